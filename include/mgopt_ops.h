@@ -1,0 +1,60 @@
+/*
+ * mgopt_ops.h -- C ABI of the operators of a training step around its matrix
+ * products and attention (libmgopt.so): token embedding, query/key norms with
+ * the rotary rotation, the MLP's activation with an 8-bit checkpoint, and the
+ * clipped policy loss.  Their gradients are the ones the optimizer step
+ * (mgopt.h) reads.
+ *
+ * Conventions are those of mgopt.h: *_dev arguments are device pointers to
+ * memory of the caller's, calls are asynchronous on `stream` and wait for
+ * nothing, the return value is 0 or a hipError_t / MGOPT_E_* code that
+ * mgopt_last_error() explains.  Calls launch on the current device, which must
+ * be the stream's.  They allocate nothing, so they can be captured in a graph.
+ * Element types are MGOPT_F32, MGOPT_F16 and MGOPT_BF16; strides count
+ * elements; the last dimension is always contiguous.  Arithmetic, sums and
+ * statistics are held in 32 bits or more and rounded once to the output's type.
+ * Same inputs give the same bits: no result depends on the order of atomics.
+ */
+#ifndef MGOPT_OPS_H
+#define MGOPT_OPS_H
+
+#include <stdint.h>
+
+#include "mgopt.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- the MLP's activation ------------------------------------------------ */
+
+#define MGOPT_ACT_SILU 0       /* x / (1 + exp(-x)) */
+#define MGOPT_ACT_GELU_TANH 1  /* x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2 */
+#define MGOPT_ACT_GROUP 128    /* elements of a row that share a scale in a checkpoint */
+
+/* y = act(gate) * up, or act(gate) where up_dev is NULL, for `rows` rows of
+ * `width` elements; y is contiguous.  With codes_dev and scales_dev, also the
+ * 8-bit checkpoint of gate and up that mgopt_gated_act_backward reads: with
+ * G = ceil(width / 128) groups a row, codes_dev (8-byte aligned) holds
+ * [inputs][rows][G * 128] int8 and scales_dev [inputs][rows][G] floats, inputs
+ * being gate and, where there is one, up.  A group whose largest magnitude is
+ * m holds scale = m * (1/127) and the integers nearest to x * (127 / m), ties
+ * to even; m below 2^-119 counts as 0, and a group with an inf or a NaN has
+ * the scale NaN. */
+MGOPT_API int mgopt_gated_act(const void* gate_dev, int64_t gate_stride, const void* up_dev, int64_t up_stride,
+                              int32_t dtype, int64_t rows, int64_t width, int32_t act, void* y_dev, int8_t* codes_dev,
+                              float* scales_dev, void* stream);
+
+/* From the gradient of y and the checkpoint (g, u): d_gate = dy * u * act'(g),
+ * d_up = dy * act(g) (d_up_dev is NULL exactly where gated is 0, and u is 1
+ * then), and, where y_dev is not NULL, y = act(g) * u again, contiguous. */
+MGOPT_API int mgopt_gated_act_backward(const void* grad_out_dev, int64_t grad_out_stride, const int8_t* codes_dev,
+                                       const float* scales_dev, int32_t gated, int32_t dtype, int64_t rows,
+                                       int64_t width, int32_t act, void* d_gate_dev, int64_t d_gate_stride,
+                                       void* d_up_dev, int64_t d_up_stride, void* y_dev, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* MGOPT_OPS_H */

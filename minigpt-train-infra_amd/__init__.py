@@ -9,7 +9,12 @@ Drop-in replacements for the torch calls of the reference's training loop
 
 plus the loop's host helpers (build_adamw_param_groups, set_optimizer_lr,
 cosine_lr, optimizer_completed_steps) and the checkpoint loaders it calls on
-resume (load_optimizer_state, load_grad_scaler_state).  The arithmetic runs
+resume (load_optimizer_state, load_grad_scaler_state).  Beside them, the
+operators of a training step around its matrix products and attention:
+
+    gated_act       the MLP's activation with an 8-bit checkpoint
+
+The arithmetic runs
 in hand-written gfx950 kernels (libmgopt.so, C ABI in include/mgopt.h); there
 is no CPU path.
 
@@ -19,6 +24,7 @@ importlib.import_module("minigpt-train-infra_amd").
 
 from .adamw import AdamW
 from .clip_grad import clip_grad_norm_
+from .gated_act import ActCheckpoint, gated_act, gated_act_backward, gated_act_pack
 from .grad_scaler import GradScaler
 from .schedule import build_adamw_param_groups, cosine_lr, optimizer_completed_steps, set_optimizer_lr
 from .state_load import load_grad_scaler_state, load_optimizer_state
@@ -35,4 +41,8 @@ __all__ = [
     "load_optimizer_state",
     "load_grad_scaler_state",
     "paramsets",
+    "ActCheckpoint",
+    "gated_act",
+    "gated_act_backward",
+    "gated_act_pack",
 ]

@@ -38,6 +38,11 @@ EXPORTS = (
     "mgopt_last_error",
     "mgopt_version",
 )
+#: every symbol include/mgopt_ops.h declares; the host helper calls them by address
+OPS_EXPORTS = (
+    "mgopt_gated_act",
+    "mgopt_gated_act_backward",
+)
 
 
 class TensorDesc(ctypes.Structure):
@@ -166,6 +171,19 @@ def entry_address(name: str) -> int:
     if addr is None:
         addr = _addresses[name] = ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
     return addr
+
+
+_ops = None
+
+
+def ops():
+    """The host helper with the training-step operators' entry points bound."""
+    global _ops
+    if _ops is None:
+        h = host()
+        h.bind_ops({name: entry_address(name) for name in (*OPS_EXPORTS, "mgopt_last_error")}, MgoptError)
+        _ops = h
+    return _ops
 
 
 def check(rc: int, what: str) -> None:

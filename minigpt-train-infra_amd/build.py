@@ -13,7 +13,8 @@ import sys
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
-SRC = HERE / "csrc" / "mgopt.hip"
+#: the optimizer step and the training-step operators
+SRCS = [HERE / "csrc" / name for name in ("mgopt.hip", "ops_gated_act.hip")]
 INCLUDE = HERE.parent / "include"
 OUT_DIR = HERE / "_build"
 LIB = OUT_DIR / "libmgopt.so"
@@ -23,7 +24,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     # every fused multiply-add in the kernels is written out explicitly
     "-ffp-contract=off",
     # no packed-fp32 instructions (v_pk_*_f32) anywhere in the device code
@@ -42,21 +42,32 @@ def hipcc() -> str:
 
 def build(verbose: bool = False) -> Path:
     OUT_DIR.mkdir(exist_ok=True)
+    objects = [OUT_DIR / f"{src.stem}.o" for src in SRCS]
+    compile_ = [[hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", "-c", str(src), "-o", str(obj)] for src, obj in zip(SRCS, objects)]
+    _run(compile_, verbose)
     tmp = LIB.with_suffix(".so.tmp")
-    cmd = [hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", str(SRC), "-o", str(tmp)]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
-    noise = [ln for ln in proc.stderr.splitlines() if "packed-fp32-ops" not in ln and ln.strip()]
-    if verbose and noise:
-        print("\n".join(noise), file=sys.stderr)
+    _run([[hipcc(), *HIPCC_FLAGS, "-shared", *map(str, objects), "-o", str(tmp)]], verbose)
     os.replace(tmp, LIB)
     return LIB
 
 
-HOST_SRC = HERE / "csrc" / "host_ptrs.cpp"
+def _run(commands: list[list[str]], verbose: bool) -> None:
+    """Runs the commands side by side; raises with the output of the first that fails."""
+    procs = []
+    for cmd in commands:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        procs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True))
+    results = [(p, *p.communicate()) for p in procs]
+    for p, out, err in results:
+        if p.returncode != 0:
+            raise RuntimeError(f"hipcc failed ({p.returncode}):\n{out}\n{err}")
+        noise = [ln for ln in err.splitlines() if "packed-fp32-ops" not in ln and ln.strip()]
+        if verbose and noise:
+            print("\n".join(noise), file=sys.stderr)
+
+
+HOST_SRCS = [HERE / "csrc" / name for name in ("host_ptrs.cpp", "host_ops.cpp")]
 HOST_DIR = OUT_DIR / "host"
 
 
@@ -67,7 +78,8 @@ def build_host(verbose: bool = False) -> Path:
     if HOST_DIR.exists():
         shutil.rmtree(HOST_DIR)
     HOST_DIR.mkdir(parents=True)
-    load(name="mgopt_host", sources=[str(HOST_SRC)], build_directory=str(HOST_DIR), extra_cflags=["-O2"],
+    load(name="mgopt_host", sources=list(map(str, HOST_SRCS)), build_directory=str(HOST_DIR), extra_cflags=["-O2"],
+         extra_include_paths=[str(INCLUDE)],
          verbose=verbose)
     return HOST_DIR / "mgopt_host.so"
 

@@ -270,6 +270,8 @@ int scaler_update(uint64_t fn, uint64_t scale, uint64_t tracker, uint64_t found,
 
 }  // namespace
 
+void define_ops(py::module_& m);  // host_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     py::class_<ParamSet>(m, "ParamSet")
         .def(py::init<std::vector<at::Tensor>, std::vector<c10::optional<at::Tensor>>>())
@@ -286,4 +288,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("scaler_update", &scaler_update);
     m.def("clip_table", &clip_table);
     m.def("clip_launch", &clip_launch);
+    define_ops(m);
 }

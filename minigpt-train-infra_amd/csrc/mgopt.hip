@@ -1279,6 +1279,15 @@ int hip_fail(hipError_t e, const char* what) {
     return fail(static_cast<int>(e), std::string(what) + ": " + hipGetErrorString(e));
 }
 
+}  // namespace
+
+namespace mgopt {
+// for the operators' translation units (ops_common.h)
+int set_error(int code, const std::string& msg) { return fail(code, msg); }
+}  // namespace mgopt
+
+namespace {
+
 #define HIP_TRY(expr)                                   \
     do {                                                \
         hipError_t _e = (expr);                         \
