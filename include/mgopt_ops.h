@@ -53,6 +53,73 @@ MGOPT_API int mgopt_gated_act_backward(const void* grad_out_dev, int64_t grad_ou
                                        int64_t width, int32_t act, void* d_gate_dev, int64_t d_gate_stride,
                                        void* d_up_dev, int64_t d_up_stride, void* y_dev, void* stream);
 
+/* ---- the clipped policy loss ---------------------------------------------- */
+
+#define MGOPT_MASK_NONE 0   /* every row counts once */
+#define MGOPT_MASK_BYTES 1  /* one byte a row: 0 leaves it out */
+#define MGOPT_MASK_F32 2    /* a weight a row */
+
+/* Row n holds the logits of one token.
+ *   logits_dev     [rows] of `vocab` elements, logits_stride elements apart.
+ *   targets_dev    the token that was taken, of target_bytes (4 or 8) bytes.
+ *   old_logp_dev, advantages_dev, ref_logp_dev (NULL: no KL term): [rows].
+ *   mask_dev       by mask_kind.  A row of weight 0 is not read: its target,
+ *                  logits and other values may be anything.
+ *   clip_low,
+ *   clip_high      the ratio is clipped to [1 - clip_low, 1 + clip_high].
+ *   grad_scale_dev a factor of the gradient (a loss scaler's scale, or the
+ *                  gradient of the loss), or NULL.
+ *   log_probs_dev  [rows]: each row's log-probability of its target, 0 for a
+ *                  row of weight 0.
+ *   d_logits_dev   the gradient, of the logits' type, or NULL; it may be
+ *                  logits_dev itself with the same stride.
+ *   workspace_dev  mgopt_policy_workspace(rows) bytes, 16-byte aligned.
+ * A target outside [0, vocab) in a row that counts makes the loss and that
+ * row's gradient NaN. */
+typedef struct mgopt_policy_args {
+    const void* logits_dev;
+    const void* targets_dev;
+    const float* old_logp_dev;
+    const float* advantages_dev;
+    const float* ref_logp_dev;
+    const void* mask_dev;
+    const float* grad_scale_dev;
+    float* log_probs_dev;
+    void* d_logits_dev;
+    void* workspace_dev;
+    int64_t rows;
+    int64_t vocab;
+    int64_t logits_stride;
+    int64_t d_logits_stride;
+    double clip_low;
+    double clip_high;
+    double kl_coef;
+    double temperature;
+    int32_t dtype;
+    int32_t target_bytes;
+    int32_t mask_kind;
+    int32_t reserved;
+} mgopt_policy_args;
+
+MGOPT_API int64_t mgopt_policy_workspace(int64_t rows);
+
+/* Writes log_probs_dev.  Reads logits, targets and mask; needs no workspace. */
+MGOPT_API int mgopt_token_log_probs(const mgopt_policy_args* args, void* stream);
+
+/* With logp = log_softmax(logits / temperature)[target], ratio =
+ * exp(logp - old_logp) and r = ref_logp - logp:
+ *   policy = -min(ratio * A, clip(ratio) * A)    kl = exp(r) - r - 1
+ * loss_dev[0] = mean(policy) + kl_coef * mean(kl), parts_dev[0..2] =
+ * mean(policy), mean(kl) and the share of rows whose gradient the clip holds at
+ * 0, all weighted by the mask (0 where every weight is 0).  With d_logits_dev,
+ * also the gradient of grad_scale * loss, reading the logits once; without it,
+ * the workspace keeps what mgopt_policy_loss_backward needs. */
+MGOPT_API int mgopt_policy_loss(const mgopt_policy_args* args, float* loss_dev, float* parts_dev, void* stream);
+
+/* The gradient of grad_scale * loss, after mgopt_policy_loss without
+ * d_logits_dev on the same arguments, log_probs_dev and workspace_dev. */
+MGOPT_API int mgopt_policy_loss_backward(const mgopt_policy_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@ resume (load_optimizer_state, load_grad_scaler_state).  Beside them, the
 operators of a training step around its matrix products and attention:
 
     gated_act       the MLP's activation with an 8-bit checkpoint
+    policy_loss     the clipped policy loss with a KL term over the logits
 
 The arithmetic runs
 in hand-written gfx950 kernels (libmgopt.so, C ABI in include/mgopt.h); there
@@ -26,6 +27,7 @@ from .adamw import AdamW
 from .clip_grad import clip_grad_norm_
 from .gated_act import ActCheckpoint, gated_act, gated_act_backward, gated_act_pack
 from .grad_scaler import GradScaler
+from .policy_loss import PolicyLoss, policy_loss, policy_loss_grad, token_log_probs
 from .schedule import build_adamw_param_groups, cosine_lr, optimizer_completed_steps, set_optimizer_lr
 from .state_load import load_grad_scaler_state, load_optimizer_state
 from . import paramsets
@@ -45,4 +47,8 @@ __all__ = [
     "gated_act",
     "gated_act_backward",
     "gated_act_pack",
+    "PolicyLoss",
+    "policy_loss",
+    "policy_loss_grad",
+    "token_log_probs",
 ]

@@ -42,6 +42,10 @@ EXPORTS = (
 OPS_EXPORTS = (
     "mgopt_gated_act",
     "mgopt_gated_act_backward",
+    "mgopt_policy_workspace",
+    "mgopt_token_log_probs",
+    "mgopt_policy_loss",
+    "mgopt_policy_loss_backward",
 )
 
 
@@ -205,6 +209,12 @@ def stream_handle(device) -> int:
     if raw is not None:
         return raw(index)
     return torch.cuda.current_stream(index).cuda_stream
+
+
+def ops_stream(t) -> int:
+    """The stream an operator on tensor `t` runs on (0 for a tensor that is not
+    on a GPU, which the operator refuses)."""
+    return stream_handle(t.device) if t.is_cuda else 0
 
 
 def dtype_code(dtype) -> int:

@@ -7,6 +7,7 @@
 
 #include <torch/extension.h>
 
+#include <cmath>
 #include <cstdint>
 #include <string>
 #include <tuple>
@@ -22,6 +23,10 @@ using c10::optional;
 struct Entries {
     decltype(&mgopt_gated_act) gated_act = nullptr;
     decltype(&mgopt_gated_act_backward) gated_act_backward = nullptr;
+    decltype(&mgopt_policy_workspace) policy_workspace = nullptr;
+    decltype(&mgopt_token_log_probs) token_log_probs = nullptr;
+    decltype(&mgopt_policy_loss) policy_loss = nullptr;
+    decltype(&mgopt_policy_loss_backward) policy_loss_backward = nullptr;
     decltype(&mgopt_last_error) last_error = nullptr;
     PyObject* error = nullptr;  // the package's MgoptError
 } lib;
@@ -33,6 +38,10 @@ void bind_ops(const py::dict& addresses, const py::object& error) {
     };
     take(lib.gated_act, "mgopt_gated_act");
     take(lib.gated_act_backward, "mgopt_gated_act_backward");
+    take(lib.policy_workspace, "mgopt_policy_workspace");
+    take(lib.token_log_probs, "mgopt_token_log_probs");
+    take(lib.policy_loss, "mgopt_policy_loss");
+    take(lib.policy_loss_backward, "mgopt_policy_loss_backward");
     take(lib.last_error, "mgopt_last_error");
     Py_XDECREF(lib.error);
     lib.error = error.inc_ref().ptr();
@@ -172,10 +181,155 @@ std::tuple<Tensor, optional<Tensor>, optional<Tensor>> gated_act_backward(const 
     return {d_gate, d_up, y};
 }
 
+// ------------------------------------------------------------ policy_loss
+
+// One value per row, in the rows' order.
+Tensor per_row(const Tensor& t, const Tensor& logits, int64_t rows, const char* name) {
+    beside(t, logits, name);
+    if (t.numel() != rows)
+        refuse(std::string(name) + " has " + std::to_string(t.numel()) + " values for " + std::to_string(rows) + " rows");
+    return t.contiguous();
+}
+Tensor float_per_row(const Tensor& t, const Tensor& logits, int64_t rows, const char* name) {
+    if (t.scalar_type() != at::kFloat)
+        throw py::type_error(std::string(name) + " must be float32, got " + c10::toString(t.scalar_type()));
+    return per_row(t, logits, rows, name);
+}
+
+// The arguments all three entry points share, with the tensors that keep them alive.
+struct Policy {
+    mgopt_policy_args a{};
+    Rows logits;
+    Tensor targets, mask, log_probs;
+};
+Policy policy_args(const Tensor& logits, const Tensor& targets, const optional<Tensor>& mask, double temperature) {
+    Policy p;
+    on_gpu(logits, "logits");
+    p.a.dtype = code_of(logits, "logits");
+    if (logits.dim() < 1 || logits.size(-1) < 1) refuse("logits need a last dimension of at least 1, got " + shape_of(logits));
+    if (!(temperature > 0.0) || !std::isfinite(temperature)) refuse("the temperature must be positive and finite");
+    p.logits = rows_of(logits);
+    const int64_t rows = p.logits.rows;
+    if (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt)
+        throw py::type_error("targets must be int64 or int32");
+    p.targets = per_row(targets, logits, rows, "targets");
+    if (mask.has_value()) {
+        if (mask->scalar_type() != at::kBool && mask->scalar_type() != at::kFloat)
+            throw py::type_error("mask must be bool or float32");
+        p.mask = per_row(*mask, logits, rows, "mask");
+        p.a.mask_kind = mask->scalar_type() == at::kBool ? MGOPT_MASK_BYTES : MGOPT_MASK_F32;
+        p.a.mask_dev = p.mask.data_ptr();
+    }
+    p.a.logits_dev = p.logits.t.data_ptr();
+    p.a.logits_stride = p.logits.stride;
+    p.a.targets_dev = p.targets.data_ptr();
+    p.a.target_bytes = static_cast<int32_t>(p.targets.element_size());
+    p.a.rows = rows;
+    p.a.vocab = p.logits.width;
+    p.a.temperature = temperature;
+    return p;
+}
+
+std::vector<int64_t> all_but_last(const Tensor& t) { return {t.sizes().begin(), t.sizes().end() - 1}; }
+
+Tensor token_log_probs(const Tensor& logits, const Tensor& targets, const optional<Tensor>& mask, double temperature,
+                       uint64_t stream) {
+    Policy p = policy_args(logits, targets, mask, temperature);
+    const c10::DeviceGuard guard(logits.device());
+    Tensor out = at::empty(all_but_last(logits), logits.options().dtype(at::kFloat));
+    p.a.log_probs_dev = out.data_ptr<float>();
+    check(lib.token_log_probs(&p.a, as_stream(stream)), "token_log_probs");
+    return out;
+}
+
+// The loss's inputs beside the logits, as one call's arguments.
+struct Loss {
+    Policy p;
+    Tensor old_logp, advantages, ref, scale;
+};
+Loss loss_args(const Tensor& logits, const Tensor& targets, const Tensor& old_logp, const Tensor& advantages,
+               const optional<Tensor>& ref, const optional<Tensor>& mask, double clip_low, double clip_high, double kl_coef,
+               double temperature, const optional<Tensor>& scale) {
+    Loss l;
+    l.p = policy_args(logits, targets, mask, temperature);
+    mgopt_policy_args& a = l.p.a;
+    if (!(clip_low >= 0.0) || !(clip_high >= 0.0)) refuse("the clip range must not be negative");
+    l.old_logp = float_per_row(old_logp, logits, a.rows, "old_logp");
+    l.advantages = float_per_row(advantages, logits, a.rows, "advantages");
+    a.old_logp_dev = l.old_logp.data_ptr<float>();
+    a.advantages_dev = l.advantages.data_ptr<float>();
+    if (ref.has_value()) {
+        l.ref = float_per_row(*ref, logits, a.rows, "ref_logp");
+        a.ref_logp_dev = l.ref.data_ptr<float>();
+    }
+    if (scale.has_value()) {
+        beside(*scale, logits, "grad_scale");
+        if (scale->scalar_type() != at::kFloat || scale->numel() != 1) refuse("grad_scale must be one float32 value");
+        l.scale = *scale;
+        a.grad_scale_dev = l.scale.data_ptr<float>();
+    }
+    a.clip_low = clip_low, a.clip_high = clip_high, a.kl_coef = kl_coef;
+    return l;
+}
+
+// (loss, log_probs, policy, kl, clip_fraction, gradient or None, workspace)
+py::tuple policy_loss(const Tensor& logits, const Tensor& targets, const Tensor& old_logp, const Tensor& advantages,
+                      const optional<Tensor>& ref, const optional<Tensor>& mask, double clip_low, double clip_high,
+                      double kl_coef, double temperature, const optional<Tensor>& scale, bool want_grad,
+                      const optional<Tensor>& out, uint64_t stream) {
+    Loss l = loss_args(logits, targets, old_logp, advantages, ref, mask, clip_low, clip_high, kl_coef, temperature, scale);
+    mgopt_policy_args& a = l.p.a;
+    const c10::DeviceGuard guard(logits.device());
+    const auto f32 = logits.options().dtype(at::kFloat);
+    Tensor log_probs = at::empty(all_but_last(logits), f32), loss = at::empty({}, f32), parts = at::empty({3}, f32);
+    Tensor work = at::empty({lib.policy_workspace(a.rows)}, logits.options().dtype(at::kByte));
+    a.log_probs_dev = log_probs.data_ptr<float>();
+    a.workspace_dev = work.data_ptr();
+    optional<Tensor> grad;
+    if (want_grad) {
+        if (out.has_value()) {
+            beside(*out, logits, "out");
+            same_dtype(*out, logits, "out");
+            if (out->sizes() != logits.sizes()) refuse("out has shape " + shape_of(*out) + ", logits " + shape_of(logits));
+            const Rows r = rows_of(*out);
+            if (!r.t.is_same(*out)) refuse("out needs rows that are contiguous and evenly spaced");
+            if (out->data_ptr() == logits.data_ptr() && (l.p.logits.stride != r.stride || !l.p.logits.t.is_same(logits)))
+                refuse("out overlaps the logits and is not them");
+            grad = *out;
+            a.d_logits_stride = r.stride;
+        } else {
+            grad = at::empty(logits.sizes(), logits.options());
+            a.d_logits_stride = a.vocab;
+        }
+        a.d_logits_dev = grad->data_ptr();
+    }
+    check(lib.policy_loss(&a, loss.data_ptr<float>(), parts.data_ptr<float>(), as_stream(stream)), "policy_loss");
+    return py::make_tuple(loss, log_probs, parts.select(0, 0), parts.select(0, 1), parts.select(0, 2), grad, work);
+}
+
+Tensor policy_loss_backward(const Tensor& logits, const Tensor& targets, const Tensor& old_logp, const Tensor& advantages,
+                            const optional<Tensor>& ref, const optional<Tensor>& mask, double clip_low, double clip_high,
+                            double kl_coef, double temperature, const Tensor& scale, const Tensor& log_probs,
+                            const Tensor& work, uint64_t stream) {
+    Loss l = loss_args(logits, targets, old_logp, advantages, ref, mask, clip_low, clip_high, kl_coef, temperature, scale);
+    mgopt_policy_args& a = l.p.a;
+    const c10::DeviceGuard guard(logits.device());
+    Tensor grad = at::empty(logits.sizes(), logits.options());
+    a.log_probs_dev = log_probs.data_ptr<float>();
+    a.workspace_dev = work.data_ptr();
+    a.d_logits_dev = grad.data_ptr();
+    a.d_logits_stride = a.vocab;
+    check(lib.policy_loss_backward(&a, as_stream(stream)), "policy_loss_backward");
+    return grad;
+}
+
 }  // namespace
 
 void define_ops(py::module_& m) {
     m.def("bind_ops", &bind_ops);
     m.def("gated_act", &gated_act);
     m.def("gated_act_backward", &gated_act_backward);
+    m.def("token_log_probs", &token_log_probs);
+    m.def("policy_loss", &policy_loss);
+    m.def("policy_loss_backward", &policy_loss_backward);
 }

@@ -1,0 +1,346 @@
+// ops_policy_loss.hip -- the clipped policy loss with a KL term over a batch's
+// logits, its gradient, and the log-probabilities it is made of.
+//
+// For row n with logits x, target y, temperature T and weight w_n (the mask):
+//
+//     logp   = x_y / T - log sum_j exp(x_j / T)        ratio = exp(logp - old)
+//     policy = -min(ratio * A, clip(ratio, lo, hi) * A)
+//     kl     = exp(r) - r - 1,  r = ref - logp
+//     loss   = sum_n w_n (policy + kl_coef * kl) / sum_n w_n
+//
+// and, with p the softmax and [.] one where it holds,
+//
+//     slope  = w_n / sum(w) * ((clipped ? 0 : -ratio * A) + kl_coef * (1 - exp(r)))
+//     dx_j   = scale * slope / T * ([j = y] - p_j)
+//
+// A row is one work-group's: a pass over it keeps, per thread, the maximum m
+// and the sum s of exp((x - m) / T); the row's scalars are formed once, in 64
+// bits; a second pass writes the gradient.  The exponent is ((x - m) * log2(e) / T):
+// subtracting first keeps rows of the type's lowest value (m is that value)
+// and entries of it finite, and small differences exact.  Rows of weight 0 are
+// not read.
+//
+// Bound by memory: a row's logits once, its gradient once.
+#include "ops_common.h"
+
+namespace mgopt {
+namespace {
+
+enum Mode { kLogp, kLoss, kLossGrad, kGrad };
+
+struct PolicyArgs {
+    const void* logits;
+    int64_t row_stride, rows, vocab, first_row;
+    const void* targets;
+    int32_t target_bytes, mask_kind;
+    const float *old_logp, *ref_logp, *advantages;
+    const void* mask;
+    double low, high, kl_coef, inv_temp;
+    float c;                     // log2(e) / T
+    const float* grad_scale;     // may be NULL
+    const double* weight_sum;    // NULL: every row's weight is 1
+    float* log_probs;
+    float2* stats;               // m and s of each row: written by kLoss, read by kGrad
+    float4* terms;               // w * policy, w * kl, w * clipped
+    void* d_logits;
+    int64_t d_stride;
+};
+
+__device__ __forceinline__ float weight_at(const void* mask, int32_t kind, int64_t n) {
+    if (kind == MGOPT_MASK_NONE) return 1.0f;
+    if (kind == MGOPT_MASK_BYTES) return static_cast<const uint8_t*>(mask)[n] != 0 ? 1.0f : 0.0f;
+    return static_cast<const float*>(mask)[n];
+}
+
+// m and s of a running sum of exp2((x - m) * c).  m is -inf until a larger
+// value was seen; the differences are then taken to 0, so that -inf - -inf
+// does not occur (a row of nothing but -inf keeps s = 0, and its log is -inf).
+struct Running {
+    float m, s;
+};
+__device__ __forceinline__ float base(float m) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ Running join(Running a, Running b, float c) {
+    const float m = fmaxf(a.m, b.m), o = base(m);
+    return {m, a.s * exp2_hw((a.m - o) * c) + b.s * exp2_hw((b.m - o) * c)};
+}
+template <int N>
+__device__ __forceinline__ void take(Running& r, const float (&x)[N], float c) {
+    float m = r.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+    const float o = base(m);
+    float s = r.s * exp2_hw((r.m - o) * c);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += exp2_hw((x[i] - o) * c);
+    r = {m, s};
+}
+
+template <int NT>
+__device__ __forceinline__ Running join_block(Running r, float c) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) r = join(r, Running{__shfl_xor(r.m, off), __shfl_xor(r.s, off)}, c);
+    if constexpr (NT > 64) {
+        __shared__ Running part[NT / 64];
+        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = r;
+        __syncthreads();
+        r = part[0];
+#pragma unroll
+        for (int i = 1; i < NT / 64; ++i) r = join(r, part[i], c);
+    }
+    return r;
+}
+
+struct RowResult {
+    float slope, k;  // of the gradient: slope * [j = y] + k * exp2((x - m) * c)
+};
+
+// What one row adds to the loss, and its slope, from m and s.
+template <typename T, Mode MODE>
+__device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, float w, float m, float s) {
+    const int64_t y = id_at(a.targets, n, a.target_bytes);
+    double logp;
+    if constexpr (MODE == kGrad) {
+        logp = a.log_probs[n];
+    } else {
+        const double x = y >= 0 && y < a.vocab
+                             ? static_cast<double>(static_cast<float>(static_cast<const T*>(a.logits)[n * a.row_stride + y]))
+                             : __builtin_nan("");
+        logp = (x - static_cast<double>(base(m))) * a.inv_temp - log(static_cast<double>(s));
+        a.log_probs[n] = static_cast<float>(logp);
+    }
+    if constexpr (MODE == kLogp) return {};
+    const double A = a.advantages[n], ratio = exp(logp - static_cast<double>(a.old_logp[n]));
+    const double s1 = ratio * A, s2 = fmin(fmax(ratio, a.low), a.high) * A;
+    const bool held = s2 < s1;
+    double slope = held ? 0.0 : -s1, kl = 0.0;
+    if (a.ref_logp != nullptr) {
+        const double r = static_cast<double>(a.ref_logp[n]) - logp, e = expm1(r);
+        kl = e - r;
+        slope -= a.kl_coef * e;
+    }
+    if constexpr (MODE != kGrad)
+        a.terms[n] = make_float4(static_cast<float>(w * -(held ? s2 : s1)), static_cast<float>(w * kl), held ? w : 0.0f, 0.0f);
+    if constexpr (MODE == kLoss) a.stats[n] = make_float2(m, s);
+    if constexpr (MODE == kLoss) return {};
+    const double total = a.weight_sum != nullptr ? *a.weight_sum : static_cast<double>(a.rows);
+    slope *= w / total * a.inv_temp;
+    if (a.grad_scale != nullptr) slope *= static_cast<double>(*a.grad_scale);
+    return {static_cast<float>(slope), static_cast<float>(-slope / static_cast<double>(s))};
+}
+
+template <typename T, int NT, Mode MODE>
+__global__ __launch_bounds__(NT) void policy_kernel(PolicyArgs a) {
+    constexpr int N = 16 / sizeof(T);
+    const int64_t n = a.first_row + blockIdx.x, V = a.vocab;
+    const float w = weight_at(a.mask, a.mask_kind, n);
+    const T* x = static_cast<const T*>(a.logits) + n * a.row_stride;
+    T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
+    const int64_t start = static_cast<int64_t>(threadIdx.x) * N;
+    constexpr int64_t kStep = int64_t{NT} * N;
+    if (w == 0.0f) {
+        if (MODE != kGrad && threadIdx.x == 0) {
+            a.log_probs[n] = 0.0f;
+            if (MODE != kLogp) a.terms[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        if constexpr (MODE == kLossGrad || MODE == kGrad) {
+            const float zero[N] = {};
+            for (int64_t i = start; i < V; i += kStep) store_some<N>(dx + i, zero, V - i);
+        }
+        return;
+    }
+    Running r{-INFINITY, 0.0f};
+    if constexpr (MODE == kGrad) {
+        const float2 q = a.stats[n];
+        r = {q.x, q.y};
+    } else {
+        int64_t i = start;
+        for (; i + N <= V; i += kStep) {
+            float v[N];
+            load<N>(v, x + i);
+            take<N>(r, v, a.c);
+        }
+        for (; i < V; ++i) {  // the row's last vector, where it is cut short
+            const float v[1] = {static_cast<float>(x[i])};
+            take<1>(r, v, a.c);
+        }
+        r = join_block<NT>(r, a.c);
+    }
+    __shared__ RowResult shared;
+    if (threadIdx.x == 0) {
+        const RowResult q = row_scalars<T, MODE>(a, n, w, r.m, r.s);
+        if constexpr (MODE == kLossGrad || MODE == kGrad) shared = q;
+    }
+    if constexpr (MODE == kLossGrad || MODE == kGrad) {
+        __syncthreads();
+        const RowResult q = shared;
+        const float o = base(r.m);
+        const int64_t y = id_at(a.targets, n, a.target_bytes);
+        for (int64_t i = start; i < V; i += kStep) {
+            float v[N];
+            load_some<N>(v, x + i, V - i);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = q.k * exp2_hw((v[j] - o) * a.c);
+            if (y >= i && y < i + N) {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (y == i + j) v[j] += q.slope;
+            }
+            store_some<N>(dx + i, v, V - i);
+        }
+    }
+}
+
+constexpr int kSumBlock = 1024;
+
+template <typename X>
+__device__ __forceinline__ X sum_block(X x) {
+    __shared__ X part[kSumBlock / 64];
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
+    __syncthreads();  // an earlier call's reads
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
+    __syncthreads();
+    x = part[0];
+#pragma unroll
+    for (int i = 1; i < kSumBlock / 64; ++i) x += part[i];
+    return x;
+}
+
+__global__ __launch_bounds__(kSumBlock) void weight_sum_kernel(const void* mask, int32_t kind, int64_t rows, double* out) {
+    double x = 0.0;
+    for (int64_t n = threadIdx.x; n < rows; n += kSumBlock) x += weight_at(mask, kind, n);
+    x = sum_block(x);
+    if (threadIdx.x == 0) *out = x;
+}
+
+// loss, policy, kl, clipped share from the rows' terms.  Rows that all have
+// weight 0 make all four 0.
+__global__ __launch_bounds__(kSumBlock) void policy_sum_kernel(const float4* terms, int64_t rows, const double* weight_sum,
+                                                               double kl_coef, float* loss, float* parts) {
+    double p = 0.0, k = 0.0, h = 0.0;
+    for (int64_t n = threadIdx.x; n < rows; n += kSumBlock) {
+        const float4 t = terms[n];
+        p += t.x, k += t.y, h += t.z;
+    }
+    p = sum_block(p), k = sum_block(k), h = sum_block(h);
+    if (threadIdx.x == 0) {
+        const double total = weight_sum != nullptr ? *weight_sum : static_cast<double>(rows);
+        const double inv = total == 0.0 ? 0.0 : 1.0 / total;
+        *loss = static_cast<float>((p + kl_coef * k) * inv);
+        parts[0] = static_cast<float>(p * inv);
+        parts[1] = static_cast<float>(k * inv);
+        parts[2] = static_cast<float>(h * inv);
+    }
+}
+
+// Threads of a row: enough to keep a row's loads in flight, few enough that
+// short rows do not idle.
+template <typename T, Mode MODE>
+int launch_rows(PolicyArgs a, hipStream_t s) {
+    constexpr int N = 16 / sizeof(T);
+    const int64_t most = max_blocks(1024);
+    for (a.first_row = 0; a.first_row < a.rows; a.first_row += most) {
+        const dim3 grid(static_cast<uint32_t>(a.rows - a.first_row < most ? a.rows - a.first_row : most));
+        if (a.vocab <= 256 * N) hipLaunchKernelGGL((policy_kernel<T, 64, MODE>), grid, dim3(64), 0, s, a);
+        else if (a.vocab <= 2048 * N) hipLaunchKernelGGL((policy_kernel<T, 256, MODE>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((policy_kernel<T, 1024, MODE>), grid, dim3(1024), 0, s, a);
+        if (int rc = launched("policy_kernel")) return rc;
+    }
+    return 0;
+}
+
+int check(const mgopt_policy_args* p, const char* what) {
+    const std::string w(what);
+    if (!p) return set_error(MGOPT_E_INVALID, w + ": NULL arguments");
+    if (!known_dtype(p->dtype)) return set_error(MGOPT_E_INVALID, w + ": bad dtype");
+    if (p->rows < 0 || p->vocab < 1) return set_error(MGOPT_E_INVALID, w + ": need rows >= 0 and vocab >= 1");
+    if (p->target_bytes != 4 && p->target_bytes != 8) return set_error(MGOPT_E_INVALID, w + ": targets have 4 or 8 bytes");
+    if (p->mask_kind < MGOPT_MASK_NONE || p->mask_kind > MGOPT_MASK_F32) return set_error(MGOPT_E_INVALID, w + ": bad mask kind");
+    if (!(p->temperature > 0.0) || !std::isfinite(p->temperature))
+        return set_error(MGOPT_E_INVALID, w + ": the temperature must be positive and finite");
+    if (p->rows > 0 && (!p->logits_dev || !p->targets_dev || !p->log_probs_dev))
+        return set_error(MGOPT_E_INVALID, w + ": NULL argument");
+    if ((p->mask_kind != MGOPT_MASK_NONE) != (p->mask_dev != nullptr) && p->rows > 0)
+        return set_error(MGOPT_E_INVALID, w + ": mask and mask kind disagree");
+    return 0;
+}
+
+// What the loss needs beyond the log-probabilities.
+int check_loss(const mgopt_policy_args* p, const char* what) {
+    if (int rc = check(p, what)) return rc;
+    const std::string w(what);
+    if (!(p->clip_low >= 0.0) || !(p->clip_high >= 0.0)) return set_error(MGOPT_E_INVALID, w + ": negative clip range");
+    if (!p->workspace_dev || reinterpret_cast<uintptr_t>(p->workspace_dev) % 16 != 0)
+        return set_error(MGOPT_E_ALIGN, w + ": the workspace must be 16-byte aligned");
+    if (p->rows > 0 && (!p->old_logp_dev || !p->advantages_dev)) return set_error(MGOPT_E_INVALID, w + ": NULL argument");
+    return 0;
+}
+
+PolicyArgs args_of(const mgopt_policy_args* p) {
+    PolicyArgs a{};
+    a.logits = p->logits_dev, a.row_stride = p->logits_stride, a.rows = p->rows, a.vocab = p->vocab;
+    a.targets = p->targets_dev, a.target_bytes = p->target_bytes, a.mask_kind = p->mask_kind, a.mask = p->mask_dev;
+    a.old_logp = p->old_logp_dev, a.ref_logp = p->ref_logp_dev, a.advantages = p->advantages_dev;
+    a.low = 1.0 - p->clip_low, a.high = 1.0 + p->clip_high, a.kl_coef = p->kl_coef;
+    a.inv_temp = 1.0 / p->temperature, a.c = static_cast<float>(1.4426950408889634 / p->temperature);
+    a.grad_scale = p->grad_scale_dev, a.log_probs = p->log_probs_dev;
+    a.d_logits = p->d_logits_dev, a.d_stride = p->d_logits_stride;
+    // workspace: the sum of the weights, then the rows' terms, then their m and s
+    char* at = static_cast<char*>(p->workspace_dev);
+    if (at != nullptr) {
+        a.weight_sum = p->mask_kind == MGOPT_MASK_NONE ? nullptr : reinterpret_cast<const double*>(at);
+        a.terms = reinterpret_cast<float4*>(at + 16);
+        a.stats = reinterpret_cast<float2*>(at + 16 + 16 * p->rows);
+    }
+    return a;
+}
+
+}  // namespace
+}  // namespace mgopt
+
+using namespace mgopt;
+
+extern "C" {
+
+MGOPT_API int64_t mgopt_policy_workspace(int64_t rows) { return rows < 0 ? -1 : 16 + 24 * rows; }
+
+MGOPT_API int mgopt_token_log_probs(const mgopt_policy_args* p, void* stream) {
+    if (int rc = check(p, "token_log_probs")) return rc;
+    if (p->rows == 0) return 0;
+    return with_dtype(p->dtype, [&](auto t) {
+        return launch_rows<decltype(t), kLogp>(args_of(p), static_cast<hipStream_t>(stream));
+    });
+}
+
+MGOPT_API int mgopt_policy_loss(const mgopt_policy_args* p, float* loss_dev, float* parts_dev, void* stream) {
+    if (int rc = check_loss(p, "policy_loss")) return rc;
+    if (!loss_dev || !parts_dev) return set_error(MGOPT_E_INVALID, "policy_loss: NULL argument");
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const PolicyArgs a = args_of(p);
+    if (a.weight_sum != nullptr) {
+        hipLaunchKernelGGL(weight_sum_kernel, dim3(1), dim3(kSumBlock), 0, s, a.mask, a.mask_kind, a.rows,
+                           static_cast<double*>(p->workspace_dev));
+        if (int rc = launched("weight_sum_kernel")) return rc;
+    }
+    if (p->rows > 0) {
+        const int rc = with_dtype(p->dtype, [&](auto t) {
+            using T = decltype(t);
+            return a.d_logits != nullptr ? launch_rows<T, kLossGrad>(a, s) : launch_rows<T, kLoss>(a, s);
+        });
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(kSumBlock), 0, s, a.terms, a.rows, a.weight_sum, a.kl_coef, loss_dev,
+                       parts_dev);
+    return launched("policy_sum_kernel");
+}
+
+MGOPT_API int mgopt_policy_loss_backward(const mgopt_policy_args* p, void* stream) {
+    if (int rc = check_loss(p, "policy_loss_backward")) return rc;
+    if (p->rows == 0) return 0;
+    if (!p->d_logits_dev) return set_error(MGOPT_E_INVALID, "policy_loss_backward: NULL argument");
+    return with_dtype(p->dtype, [&](auto t) {
+        return launch_rows<decltype(t), kGrad>(args_of(p), static_cast<hipStream_t>(stream));
+    });
+}
+
+}  // extern "C"

@@ -26,17 +26,12 @@ class ActCheckpoint(NamedTuple):
     act: str
 
 
-def _stream(t: torch.Tensor) -> int:
-    N.lib()
-    return N.stream_handle(t.device) if t.is_cuda else 0
-
-
 def gated_act_pack(gate: torch.Tensor, up: torch.Tensor | None = None, *,
                    act: str = "silu") -> tuple[torch.Tensor, ActCheckpoint]:
     """(y, checkpoint) of gate and up, of any shape and any strides whose rows
     (the last dimension) are contiguous and evenly spaced; others are copied
     first.  act: "silu" or "gelu_tanh".  Nothing is recorded for autograd."""
-    y, codes, scales = N.ops().gated_act(gate, up, act, True, _stream(gate))
+    y, codes, scales = N.ops().gated_act(gate, up, act, True, N.ops_stream(gate))
     return y, ActCheckpoint(codes, scales, act)
 
 
@@ -44,7 +39,7 @@ def gated_act_backward(grad_out: torch.Tensor, saved: ActCheckpoint, *,
                        want_y: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
     """(d_gate, d_up, y) from the gradient of y: d_up is None without a gate, y
     without want_y.  The outputs have grad_out's shape and dtype."""
-    return N.ops().gated_act_backward(grad_out, saved.codes, saved.scales, saved.act, want_y, _stream(grad_out))
+    return N.ops().gated_act_backward(grad_out, saved.codes, saved.scales, saved.act, want_y, N.ops_stream(grad_out))
 
 
 class _GatedAct(torch.autograd.Function):
@@ -67,4 +62,4 @@ def gated_act(gate: torch.Tensor, up: torch.Tensor | None = None, *, act: str = 
     keeps the 8-bit checkpoint and neither gate nor up."""
     if torch.is_grad_enabled() and (gate.requires_grad or (up is not None and up.requires_grad)):
         return _GatedAct.apply(gate, up, act)
-    return N.ops().gated_act(gate, up, act, False, _stream(gate))[0]
+    return N.ops().gated_act(gate, up, act, False, N.ops_stream(gate))[0]

@@ -3,6 +3,7 @@ work is launched)."""
 
 from __future__ import annotations
 
+import ctypes
 import importlib
 import re
 import subprocess
@@ -45,8 +46,6 @@ def _refused(lib, rc, code, text):
 
 
 def _gated_act(lib, gate=P, up=None, dtype=0, rows=4, width=8, act=0, y=P, codes=None, scales=None):
-    import ctypes
-
     vp, i64 = ctypes.c_void_p, ctypes.c_int64
     return lib.mgopt_gated_act(vp(gate), i64(8), vp(up), i64(8), dtype, i64(rows), i64(width), act, vp(y), vp(codes),
                                vp(scales), vp(None))
@@ -61,8 +60,50 @@ def test_gated_act_rejects_bad_arguments(native):
     assert _gated_act(lib, gate=None, rows=0) == 0
 
 
+class PolicyArgs(ctypes.Structure):            # mgopt_policy_args
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "targets", "old_logp", "advantages", "ref_logp", "mask",
+                                               "grad_scale", "log_probs", "d_logits", "workspace")]
+    _fields_ += [(n, ctypes.c_int64) for n in ("rows", "vocab", "logits_stride", "d_logits_stride")]
+    _fields_ += [(n, ctypes.c_double) for n in ("clip_low", "clip_high", "kl_coef", "temperature")]
+    _fields_ += [(n, ctypes.c_int32) for n in ("dtype", "target_bytes", "mask_kind", "reserved")]
+
+
+def _policy(**more):
+    a = PolicyArgs(logits=P, targets=P, old_logp=P, advantages=P, log_probs=P, d_logits=P, workspace=P, rows=4, vocab=8,
+                   logits_stride=8, d_logits_stride=8, clip_low=0.2, clip_high=0.2, temperature=1.0, target_bytes=8)
+    for k, v in more.items():
+        setattr(a, k, v)
+    return ctypes.byref(a)
+
+
+def test_policy_loss_rejects_bad_arguments(native):
+    lib = native.load_library()
+    vp = ctypes.c_void_p
+    lib.mgopt_policy_workspace.restype = ctypes.c_int64
+    assert lib.mgopt_policy_workspace(ctypes.c_int64(100)) >= 2400 and lib.mgopt_policy_workspace(ctypes.c_int64(-1)) == -1
+    calls = {"log_probs": lambda a: lib.mgopt_token_log_probs(a, vp(None)),
+             "policy_loss": lambda a: lib.mgopt_policy_loss(a, vp(P), vp(P), vp(None)),
+             "backward": lambda a: lib.mgopt_policy_loss_backward(a, vp(None))}
+    for name, call in calls.items():
+        for bad in (dict(dtype=5), dict(rows=-1), dict(vocab=0), dict(target_bytes=2), dict(mask_kind=3),
+                    dict(temperature=0.0), dict(temperature=float("nan")), dict(logits=None), dict(targets=None),
+                    dict(log_probs=None), dict(mask_kind=1), dict(mask=P)):
+            _refused(lib, call(_policy(**bad)), E_INVALID, name.encode())
+        _refused(lib, call(None), E_INVALID, b"NULL")
+        if name != "log_probs":
+            for bad in (dict(clip_low=-0.1), dict(clip_high=float("nan")), dict(old_logp=None), dict(advantages=None)):
+                _refused(lib, call(_policy(**bad)), E_INVALID, name.encode())
+            for bad in (dict(workspace=None), dict(workspace=P + 8)):
+                _refused(lib, call(_policy(**bad)), E_ALIGN, b"workspace")
+    _refused(lib, calls["backward"](_policy(d_logits=None)), E_INVALID, b"NULL")
+    _refused(lib, lib.mgopt_policy_loss(_policy(), vp(None), vp(P), vp(None)), E_INVALID, b"NULL")
+    assert calls["log_probs"](_policy(rows=0)) == 0 and calls["backward"](_policy(rows=0)) == 0
+
+
 def test_operators_have_no_cpu_path(mg):
     if torch.cuda.is_available():
         pytest.skip("a GPU is visible")
     with pytest.raises(RuntimeError, match="no CPU"):
         mg.gated_act(torch.ones(3, 4))
+    with pytest.raises(RuntimeError, match="no CPU"):
+        mg.token_log_probs(torch.ones(3, 4), torch.zeros(3, dtype=torch.int64))
