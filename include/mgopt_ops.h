@@ -53,6 +53,65 @@ MGOPT_API int mgopt_gated_act_backward(const void* grad_out_dev, int64_t grad_ou
                                        int64_t width, int32_t act, void* d_gate_dev, int64_t d_gate_stride,
                                        void* d_up_dev, int64_t d_up_stride, void* y_dev, void* stream);
 
+/* ---- query/key norms and the rotation -------------------------------------- */
+
+#define MGOPT_MAX_HEAD_DIM 512
+
+/* The heads of one side.  Every *_stride is {batch, token, head}, in elements;
+ * a head's `dim` elements are contiguous.
+ *   x_dev         the projection's output; out_dev the result (forward only).
+ *   grad_dev      the gradient of out, d_x_dev that of x, d_weight_dev that of
+ *                 weight_dev, of its type (backward only). */
+typedef struct mgopt_heads {
+    const void* x_dev;
+    const void* weight_dev;
+    void* out_dev;
+    const void* grad_dev;
+    void* d_x_dev;
+    void* d_weight_dev;
+    int64_t x_stride[3];
+    int64_t out_stride[3];
+    int64_t grad_stride[3];
+    int64_t d_x_stride[3];
+    int32_t heads;
+    int32_t reserved;
+} mgopt_heads;
+
+/* cos_dev and sin_dev hold table_rows rows of rotary / 2 floats, one per
+ * position.  positions_dev: of position_bytes (4 or 8) bytes, position_stride
+ * apart from one sequence to the next (0: all alike), or NULL for 0, 1, ...  A
+ * position outside the table makes its token's rotated elements NaN.  Pairs are
+ * (i, i + rotary / 2), or (2i, 2i + 1) with interleaved; elements from `rotary`
+ * on are not rotated.  At most 2^28 tokens. */
+typedef struct mgopt_qk_args {
+    mgopt_heads q;
+    mgopt_heads k;
+    const float* cos_dev;
+    const float* sin_dev;
+    const void* positions_dev;
+    void* workspace_dev; /* backward: mgopt_qk_norm_rope_workspace(dim) bytes */
+    int64_t table_rows;
+    int64_t position_stride;
+    int64_t batch;
+    int64_t length;
+    int32_t dim;
+    int32_t rotary;
+    int32_t dtype;
+    int32_t weight_dtype;
+    int32_t position_bytes;
+    int32_t interleaved;
+    float eps;
+    int32_t reserved;
+} mgopt_qk_args;
+
+/* out = rotate(x / sqrt(mean(x^2) + eps) * weight) for every head. */
+MGOPT_API int mgopt_qk_norm_rope(const mgopt_qk_args* args, void* stream);
+
+MGOPT_API int64_t mgopt_qk_norm_rope_workspace(int32_t dim);
+
+/* d_x and d_weight from x and the gradient of out. */
+MGOPT_API int mgopt_qk_norm_rope_backward(const mgopt_qk_args* args, void* stream);
+
 /* ---- the clipped policy loss ---------------------------------------------- */
 
 #define MGOPT_MASK_NONE 0   /* every row counts once */

@@ -12,6 +12,7 @@ cosine_lr, optimizer_completed_steps) and the checkpoint loaders it calls on
 resume (load_optimizer_state, load_grad_scaler_state).  Beside them, the
 operators of a training step around its matrix products and attention:
 
+    qk_norm_rope    RMS norms of query and key heads and the rotary rotation
     gated_act       the MLP's activation with an 8-bit checkpoint
     policy_loss     the clipped policy loss with a KL term over the logits
 
@@ -28,6 +29,7 @@ from .clip_grad import clip_grad_norm_
 from .gated_act import ActCheckpoint, gated_act, gated_act_backward, gated_act_pack
 from .grad_scaler import GradScaler
 from .policy_loss import PolicyLoss, policy_loss, policy_loss_grad, token_log_probs
+from .qk_norm_rope import qk_norm_rope, qk_norm_rope_backward, rope_tables
 from .schedule import build_adamw_param_groups, cosine_lr, optimizer_completed_steps, set_optimizer_lr
 from .state_load import load_grad_scaler_state, load_optimizer_state
 from . import paramsets
@@ -50,5 +52,8 @@ __all__ = [
     "PolicyLoss",
     "policy_loss",
     "policy_loss_grad",
+    "qk_norm_rope",
+    "qk_norm_rope_backward",
+    "rope_tables",
     "token_log_probs",
 ]

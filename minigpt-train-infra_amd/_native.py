@@ -42,6 +42,9 @@ EXPORTS = (
 OPS_EXPORTS = (
     "mgopt_gated_act",
     "mgopt_gated_act_backward",
+    "mgopt_qk_norm_rope",
+    "mgopt_qk_norm_rope_workspace",
+    "mgopt_qk_norm_rope_backward",
     "mgopt_policy_workspace",
     "mgopt_token_log_probs",
     "mgopt_policy_loss",

@@ -23,6 +23,9 @@ using c10::optional;
 struct Entries {
     decltype(&mgopt_gated_act) gated_act = nullptr;
     decltype(&mgopt_gated_act_backward) gated_act_backward = nullptr;
+    decltype(&mgopt_qk_norm_rope) qk_norm_rope = nullptr;
+    decltype(&mgopt_qk_norm_rope_workspace) qk_norm_rope_workspace = nullptr;
+    decltype(&mgopt_qk_norm_rope_backward) qk_norm_rope_backward = nullptr;
     decltype(&mgopt_policy_workspace) policy_workspace = nullptr;
     decltype(&mgopt_token_log_probs) token_log_probs = nullptr;
     decltype(&mgopt_policy_loss) policy_loss = nullptr;
@@ -38,6 +41,9 @@ void bind_ops(const py::dict& addresses, const py::object& error) {
     };
     take(lib.gated_act, "mgopt_gated_act");
     take(lib.gated_act_backward, "mgopt_gated_act_backward");
+    take(lib.qk_norm_rope, "mgopt_qk_norm_rope");
+    take(lib.qk_norm_rope_workspace, "mgopt_qk_norm_rope_workspace");
+    take(lib.qk_norm_rope_backward, "mgopt_qk_norm_rope_backward");
     take(lib.policy_workspace, "mgopt_policy_workspace");
     take(lib.token_log_probs, "mgopt_token_log_probs");
     take(lib.policy_loss, "mgopt_policy_loss");
@@ -179,6 +185,115 @@ std::tuple<Tensor, optional<Tensor>, optional<Tensor>> gated_act_backward(const 
                                  as_stream(stream)),
           "gated_act_backward");
     return {d_gate, d_up, y};
+}
+
+// ----------------------------------------------------------- qk_norm_rope
+
+// t with contiguous last dimension, and its strides by batch, token and head.
+Tensor heads_in(const Tensor& t, int64_t (&stride)[3], bool heads_first) {
+    const Tensor u = t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous();
+    stride[0] = u.stride(0);
+    stride[1] = u.stride(heads_first ? 2 : 1);
+    stride[2] = u.stride(heads_first ? 1 : 2);
+    return u;
+}
+
+// The arguments both passes share, with the tensors that keep them alive.
+struct Rope {
+    mgopt_qk_args a{};
+    Tensor q, k, wq, wk, cos, sin, positions;
+};
+Rope rope_args(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos, const Tensor& sin,
+               const optional<Tensor>& positions, double eps, bool interleaved) {
+    Rope r;
+    mgopt_qk_args& a = r.a;
+    on_gpu(q, "q");
+    a.dtype = code_of(q, "q");
+    beside(k, q, "k");
+    same_dtype(k, q, "k");
+    if (q.dim() != 4 || k.dim() != 4 || q.size(0) != k.size(0) || q.size(1) != k.size(1) || q.size(3) != k.size(3) ||
+        q.size(2) < 1 || k.size(2) < 1 || q.size(3) < 1)
+        refuse("q and k need shapes (batch, length, heads, dim) that differ in heads only, got " + shape_of(q) + " and " +
+               shape_of(k));
+    const int64_t dim = q.size(3);
+    if (dim > MGOPT_MAX_HEAD_DIM) refuse("heads of more than " + std::to_string(MGOPT_MAX_HEAD_DIM) + " elements");
+    beside(wq, q, "q_weight");
+    beside(wk, q, "k_weight");
+    a.weight_dtype = code_of(wq, "q_weight");
+    same_dtype(wk, wq, "k_weight");
+    if (wq.dim() != 1 || wk.dim() != 1 || wq.size(0) != dim || wk.size(0) != dim)
+        refuse("q_weight and k_weight need shape (" + std::to_string(dim) + ",), got " + shape_of(wq) + " and " + shape_of(wk));
+    beside(cos, q, "cos");
+    beside(sin, q, "sin");
+    if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat) throw py::type_error("cos and sin must be float32");
+    if (cos.dim() != 2 || cos.sizes() != sin.sizes() || 2 * cos.size(1) > dim)
+        refuse("cos and sin need one shape (positions, rotary / 2) with rotary at most dim, got " + shape_of(cos) + " and " +
+               shape_of(sin));
+    if (!(eps >= 0.0)) refuse("eps must not be negative");
+    a.batch = q.size(0), a.length = q.size(1), a.dim = static_cast<int32_t>(dim);
+    if (positions.has_value()) {
+        beside(*positions, q, "positions");
+        if (positions->scalar_type() != at::kLong && positions->scalar_type() != at::kInt)
+            throw py::type_error("positions must be int64 or int32");
+        const bool per_batch = positions->dim() == 2;
+        if (!(positions->dim() == 1 || (per_batch && (positions->size(0) == a.batch || positions->size(0) == 1))) ||
+            positions->size(-1) != a.length)
+            refuse("positions need shape (length,) or (batch, length), got " + shape_of(*positions) + " for " + shape_of(q));
+        r.positions = positions->contiguous();
+        a.positions_dev = r.positions.data_ptr();
+        a.position_bytes = static_cast<int32_t>(r.positions.element_size());
+        a.position_stride = per_batch && r.positions.size(0) > 1 ? a.length : 0;
+    }
+    r.q = heads_in(q, a.q.x_stride, false), r.k = heads_in(k, a.k.x_stride, false);
+    r.wq = wq.contiguous(), r.wk = wk.contiguous(), r.cos = cos.contiguous(), r.sin = sin.contiguous();
+    a.q.x_dev = r.q.data_ptr(), a.k.x_dev = r.k.data_ptr();
+    a.q.weight_dev = r.wq.data_ptr(), a.k.weight_dev = r.wk.data_ptr();
+    a.q.heads = static_cast<int32_t>(q.size(2)), a.k.heads = static_cast<int32_t>(k.size(2));
+    a.cos_dev = r.cos.data_ptr<float>(), a.sin_dev = r.sin.data_ptr<float>();
+    a.table_rows = cos.size(0), a.rotary = static_cast<int32_t>(2 * cos.size(1));
+    a.interleaved = interleaved, a.eps = static_cast<float>(eps);
+    return r;
+}
+
+std::vector<int64_t> heads_shape(const Tensor& t, bool heads_first) {
+    return heads_first ? std::vector<int64_t>{t.size(0), t.size(2), t.size(1), t.size(3)} : t.sizes().vec();
+}
+
+py::tuple qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+                       const Tensor& sin, const optional<Tensor>& positions, double eps, bool interleaved, bool heads_first,
+                       uint64_t stream) {
+    Rope r = rope_args(q, k, wq, wk, cos, sin, positions, eps, interleaved);
+    const c10::DeviceGuard guard(q.device());
+    Tensor oq = at::empty(heads_shape(q, heads_first), q.options()), ok = at::empty(heads_shape(k, heads_first), k.options());
+    heads_in(oq, r.a.q.out_stride, heads_first), heads_in(ok, r.a.k.out_stride, heads_first);
+    r.a.q.out_dev = oq.data_ptr(), r.a.k.out_dev = ok.data_ptr();
+    check(lib.qk_norm_rope(&r.a, as_stream(stream)), "qk_norm_rope");
+    return py::make_tuple(oq, ok);
+}
+
+py::tuple qk_norm_rope_backward(const Tensor& gq, const Tensor& gk, const Tensor& q, const Tensor& k, const Tensor& wq,
+                                const Tensor& wk, const Tensor& cos, const Tensor& sin, const optional<Tensor>& positions,
+                                double eps, bool interleaved, bool heads_first, uint64_t stream) {
+    Rope r = rope_args(q, k, wq, wk, cos, sin, positions, eps, interleaved);
+    mgopt_qk_args& a = r.a;
+    beside(gq, q, "grad_q");
+    beside(gk, q, "grad_k");
+    same_dtype(gq, q, "grad_q");
+    same_dtype(gk, q, "grad_k");
+    if (gq.sizes() != at::IntArrayRef(heads_shape(q, heads_first)) || gk.sizes() != at::IntArrayRef(heads_shape(k, heads_first)))
+        refuse("grad_q and grad_k need the outputs' shapes, got " + shape_of(gq) + " and " + shape_of(gk));
+    const c10::DeviceGuard guard(q.device());
+    const Tensor cq = heads_in(gq, a.q.grad_stride, heads_first), ck = heads_in(gk, a.k.grad_stride, heads_first);
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
+    Tensor dwq = at::empty(wq.sizes(), wq.options()), dwk = at::empty(wk.sizes(), wk.options());
+    Tensor work = at::empty({lib.qk_norm_rope_workspace(a.dim)}, q.options().dtype(at::kByte));
+    heads_in(dq, a.q.d_x_stride, false), heads_in(dk, a.k.d_x_stride, false);
+    a.q.grad_dev = cq.data_ptr(), a.k.grad_dev = ck.data_ptr();
+    a.q.d_x_dev = dq.data_ptr(), a.k.d_x_dev = dk.data_ptr();
+    a.q.d_weight_dev = dwq.data_ptr(), a.k.d_weight_dev = dwk.data_ptr();
+    a.workspace_dev = work.data_ptr();
+    check(lib.qk_norm_rope_backward(&a, as_stream(stream)), "qk_norm_rope_backward");
+    return py::make_tuple(dq, dk, dwq, dwk);
 }
 
 // ------------------------------------------------------------ policy_loss
@@ -329,6 +444,8 @@ void define_ops(py::module_& m) {
     m.def("bind_ops", &bind_ops);
     m.def("gated_act", &gated_act);
     m.def("gated_act_backward", &gated_act_backward);
+    m.def("qk_norm_rope", &qk_norm_rope);
+    m.def("qk_norm_rope_backward", &qk_norm_rope_backward);
     m.def("token_log_probs", &token_log_probs);
     m.def("policy_loss", &policy_loss);
     m.def("policy_loss_backward", &policy_loss_backward);

@@ -31,6 +31,14 @@ def case(*what):
     live("case: " + " ".join(str(w) for w in what))
 
 
+def same_bits(got, want) -> bool:
+    """Whether the tensors of both lists have the same bits (NaN among them)."""
+    whole = {2: torch.int16, 4: torch.int32}
+    return all(a.shape == b.shape and torch.equal(a.contiguous().view(whole[a.element_size()]),
+                                                  b.contiguous().view(whole[b.element_size()]))
+               for a, b in zip(got, want, strict=True))
+
+
 def near(got: torch.Tensor, want: torch.Tensor, within: torch.Tensor, what: str) -> None:
     """got against want (64 bits): off by at most `within` (the error of the
     32-bit arithmetic) plus the rounding to got's type."""

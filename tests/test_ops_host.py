@@ -100,6 +100,65 @@ def test_policy_loss_rejects_bad_arguments(native):
     assert calls["log_probs"](_policy(rows=0)) == 0 and calls["backward"](_policy(rows=0)) == 0
 
 
+class Heads(ctypes.Structure):                 # mgopt_heads
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "out", "grad", "d_x", "d_weight")]
+    _fields_ += [(n, ctypes.c_int64 * 3) for n in ("x_stride", "out_stride", "grad_stride", "d_x_stride")]
+    _fields_ += [("heads", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class QkArgs(ctypes.Structure):                # mgopt_qk_args
+    _fields_ = [("q", Heads), ("k", Heads)]
+    _fields_ += [(n, ctypes.c_void_p) for n in ("cos", "sin", "positions", "workspace")]
+    _fields_ += [(n, ctypes.c_int64) for n in ("table_rows", "position_stride", "batch", "length")]
+    _fields_ += [(n, ctypes.c_int32) for n in ("dim", "rotary", "dtype", "weight_dtype", "position_bytes", "interleaved")]
+    _fields_ += [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+def _qk(side=None, **more):
+    heads = dict(x=P, weight=P, out=P, grad=P, d_x=P, d_weight=P, heads=2)
+    a = QkArgs(q=Heads(**heads), k=Heads(**heads), cos=P, sin=P, workspace=P, table_rows=4, batch=1, length=2, dim=64,
+               rotary=64, eps=1e-6)
+    for k, v in more.items():
+        setattr(a if side is None else getattr(a, side), k, v)
+    return ctypes.byref(a)
+
+
+def test_qk_norm_rope_rejects_bad_arguments(native):
+    lib = native.load_library()
+    vp = ctypes.c_void_p
+    lib.mgopt_qk_norm_rope_workspace.restype = ctypes.c_int64
+    assert lib.mgopt_qk_norm_rope_workspace(64) > 0 and lib.mgopt_qk_norm_rope_workspace(0) == -1
+    forward, backward = lib.mgopt_qk_norm_rope, lib.mgopt_qk_norm_rope_backward
+    for call in (forward, backward):
+        for bad in (dict(dtype=3), dict(weight_dtype=-1), dict(batch=-1), dict(length=-1), dict(dim=0), dict(rotary=63),
+                    dict(rotary=66), dict(rotary=-2), dict(eps=-1.0), dict(eps=float("nan")), dict(cos=None), dict(sin=None),
+                    dict(positions=P, position_bytes=2)):
+            _refused(lib, call(_qk(**bad), vp(None)), E_INVALID, b"qk_norm_rope")
+        for bad in (dict(dim=514, rotary=64), dict(batch=2**20, length=2**20)):
+            _refused(lib, call(_qk(**bad), vp(None)), E_LIMIT, b"more than")
+        for side in ("q", "k"):
+            for bad in (dict(heads=0), dict(x=None), dict(weight=None)):
+                _refused(lib, call(_qk(side, **bad), vp(None)), E_INVALID, b"qk_norm_rope")
+            _refused(lib, call(_qk(side, heads=2**21), vp(None)), E_LIMIT, b"heads")
+        _refused(lib, call(None, vp(None)), E_INVALID, b"NULL")
+    _refused(lib, forward(_qk("k", out=None), vp(None)), E_INVALID, b"NULL")
+    for bad in (dict(grad=None), dict(d_x=None), dict(d_weight=None)):
+        _refused(lib, backward(_qk("q", **bad), vp(None)), E_INVALID, b"NULL")
+    _refused(lib, backward(_qk(workspace=None), vp(None)), E_ALIGN, b"workspace")
+    assert forward(_qk(batch=0), vp(None)) == 0
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    """The sizes of the structs as gcc lays them out are those declared here."""
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "mgopt_ops.h"\nint main(void) { printf("%zu %zu %zu\\n", '
+                   "sizeof(mgopt_policy_args), sizeof(mgopt_heads), sizeof(mgopt_qk_args)); return 0; }\n")
+    exe = tmp_path / "sizes"
+    subprocess.run(["gcc", "-std=c99", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
+    got = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(x) for x in got] == [ctypes.sizeof(c) for c in (PolicyArgs, Heads, QkArgs)]
+
+
 def test_operators_have_no_cpu_path(mg):
     if torch.cuda.is_available():
         pytest.skip("a GPU is visible")
@@ -107,3 +166,6 @@ def test_operators_have_no_cpu_path(mg):
         mg.gated_act(torch.ones(3, 4))
     with pytest.raises(RuntimeError, match="no CPU"):
         mg.token_log_probs(torch.ones(3, 4), torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="no CPU"):
+        x, w = torch.ones(1, 2, 3, 4), torch.ones(4)
+        mg.qk_norm_rope(x, x, w, w, *mg.rope_tables(2, 4))
