@@ -26,6 +26,28 @@
 extern "C" {
 #endif
 
+/* ---- token embedding -------------------------------------------------------- */
+
+/* out[t] = scale * weight[ids[t]] for n ids of id_bytes (4 or 8) bytes; weight
+ * is [rows][width], out [n][width], both contiguous.  An id outside
+ * [0, rows) gives a row of NaN. */
+MGOPT_API int mgopt_embedding(const void* ids_dev, int32_t id_bytes, int64_t n, const void* weight_dev,
+                              int32_t weight_dtype, int64_t rows, int64_t width, float scale, void* out_dev,
+                              int32_t out_dtype, void* stream);
+
+MGOPT_API int64_t mgopt_embedding_grad_workspace(int64_t n, int64_t rows, int64_t width);
+
+/* grad[v] = scale * sum of grad_out[t] over the t with ids[t] = v, and, with
+ * accumulate, added to what grad[v] holds: then only rows that the ids name are
+ * read and written, otherwise every row is written.  grad_out is [n][width],
+ * grad [rows][width], both contiguous.  Ids outside [0, rows) and equal to
+ * padding_idx (-1: none) add nothing.  workspace_dev:
+ * mgopt_embedding_grad_workspace bytes, 16-byte aligned. */
+MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_t n, const void* grad_out_dev,
+                                   int32_t grad_out_dtype, void* grad_dev, int32_t grad_dtype, int64_t rows,
+                                   int64_t width, float scale, int64_t padding_idx, int32_t accumulate,
+                                   void* workspace_dev, void* stream);
+
 /* ---- the MLP's activation ------------------------------------------------ */
 
 #define MGOPT_ACT_SILU 0       /* x / (1 + exp(-x)) */

@@ -12,6 +12,7 @@ cosine_lr, optimizer_completed_steps) and the checkpoint loaders it calls on
 resume (load_optimizer_state, load_grad_scaler_state).  Beside them, the
 operators of a training step around its matrix products and attention:
 
+    embedding       lookup of scaled rows, and the weight's gradient
     qk_norm_rope    RMS norms of query and key heads and the rotary rotation
     gated_act       the MLP's activation with an 8-bit checkpoint
     policy_loss     the clipped policy loss with a KL term over the logits
@@ -26,6 +27,7 @@ importlib.import_module("minigpt-train-infra_amd").
 
 from .adamw import AdamW
 from .clip_grad import clip_grad_norm_
+from .embedding import embedding, embedding_grad_
 from .gated_act import ActCheckpoint, gated_act, gated_act_backward, gated_act_pack
 from .grad_scaler import GradScaler
 from .policy_loss import PolicyLoss, policy_loss, policy_loss_grad, token_log_probs
@@ -45,6 +47,8 @@ __all__ = [
     "load_optimizer_state",
     "load_grad_scaler_state",
     "paramsets",
+    "embedding",
+    "embedding_grad_",
     "ActCheckpoint",
     "gated_act",
     "gated_act_backward",

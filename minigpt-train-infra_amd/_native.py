@@ -40,6 +40,9 @@ EXPORTS = (
 )
 #: every symbol include/mgopt_ops.h declares; the host helper calls them by address
 OPS_EXPORTS = (
+    "mgopt_embedding",
+    "mgopt_embedding_grad_workspace",
+    "mgopt_embedding_grad",
     "mgopt_gated_act",
     "mgopt_gated_act_backward",
     "mgopt_qk_norm_rope",

@@ -21,6 +21,9 @@ using at::Tensor;
 using c10::optional;
 
 struct Entries {
+    decltype(&mgopt_embedding) embedding = nullptr;
+    decltype(&mgopt_embedding_grad_workspace) embedding_grad_workspace = nullptr;
+    decltype(&mgopt_embedding_grad) embedding_grad = nullptr;
     decltype(&mgopt_gated_act) gated_act = nullptr;
     decltype(&mgopt_gated_act_backward) gated_act_backward = nullptr;
     decltype(&mgopt_qk_norm_rope) qk_norm_rope = nullptr;
@@ -39,6 +42,9 @@ void bind_ops(const py::dict& addresses, const py::object& error) {
     auto take = [&](auto& fn, const char* name) {
         fn = reinterpret_cast<std::decay_t<decltype(fn)>>(addresses[name].cast<uintptr_t>());
     };
+    take(lib.embedding, "mgopt_embedding");
+    take(lib.embedding_grad_workspace, "mgopt_embedding_grad_workspace");
+    take(lib.embedding_grad, "mgopt_embedding_grad");
     take(lib.gated_act, "mgopt_gated_act");
     take(lib.gated_act_backward, "mgopt_gated_act_backward");
     take(lib.qk_norm_rope, "mgopt_qk_norm_rope");
@@ -116,6 +122,63 @@ Rows rows_of(const Tensor& x) {
     }
     if (plain) return {x, rows, width, stride};
     return {x.contiguous(), rows, width, width};
+}
+
+// ------------------------------------------------------------- embedding
+
+Tensor ids_of(const Tensor& ids, const Tensor& first) {
+    beside(ids, first, "ids");
+    if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) throw py::type_error("ids must be int64 or int32");
+    return ids.contiguous();
+}
+
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, const optional<py::object>& dtype, uint64_t stream) {
+    on_gpu(weight, "weight");
+    const int32_t code = code_of(weight, "weight");
+    if (weight.dim() != 2 || weight.size(0) < 1 || weight.size(1) < 1)
+        refuse("weight needs shape (rows, width), got " + shape_of(weight));
+    if (!std::isfinite(scale)) refuse("the scale must be finite");
+    const c10::DeviceGuard guard(weight.device());
+    const Tensor i = ids_of(ids, weight), w = weight.contiguous();
+    std::vector<int64_t> shape = ids.sizes().vec();
+    shape.push_back(weight.size(1));
+    auto options = weight.options();
+    if (dtype.has_value()) options = options.dtype(torch::python::detail::py_object_to_dtype(*dtype));
+    Tensor out = at::empty(shape, options);
+    check(lib.embedding(i.data_ptr(), static_cast<int32_t>(i.element_size()), i.numel(), w.data_ptr(), code, w.size(0),
+                        w.size(1), static_cast<float>(scale), out.data_ptr(), code_of(out, "the output"), as_stream(stream)),
+          "embedding");
+    return out;
+}
+
+void embedding_grad(const Tensor& grad, const Tensor& ids, const Tensor& grad_out, double scale,
+                    const optional<int64_t>& padding_idx, bool accumulate, uint64_t stream) {
+    on_gpu(grad, "grad");
+    const int32_t code = code_of(grad, "grad");
+    if (grad.dim() != 2 || grad.size(0) < 1 || grad.size(1) < 1 || !grad.is_contiguous())
+        refuse("grad needs shape (rows, width) and to be contiguous, got " + shape_of(grad));
+    beside(grad_out, grad, "grad_out");
+    const int32_t out_code = code_of(grad_out, "grad_out");
+    std::vector<int64_t> shape = ids.sizes().vec();
+    shape.push_back(grad.size(1));
+    if (grad_out.sizes() != at::IntArrayRef(shape))
+        refuse("grad_out needs the ids' shape and grad's width, got " + shape_of(grad_out) + " for ids " + shape_of(ids) +
+               " and grad " + shape_of(grad));
+    if (!std::isfinite(scale)) refuse("the scale must be finite");
+    int64_t padding = -1;
+    if (padding_idx.has_value()) {
+        padding = *padding_idx < 0 ? *padding_idx + grad.size(0) : *padding_idx;
+        if (padding < 0 || padding >= grad.size(0))
+            refuse("padding_idx " + std::to_string(*padding_idx) + " is outside " + std::to_string(grad.size(0)) + " rows");
+    }
+    const c10::DeviceGuard guard(grad.device());
+    const Tensor i = ids_of(ids, grad), g = grad_out.contiguous();
+    const int64_t rows = grad.size(0), width = grad.size(1);
+    Tensor work = at::empty({lib.embedding_grad_workspace(i.numel(), rows, width)}, grad.options().dtype(at::kByte));
+    check(lib.embedding_grad(i.data_ptr(), static_cast<int32_t>(i.element_size()), i.numel(), g.data_ptr(), out_code,
+                             grad.data_ptr(), code, rows, width, static_cast<float>(scale), padding, accumulate,
+                             work.data_ptr(), as_stream(stream)),
+          "embedding_grad_");
 }
 
 // ------------------------------------------------------------- gated_act
@@ -442,6 +505,8 @@ Tensor policy_loss_backward(const Tensor& logits, const Tensor& targets, const T
 
 void define_ops(py::module_& m) {
     m.def("bind_ops", &bind_ops);
+    m.def("embedding", &embedding);
+    m.def("embedding_grad", &embedding_grad);
     m.def("gated_act", &gated_act);
     m.def("gated_act_backward", &gated_act_backward);
     m.def("qk_norm_rope", &qk_norm_rope);

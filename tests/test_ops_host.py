@@ -45,6 +45,35 @@ def _refused(lib, rc, code, text):
     assert rc == code and text in lib.mgopt_last_error(), (rc, lib.mgopt_last_error())
 
 
+def test_embedding_rejects_bad_arguments(native):
+    lib = native.load_library()
+    vp, i64, f = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float
+    lib.mgopt_embedding_grad_workspace.restype = i64
+    assert lib.mgopt_embedding_grad_workspace(i64(10), i64(10), i64(10)) > 0
+    for bad in ((-1, 10, 10), (10, 0, 10), (10, 10, 0)):
+        assert lib.mgopt_embedding_grad_workspace(*map(i64, bad)) == -1
+
+    def lookup(ids=P, id_bytes=8, n=4, weight=P, wd=0, rows=5, width=8, scale=1.0, out=P, od=0):
+        return lib.mgopt_embedding(vp(ids), id_bytes, i64(n), vp(weight), wd, i64(rows), i64(width), f(scale), vp(out), od,
+                                   vp(None))
+
+    def grad(ids=P, id_bytes=8, n=4, grad_out=P, wd=0, dst=P, od=0, rows=5, width=8, scale=1.0, pad=-1, acc=1, work=P):
+        return lib.mgopt_embedding_grad(vp(ids), id_bytes, i64(n), vp(grad_out), wd, vp(dst), od, i64(rows), i64(width),
+                                        f(scale), i64(pad), acc, vp(work), vp(None))
+
+    for call in (lookup, grad):
+        for bad in (dict(id_bytes=2), dict(n=-1), dict(rows=0), dict(width=0), dict(wd=3), dict(od=-1), dict(ids=None),
+                    dict(scale=float("nan"))):
+            _refused(lib, call(**bad), E_INVALID, b"embedding")
+    for bad in (dict(weight=None), dict(out=None)):
+        _refused(lib, lookup(**bad), E_INVALID, b"NULL")
+    for bad in (dict(grad_out=None), dict(dst=None), dict(pad=5), dict(pad=-2)):
+        _refused(lib, grad(**bad), E_INVALID, b"embedding_grad")
+    for bad in (dict(work=None), dict(work=P + 8)):
+        _refused(lib, grad(**bad), E_ALIGN, b"workspace")
+    assert lookup(n=0) == 0 and grad(n=0) == 0
+
+
 def _gated_act(lib, gate=P, up=None, dtype=0, rows=4, width=8, act=0, y=P, codes=None, scales=None):
     vp, i64 = ctypes.c_void_p, ctypes.c_int64
     return lib.mgopt_gated_act(vp(gate), i64(8), vp(up), i64(8), dtype, i64(rows), i64(width), act, vp(y), vp(codes),
@@ -164,6 +193,8 @@ def test_operators_have_no_cpu_path(mg):
         pytest.skip("a GPU is visible")
     with pytest.raises(RuntimeError, match="no CPU"):
         mg.gated_act(torch.ones(3, 4))
+    with pytest.raises(RuntimeError, match="no CPU"):
+        mg.embedding(torch.zeros(3, dtype=torch.int64), torch.ones(3, 4))
     with pytest.raises(RuntimeError, match="no CPU"):
         mg.token_log_probs(torch.ones(3, 4), torch.zeros(3, dtype=torch.int64))
     with pytest.raises(RuntimeError, match="no CPU"):
