@@ -135,6 +135,315 @@ __global__ __launch_bounds__(kBlock) void grad_by_row_kernel(GradArgs a) {
     store_some<N>(out, sum, left);
 }
 
+// Everything else sorts: the tokens by id, stably, so that a row's tokens are
+// neighbours in their order; then the sorted list is cut in pieces of equal
+// length, whatever rows they touch, and the pieces' sums are joined.
+//
+// The sort is a radix sort, kDigitBits a pass, from the low digit up.  A pass
+// counts every tile's digits, and then places each token behind the tokens of
+// smaller digits, those of its digit in earlier tiles, and those before it in
+// its tile.  Ids that name no row, and the padding's, become the key `rows`
+// and end up last.
+
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
+constexpr int kSortBlock = 512, kSortItems = 4, kTile = kSortBlock * kSortItems, kSortWaves = kSortBlock / 64;
+static_assert(kSortBlock == kDigits, "a thread a digit");
+
+struct SortArgs {
+    const void* ids;           // first pass
+    const uint32_t *keys, *tokens;
+    uint32_t *keys_out, *tokens_out;
+    uint32_t* counts;          // [tiles][kDigits]
+    int64_t rows, padding;
+    uint32_t n, tiles;
+    int32_t id_bytes, shift;   // the digit's lowest bit
+    char* zeros;               // first pass: what the work-groups past the tiles clear
+    int64_t zero_bytes;
+};
+
+__device__ __forceinline__ uint32_t key_at(const SortArgs& a, uint32_t t) {
+    if (a.keys != nullptr) return a.keys[t];
+    const int64_t id = id_at(a.ids, t, a.id_bytes);
+    return static_cast<uint32_t>(id < 0 || id >= a.rows || id == a.padding ? a.rows : id);
+}
+
+// Clears a.zeros with the work-groups from `first` on.
+__device__ __forceinline__ void clear(const SortArgs& a, uint32_t first) {
+    const int64_t vecs = a.zero_bytes / 16, step = static_cast<int64_t>(gridDim.x - first) * kSortBlock;
+    const vec_t<uint16_t, 8> zero = {};
+    int64_t i = static_cast<int64_t>(blockIdx.x - first) * kSortBlock + threadIdx.x;
+    if (i < a.zero_bytes % 16 / 2) reinterpret_cast<uint16_t*>(a.zeros)[vecs * 8 + i] = 0;
+    for (; i < vecs; i += step) reinterpret_cast<vec_t<uint16_t, 8>*>(a.zeros)[i] = zero;
+}
+
+__global__ __launch_bounds__(kSortBlock) void count_kernel(SortArgs a) {
+    if (blockIdx.x >= a.tiles) return clear(a, a.tiles);
+    __shared__ uint32_t count[kDigits];
+    count[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t t = blockIdx.x * kTile + k * kSortBlock + threadIdx.x;
+        if (t < a.n) atomicAdd(&count[key_at(a, t) >> a.shift & (kDigits - 1)], 1u);
+    }
+    __syncthreads();
+    a.counts[static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = count[threadIdx.x];
+}
+
+// The exclusive sum of x over the work-group's threads.
+__device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* wave_sums) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    uint32_t run = x;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t y = __shfl_up(run, off);
+        if (lane >= static_cast<uint32_t>(off)) run += y;
+    }
+    if (lane == 63) wave_sums[wave] = run;
+    __syncthreads();
+    uint32_t base = 0;
+    for (uint32_t w = 0; w < wave; ++w) base += wave_sums[w];
+    __syncthreads();  // before the next use
+    return base + run - x;
+}
+
+// The places within the tile's digits of a thread's items, which are the
+// tile's elements wave * 256 + k * 64 + lane; used[w][d] becomes the number of
+// elements of digit d in waves before w, and the return value of thread d the
+// number in the tile.
+struct Places {
+    uint32_t rank[kSortItems];
+};
+__device__ __forceinline__ uint32_t rank_tile(const uint32_t (&digit)[kSortItems], const bool (&on)[kSortItems],
+                                              uint32_t (&used)[kSortWaves][kDigits], Places& p) {
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) used[w][threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        uint64_t same = __ballot(on[k]);
+#pragma unroll
+        for (int bit = 0; bit < kDigitBits; ++bit) {
+            const bool b = digit[k] >> bit & 1u;
+            const uint64_t vote = __ballot(b);
+            same &= b ? vote : ~vote;
+        }
+        const uint32_t before = static_cast<uint32_t>(__popcll(same & ((uint64_t{1} << lane) - 1)));
+        // the wave's lanes read the counter, then the first of each digit moves it on
+        uint32_t* counter = &used[wave][digit[k]];
+        const uint32_t old = *reinterpret_cast<volatile uint32_t*>(counter);
+        __builtin_amdgcn_wave_barrier();
+        if (on[k] && before == 0) *reinterpret_cast<volatile uint32_t*>(counter) = old + static_cast<uint32_t>(__popcll(same));
+        __builtin_amdgcn_wave_barrier();
+        p.rank[k] = old + before;
+    }
+    __syncthreads();
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+        const uint32_t x = used[w][threadIdx.x];
+        used[w][threadIdx.x] = sum;
+        sum += x;
+    }
+    __syncthreads();
+    return sum;
+}
+
+__global__ __launch_bounds__(kSortBlock) void place_kernel(SortArgs a) {
+    __shared__ uint32_t used[kSortWaves][kDigits], base[kDigits], wave_sums[kSortWaves];
+    const uint32_t d = threadIdx.x, lane = d % 64, wave = d / 64;
+    uint32_t all = 0, earlier = 0;
+#pragma unroll 8
+    for (uint32_t b = 0; b < a.tiles; ++b) {
+        const uint32_t x = a.counts[static_cast<int64_t>(b) * kDigits + d];
+        all += x;
+        if (b < blockIdx.x) earlier += x;
+    }
+    base[d] = sum_before(all, wave_sums) + earlier;
+    uint32_t key[kSortItems], token[kSortItems], digit[kSortItems];
+    bool on[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t t = blockIdx.x * kTile + wave * (64 * kSortItems) + k * 64 + lane;
+        on[k] = t < a.n;
+        key[k] = on[k] ? key_at(a, t) : 0;
+        token[k] = on[k] && a.tokens != nullptr ? a.tokens[t] : t;
+        digit[k] = key[k] >> a.shift & (kDigits - 1);
+    }
+    Places p;
+    rank_tile(digit, on, used, p);
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        if (!on[k]) continue;
+        const uint32_t at = base[digit[k]] + used[wave][digit[k]] + p.rank[k];
+        a.keys_out[at] = key[k];
+        a.tokens_out[at] = token[k];
+    }
+}
+
+// All passes over one tile, in LDS.
+__global__ __launch_bounds__(kSortBlock) void sort_tile_kernel(SortArgs a, int32_t bits) {
+    if (blockIdx.x >= 1) return clear(a, 1);
+    __shared__ uint32_t used[kSortWaves][kDigits], base[kDigits], wave_sums[kSortWaves], keys[kTile], tokens[kTile];
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    uint32_t key[kSortItems], token[kSortItems], digit[kSortItems];
+    bool on[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t t = wave * (64 * kSortItems) + k * 64 + lane;
+        on[k] = t < a.n;
+        key[k] = on[k] ? key_at(a, t) : 0;
+        token[k] = t;
+    }
+    for (int32_t shift = 0; shift < bits; shift += kDigitBits) {
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) digit[k] = key[k] >> shift & (kDigits - 1);
+        Places p;
+        const uint32_t sum = rank_tile(digit, on, used, p);
+        base[threadIdx.x] = sum_before(sum, wave_sums);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) {
+            if (!on[k]) continue;
+            const uint32_t at = base[digit[k]] + used[wave][digit[k]] + p.rank[k];
+            keys[at] = key[k];
+            tokens[at] = token[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) {
+            const uint32_t t = wave * (64 * kSortItems) + k * 64 + lane;
+            if (on[k]) key[k] = keys[t], token[k] = tokens[t];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t t = wave * (64 * kSortItems) + k * 64 + lane;
+        if (on[k]) a.keys_out[t] = key[k], a.tokens_out[t] = token[k];
+    }
+}
+
+struct SumArgs {
+    const uint32_t *keys, *tokens;  // sorted
+    const void* grad_out;
+    void* grad;
+    float* partials;                // [pieces][2][width]
+    int64_t rows, width;
+    uint32_t n, piece, pieces;
+    uint32_t shift, chunks;         // as GradArgs
+    int32_t accumulate;
+    float scale;
+};
+
+template <int N, typename TW>
+__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int64_t c, float (&sum)[N]) {
+    TW* out = static_cast<TW*>(a.grad) + static_cast<int64_t>(row) * a.width + c;
+    const int64_t left = a.width - c;
+    float old[N] = {}, x[N];
+    if (a.accumulate) load_some<N>(old, out, left);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = fmaf(sum[j], a.scale, old[j]);
+    store_some<N>(out, x, left);
+}
+
+// A group of 1 << shift threads sums the rows of one piece of the sorted list
+// over its columns.  A run of one key that lies inside the piece is written to
+// its row; one that began before it goes to the piece's first partial row, one
+// that began in it and goes on after it to the second.
+template <typename TG, typename TW>
+__global__ __launch_bounds__(kBlock) void sum_pieces_kernel(SumArgs a) {
+    constexpr int N = 16 / (sizeof(TG) > sizeof(TW) ? sizeof(TG) : sizeof(TW)), kAhead = 4;
+    const uint32_t pb = blockIdx.x / a.chunks, cb = blockIdx.x - pb * a.chunks;
+    const uint32_t piece = pb * (kBlock >> a.shift) + (threadIdx.x >> a.shift);
+    const int64_t c = (static_cast<int64_t>(cb) * kBlock + (threadIdx.x & ((1u << a.shift) - 1))) * N, left = a.width - c;
+    if (piece >= a.pieces || left <= 0) return;
+    const uint32_t first = piece * a.piece, last = a.n - first < a.piece ? a.n : first + a.piece;
+    uint32_t row = a.keys[first];
+    if (row >= a.rows) return;  // the ids that name no row come last
+    bool head = first > 0 && a.keys[first - 1] == row;
+    float sum[N] = {};
+    for (uint32_t i = first; i < last; i += kAhead) {
+        float v[kAhead][N];
+        uint32_t key[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            key[u] = i + u < last ? a.keys[i + u] : static_cast<uint32_t>(a.rows);
+            if (key[u] < a.rows)
+                load_some<N>(v[u], static_cast<const TG*>(a.grad_out) + static_cast<int64_t>(a.tokens[i + u]) * a.width + c, left);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (i + u >= last) break;
+            if (key[u] != row) {
+                if (row < a.rows) {
+                    if (head) store_some<N>(a.partials + static_cast<int64_t>(piece) * 2 * a.width + c, sum, left);
+                    else write_row<N, TW>(a, row, c, sum);
+                }
+                row = key[u];
+                head = false;
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum[j] = 0.0f;
+            }
+            if (row < a.rows) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum[j] += v[u][j];
+            }
+        }
+    }
+    if (row >= a.rows) return;
+    const bool tail = last < a.n && a.keys[last] == row;
+    if (!head && !tail) write_row<N, TW>(a, row, c, sum);
+    else store_some<N>(a.partials + (static_cast<int64_t>(piece) * 2 + (head ? 0 : 1)) * a.width + c, sum, left);
+}
+
+// Joins the runs that cross pieces: the group of the piece in which a run began
+// adds the partial rows of the pieces it goes on through, in their order.
+template <int N, typename TW>
+__global__ __launch_bounds__(kBlock) void join_pieces_kernel(SumArgs a) {
+    const uint32_t pb = blockIdx.x / a.chunks, cb = blockIdx.x - pb * a.chunks;
+    const uint32_t piece = pb * (kBlock >> a.shift) + (threadIdx.x >> a.shift);
+    const int64_t c = (static_cast<int64_t>(cb) * kBlock + (threadIdx.x & ((1u << a.shift) - 1))) * N, left = a.width - c;
+    if (piece + 1 >= a.pieces || left <= 0) return;
+    const uint32_t first = piece * a.piece, next = first + a.piece, row = a.keys[next];
+    if (row >= a.rows || a.keys[next - 1] != row) return;             // nothing crosses this piece's end
+    if (a.keys[first] == row && first > 0 && a.keys[first - 1] == row) return;  // it began before this piece
+    float sum[N];
+    load_some<N>(sum, a.partials + (static_cast<int64_t>(piece) * 2 + 1) * a.width + c, left);
+    for (uint32_t q = piece + 1; q < a.pieces && a.keys[q * a.piece] == row; ++q) {
+        float v[N];
+        load_some<N>(v, a.partials + static_cast<int64_t>(q) * 2 * a.width + c, left);
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[j] += v[j];
+    }
+    write_row<N, TW>(a, row, c, sum);
+}
+
+// Which form: the sort's launches cost what reading all ids for each of a few
+// thousand rows does.
+constexpr int64_t kByRowWork = int64_t{1} << 20;  // rows * tokens
+bool by_row(int64_t n, int64_t rows) {
+    return n >= (int64_t{1} << 30) || rows >= (int64_t{1} << 31) || n == 0 || rows <= kByRowWork / n;
+}
+
+// Sorted positions per piece: enough pieces to fill the chip, long ones otherwise.
+uint32_t piece_for(int64_t n) { return n <= 32768 ? 16 : 64; }
+
+struct Work {
+    int64_t counts, keys[2], tokens[2], partials, bytes;
+};
+Work work_of(int64_t n, int64_t width) {
+    const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    Work w{};
+    const int64_t tiles = (n + kTile - 1) / kTile, list = up(4 * n);
+    w.keys[0] = up(4 * tiles * kDigits);
+    w.tokens[0] = w.keys[0] + list, w.keys[1] = w.tokens[0] + list, w.tokens[1] = w.keys[1] + list;
+    w.partials = w.tokens[1] + list;
+    w.bytes = w.partials + (n + piece_for(n) - 1) / piece_for(n) * 2 * width * 4;
+    return w;
+}
+
 uint32_t shift_for(int64_t vecs) {
     uint32_t s = 0;
     while ((1 << s) < kBlock && (int64_t{1} << s) < vecs) ++s;
@@ -182,7 +491,8 @@ MGOPT_API int mgopt_embedding(const void* ids_dev, int32_t id_bytes, int64_t n, 
 }
 
 MGOPT_API int64_t mgopt_embedding_grad_workspace(int64_t n, int64_t rows, int64_t width) {
-    return n < 0 || rows < 1 || width < 1 ? -1 : 16;
+    if (n < 0 || rows < 1 || width < 1) return -1;
+    return by_row(n, rows) ? 16 : work_of(n, width).bytes;
 }
 
 MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_t n, const void* grad_out_dev,
@@ -203,14 +513,58 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
             constexpr int N = 16 / (sizeof(TG) > sizeof(TW) ? sizeof(TG) : sizeof(TW));
             const int64_t vecs = (width + N - 1) / N, chunks = (vecs + kBlock - 1) / kBlock;
             if (chunks > max_blocks(kBlock)) return set_error(MGOPT_E_LIMIT, "embedding_grad: rows too long");
-            a.shift = shift_for(vecs);
-            a.chunks = static_cast<uint32_t>(chunks);
-            const int64_t most = max_blocks(kBlock) / chunks;
-            for (a.first_row = 0; a.first_row < rows; a.first_row += most) {
-                const int64_t blocks = std::min(rows - a.first_row, most) * chunks;
-                hipLaunchKernelGGL((grad_by_row_kernel<TG, TW>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, a);
-                if (int rc = launched("grad_by_row_kernel")) return rc;
+            const uint32_t shift = shift_for(vecs);
+            if (by_row(n, rows)) {
+                a.shift = shift;
+                a.chunks = static_cast<uint32_t>(chunks);
+                const int64_t most = max_blocks(kBlock) / chunks;
+                for (a.first_row = 0; a.first_row < rows; a.first_row += most) {
+                    const int64_t blocks = std::min(rows - a.first_row, most) * chunks;
+                    hipLaunchKernelGGL((grad_by_row_kernel<TG, TW>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, a);
+                    if (int rc = launched("grad_by_row_kernel")) return rc;
+                }
+                return 0;
             }
+            const Work work = work_of(n, width);
+            char* const at = static_cast<char*>(workspace_dev);
+            const auto list = [&](int64_t offset) { return reinterpret_cast<uint32_t*>(at + offset); };
+            const uint32_t tiles = static_cast<uint32_t>((n + kTile - 1) / kTile);
+            SortArgs o{ids_dev, nullptr, nullptr, nullptr, nullptr, list(work.counts), rows, padding_idx, static_cast<uint32_t>(n),
+                       tiles, id_bytes, 0, static_cast<char*>(grad_dev), 0};
+            // a gradient that is written whole is cleared beside the first pass, which leaves most of the chip idle
+            uint32_t clearing = 0;
+            if (!accumulate) {
+                o.zero_bytes = rows * width * static_cast<int64_t>(sizeof(TW));
+                clearing = static_cast<uint32_t>(std::min<int64_t>((o.zero_bytes + 16 * kSortBlock - 1) / (16 * kSortBlock), 2048));
+            }
+            int32_t bits = 1;
+            while (rows >> bits) ++bits;  // of the largest key, `rows`
+            int side = 0;
+            if (tiles == 1) {
+                o.keys_out = list(work.keys[0]), o.tokens_out = list(work.tokens[0]);
+                hipLaunchKernelGGL(sort_tile_kernel, dim3(1 + clearing), dim3(kSortBlock), 0, s, o, bits);
+                if (int rc = launched("sort_tile_kernel")) return rc;
+                side = 1;
+            } else {
+                for (o.shift = 0; o.shift < bits; o.shift += kDigitBits, side ^= 1, clearing = 0) {
+                    o.keys_out = list(work.keys[side]), o.tokens_out = list(work.tokens[side]);
+                    hipLaunchKernelGGL(count_kernel, dim3(tiles + clearing), dim3(kSortBlock), 0, s, o);
+                    if (int rc = launched("count_kernel")) return rc;
+                    hipLaunchKernelGGL(place_kernel, dim3(tiles), dim3(kSortBlock), 0, s, o);
+                    if (int rc = launched("place_kernel")) return rc;
+                    o.keys = o.keys_out, o.tokens = o.tokens_out;
+                }
+            }
+            SumArgs m{list(work.keys[side ^ 1]), list(work.tokens[side ^ 1]), grad_out_dev, grad_dev,
+                      reinterpret_cast<float*>(at + work.partials), rows, width, static_cast<uint32_t>(n), piece_for(n), 0, shift,
+                      static_cast<uint32_t>(chunks), accumulate, scale};
+            m.pieces = static_cast<uint32_t>((n + m.piece - 1) / m.piece);
+            const int64_t per_block = kBlock >> shift, blocks = (m.pieces + per_block - 1) / per_block * chunks;
+            if (blocks > max_blocks(kBlock)) return set_error(MGOPT_E_LIMIT, "embedding_grad: too many tokens of long rows");
+            hipLaunchKernelGGL((sum_pieces_kernel<TG, TW>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, m);
+            if (int rc = launched("sum_pieces_kernel")) return rc;
+            hipLaunchKernelGGL((join_pieces_kernel<N, TW>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, m);
+            if (int rc = launched("join_pieces_kernel")) return rc;
             return 0;
         });
     });
