@@ -20,6 +20,10 @@
 // and entries of it finite, and small differences exact.  Rows of weight 0 are
 // not read.
 //
+// A row that fits is held in registers between the passes (cached_kernel), as
+// it came, so that it is read once; longer rows are read again, from the
+// Infinity Cache in part.
+//
 // Bound by memory: a row's logits once, its gradient once.
 #include "ops_common.h"
 
@@ -90,31 +94,51 @@ __device__ __forceinline__ Running join_block(Running r, float c) {
     return r;
 }
 
+// What the row's scalars are made of, read before the row so that nothing
+// waits for them after it.
+struct RowInputs {
+    int64_t target;
+    float x, old_logp, advantage, ref;  // x: the target's logit, NaN for a target outside the vocabulary
+    float scale;                        // of the gradient, with the weights' sum
+    double total;
+};
+template <typename T, Mode MODE>
+__device__ __forceinline__ RowInputs row_inputs(const PolicyArgs& a, int64_t n) {
+    RowInputs r{};
+    r.target = id_at(a.targets, n, a.target_bytes);
+    if (MODE != kGrad)
+        r.x = r.target >= 0 && r.target < a.vocab
+                  ? static_cast<float>(static_cast<const T*>(a.logits)[n * a.row_stride + r.target])
+                  : __builtin_nanf("");
+    if (MODE == kLogp) return r;
+    r.old_logp = a.old_logp[n], r.advantage = a.advantages[n];
+    if (a.ref_logp != nullptr) r.ref = a.ref_logp[n];
+    r.scale = a.grad_scale != nullptr ? *a.grad_scale : 1.0f;
+    r.total = a.weight_sum != nullptr ? *a.weight_sum : static_cast<double>(a.rows);
+    return r;
+}
+
 struct RowResult {
     float slope, k;  // of the gradient: slope * [j = y] + k * exp2((x - m) * c)
 };
 
 // What one row adds to the loss, and its slope, from m and s.
-template <typename T, Mode MODE>
-__device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, float w, float m, float s) {
-    const int64_t y = id_at(a.targets, n, a.target_bytes);
+template <Mode MODE>
+__device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs& in, float w, float m, float s) {
     double logp;
     if constexpr (MODE == kGrad) {
         logp = a.log_probs[n];
     } else {
-        const double x = y >= 0 && y < a.vocab
-                             ? static_cast<double>(static_cast<float>(static_cast<const T*>(a.logits)[n * a.row_stride + y]))
-                             : __builtin_nan("");
-        logp = (x - static_cast<double>(base(m))) * a.inv_temp - log(static_cast<double>(s));
+        logp = (static_cast<double>(in.x) - static_cast<double>(base(m))) * a.inv_temp - log(static_cast<double>(s));
         a.log_probs[n] = static_cast<float>(logp);
     }
     if constexpr (MODE == kLogp) return {};
-    const double A = a.advantages[n], ratio = exp(logp - static_cast<double>(a.old_logp[n]));
+    const double A = in.advantage, ratio = exp(logp - static_cast<double>(in.old_logp));
     const double s1 = ratio * A, s2 = fmin(fmax(ratio, a.low), a.high) * A;
     const bool held = s2 < s1;
     double slope = held ? 0.0 : -s1, kl = 0.0;
     if (a.ref_logp != nullptr) {
-        const double r = static_cast<double>(a.ref_logp[n]) - logp, e = expm1(r);
+        const double r = static_cast<double>(in.ref) - logp, e = expm1(r);
         kl = e - r;
         slope -= a.kl_coef * e;
     }
@@ -122,10 +146,100 @@ __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, float w, float 
         a.terms[n] = make_float4(static_cast<float>(w * -(held ? s2 : s1)), static_cast<float>(w * kl), held ? w : 0.0f, 0.0f);
     if constexpr (MODE == kLoss) a.stats[n] = make_float2(m, s);
     if constexpr (MODE == kLoss) return {};
-    const double total = a.weight_sum != nullptr ? *a.weight_sum : static_cast<double>(a.rows);
-    slope *= w / total * a.inv_temp;
-    if (a.grad_scale != nullptr) slope *= static_cast<double>(*a.grad_scale);
+    slope *= w / in.total * a.inv_temp * static_cast<double>(in.scale);
     return {static_cast<float>(slope), static_cast<float>(-slope / static_cast<double>(s))};
+}
+
+// A row of weight 0: its outputs are zeros.
+template <typename T, int NT, Mode MODE>
+__device__ __forceinline__ void skip_row(const PolicyArgs& a, int64_t n, T* dx) {
+    constexpr int N = 16 / sizeof(T);
+    if (MODE != kGrad && threadIdx.x == 0) {
+        a.log_probs[n] = 0.0f;
+        if (MODE != kLogp) a.terms[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    if constexpr (MODE == kLossGrad || MODE == kGrad) {
+        const float zero[N] = {};
+        for (int64_t i = static_cast<int64_t>(threadIdx.x) * N; i < a.vocab; i += int64_t{NT} * N)
+            store_some<N>(dx + i, zero, a.vocab - i);
+    }
+}
+
+// One vector of the gradient, from column i on.
+template <int N>
+__device__ __forceinline__ void to_gradient(float (&v)[N], const RowResult& q, float o, float c, int64_t y, int64_t i) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = q.k * exp2_hw((v[j] - o) * c);
+    if (y >= i && y < i + N) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (y == i + j) v[j] += q.slope;
+    }
+}
+
+// 16 bytes of a row as they came, and their values.
+typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+template <typename T, int N>
+__device__ __forceinline__ void widen(float (&v)[N], const Raw& raw) {
+    const vec_t<T, N> q = __builtin_bit_cast(vec_t<T, N>, raw);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = static_cast<float>(q[j]);
+}
+
+// The loss and its gradient for rows of at most NT * NV vectors (and a tail of
+// less than one): each thread holds NV of them.  All loads are issued before
+// the first is used; vectors past the row's end repeat its last one and are
+// not counted.
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
+    constexpr int N = 16 / sizeof(T);
+    const int64_t n = a.first_row + blockIdx.x;
+    const float w = weight_at(a.mask, a.mask_kind, n);
+    const T* x = static_cast<const T*>(a.logits) + n * a.row_stride;
+    T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
+    if (w == 0.0f) return skip_row<T, NT, kLossGrad>(a, n, dx);
+    const int V = static_cast<int>(a.vocab), full = V / N, tail = V - full * N, t = threadIdx.x;
+    Raw raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = i * NT + t;
+        raw[i] = __builtin_bit_cast(
+            Raw, __builtin_nontemporal_load(reinterpret_cast<const vec_t<T, N>*>(x) + (v < full ? v : full - 1)));
+    }
+    float last[1] = {t < tail ? static_cast<float>(x[full * N + t]) : -INFINITY};
+    __shared__ RowInputs in;  // not in registers, which the row needs
+    if (t == 0) in = row_inputs<T, kLossGrad>(a, n);
+    Running r{-INFINITY, 0.0f};
+    take<1>(r, last, a.c);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        __builtin_amdgcn_sched_barrier(0);  // one vector's values at a time: all of them widened do not fit
+        float v[N];
+        widen<T, N>(v, raw[i]);
+        if (i * NT + t < full) take<N>(r, v, a.c);
+        asm("" : "+v"(raw[i]));             // widened again below, not kept
+    }
+    r = join_block<NT>(r, a.c);
+    __shared__ RowResult shared;
+    if (t == 0) shared = row_scalars<kLossGrad>(a, n, in, w, r.m, r.s);
+    __syncthreads();
+    const RowResult q = shared;
+    const float o = base(r.m);
+    const int64_t y = id_at(a.targets, n, a.target_bytes);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = i * NT + t;
+        if (at >= full) continue;
+        __builtin_amdgcn_sched_barrier(0);
+        float v[N];
+        widen<T, N>(v, raw[i]);
+        to_gradient<N>(v, q, o, a.c, y, static_cast<int64_t>(at) * N);
+        store_nt<N>(dx + static_cast<int64_t>(at) * N, v);
+    }
+    if (t < tail) {
+        to_gradient<1>(last, q, o, a.c, y, full * N + t);
+        dx[full * N + t] = static_cast<T>(last[0]);
+    }
 }
 
 template <typename T, int NT, Mode MODE>
@@ -137,37 +251,30 @@ __global__ __launch_bounds__(NT) void policy_kernel(PolicyArgs a) {
     T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
     const int64_t start = static_cast<int64_t>(threadIdx.x) * N;
     constexpr int64_t kStep = int64_t{NT} * N;
-    if (w == 0.0f) {
-        if (MODE != kGrad && threadIdx.x == 0) {
-            a.log_probs[n] = 0.0f;
-            if (MODE != kLogp) a.terms[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-        if constexpr (MODE == kLossGrad || MODE == kGrad) {
-            const float zero[N] = {};
-            for (int64_t i = start; i < V; i += kStep) store_some<N>(dx + i, zero, V - i);
-        }
-        return;
-    }
+    if (w == 0.0f) return skip_row<T, NT, MODE>(a, n, dx);
+    RowInputs in{};
+    if (threadIdx.x == 0) in = row_inputs<T, MODE>(a, n);
     Running r{-INFINITY, 0.0f};
     if constexpr (MODE == kGrad) {
         const float2 q = a.stats[n];
         r = {q.x, q.y};
     } else {
-        int64_t i = start;
-        for (; i + N <= V; i += kStep) {
+        // the elements after the last whole vector first, as cached_kernel does: the same bits
+        const int64_t full = V / N * N;
+        if (threadIdx.x < V - full) {
+            const float v[1] = {static_cast<float>(x[full + threadIdx.x])};
+            take<1>(r, v, a.c);
+        }
+        for (int64_t i = start; i < full; i += kStep) {
             float v[N];
             load<N>(v, x + i);
             take<N>(r, v, a.c);
-        }
-        for (; i < V; ++i) {  // the row's last vector, where it is cut short
-            const float v[1] = {static_cast<float>(x[i])};
-            take<1>(r, v, a.c);
         }
         r = join_block<NT>(r, a.c);
     }
     __shared__ RowResult shared;
     if (threadIdx.x == 0) {
-        const RowResult q = row_scalars<T, MODE>(a, n, w, r.m, r.s);
+        const RowResult q = row_scalars<MODE>(a, n, in, w, r.m, r.s);
         if constexpr (MODE == kLossGrad || MODE == kGrad) shared = q;
     }
     if constexpr (MODE == kLossGrad || MODE == kGrad) {
@@ -178,13 +285,7 @@ __global__ __launch_bounds__(NT) void policy_kernel(PolicyArgs a) {
         for (int64_t i = start; i < V; i += kStep) {
             float v[N];
             load_some<N>(v, x + i, V - i);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = q.k * exp2_hw((v[j] - o) * a.c);
-            if (y >= i && y < i + N) {
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (y == i + j) v[j] += q.slope;
-            }
+            to_gradient<N>(v, q, o, a.c, y, i);
             store_some<N>(dx + i, v, V - i);
         }
     }
@@ -233,6 +334,11 @@ __global__ __launch_bounds__(kSumBlock) void policy_sum_kernel(const float4* ter
     }
 }
 
+template <typename T, int NV>
+void launch_cached(const PolicyArgs& a, dim3 grid, hipStream_t s) {
+    hipLaunchKernelGGL((cached_kernel<T, 1024, NV>), grid, dim3(1024), 0, s, a);
+}
+
 // Threads of a row: enough to keep a row's loads in flight, few enough that
 // short rows do not idle.
 template <typename T, Mode MODE>
@@ -243,7 +349,14 @@ int launch_rows(PolicyArgs a, hipStream_t s) {
         const dim3 grid(static_cast<uint32_t>(a.rows - a.first_row < most ? a.rows - a.first_row : most));
         if (a.vocab <= 256 * N) hipLaunchKernelGGL((policy_kernel<T, 64, MODE>), grid, dim3(64), 0, s, a);
         else if (a.vocab <= 2048 * N) hipLaunchKernelGGL((policy_kernel<T, 256, MODE>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((policy_kernel<T, 1024, MODE>), grid, dim3(1024), 0, s, a);
+        else if (MODE == kLossGrad && a.vocab <= 20 * 1024 * N) {
+            const int nv = static_cast<int>((a.vocab / N + 1023) / 1024);
+            if (nv <= 4) launch_cached<T, 4>(a, grid, s);
+            else if (nv <= 8) launch_cached<T, 8>(a, grid, s);
+            else if (nv <= 12) launch_cached<T, 12>(a, grid, s);
+            else if (nv <= 16) launch_cached<T, 16>(a, grid, s);
+            else launch_cached<T, 20>(a, grid, s);
+        } else hipLaunchKernelGGL((policy_kernel<T, 1024, MODE>), grid, dim3(1024), 0, s, a);
         if (int rc = launched("policy_kernel")) return rc;
     }
     return 0;
