@@ -14,11 +14,16 @@
 //     dx_j   = scale * slope / T * ([j = y] - p_j)
 //
 // A row is one work-group's: a pass over it keeps, per thread, the maximum m
-// and the sum s of exp((x - m) / T); the row's scalars are formed once, in 64
-// bits; a second pass writes the gradient.  The exponent is ((x - m) * log2(e) / T):
-// subtracting first keeps rows of the type's lowest value (m is that value)
-// and entries of it finite, and small differences exact.  Rows of weight 0 are
-// not read.
+// and a sum s of powers of two; the row's scalars are formed once, in 64 bits; a
+// second pass writes the gradient.  Rows of weight 0 are not read.
+//
+// With c = log2(e) / T and B the integer nearest to m c, s = sum 2^(x c - B):
+// one fused multiply-add forms the exponent with one rounding, of the exponent
+// itself, and sums of other B are joined by exact powers of two.  Where m c
+// passes 2^100 -- a row of the type's lowest value, or a largest one -- all
+// that differs from m is further from it than any exponent reaches, so 1/4
+// takes c's place, which keeps the products finite: what equals m counts 1,
+// all else 0.
 //
 // A row that fits is held in registers between the passes (cached_kernel), as
 // it came, so that it is read once; longer rows are read again, from the
@@ -29,6 +34,8 @@
 
 namespace mgopt {
 namespace {
+
+constexpr double kLn2 = 0.6931471805599453;
 
 enum Mode { kLogp, kLoss, kLossGrad, kGrad };
 
@@ -56,40 +63,47 @@ __device__ __forceinline__ float weight_at(const void* mask, int32_t kind, int64
     return static_cast<const float*>(mask)[n];
 }
 
-// m and s of a running sum of exp2((x - m) * c).  m is -inf until a larger
-// value was seen; the differences are then taken to 0, so that -inf - -inf
-// does not occur (a row of nothing but -inf keeps s = 0, and its log is -inf).
-struct Running {
-    float m, s;
+// The exponents' factor and offset (-B) at maximum m.  Without a maximum yet
+// (-inf) the offset is finite, so that -inf - -inf does not occur: -inf then
+// counts 0, and a row of nothing else has s = 0, whose log is -inf.
+struct Frame {
+    float c, offset;
 };
-__device__ __forceinline__ float base(float m) { return m == -INFINITY ? 0.0f : m; }
-__device__ __forceinline__ Running join(Running a, Running b, float c) {
-    const float m = fmaxf(a.m, b.m), o = base(m);
-    return {m, a.s * exp2_hw((a.m - o) * c) + b.s * exp2_hw((b.m - o) * c)};
+__device__ __forceinline__ Frame frame(float m, float c) {
+    const float k = fabsf(m * c) < 0x1p100f ? c : 0.25f;
+    return {k, m == -INFINITY ? 3e38f : -rintf(m * k)};
+}
+struct Running {
+    float m = -INFINITY, s = 0.0f, offset = 3e38f;  // of frame(m)
+};
+__device__ __forceinline__ Running join(Running a, Running b) {
+    const bool up = b.m > a.m;
+    const float o = up ? b.offset : a.offset;
+    return {up ? b.m : a.m, a.s * exp2_hw(o - a.offset) + b.s * exp2_hw(o - b.offset), o};
 }
 template <int N>
 __device__ __forceinline__ void take(Running& r, const float (&x)[N], float c) {
-    float m = r.m;
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
-    const float o = base(m);
-    float s = r.s * exp2_hw((r.m - o) * c);
+    for (int i = 0; i < N; ++i) r.m = fmaxf(r.m, x[i]);
+    const Frame f = frame(r.m, c);
+    r.s *= exp2_hw(f.offset - r.offset);
+    r.offset = f.offset;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += exp2_hw((x[i] - o) * c);
-    r = {m, s};
+    for (int i = 0; i < N; ++i) r.s += exp2_hw(fmaf(x[i], f.c, f.offset));
 }
 
 template <int NT>
-__device__ __forceinline__ Running join_block(Running r, float c) {
+__device__ __forceinline__ Running join_block(Running r) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) r = join(r, Running{__shfl_xor(r.m, off), __shfl_xor(r.s, off)}, c);
+    for (int off = 1; off < 64; off <<= 1) r = join(r, Running{__shfl_xor(r.m, off), __shfl_xor(r.s, off), __shfl_xor(r.offset, off)});
     if constexpr (NT > 64) {
-        __shared__ Running part[NT / 64];
-        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = r;
+        __shared__ float part_m[NT / 64], part_s[NT / 64], part_o[NT / 64];
+        const int wave = threadIdx.x / 64;
+        if (threadIdx.x % 64 == 0) part_m[wave] = r.m, part_s[wave] = r.s, part_o[wave] = r.offset;
         __syncthreads();
-        r = part[0];
-#pragma unroll
-        for (int i = 1; i < NT / 64; ++i) r = join(r, part[i], c);
+        r = {part_m[0], part_s[0], part_o[0]};
+#pragma unroll 1
+        for (int i = 1; i < NT / 64; ++i) r = join(r, Running{part_m[i], part_s[i], part_o[i]});
     }
     return r;
 }
@@ -119,7 +133,7 @@ __device__ __forceinline__ RowInputs row_inputs(const PolicyArgs& a, int64_t n) 
 }
 
 struct RowResult {
-    float slope, k;  // of the gradient: slope * [j = y] + k * exp2((x - m) * c)
+    float slope, k;  // of the gradient: slope * [j = y] + k * 2^(x c - B)
 };
 
 // What one row adds to the loss, and its slope, from m and s.
@@ -129,7 +143,11 @@ __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs
     if constexpr (MODE == kGrad) {
         logp = a.log_probs[n];
     } else {
-        logp = (static_cast<double>(in.x) - static_cast<double>(base(m))) * a.inv_temp - log(static_cast<double>(s));
+        // to the maximum exactly, and from there as the sum was formed
+        const Frame f = frame(m, a.c);
+        logp = (static_cast<double>(in.x) - static_cast<double>(m)) * a.inv_temp +
+               fma(static_cast<double>(m), static_cast<double>(f.c), static_cast<double>(f.offset)) * kLn2 -
+               log(static_cast<double>(s));
         a.log_probs[n] = static_cast<float>(logp);
     }
     if constexpr (MODE == kLogp) return {};
@@ -167,9 +185,9 @@ __device__ __forceinline__ void skip_row(const PolicyArgs& a, int64_t n, T* dx) 
 
 // One vector of the gradient, from column i on.
 template <int N>
-__device__ __forceinline__ void to_gradient(float (&v)[N], const RowResult& q, float o, float c, int64_t y, int64_t i) {
+__device__ __forceinline__ void to_gradient(float (&v)[N], const RowResult& q, const Frame& f, int64_t y, int64_t i) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = q.k * exp2_hw((v[j] - o) * c);
+    for (int j = 0; j < N; ++j) v[j] = q.k * exp2_hw(fmaf(v[j], f.c, f.offset));
     if (y >= i && y < i + N) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -186,30 +204,31 @@ __device__ __forceinline__ void widen(float (&v)[N], const Raw& raw) {
     for (int j = 0; j < N; ++j) v[j] = static_cast<float>(q[j]);
 }
 
-// The loss and its gradient for rows of at most NT * NV vectors (and a tail of
-// less than one): each thread holds NV of them.  All loads are issued before
+// Rows of at most NT * NV vectors (and a tail of less than one): each thread
+// holds NV of them.  All loads are issued before
 // the first is used; vectors past the row's end repeat its last one and are
 // not counted.
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, Mode MODE>
 __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
     constexpr int N = 16 / sizeof(T);
     const int64_t n = a.first_row + blockIdx.x;
     const float w = weight_at(a.mask, a.mask_kind, n);
     const T* x = static_cast<const T*>(a.logits) + n * a.row_stride;
     T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
-    if (w == 0.0f) return skip_row<T, NT, kLossGrad>(a, n, dx);
+    if (w == 0.0f) return skip_row<T, NT, MODE>(a, n, dx);
     const int V = static_cast<int>(a.vocab), full = V / N, tail = V - full * N, t = threadIdx.x;
     Raw raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int v = i * NT + t;
-        raw[i] = __builtin_bit_cast(
-            Raw, __builtin_nontemporal_load(reinterpret_cast<const vec_t<T, N>*>(x) + (v < full ? v : full - 1)));
+        raw[i] = full > 0 ? __builtin_bit_cast(Raw, __builtin_nontemporal_load(reinterpret_cast<const vec_t<T, N>*>(x) +
+                                                                              (v < full ? v : full - 1)))
+                          : Raw{};
     }
     float last[1] = {t < tail ? static_cast<float>(x[full * N + t]) : -INFINITY};
     __shared__ RowInputs in;  // not in registers, which the row needs
-    if (t == 0) in = row_inputs<T, kLossGrad>(a, n);
-    Running r{-INFINITY, 0.0f};
+    if (t == 0) in = row_inputs<T, MODE>(a, n);
+    Running r;
     take<1>(r, last, a.c);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -219,12 +238,13 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
         if (i * NT + t < full) take<N>(r, v, a.c);
         asm("" : "+v"(raw[i]));             // widened again below, not kept
     }
-    r = join_block<NT>(r, a.c);
+    r = join_block<NT>(r);
     __shared__ RowResult shared;
-    if (t == 0) shared = row_scalars<kLossGrad>(a, n, in, w, r.m, r.s);
+    if (t == 0) shared = row_scalars<MODE>(a, n, in, w, r.m, r.s);
+    if constexpr (MODE != kLossGrad) return;
     __syncthreads();
     const RowResult q = shared;
-    const float o = base(r.m);
+    const Frame f = frame(r.m, a.c);
     const int64_t y = id_at(a.targets, n, a.target_bytes);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -233,14 +253,17 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         float v[N];
         widen<T, N>(v, raw[i]);
-        to_gradient<N>(v, q, o, a.c, y, static_cast<int64_t>(at) * N);
+        to_gradient<N>(v, q, f, y, static_cast<int64_t>(at) * N);
         store_nt<N>(dx + static_cast<int64_t>(at) * N, v);
     }
     if (t < tail) {
-        to_gradient<1>(last, q, o, a.c, y, full * N + t);
+        to_gradient<1>(last, q, f, y, full * N + t);
         dx[full * N + t] = static_cast<T>(last[0]);
     }
 }
+
+template <int V>
+using Int = std::integral_constant<int, V>;
 
 template <typename T, int NT, Mode MODE>
 __global__ __launch_bounds__(NT) void policy_kernel(PolicyArgs a) {
@@ -254,10 +277,10 @@ __global__ __launch_bounds__(NT) void policy_kernel(PolicyArgs a) {
     if (w == 0.0f) return skip_row<T, NT, MODE>(a, n, dx);
     RowInputs in{};
     if (threadIdx.x == 0) in = row_inputs<T, MODE>(a, n);
-    Running r{-INFINITY, 0.0f};
+    Running r;
     if constexpr (MODE == kGrad) {
         const float2 q = a.stats[n];
-        r = {q.x, q.y};
+        r.m = q.x, r.s = q.y;
     } else {
         // the elements after the last whole vector first, as cached_kernel does: the same bits
         const int64_t full = V / N * N;
@@ -270,7 +293,7 @@ __global__ __launch_bounds__(NT) void policy_kernel(PolicyArgs a) {
             load<N>(v, x + i);
             take<N>(r, v, a.c);
         }
-        r = join_block<NT>(r, a.c);
+        r = join_block<NT>(r);
     }
     __shared__ RowResult shared;
     if (threadIdx.x == 0) {
@@ -280,12 +303,12 @@ __global__ __launch_bounds__(NT) void policy_kernel(PolicyArgs a) {
     if constexpr (MODE == kLossGrad || MODE == kGrad) {
         __syncthreads();
         const RowResult q = shared;
-        const float o = base(r.m);
+        const Frame f = frame(r.m, a.c);
         const int64_t y = id_at(a.targets, n, a.target_bytes);
         for (int64_t i = start; i < V; i += kStep) {
             float v[N];
             load_some<N>(v, x + i, V - i);
-            to_gradient<N>(v, q, o, a.c, y, i);
+            to_gradient<N>(v, q, f, y, i);
             store_some<N>(dx + i, v, V - i);
         }
     }
@@ -334,29 +357,33 @@ __global__ __launch_bounds__(kSumBlock) void policy_sum_kernel(const float4* ter
     }
 }
 
-template <typename T, int NV>
-void launch_cached(const PolicyArgs& a, dim3 grid, hipStream_t s) {
-    hipLaunchKernelGGL((cached_kernel<T, 1024, NV>), grid, dim3(1024), 0, s, a);
-}
-
-// Threads of a row: enough to keep a row's loads in flight, few enough that
-// short rows do not idle.
+// The kernel for rows of this length: threads enough to keep a row's loads in
+// flight, few enough that short rows do not idle.
 template <typename T, Mode MODE>
 int launch_rows(PolicyArgs a, hipStream_t s) {
     constexpr int N = 16 / sizeof(T);
-    const int64_t most = max_blocks(1024);
+    const int64_t most = max_blocks(1024), vecs = a.vocab / N;
     for (a.first_row = 0; a.first_row < a.rows; a.first_row += most) {
         const dim3 grid(static_cast<uint32_t>(a.rows - a.first_row < most ? a.rows - a.first_row : most));
-        if (a.vocab <= 256 * N) hipLaunchKernelGGL((policy_kernel<T, 64, MODE>), grid, dim3(64), 0, s, a);
-        else if (a.vocab <= 2048 * N) hipLaunchKernelGGL((policy_kernel<T, 256, MODE>), grid, dim3(256), 0, s, a);
-        else if (MODE == kLossGrad && a.vocab <= 20 * 1024 * N) {
-            const int nv = static_cast<int>((a.vocab / N + 1023) / 1024);
-            if (nv <= 4) launch_cached<T, 4>(a, grid, s);
-            else if (nv <= 8) launch_cached<T, 8>(a, grid, s);
-            else if (nv <= 12) launch_cached<T, 12>(a, grid, s);
-            else if (nv <= 16) launch_cached<T, 16>(a, grid, s);
-            else launch_cached<T, 20>(a, grid, s);
-        } else hipLaunchKernelGGL((policy_kernel<T, 1024, MODE>), grid, dim3(1024), 0, s, a);
+        const auto cached = [&](auto threads, auto held) {
+            constexpr int NT = decltype(threads)::value, NV = decltype(held)::value;
+            if (vecs > NT * NV) return false;
+            hipLaunchKernelGGL((cached_kernel<T, NT, NV, MODE>), grid, dim3(NT), 0, s, a);
+            return true;
+        };
+        const auto again = [&](auto threads) {
+            constexpr int NT = decltype(threads)::value;
+            hipLaunchKernelGGL((policy_kernel<T, NT, MODE>), grid, dim3(NT), 0, s, a);
+        };
+        if constexpr (MODE == kGrad) {
+            if (vecs <= 256) again(Int<64>{});
+            else if (vecs <= 2048) again(Int<256>{});
+            else again(Int<1024>{});
+        } else if (!(cached(Int<64>{}, Int<4>{}) || cached(Int<256>{}, Int<8>{}) || cached(Int<1024>{}, Int<4>{}) ||
+                     cached(Int<1024>{}, Int<8>{}) || cached(Int<1024>{}, Int<12>{}) || cached(Int<1024>{}, Int<16>{}) ||
+                     cached(Int<1024>{}, Int<20>{}))) {
+            again(Int<1024>{});
+        }
         if (int rc = launched("policy_kernel")) return rc;
     }
     return 0;
