@@ -29,27 +29,46 @@ struct LookupArgs {
     float scale;
 };
 
-template <typename TW, typename TO>
+// N elements as they came; those past `left` are zeros.
+template <typename T, int N>
+__device__ __forceinline__ vec_t<T, N> load_raw(const T* p, int64_t left) {
+    if (left >= N) return *reinterpret_cast<const vec_t<T, N>*>(p);
+    vec_t<T, N> v = {};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < left) v[i] = p[i];
+    return v;
+}
+
+// K tokens a thread, kBlock >> shift apart: the ids and then the rows of all of
+// them are on their way before the first is written.
+template <typename TW, typename TO, int K>
 __global__ __launch_bounds__(kBlock) void lookup_kernel(LookupArgs a) {
     constexpr int N = 16 / (sizeof(TW) > sizeof(TO) ? sizeof(TW) : sizeof(TO));
-    const int64_t t = a.first + static_cast<int64_t>(blockIdx.x) * (kBlock >> a.shift) + (threadIdx.x >> a.shift);
-    if (t >= a.n) return;
-    const int64_t id = id_at(a.ids, t, a.id_bytes);
-    const bool known = id >= 0 && id < a.rows;
-    const TW* w = static_cast<const TW*>(a.weight) + (known ? id : 0) * a.width;
-    TO* out = static_cast<TO*>(a.out) + t * a.width;
+    const int64_t per = kBlock >> a.shift;
+    const int64_t t0 = a.first + static_cast<int64_t>(blockIdx.x) * (per * K) + (threadIdx.x >> a.shift);
+    int64_t id[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int64_t t = t0 + k * per;
+        id[k] = t < a.n ? id_at(a.ids, t, a.id_bytes) : -1;
+    }
     const int64_t step = int64_t{N} << a.shift;
     for (int64_t c = static_cast<int64_t>(threadIdx.x & ((1u << a.shift) - 1)) * N; c < a.width; c += step) {
-        float v[N];
-        if (known) {
-            load_some<N>(v, w + c, a.width - c);
+        vec_t<TW, N> w[K];
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] *= a.scale;
-        } else {
+        for (int k = 0; k < K; ++k)
+            if (id[k] >= 0 && id[k] < a.rows) w[k] = load_raw<TW, N>(static_cast<const TW*>(a.weight) + id[k] * a.width + c, a.width - c);
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = __builtin_nanf("");
+        for (int k = 0; k < K; ++k) {
+            const int64_t t = t0 + k * per;
+            if (t >= a.n) break;
+            const bool known = id[k] >= 0 && id[k] < a.rows;
+            float v[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = known ? static_cast<float>(w[k][i]) * a.scale : __builtin_nanf("");
+            store_some<N>(static_cast<TO*>(a.out) + t * a.width + c, v, a.width - c);
         }
-        store_some<N>(out + c, v, a.width - c);
     }
 }
 
@@ -337,87 +356,108 @@ struct SumArgs {
     float scale;
 };
 
-template <int N, typename TW>
-__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int64_t c, float (&sum)[N]) {
-    TW* out = static_cast<TW*>(a.grad) + static_cast<int64_t>(row) * a.width + c;
-    const int64_t left = a.width - c;
-    float old[N] = {}, x[N];
-    if (a.accumulate) load_some<N>(old, out, left);
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = fmaf(sum[j], a.scale, old[j]);
-    store_some<N>(out, x, left);
-}
-
 // A group of 1 << shift threads sums the rows of one piece of the sorted list
 // over its columns.  A run of one key that lies inside the piece is written to
 // its row; one that began before it goes to the piece's first partial row, one
-// that began in it and goes on after it to the second.
-template <typename TG, typename TW>
+// that began in it and goes on after it to the second.  The rows of kAhead
+// tokens, and what the weight rows that end among them hold, are on their way
+// at once.  WIDE: a wave has one piece, so that its keys are scalars.
+template <typename TG, typename TW, bool WIDE>
 __global__ __launch_bounds__(kBlock) void sum_pieces_kernel(SumArgs a) {
-    constexpr int N = 16 / (sizeof(TG) > sizeof(TW) ? sizeof(TG) : sizeof(TW)), kAhead = 4;
+    constexpr int N = 16 / (sizeof(TG) > sizeof(TW) ? sizeof(TG) : sizeof(TW)), kAhead = 8;
     const uint32_t pb = blockIdx.x / a.chunks, cb = blockIdx.x - pb * a.chunks;
-    const uint32_t piece = pb * (kBlock >> a.shift) + (threadIdx.x >> a.shift);
+    uint32_t piece = pb * (kBlock >> a.shift) + (threadIdx.x >> a.shift);
+    if constexpr (WIDE) piece = __builtin_amdgcn_readfirstlane(piece);
     const int64_t c = (static_cast<int64_t>(cb) * kBlock + (threadIdx.x & ((1u << a.shift) - 1))) * N, left = a.width - c;
     if (piece >= a.pieces || left <= 0) return;
-    const uint32_t first = piece * a.piece, last = a.n - first < a.piece ? a.n : first + a.piece;
-    uint32_t row = a.keys[first];
-    if (row >= a.rows) return;  // the ids that name no row come last
-    bool head = first > 0 && a.keys[first - 1] == row;
+    const uint32_t none = static_cast<uint32_t>(a.rows), first = piece * a.piece;
+    const uint32_t last = a.n - first < a.piece ? a.n : first + a.piece;
+    bool head = first > 0 && a.keys[first - 1] == a.keys[first];  // its first run began before it
+    bool open = false;                                            // the run at hand goes on
     float sum[N] = {};
     for (uint32_t i = first; i < last; i += kAhead) {
-        float v[kAhead][N];
-        uint32_t key[kAhead];
+        uint32_t key[kAhead + 1];
+#pragma unroll
+        for (int u = 0; u <= kAhead; ++u) key[u] = i + u < a.n ? a.keys[i + u] : none;
+        if (key[0] == none) break;  // the ids that name no row come last
+        vec_t<TG, N> v[kAhead];
+        vec_t<TW, N> old[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            key[u] = i + u < last ? a.keys[i + u] : static_cast<uint32_t>(a.rows);
-            if (key[u] < a.rows)
-                load_some<N>(v[u], static_cast<const TG*>(a.grad_out) + static_cast<int64_t>(a.tokens[i + u]) * a.width + c, left);
+            if (i + u >= last || key[u] == none) continue;
+            v[u] = load_raw<TG, N>(static_cast<const TG*>(a.grad_out) + static_cast<int64_t>(a.tokens[i + u]) * a.width + c, left);
+            if (a.accumulate && key[u + 1] != key[u])
+                old[u] = load_raw<TW, N>(static_cast<const TW*>(a.grad) + static_cast<int64_t>(key[u]) * a.width + c, left);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (i + u >= last) break;
-            if (key[u] != row) {
-                if (row < a.rows) {
-                    if (head) store_some<N>(a.partials + static_cast<int64_t>(piece) * 2 * a.width + c, sum, left);
-                    else write_row<N, TW>(a, row, c, sum);
-                }
-                row = key[u];
-                head = false;
+            if (i + u >= last || key[u] == none) continue;
 #pragma unroll
-                for (int j = 0; j < N; ++j) sum[j] = 0.0f;
-            }
-            if (row < a.rows) {
+            for (int j = 0; j < N; ++j) sum[j] += static_cast<float>(v[u][j]);
+            open = key[u + 1] == key[u];
+            if (open) continue;
+            if (head) {
+                store_some<N>(a.partials + static_cast<int64_t>(piece) * 2 * a.width + c, sum, left);
+            } else {
 #pragma unroll
-                for (int j = 0; j < N; ++j) sum[j] += v[u][j];
+                for (int j = 0; j < N; ++j) sum[j] = a.accumulate ? fmaf(sum[j], a.scale, static_cast<float>(old[u][j])) : sum[j] * a.scale;
+                store_some<N>(static_cast<TW*>(a.grad) + static_cast<int64_t>(key[u]) * a.width + c, sum, left);
             }
+            head = false;
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum[j] = 0.0f;
         }
     }
-    if (row >= a.rows) return;
-    const bool tail = last < a.n && a.keys[last] == row;
-    if (!head && !tail) write_row<N, TW>(a, row, c, sum);
-    else store_some<N>(a.partials + (static_cast<int64_t>(piece) * 2 + (head ? 0 : 1)) * a.width + c, sum, left);
+    if (open) store_some<N>(a.partials + (static_cast<int64_t>(piece) * 2 + (head ? 0 : 1)) * a.width + c, sum, left);
 }
 
-// Joins the runs that cross pieces: the group of the piece in which a run began
-// adds the partial rows of the pieces it goes on through, in their order.
+// Joins the runs that cross pieces.  The work-group of the piece in which a run
+// began adds the partial rows of the pieces that it goes on through: 64 lanes
+// over the columns, its waves over the pieces in turn, joined in a fixed order.
 template <int N, typename TW>
 __global__ __launch_bounds__(kBlock) void join_pieces_kernel(SumArgs a) {
-    const uint32_t pb = blockIdx.x / a.chunks, cb = blockIdx.x - pb * a.chunks;
-    const uint32_t piece = pb * (kBlock >> a.shift) + (threadIdx.x >> a.shift);
-    const int64_t c = (static_cast<int64_t>(cb) * kBlock + (threadIdx.x & ((1u << a.shift) - 1))) * N, left = a.width - c;
-    if (piece + 1 >= a.pieces || left <= 0) return;
+    constexpr uint32_t kWaves = kBlock / 64;
+    __shared__ float part[kWaves][64][N + 1];
+    const uint32_t piece = blockIdx.x / a.chunks, cb = blockIdx.x - piece * a.chunks;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    if (piece + 1 >= a.pieces) return;
     const uint32_t first = piece * a.piece, next = first + a.piece, row = a.keys[next];
-    if (row >= a.rows || a.keys[next - 1] != row) return;             // nothing crosses this piece's end
+    if (row >= a.rows || a.keys[next - 1] != row) return;                       // nothing crosses this piece's end
     if (a.keys[first] == row && first > 0 && a.keys[first - 1] == row) return;  // it began before this piece
-    float sum[N];
-    load_some<N>(sum, a.partials + (static_cast<int64_t>(piece) * 2 + 1) * a.width + c, left);
-    for (uint32_t q = piece + 1; q < a.pieces && a.keys[q * a.piece] == row; ++q) {
-        float v[N];
-        load_some<N>(v, a.partials + static_cast<int64_t>(q) * 2 * a.width + c, left);
-#pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] += v[j];
+    // the pieces it goes on through: those whose first key is its
+    uint32_t more = 0;
+    for (uint32_t q = piece + 1;; q += kBlock) {
+        const uint32_t here = q + threadIdx.x;
+        const int n = __syncthreads_count(here < a.pieces && a.keys[here * a.piece] == row);
+        more += static_cast<uint32_t>(n);
+        if (n < kBlock) break;
     }
-    write_row<N, TW>(a, row, c, sum);
+    const int64_t c = (static_cast<int64_t>(cb) * 64 + lane) * N, left = a.width - c;
+    float sum[N] = {};
+    if (left > 0) {
+        const float* at = a.partials + static_cast<int64_t>(piece + 1) * 2 * a.width + c;
+        if (wave == 0) load_some<N>(sum, at - a.width, left);
+#pragma unroll 8
+        for (uint32_t q = wave; q < more; q += kWaves) {
+            float v[N];
+            load_some<N>(v, at + static_cast<int64_t>(q) * 2 * a.width, left);
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum[j] += v[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) part[wave][lane][j] = sum[j];
+    __syncthreads();
+    if (wave != 0 || left <= 0) return;
+    for (uint32_t w = 1; w < kWaves; ++w)
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[j] += part[w][lane][j];
+    TW* out = static_cast<TW*>(a.grad) + static_cast<int64_t>(row) * a.width + c;
+    float old[N] = {};
+    if (a.accumulate) load_some<N>(old, out, left);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = fmaf(sum[j], a.scale, old[j]);
+    store_some<N>(out, sum, left);
 }
 
 // Which form: the sort's launches cost what reading all ids for each of a few
@@ -478,11 +518,14 @@ MGOPT_API int mgopt_embedding(const void* ids_dev, int32_t id_bytes, int64_t n, 
             using TO = decltype(o);
             constexpr int N = 16 / (sizeof(TW) > sizeof(TO) ? sizeof(TW) : sizeof(TO));
             a.shift = shift_for((width + N - 1) / N);
-            const int64_t per_block = kBlock >> a.shift, most = max_blocks(kBlock) * per_block;
+            const int64_t per_block = kBlock >> a.shift;
+            // four tokens a thread where that leaves work-groups enough for the chip
+            const bool four = n >= 4 * 1024 * per_block;
+            const int64_t tokens = per_block * (four ? 4 : 1), most = max_blocks(kBlock) * tokens;
             for (a.first = 0; a.first < n; a.first += most) {
-                const int64_t blocks = (std::min(n - a.first, most) + per_block - 1) / per_block;
-                hipLaunchKernelGGL((lookup_kernel<TW, TO>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0,
-                                   static_cast<hipStream_t>(stream), a);
+                const dim3 grid(static_cast<uint32_t>((std::min(n - a.first, most) + tokens - 1) / tokens));
+                if (four) hipLaunchKernelGGL((lookup_kernel<TW, TO, 4>), grid, dim3(kBlock), 0, static_cast<hipStream_t>(stream), a);
+                else hipLaunchKernelGGL((lookup_kernel<TW, TO, 1>), grid, dim3(kBlock), 0, static_cast<hipStream_t>(stream), a);
                 if (int rc = launched("lookup_kernel")) return rc;
             }
             return 0;
@@ -561,9 +604,15 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
             m.pieces = static_cast<uint32_t>((n + m.piece - 1) / m.piece);
             const int64_t per_block = kBlock >> shift, blocks = (m.pieces + per_block - 1) / per_block * chunks;
             if (blocks > max_blocks(kBlock)) return set_error(MGOPT_E_LIMIT, "embedding_grad: too many tokens of long rows");
-            hipLaunchKernelGGL((sum_pieces_kernel<TG, TW>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, m);
+            if (shift >= 6)
+                hipLaunchKernelGGL((sum_pieces_kernel<TG, TW, true>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, m);
+            else
+                hipLaunchKernelGGL((sum_pieces_kernel<TG, TW, false>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, m);
             if (int rc = launched("sum_pieces_kernel")) return rc;
-            hipLaunchKernelGGL((join_pieces_kernel<N, TW>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, m);
+            m.chunks = static_cast<uint32_t>((vecs + 63) / 64);
+            if (static_cast<int64_t>(m.chunks) * m.pieces > max_blocks(kBlock))
+                return set_error(MGOPT_E_LIMIT, "embedding_grad: too many tokens of long rows");
+            hipLaunchKernelGGL((join_pieces_kernel<N, TW>), dim3(m.pieces * m.chunks), dim3(kBlock), 0, s, m);
             if (int rc = launched("join_pieces_kernel")) return rc;
             return 0;
         });
