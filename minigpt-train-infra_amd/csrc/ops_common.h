@@ -82,16 +82,24 @@ __device__ __forceinline__ void store_nt(T* p, const float (&f)[N]) {
 }
 
 // The first n of N elements (n may exceed N or be negative), zeros for the others.
-template <int N, typename T>
+template <int N, bool NT = false, typename T>
 __device__ __forceinline__ void load_some(float (&f)[N], const T* p, int64_t n) {
-    if (n >= N) return load<N>(f, p);
+    if (n >= N) {
+        if constexpr (NT) load_nt<N>(f, p);
+        else load<N>(f, p);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = i < n ? static_cast<float>(p[i]) : 0.0f;
 }
 
-template <int N, typename T>
+template <int N, bool NT = false, typename T>
 __device__ __forceinline__ void store_some(T* p, const float (&f)[N], int64_t n) {
-    if (n >= N) return store<N>(p, f);
+    if (n >= N) {
+        if constexpr (NT) store_nt<N>(p, f);
+        else store<N>(p, f);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i)
         if (i < n) p[i] = static_cast<T>(f[i]);

@@ -29,10 +29,13 @@ struct LookupArgs {
     float scale;
 };
 
-// N elements as they came; those past `left` are zeros.
-template <typename T, int N>
+// N elements as they came; those past `left` are zeros.  NT: streamed.
+template <typename T, int N, bool NT = false>
 __device__ __forceinline__ vec_t<T, N> load_raw(const T* p, int64_t left) {
-    if (left >= N) return *reinterpret_cast<const vec_t<T, N>*>(p);
+    if (left >= N) {
+        if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const vec_t<T, N>*>(p));
+        else return *reinterpret_cast<const vec_t<T, N>*>(p);
+    }
     vec_t<T, N> v = {};
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -158,7 +161,7 @@ __global__ __launch_bounds__(kBlock) void grad_by_row_kernel(GradArgs a) {
 // neighbours in their order; then the sorted list is cut in pieces of equal
 // length, whatever rows they touch, and the pieces' sums are joined.
 //
-// The sort is a radix sort, kDigitBits a pass, from the low digit up.  A pass
+// The sort is a radix sort, at most kDigitBits a pass, from the low digit up.  A pass
 // counts every tile's digits, and then places each token behind the tokens of
 // smaller digits, those of its digit in earlier tiles, and those before it in
 // its tile.  Ids that name no row, and the padding's, become the key `rows`
@@ -175,8 +178,8 @@ struct SortArgs {
     uint32_t* counts;          // [tiles][kDigits]
     int64_t rows, padding;
     uint32_t n, tiles;
-    int32_t id_bytes, shift;   // the digit's lowest bit
-    char* zeros;               // first pass: what the work-groups past the tiles clear
+    int32_t id_bytes, shift, digit_bits;  // the digit's lowest bit and its length
+    char* zeros;               // what the work-groups past the tiles clear: a multiple of 16 bytes but in the last launch
     int64_t zero_bytes;
 };
 
@@ -188,9 +191,9 @@ __device__ __forceinline__ uint32_t key_at(const SortArgs& a, uint32_t t) {
 
 // Clears a.zeros with the work-groups from `first` on.
 __device__ __forceinline__ void clear(const SortArgs& a, uint32_t first) {
-    const int64_t vecs = a.zero_bytes / 16, step = static_cast<int64_t>(gridDim.x - first) * kSortBlock;
+    const int64_t vecs = a.zero_bytes / 16, step = static_cast<int64_t>(gridDim.x - first) * blockDim.x;
     const vec_t<uint16_t, 8> zero = {};
-    int64_t i = static_cast<int64_t>(blockIdx.x - first) * kSortBlock + threadIdx.x;
+    int64_t i = static_cast<int64_t>(blockIdx.x - first) * blockDim.x + threadIdx.x;
     if (i < a.zero_bytes % 16 / 2) reinterpret_cast<uint16_t*>(a.zeros)[vecs * 8 + i] = 0;
     for (; i < vecs; i += step) reinterpret_cast<vec_t<uint16_t, 8>*>(a.zeros)[i] = zero;
 }
@@ -203,13 +206,14 @@ __global__ __launch_bounds__(kSortBlock) void count_kernel(SortArgs a) {
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const uint32_t t = blockIdx.x * kTile + k * kSortBlock + threadIdx.x;
-        if (t < a.n) atomicAdd(&count[key_at(a, t) >> a.shift & (kDigits - 1)], 1u);
+        if (t < a.n) atomicAdd(&count[key_at(a, t) >> a.shift & ((1u << a.digit_bits) - 1)], 1u);
     }
     __syncthreads();
     a.counts[static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = count[threadIdx.x];
 }
 
-// The exclusive sum of x over the work-group's threads.
+// The exclusive sum of x over the work-group's WAVES waves.
+template <int WAVES>
 __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* wave_sums) {
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     uint32_t run = x;
@@ -226,122 +230,126 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* wave_sums) 
     return base + run - x;
 }
 
-// The places within the tile's digits of a thread's items, which are the
-// tile's elements wave * 256 + k * 64 + lane; used[w][d] becomes the number of
-// elements of digit d in waves before w, and the return value of thread d the
-// number in the tile.
-struct Places {
-    uint32_t rank[kSortItems];
-};
-__device__ __forceinline__ uint32_t rank_tile(const uint32_t (&digit)[kSortItems], const bool (&on)[kSortItems],
-                                              uint32_t (&used)[kSortWaves][kDigits], Places& p) {
+// The places within their digits of a tile's elements: element k of a thread
+// is the tile's wave * 64 * ITEMS + k * 64 + lane.  rank counts those of its
+// digit before it in its wave, used[w][d] becomes the number of digit d in the
+// waves before w, and thread d's return value the number in the tile.  The
+// lanes of one digit are found by a vote per bit.
+template <int WAVES, int ITEMS>
+__device__ __forceinline__ uint32_t rank_tile(const uint32_t (&digit)[ITEMS], const bool (&on)[ITEMS],
+                                              uint16_t (&used)[WAVES][kDigits], uint32_t (&rank)[ITEMS], int digit_bits) {
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-#pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) used[w][threadIdx.x] = 0;
+    for (uint32_t i = threadIdx.x; i < WAVES * kDigits / 2; i += WAVES * 64) reinterpret_cast<uint32_t*>(used)[i] = 0;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
+    for (int k = 0; k < ITEMS; ++k) {
         uint64_t same = __ballot(on[k]);
-#pragma unroll
-        for (int bit = 0; bit < kDigitBits; ++bit) {
+        for (int bit = 0; bit < digit_bits; ++bit) {
             const bool b = digit[k] >> bit & 1u;
             const uint64_t vote = __ballot(b);
             same &= b ? vote : ~vote;
         }
         const uint32_t before = static_cast<uint32_t>(__popcll(same & ((uint64_t{1} << lane) - 1)));
         // the wave's lanes read the counter, then the first of each digit moves it on
-        uint32_t* counter = &used[wave][digit[k]];
-        const uint32_t old = *reinterpret_cast<volatile uint32_t*>(counter);
+        volatile uint16_t* counter = &used[wave][digit[k]];
+        const uint32_t old = *counter;
         __builtin_amdgcn_wave_barrier();
-        if (on[k] && before == 0) *reinterpret_cast<volatile uint32_t*>(counter) = old + static_cast<uint32_t>(__popcll(same));
+        if (on[k] && before == 0) *counter = static_cast<uint16_t>(old + static_cast<uint32_t>(__popcll(same)));
         __builtin_amdgcn_wave_barrier();
-        p.rank[k] = old + before;
+        rank[k] = old + before;
     }
     __syncthreads();
     uint32_t sum = 0;
+    if (threadIdx.x < kDigits) {
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t x = used[w][threadIdx.x];
-        used[w][threadIdx.x] = sum;
-        sum += x;
+        for (int w = 0; w < WAVES; ++w) {
+            const uint32_t x = used[w][threadIdx.x];
+            used[w][threadIdx.x] = static_cast<uint16_t>(sum);
+            sum += x;
+        }
     }
     __syncthreads();
     return sum;
 }
 
 __global__ __launch_bounds__(kSortBlock) void place_kernel(SortArgs a) {
-    __shared__ uint32_t used[kSortWaves][kDigits], base[kDigits], wave_sums[kSortWaves];
-    const uint32_t d = threadIdx.x, lane = d % 64, wave = d / 64;
-    uint32_t all = 0, earlier = 0;
+    if (blockIdx.x >= a.tiles) return clear(a, a.tiles);
+    __shared__ uint16_t used[kSortWaves][kDigits];
+    __shared__ uint32_t base[kDigits], wave_sums[kSortWaves];
+    const uint32_t d = threadIdx.x, lane = d % 64, wave = d / 64, begin = blockIdx.x * kTile;
+    uint32_t earlier = 0, all = 0;  // elements of digit d
 #pragma unroll 8
     for (uint32_t b = 0; b < a.tiles; ++b) {
         const uint32_t x = a.counts[static_cast<int64_t>(b) * kDigits + d];
         all += x;
-        if (b < blockIdx.x) earlier += x;
+        earlier += b < blockIdx.x ? x : 0;
     }
-    base[d] = sum_before(all, wave_sums) + earlier;
     uint32_t key[kSortItems], token[kSortItems], digit[kSortItems];
     bool on[kSortItems];
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
-        const uint32_t t = blockIdx.x * kTile + wave * (64 * kSortItems) + k * 64 + lane;
+        const uint32_t t = begin + wave * (64 * kSortItems) + k * 64 + lane;
         on[k] = t < a.n;
         key[k] = on[k] ? key_at(a, t) : 0;
         token[k] = on[k] && a.tokens != nullptr ? a.tokens[t] : t;
-        digit[k] = key[k] >> a.shift & (kDigits - 1);
+        digit[k] = key[k] >> a.shift & ((1u << a.digit_bits) - 1);
     }
-    Places p;
-    rank_tile(digit, on, used, p);
+    uint32_t rank[kSortItems];
+    rank_tile(digit, on, used, rank, a.digit_bits);
+    base[d] = sum_before<kSortWaves>(all, wave_sums) + earlier;
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         if (!on[k]) continue;
-        const uint32_t at = base[digit[k]] + used[wave][digit[k]] + p.rank[k];
+        const uint32_t at = base[digit[k]] + used[wave][digit[k]] + rank[k];
         a.keys_out[at] = key[k];
         a.tokens_out[at] = token[k];
     }
 }
 
-// All passes over one tile, in LDS.
-__global__ __launch_bounds__(kSortBlock) void sort_tile_kernel(SortArgs a, int32_t bits) {
+// All passes over a list of at most WAVES * 64 * ITEMS tokens by one
+// work-group, in LDS.
+template <int WAVES, int ITEMS>
+__global__ __launch_bounds__(WAVES * 64) void sort_whole_kernel(SortArgs a, int32_t bits) {
+    constexpr int kMost = WAVES * 64 * ITEMS;
+    static_assert(kMost <= 65536 && WAVES * 64 >= kDigits, "16-bit places, a thread a digit");
     if (blockIdx.x >= 1) return clear(a, 1);
-    __shared__ uint32_t used[kSortWaves][kDigits], base[kDigits], wave_sums[kSortWaves], keys[kTile], tokens[kTile];
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    uint32_t key[kSortItems], token[kSortItems], digit[kSortItems];
-    bool on[kSortItems];
+    __shared__ uint32_t keys[kMost], base[kDigits], wave_sums[WAVES];
+    __shared__ uint16_t used[WAVES][kDigits], tokens[kMost];
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, begin = wave * (64 * ITEMS) + lane;
+    uint32_t key[ITEMS], digit[ITEMS], rank[ITEMS];
+    uint16_t token[ITEMS];
+    bool on[ITEMS];
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const uint32_t t = wave * (64 * kSortItems) + k * 64 + lane;
+    for (int k = 0; k < ITEMS; ++k) {
+        const uint32_t t = begin + k * 64;
         on[k] = t < a.n;
         key[k] = on[k] ? key_at(a, t) : 0;
-        token[k] = t;
+        token[k] = static_cast<uint16_t>(t);
     }
-    for (int32_t shift = 0; shift < bits; shift += kDigitBits) {
+    for (int32_t shift = 0; shift < bits; shift += a.digit_bits) {
 #pragma unroll
-        for (int k = 0; k < kSortItems; ++k) digit[k] = key[k] >> shift & (kDigits - 1);
-        Places p;
-        const uint32_t sum = rank_tile(digit, on, used, p);
-        base[threadIdx.x] = sum_before(sum, wave_sums);
+        for (int k = 0; k < ITEMS; ++k) digit[k] = key[k] >> shift & ((1u << a.digit_bits) - 1);
+        const uint32_t sum = rank_tile(digit, on, used, rank, a.digit_bits);
+        const uint32_t before = sum_before<WAVES>(sum, wave_sums);
+        if (threadIdx.x < kDigits) base[threadIdx.x] = before;
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kSortItems; ++k) {
+        for (int k = 0; k < ITEMS; ++k) {
             if (!on[k]) continue;
-            const uint32_t at = base[digit[k]] + used[wave][digit[k]] + p.rank[k];
+            const uint32_t at = base[digit[k]] + used[wave][digit[k]] + rank[k];
             keys[at] = key[k];
             tokens[at] = token[k];
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kSortItems; ++k) {
-            const uint32_t t = wave * (64 * kSortItems) + k * 64 + lane;
-            if (on[k]) key[k] = keys[t], token[k] = tokens[t];
-        }
+        for (int k = 0; k < ITEMS; ++k)
+            if (on[k]) key[k] = keys[begin + k * 64], token[k] = tokens[begin + k * 64];
         __syncthreads();
     }
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const uint32_t t = wave * (64 * kSortItems) + k * 64 + lane;
-        if (on[k]) a.keys_out[t] = key[k], a.tokens_out[t] = token[k];
-    }
+    for (int k = 0; k < ITEMS; ++k)
+        if (on[k]) a.keys_out[begin + k * 64] = key[k], a.tokens_out[begin + k * 64] = token[k];
 }
 
 struct SumArgs {
@@ -364,7 +372,7 @@ struct SumArgs {
 // at once.  WIDE: a wave has one piece, so that its keys are scalars.
 template <typename TG, typename TW, bool WIDE>
 __global__ __launch_bounds__(kBlock) void sum_pieces_kernel(SumArgs a) {
-    constexpr int N = 16 / (sizeof(TG) > sizeof(TW) ? sizeof(TG) : sizeof(TW)), kAhead = 8;
+    constexpr int N = 16 / (sizeof(TG) > sizeof(TW) ? sizeof(TG) : sizeof(TW)), kAhead = 4;
     const uint32_t pb = blockIdx.x / a.chunks, cb = blockIdx.x - pb * a.chunks;
     uint32_t piece = pb * (kBlock >> a.shift) + (threadIdx.x >> a.shift);
     if constexpr (WIDE) piece = __builtin_amdgcn_readfirstlane(piece);
@@ -385,7 +393,7 @@ __global__ __launch_bounds__(kBlock) void sum_pieces_kernel(SumArgs a) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             if (i + u >= last || key[u] == none) continue;
-            v[u] = load_raw<TG, N>(static_cast<const TG*>(a.grad_out) + static_cast<int64_t>(a.tokens[i + u]) * a.width + c, left);
+            v[u] = load_raw<TG, N, true>(static_cast<const TG*>(a.grad_out) + static_cast<int64_t>(a.tokens[i + u]) * a.width + c, left);
             if (a.accumulate && key[u + 1] != key[u])
                 old[u] = load_raw<TW, N>(static_cast<const TW*>(a.grad) + static_cast<int64_t>(key[u]) * a.width + c, left);
         }
@@ -437,8 +445,18 @@ __global__ __launch_bounds__(kBlock) void join_pieces_kernel(SumArgs a) {
     if (left > 0) {
         const float* at = a.partials + static_cast<int64_t>(piece + 1) * 2 * a.width + c;
         if (wave == 0) load_some<N>(sum, at - a.width, left);
-#pragma unroll 8
-        for (uint32_t q = wave; q < more; q += kWaves) {
+        constexpr uint32_t kAhead = 8;
+        uint32_t q = wave;
+        for (; left >= N && q + (kAhead - 1) * kWaves < more; q += kAhead * kWaves) {
+            float v[kAhead][N];
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u) load<N>(v[u], at + static_cast<int64_t>(q + u * kWaves) * 2 * a.width);
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u)
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum[j] += v[u][j];
+        }
+        for (; q < more; q += kWaves) {
             float v[N];
             load_some<N>(v, at + static_cast<int64_t>(q) * 2 * a.width, left);
 #pragma unroll
@@ -467,8 +485,23 @@ bool by_row(int64_t n, int64_t rows) {
     return n >= (int64_t{1} << 30) || rows >= (int64_t{1} << 31) || n == 0 || rows <= kByRowWork / n;
 }
 
-// Sorted positions per piece: enough pieces to fill the chip, long ones otherwise.
-uint32_t piece_for(int64_t n) { return n <= 32768 ? 16 : 64; }
+// Up to here one work-group sorts the whole list: at 8,183 tokens that takes
+// 23 us, beside the clearing, where the two launches of each of two passes take
+// 29; at 16,384, with 16 elements a thread, 44 us against 29.
+constexpr int64_t kSortWhole = 8192;
+
+// Sorted positions per piece, a power of two from 8 to 64: about 8,192 waves'
+// pieces, all that fit the chip at once.  Short pieces give the sums more waves,
+// long ones the joining less to do; sums and joining, traced, in us, by the
+// tokens of a piece:        4            8            16           32           64
+//   8,183 tokens of 768     10.0 + 12.7  13.2 + 7.7   14.2 + 5.3
+//   16,384 tokens of 4,096                            56.7 + 13.6  67.8 + 8.9   98.2 + 6.6
+uint32_t piece_for(int64_t n, int64_t width) {
+    const int64_t most = n * ((width + 511) / 512) / 8192;
+    uint32_t p = 8;
+    while (p < 64 && p < most) p *= 2;
+    return p;
+}
 
 struct Work {
     int64_t counts, keys[2], tokens[2], partials, bytes;
@@ -480,7 +513,8 @@ Work work_of(int64_t n, int64_t width) {
     w.keys[0] = up(4 * tiles * kDigits);
     w.tokens[0] = w.keys[0] + list, w.keys[1] = w.tokens[0] + list, w.tokens[1] = w.keys[1] + list;
     w.partials = w.tokens[1] + list;
-    w.bytes = w.partials + (n + piece_for(n) - 1) / piece_for(n) * 2 * width * 4;
+    const int64_t piece = piece_for(n, width);
+    w.bytes = w.partials + (n + piece - 1) / piece * 2 * width * 4;
     return w;
 }
 
@@ -573,33 +607,45 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
             const auto list = [&](int64_t offset) { return reinterpret_cast<uint32_t*>(at + offset); };
             const uint32_t tiles = static_cast<uint32_t>((n + kTile - 1) / kTile);
             SortArgs o{ids_dev, nullptr, nullptr, nullptr, nullptr, list(work.counts), rows, padding_idx, static_cast<uint32_t>(n),
-                       tiles, id_bytes, 0, static_cast<char*>(grad_dev), 0};
-            // a gradient that is written whole is cleared beside the first pass, which leaves most of the chip idle
-            uint32_t clearing = 0;
-            if (!accumulate) {
-                o.zero_bytes = rows * width * static_cast<int64_t>(sizeof(TW));
-                clearing = static_cast<uint32_t>(std::min<int64_t>((o.zero_bytes + 16 * kSortBlock - 1) / (16 * kSortBlock), 2048));
-            }
+                       tiles, id_bytes, 0, 0, nullptr, 0};
             int32_t bits = 1;
             while (rows >> bits) ++bits;  // of the largest key, `rows`
+            const int passes = (bits + kDigitBits - 1) / kDigitBits;
+            o.digit_bits = (bits + passes - 1) / passes;
+            const bool whole = n <= kSortWhole;
+            const int launches = whole ? 1 : 2 * passes;
+            // a gradient that is written whole is cleared beside the sort, which leaves most of the chip idle: a share
+            // with each launch, by the work-groups past the tiles
+            int64_t dirty = accumulate ? 0 : rows * width * static_cast<int64_t>(sizeof(TW));
+            const int64_t share = (dirty / launches + 15) / 16 * 16;
+            const auto clearing = [&](bool rest) {
+                if (o.zeros != nullptr) o.zeros += o.zero_bytes;
+                else o.zeros = static_cast<char*>(grad_dev);
+                o.zero_bytes = rest ? dirty : std::min(share, dirty);
+                dirty -= o.zero_bytes;
+                return static_cast<uint32_t>(std::min<int64_t>((o.zero_bytes + 16 * kSortBlock - 1) / (16 * kSortBlock), 2048));
+            };
             int side = 0;
-            if (tiles == 1) {
+            if (whole) {
                 o.keys_out = list(work.keys[0]), o.tokens_out = list(work.tokens[0]);
-                hipLaunchKernelGGL(sort_tile_kernel, dim3(1 + clearing), dim3(kSortBlock), 0, s, o, bits);
-                if (int rc = launched("sort_tile_kernel")) return rc;
+                const dim3 grid(1 + clearing(true));
+                if (n <= 2048) hipLaunchKernelGGL((sort_whole_kernel<8, 4>), grid, dim3(512), 0, s, o, bits);
+                else hipLaunchKernelGGL((sort_whole_kernel<16, 8>), grid, dim3(1024), 0, s, o, bits);
+                if (int rc = launched("sort_whole_kernel")) return rc;
                 side = 1;
             } else {
-                for (o.shift = 0; o.shift < bits; o.shift += kDigitBits, side ^= 1, clearing = 0) {
+                for (o.shift = 0; o.shift < bits; o.shift += o.digit_bits, side ^= 1) {
                     o.keys_out = list(work.keys[side]), o.tokens_out = list(work.tokens[side]);
-                    hipLaunchKernelGGL(count_kernel, dim3(tiles + clearing), dim3(kSortBlock), 0, s, o);
+                    hipLaunchKernelGGL(count_kernel, dim3(tiles + clearing(false)), dim3(kSortBlock), 0, s, o);
                     if (int rc = launched("count_kernel")) return rc;
-                    hipLaunchKernelGGL(place_kernel, dim3(tiles), dim3(kSortBlock), 0, s, o);
+                    const dim3 grid(tiles + clearing(o.shift + o.digit_bits >= bits));
+                    hipLaunchKernelGGL(place_kernel, grid, dim3(kSortBlock), 0, s, o);
                     if (int rc = launched("place_kernel")) return rc;
                     o.keys = o.keys_out, o.tokens = o.tokens_out;
                 }
             }
             SumArgs m{list(work.keys[side ^ 1]), list(work.tokens[side ^ 1]), grad_out_dev, grad_dev,
-                      reinterpret_cast<float*>(at + work.partials), rows, width, static_cast<uint32_t>(n), piece_for(n), 0, shift,
+                      reinterpret_cast<float*>(at + work.partials), rows, width, static_cast<uint32_t>(n), piece_for(n, width), 0, shift,
                       static_cast<uint32_t>(chunks), accumulate, scale};
             m.pieces = static_cast<uint32_t>((n + m.piece - 1) / m.piece);
             const int64_t per_block = kBlock >> shift, blocks = (m.pieces + per_block - 1) / per_block * chunks;

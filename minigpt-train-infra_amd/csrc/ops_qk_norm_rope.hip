@@ -28,14 +28,16 @@ namespace {
 constexpr int kRopeBlock = 256;
 constexpr int kWaves = kRopeBlock / 64;
 constexpr int kMaxDim = MGOPT_MAX_HEAD_DIM;
-constexpr uint32_t kBackwardBlocks = 1024;  // work-groups of the backward pass at most: rows of partial weight gradients
+constexpr uint32_t kBackwardBlocks = 2048;  // work-groups of the backward pass at most, a row of partial weight gradients each
 
 struct Args {
     mgopt_qk_args a;
     uint32_t tokens;
     uint32_t lanes;   // of a head: a power of two
     uint32_t parts;   // waves that share a token's heads
-    float* partials;  // backward: [work-groups][2][dim]
+    // backward
+    uint32_t q_parts, k_parts, q_blocks;
+    float* partials;  // [work-groups][dim]
 };
 
 // x summed over aligned groups of `lanes` lanes, in each of them.
@@ -191,118 +193,122 @@ __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_kernel(Args k) {
     heads(k.a.k, first_k);
 }
 
+// The first q_blocks work-groups take the queries' heads, the others the keys':
+// one side's weights and sums are all that a lane holds, which leaves registers
+// for four waves a SIMD (8,192 tokens of 32 + 8 heads of 128 in bf16: 50 us, with
+// both sides' in one wave, 185 registers, 62).
 template <typename T, int VEC, int SLOTS, bool INTER>
-__global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_backward_kernel(Args k) {
-    const uint32_t lane = threadIdx.x % 64, l = lane & (k.lanes - 1), groups = 64 / k.lanes, step = groups * k.parts;
+__global__ __launch_bounds__(kRopeBlock, 4) void qk_norm_rope_backward_kernel(Args k) {
+    const bool on_q = blockIdx.x < k.q_blocks;
+    const mgopt_heads& side = on_q ? k.a.q : k.a.k;
+    const uint32_t block = on_q ? blockIdx.x : blockIdx.x - k.q_blocks, blocks = on_q ? k.q_blocks : gridDim.x - k.q_blocks;
+    const uint32_t heads = static_cast<uint32_t>(side.heads);
+    const uint32_t lane = threadIdx.x % 64, l = lane & (k.lanes - 1), groups = 64 / k.lanes;
+    const uint32_t parts = on_q ? k.q_parts : k.k_parts, step = groups * parts;
     const float inv_dim = 1.0f / static_cast<float>(k.a.dim);
     Slot q[SLOTS];
-    Pairs<VEC, INTER> w[2][SLOTS], sum_w[2][SLOTS];
+    Pairs<VEC, INTER> w[SLOTS], sum_w[SLOTS];
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
         q[i] = slot_of<VEC, INTER>(l + i * k.lanes, k.a.dim, k.a.rotary);
-        if (q[i].on) {
-            w[0][i].read_weights(k.a.q.weight_dev, k.a.weight_dtype, q[i]);
-            w[1][i].read_weights(k.a.k.weight_dev, k.a.weight_dtype, q[i]);
-        }
+        if (q[i].on) w[i].read_weights(side.weight_dev, k.a.weight_dtype, q[i]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            sum_w[0][i].a[j] = sum_w[0][i].b[j] = sum_w[1][i].a[j] = sum_w[1][i].b[j] = 0.0f;
+        for (int j = 0; j < VEC; ++j) sum_w[i].a[j] = sum_w[i].b[j] = 0.0f;
     }
-    const uint64_t tasks = static_cast<uint64_t>(k.tokens) * k.parts;
-    for (uint64_t task = static_cast<uint64_t>(blockIdx.x) * kWaves + threadIdx.x / 64; task < tasks;
-         task += static_cast<uint64_t>(gridDim.x) * kWaves) {
-        const uint32_t n = static_cast<uint32_t>(task / k.parts), part = static_cast<uint32_t>(task - static_cast<uint64_t>(n) * k.parts);
+    const uint64_t tasks = static_cast<uint64_t>(k.tokens) * parts;
+    for (uint64_t task = static_cast<uint64_t>(block) * kWaves + threadIdx.x / 64; task < tasks;
+         task += static_cast<uint64_t>(blocks) * kWaves) {
+        const uint32_t n = static_cast<uint32_t>(task / parts), part = static_cast<uint32_t>(task - static_cast<uint64_t>(n) * parts);
         const Token t = token_of(k, n);
         float c[SLOTS][VEC], d[SLOTS][VEC];
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) angles<VEC>(k, q[i], l + i * k.lanes, t.pos, c[i], d[i]);
-        auto heads = [&](const mgopt_heads& side, const Pairs<VEC, INTER>(&w)[SLOTS], Pairs<VEC, INTER>(&sum_w)[SLOTS],
-                         uint32_t h) {
-            for (; h < static_cast<uint32_t>(side.heads); h += step) {
-                const T* x = static_cast<const T*>(side.x_dev) + offset(side.x_stride, t, h);
-                const T* grad = static_cast<const T*>(side.grad_dev) + offset(side.grad_stride, t, h);
-                T* dx = static_cast<T*>(side.d_x_dev) + offset(side.d_x_stride, t, h);
-                Pairs<VEC, INTER> v[SLOTS], g[SLOTS];
-                float sum = 0.0f, dot = 0.0f;
+        for (uint32_t h = part * groups + lane / k.lanes; h < heads; h += step) {
+            const T* x = static_cast<const T*>(side.x_dev) + offset(side.x_stride, t, h);
+            const T* grad = static_cast<const T*>(side.grad_dev) + offset(side.grad_stride, t, h);
+            T* dx = static_cast<T*>(side.d_x_dev) + offset(side.d_x_stride, t, h);
+            Pairs<VEC, INTER> v[SLOTS], g[SLOTS];
+            float sum = 0.0f, dot = 0.0f;
 #pragma unroll
-                for (int i = 0; i < SLOTS; ++i) {
-                    if (!q[i].on) continue;
-                    v[i].read(x, q[i]);
-                    g[i].read(grad, q[i]);
+            for (int i = 0; i < SLOTS; ++i) {
+                if (!q[i].on) continue;
+                v[i].read(x, q[i]);
+                g[i].read(grad, q[i]);
+            }
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const float a = g[i].a[j], b = g[i].b[j];
-                        g[i].a[j] = fmaf(a, c[i][j], b * d[i][j]);
-                        g[i].b[j] = fmaf(b, c[i][j], -a * d[i][j]);
-                        sum = fmaf(v[i].a[j], v[i].a[j], fmaf(v[i].b[j], v[i].b[j], sum));
-                        dot = fmaf(g[i].a[j] * w[i].a[j], v[i].a[j], fmaf(g[i].b[j] * w[i].b[j], v[i].b[j], dot));
-                    }
-                }
-                const float r = 1.0f / sqrtf(fmaf(sum_group(sum, k.lanes), inv_dim, k.a.eps));
-                const float m = sum_group(dot, k.lanes) * r * inv_dim;  // mean(h * xhat)
+            for (int i = 0; i < SLOTS; ++i) {
+                if (!q[i].on) continue;
 #pragma unroll
-                for (int i = 0; i < SLOTS; ++i) {
-                    if (!q[i].on) continue;
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const float xa = v[i].a[j] * r, xb = v[i].b[j] * r;
-                        sum_w[i].a[j] = fmaf(g[i].a[j], xa, sum_w[i].a[j]);
-                        sum_w[i].b[j] = fmaf(g[i].b[j], xb, sum_w[i].b[j]);
-                        v[i].a[j] = r * fmaf(-xa, m, g[i].a[j] * w[i].a[j]);
-                        v[i].b[j] = r * fmaf(-xb, m, g[i].b[j] * w[i].b[j]);
-                    }
-                    v[i].write(dx, q[i]);
+                for (int j = 0; j < VEC; ++j) {
+                    const float a = g[i].a[j], b = g[i].b[j];
+                    g[i].a[j] = fmaf(a, c[i][j], b * d[i][j]);
+                    g[i].b[j] = fmaf(b, c[i][j], -a * d[i][j]);
+                    sum = fmaf(v[i].a[j], v[i].a[j], fmaf(v[i].b[j], v[i].b[j], sum));
+                    dot = fmaf(g[i].a[j] * w[i].a[j], v[i].a[j], fmaf(g[i].b[j] * w[i].b[j], v[i].b[j], dot));
                 }
             }
-            return h - static_cast<uint32_t>(side.heads);
-        };
-        const uint32_t first_k = heads(k.a.q, w[0], sum_w[0], part * groups + lane / k.lanes);
-        heads(k.a.k, w[1], sum_w[1], first_k);
+            const float r = 1.0f / sqrtf(fmaf(sum_group(sum, k.lanes), inv_dim, k.a.eps));
+            const float m = sum_group(dot, k.lanes) * r * inv_dim;  // mean(h * xhat)
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) {
+                if (!q[i].on) continue;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float xa = v[i].a[j] * r, xb = v[i].b[j] * r;
+                    sum_w[i].a[j] = fmaf(g[i].a[j], xa, sum_w[i].a[j]);
+                    sum_w[i].b[j] = fmaf(g[i].b[j], xb, sum_w[i].b[j]);
+                    v[i].a[j] = r * fmaf(-xa, m, g[i].a[j] * w[i].a[j]);
+                    v[i].b[j] = r * fmaf(-xb, m, g[i].b[j] * w[i].b[j]);
+                }
+                v[i].write(dx, q[i]);
+            }
+        }
     }
     // over the groups of a wave, then over the work-group's waves
-    __shared__ float part[kWaves][2][kMaxDim];
+    __shared__ float part[kWaves][kMaxDim];
 #pragma unroll
-    for (int side = 0; side < 2; ++side)
+    for (int i = 0; i < SLOTS; ++i) {
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                for (uint32_t off = k.lanes; off < 64; off <<= 1) {
-                    sum_w[side][i].a[j] += __shfl_xor(sum_w[side][i].a[j], off);
-                    sum_w[side][i].b[j] += __shfl_xor(sum_w[side][i].b[j], off);
-                }
-            if (lane < k.lanes && q[i].on) sum_w[side][i].write(&part[threadIdx.x / 64][side][0], q[i]);
-        }
+        for (int j = 0; j < VEC; ++j)
+            for (uint32_t off = k.lanes; off < 64; off <<= 1) {
+                sum_w[i].a[j] += __shfl_xor(sum_w[i].a[j], off);
+                sum_w[i].b[j] += __shfl_xor(sum_w[i].b[j], off);
+            }
+        if (lane < k.lanes && q[i].on) sum_w[i].write(&part[threadIdx.x / 64][0], q[i]);
+    }
     __syncthreads();
-    for (int at = threadIdx.x; at < 2 * k.a.dim; at += kRopeBlock) {
-        const int side = at >= k.a.dim, e = at - side * k.a.dim;
+    for (int e = threadIdx.x; e < k.a.dim; e += kRopeBlock) {
         float x = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) x += part[v][side][e];
-        k.partials[(static_cast<int64_t>(blockIdx.x) * 2 + side) * k.a.dim + e] = x;
+        for (int v = 0; v < kWaves; ++v) x += part[v][e];
+        k.partials[static_cast<int64_t>(blockIdx.x) * k.a.dim + e] = x;
     }
 }
 
-// Sums `rows` rows of partial weight gradients of 2 * dim columns: a work-group
-// takes kCols columns, its threads rows in turn, joined in a fixed order.
+// Sums the rows of partial weight gradients, the first q_rows of them the
+// queries': work-group (c, s) takes kCols columns of side s, its threads rows in
+// turn, joined in a fixed order.
 constexpr int kCols = 16, kSumBlock = 1024;
-__global__ __launch_bounds__(kSumBlock) void weight_grad_kernel(const float* partials, uint32_t rows, int32_t dim, void* dq,
-                                                                void* dk, int32_t dtype) {
+__global__ __launch_bounds__(kSumBlock) void weight_grad_kernel(const float* partials, uint32_t q_rows, uint32_t k_rows,
+                                                                int32_t dim, void* dq, void* dk, int32_t dtype) {
     __shared__ float part[kSumBlock / kCols][kCols + 1];
-    const int col = threadIdx.x % kCols, row = threadIdx.x / kCols, at = blockIdx.x * kCols + col;
+    const int col = threadIdx.x % kCols, row = threadIdx.x / kCols, e = blockIdx.x * kCols + col;
+    const uint32_t rows = blockIdx.y == 0 ? q_rows : k_rows;
+    const float* at = partials + (blockIdx.y == 0 ? 0 : static_cast<int64_t>(q_rows) * dim) + e;
     float x = 0.0f;
-    if (at < 2 * dim)
-        for (uint32_t r = row; r < rows; r += kSumBlock / kCols) x += partials[static_cast<int64_t>(r) * 2 * dim + at];
+    if (e < dim) {
+#pragma unroll 8
+        for (uint32_t r = row; r < rows; r += kSumBlock / kCols) x += at[static_cast<int64_t>(r) * dim];
+    }
     part[row][col] = x;
     __syncthreads();
     for (int half = kSumBlock / kCols / 2; half > 0; half /= 2) {
         if (row < half) part[row][col] += part[row + half][col];
         __syncthreads();
     }
-    if (row != 0 || at >= 2 * dim) return;
+    if (row != 0 || e >= dim) return;
     x = part[0][col];
-    void* out = at < dim ? dq : dk;
-    const int e = at < dim ? at : at - dim;
+    void* out = blockIdx.y == 0 ? dq : dk;
     if (dtype == MGOPT_F32) static_cast<float*>(out)[e] = x;
     else if (dtype == MGOPT_F16) static_cast<_Float16*>(out)[e] = static_cast<_Float16>(x);
     else static_cast<__bf16*>(out)[e] = static_cast<__bf16>(x);
@@ -330,29 +336,37 @@ int check(const mgopt_qk_args* a, const char* what) {
 }
 
 // The kernel's form for these sizes: 16 bytes (VEC elements) of each half of the pairs per lane where
-// the head and its rotated part are made of such; else 4 elements; else single ones.
-template <typename F>
+// the head and its rotated part are made of such; else 4 elements; else single ones.  Interleaved pairs
+// of 8 elements do not fit the backward pass's registers at four waves a SIMD (40 of them spill), 4 do.
+template <bool BACKWARD, typename F>
 int with_form(const mgopt_qk_args& a, Args& k, F&& f) {
     auto shape = [&](int vec, int slots) {
         const int pieces = (a.dim + 2 * vec - 1) / (2 * vec);
         k.lanes = 1;
         while (static_cast<int>(k.lanes) * slots < pieces) k.lanes <<= 1;
         // waves that share a token's heads, while that leaves the chip's 1,024 SIMDs idle and a wave's groups have heads
-        const int64_t heads = a.q.heads + a.k.heads, groups = 64 / k.lanes;
-        k.parts = 1;
-        while (k.parts * groups < heads && static_cast<int64_t>(k.tokens) * k.parts < 4096) ++k.parts;
+        const int64_t groups = 64 / k.lanes;
+        const auto share = [&](int64_t heads) {
+            uint32_t parts = 1;
+            while (parts * groups < heads && static_cast<int64_t>(k.tokens) * parts < 4096) ++parts;
+            return parts;
+        };
+        k.parts = share(a.q.heads + a.k.heads);
+        k.q_parts = share(a.q.heads), k.k_parts = share(a.k.heads);
     };
     return with_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
         auto inter = [&](auto vec, auto slots) {
             constexpr int VEC = decltype(vec)::value, SLOTS = decltype(slots)::value;
             shape(VEC, SLOTS);
-            return a.interleaved ? f(T{}, vec, slots, std::true_type{}) : f(T{}, vec, slots, std::false_type{});
+            if constexpr (!BACKWARD || VEC < 8)
+                if (a.interleaved) return f(T{}, vec, slots, std::true_type{});
+            return f(T{}, vec, slots, std::false_type{});
         };
         auto both = [&](int n) { return a.dim % (2 * n) == 0 && a.rotary % (2 * n) == 0; };
         using One = std::integral_constant<int, 1>;
         if constexpr (sizeof(T) == 2)
-            if (both(8)) return inter(std::integral_constant<int, 8>{}, One{});
+            if (both(8) && !(BACKWARD && a.interleaved)) return inter(std::integral_constant<int, 8>{}, One{});
         if (both(4)) return inter(std::integral_constant<int, 4>{}, One{});
         if (a.dim <= 128) return inter(One{}, One{});
         return inter(One{}, std::integral_constant<int, 4>{});
@@ -374,7 +388,7 @@ MGOPT_API int mgopt_qk_norm_rope(const mgopt_qk_args* a, void* stream) {
     Args k{};
     k.a = *a;
     k.tokens = static_cast<uint32_t>(a->batch * a->length);
-    return with_form(*a, k, [&](auto t, auto vec, auto slots, auto inter) {
+    return with_form<false>(*a, k, [&](auto t, auto vec, auto slots, auto inter) {
         using T = decltype(t);
         const uint32_t blocks = static_cast<uint32_t>((static_cast<uint64_t>(k.tokens) * k.parts + kWaves - 1) / kWaves);
         hipLaunchKernelGGL((qk_norm_rope_kernel<T, decltype(vec)::value, decltype(slots)::value, decltype(inter)::value>),
@@ -384,7 +398,7 @@ MGOPT_API int mgopt_qk_norm_rope(const mgopt_qk_args* a, void* stream) {
 }
 
 MGOPT_API int64_t mgopt_qk_norm_rope_workspace(int32_t dim) {
-    return dim < 1 ? -1 : int64_t{kBackwardBlocks} * 2 * dim * static_cast<int64_t>(sizeof(float));
+    return dim < 1 ? -1 : int64_t{kBackwardBlocks} * dim * static_cast<int64_t>(sizeof(float));
 }
 
 MGOPT_API int mgopt_qk_norm_rope_backward(const mgopt_qk_args* a, void* stream) {
@@ -401,20 +415,27 @@ MGOPT_API int mgopt_qk_norm_rope_backward(const mgopt_qk_args* a, void* stream) 
     k.a = *a;
     k.tokens = static_cast<uint32_t>(a->batch * a->length);
     k.partials = static_cast<float*>(a->workspace_dev);
-    uint32_t blocks = 0;
+    uint32_t k_blocks = 0;
     if (k.tokens > 0) {
-        const int rc = with_form(*a, k, [&](auto t, auto vec, auto slots, auto inter) {
+        const int rc = with_form<true>(*a, k, [&](auto t, auto vec, auto slots, auto inter) {
             using T = decltype(t);
-            const uint64_t waves = static_cast<uint64_t>(k.tokens) * k.parts;
-            blocks = static_cast<uint32_t>(std::min<uint64_t>((waves + kWaves - 1) / kWaves, kBackwardBlocks));
+            // work-groups by the sides' shares of the heads, each no more than it has waves' work for
+            const auto blocks_for = [&](uint32_t parts, uint32_t share) {
+                const uint64_t waves = static_cast<uint64_t>(k.tokens) * parts;
+                return static_cast<uint32_t>(std::min<uint64_t>((waves + kWaves - 1) / kWaves, share));
+            };
+            const uint32_t k_share = std::max<uint32_t>(
+                1, static_cast<uint32_t>(static_cast<uint64_t>(kBackwardBlocks) * a->k.heads / (a->q.heads + a->k.heads)));
+            k.q_blocks = blocks_for(k.q_parts, kBackwardBlocks - k_share);
+            k_blocks = blocks_for(k.k_parts, k_share);
             hipLaunchKernelGGL((qk_norm_rope_backward_kernel<T, decltype(vec)::value, decltype(slots)::value, decltype(inter)::value>),
-                               dim3(blocks), dim3(kRopeBlock), 0, s, k);
+                               dim3(k.q_blocks + k_blocks), dim3(kRopeBlock), 0, s, k);
             return launched("qk_norm_rope_backward_kernel");
         });
         if (rc) return rc;
     }
-    hipLaunchKernelGGL(weight_grad_kernel, dim3((2 * a->dim + kCols - 1) / kCols), dim3(kSumBlock), 0, s, k.partials, blocks,
-                       a->dim, a->q.d_weight_dev, a->k.d_weight_dev, a->weight_dtype);
+    hipLaunchKernelGGL(weight_grad_kernel, dim3((a->dim + kCols - 1) / kCols, 2), dim3(kSumBlock), 0, s, k.partials,
+                       k.q_blocks, k_blocks, a->dim, a->q.d_weight_dev, a->k.d_weight_dev, a->weight_dtype);
     return launched("weight_grad_kernel");
 }
 
