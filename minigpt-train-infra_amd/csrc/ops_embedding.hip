@@ -167,7 +167,7 @@ __global__ __launch_bounds__(kBlock) void grad_by_row_kernel(GradArgs a) {
 // its tile.  Ids that name no row, and the padding's, become the key `rows`
 // and end up last.
 
-constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;  // at most
 constexpr int kSortBlock = 512, kSortItems = 4, kTile = kSortBlock * kSortItems, kSortWaves = kSortBlock / 64;
 static_assert(kSortBlock == kDigits, "a thread a digit");
 
@@ -178,7 +178,7 @@ struct SortArgs {
     uint32_t* counts;          // [tiles][kDigits]
     int64_t rows, padding;
     uint32_t n, tiles;
-    int32_t id_bytes, shift, digit_bits;  // the digit's lowest bit and its length
+    int32_t id_bytes, shift;   // the digit's lowest bit
     char* zeros;               // what the work-groups past the tiles clear: a multiple of 16 bytes but in the last launch
     int64_t zero_bytes;
 };
@@ -198,6 +198,7 @@ __device__ __forceinline__ void clear(const SortArgs& a, uint32_t first) {
     for (; i < vecs; i += step) reinterpret_cast<vec_t<uint16_t, 8>*>(a.zeros)[i] = zero;
 }
 
+template <int BITS>
 __global__ __launch_bounds__(kSortBlock) void count_kernel(SortArgs a) {
     if (blockIdx.x >= a.tiles) return clear(a, a.tiles);
     __shared__ uint32_t count[kDigits];
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(kSortBlock) void count_kernel(SortArgs a) {
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const uint32_t t = blockIdx.x * kTile + k * kSortBlock + threadIdx.x;
-        if (t < a.n) atomicAdd(&count[key_at(a, t) >> a.shift & ((1u << a.digit_bits) - 1)], 1u);
+        if (t < a.n) atomicAdd(&count[key_at(a, t) >> a.shift & ((1u << BITS) - 1)], 1u);
     }
     __syncthreads();
     a.counts[static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = count[threadIdx.x];
@@ -235,16 +236,17 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* wave_sums) 
 // digit before it in its wave, used[w][d] becomes the number of digit d in the
 // waves before w, and thread d's return value the number in the tile.  The
 // lanes of one digit are found by a vote per bit.
-template <int WAVES, int ITEMS>
+template <int BITS, int WAVES, int ITEMS>
 __device__ __forceinline__ uint32_t rank_tile(const uint32_t (&digit)[ITEMS], const bool (&on)[ITEMS],
-                                              uint16_t (&used)[WAVES][kDigits], uint32_t (&rank)[ITEMS], int digit_bits) {
+                                              uint16_t (&used)[WAVES][kDigits], uint32_t (&rank)[ITEMS]) {
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     for (uint32_t i = threadIdx.x; i < WAVES * kDigits / 2; i += WAVES * 64) reinterpret_cast<uint32_t*>(used)[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         uint64_t same = __ballot(on[k]);
-        for (int bit = 0; bit < digit_bits; ++bit) {
+#pragma unroll
+        for (int bit = 0; bit < BITS; ++bit) {
             const bool b = digit[k] >> bit & 1u;
             const uint64_t vote = __ballot(b);
             same &= b ? vote : ~vote;
@@ -272,6 +274,7 @@ __device__ __forceinline__ uint32_t rank_tile(const uint32_t (&digit)[ITEMS], co
     return sum;
 }
 
+template <int BITS>
 __global__ __launch_bounds__(kSortBlock) void place_kernel(SortArgs a) {
     if (blockIdx.x >= a.tiles) return clear(a, a.tiles);
     __shared__ uint16_t used[kSortWaves][kDigits];
@@ -292,10 +295,10 @@ __global__ __launch_bounds__(kSortBlock) void place_kernel(SortArgs a) {
         on[k] = t < a.n;
         key[k] = on[k] ? key_at(a, t) : 0;
         token[k] = on[k] && a.tokens != nullptr ? a.tokens[t] : t;
-        digit[k] = key[k] >> a.shift & ((1u << a.digit_bits) - 1);
+        digit[k] = key[k] >> a.shift & ((1u << BITS) - 1);
     }
     uint32_t rank[kSortItems];
-    rank_tile(digit, on, used, rank, a.digit_bits);
+    rank_tile<BITS>(digit, on, used, rank);
     base[d] = sum_before<kSortWaves>(all, wave_sums) + earlier;
     __syncthreads();
 #pragma unroll
@@ -308,48 +311,52 @@ __global__ __launch_bounds__(kSortBlock) void place_kernel(SortArgs a) {
 }
 
 // All passes over a list of at most WAVES * 64 * ITEMS tokens by one
-// work-group, in LDS.
-template <int WAVES, int ITEMS>
+// work-group, in LDS.  A key and its token share 32 bits: random accesses to the
+// LDS are what bounds it.
+constexpr int kWholeKeyBits = 19;
+template <int BITS, int WAVES, int ITEMS>
 __global__ __launch_bounds__(WAVES * 64) void sort_whole_kernel(SortArgs a, int32_t bits) {
     constexpr int kMost = WAVES * 64 * ITEMS;
-    static_assert(kMost <= 65536 && WAVES * 64 >= kDigits, "16-bit places, a thread a digit");
+    static_assert(kMost <= 1 << (32 - kWholeKeyBits) && WAVES * 64 >= kDigits, "a token's bits, a thread a digit");
     if (blockIdx.x >= 1) return clear(a, 1);
-    __shared__ uint32_t keys[kMost], base[kDigits], wave_sums[WAVES];
-    __shared__ uint16_t used[WAVES][kDigits], tokens[kMost];
+    __shared__ uint32_t list[kMost], wave_sums[WAVES];
+    __shared__ uint16_t used[WAVES][kDigits];
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, begin = wave * (64 * ITEMS) + lane;
-    uint32_t key[ITEMS], digit[ITEMS], rank[ITEMS];
-    uint16_t token[ITEMS];
+    uint32_t item[ITEMS], digit[ITEMS], rank[ITEMS];
     bool on[ITEMS];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         const uint32_t t = begin + k * 64;
         on[k] = t < a.n;
-        key[k] = on[k] ? key_at(a, t) : 0;
-        token[k] = static_cast<uint16_t>(t);
+        item[k] = (on[k] ? key_at(a, t) : 0) | t << kWholeKeyBits;
     }
-    for (int32_t shift = 0; shift < bits; shift += a.digit_bits) {
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k) digit[k] = key[k] >> shift & ((1u << a.digit_bits) - 1);
-        const uint32_t sum = rank_tile(digit, on, used, rank, a.digit_bits);
-        const uint32_t before = sum_before<WAVES>(sum, wave_sums);
-        if (threadIdx.x < kDigits) base[threadIdx.x] = before;
-        __syncthreads();
+    for (int32_t shift = 0; shift < bits; shift += BITS) {
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
-            if (!on[k]) continue;
-            const uint32_t at = base[digit[k]] + used[wave][digit[k]] + rank[k];
-            keys[at] = key[k];
-            tokens[at] = token[k];
+            digit[k] = (item[k] & ((1u << kWholeKeyBits) - 1)) >> shift & ((1u << BITS) - 1);
+        }
+        const uint32_t sum = rank_tile<BITS>(digit, on, used, rank);
+        const uint32_t before = sum_before<WAVES>(sum, wave_sums);
+        if (threadIdx.x < kDigits) {
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) used[w][threadIdx.x] += static_cast<uint16_t>(before);
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k)
-            if (on[k]) key[k] = keys[begin + k * 64], token[k] = tokens[begin + k * 64];
+            if (on[k]) list[used[wave][digit[k]] + rank[k]] = item[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k)
+            if (on[k]) item[k] = list[begin + k * 64];
         __syncthreads();
     }
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-        if (on[k]) a.keys_out[begin + k * 64] = key[k], a.tokens_out[begin + k * 64] = token[k];
+    for (int k = 0; k < ITEMS; ++k) {
+        if (!on[k]) continue;
+        a.keys_out[begin + k * 64] = item[k] & ((1u << kWholeKeyBits) - 1);
+        a.tokens_out[begin + k * 64] = item[k] >> kWholeKeyBits;
+    }
 }
 
 struct SumArgs {
@@ -380,36 +387,50 @@ __global__ __launch_bounds__(kBlock) void sum_pieces_kernel(SumArgs a) {
     if (piece >= a.pieces || left <= 0) return;
     const uint32_t none = static_cast<uint32_t>(a.rows), first = piece * a.piece;
     const uint32_t last = a.n - first < a.piece ? a.n : first + a.piece;
-    bool head = first > 0 && a.keys[first - 1] == a.keys[first];  // its first run began before it
-    bool open = false;                                            // the run at hand goes on
-    float sum[N] = {};
-    for (uint32_t i = first; i < last; i += kAhead) {
-        uint32_t key[kAhead + 1];
+    // The keys and tokens of a batch come together, and the next batch's while its
+    // rows are on their way.  The lists are longer than n by kAhead, so that no
+    // load waits for a comparison; keys from n on count as none.
+    uint32_t key[kAhead + 1], token[kAhead];
+    const auto fetch = [&](uint32_t i) {
 #pragma unroll
-        for (int u = 0; u <= kAhead; ++u) key[u] = i + u < a.n ? a.keys[i + u] : none;
-        if (key[0] == none) break;  // the ids that name no row come last
+        for (int u = 0; u <= kAhead; ++u) key[u] = a.keys[i + u];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) token[u] = a.tokens[i + u];
+#pragma unroll
+        for (int u = 0; u <= kAhead; ++u) key[u] = i + u < a.n ? key[u] : none;
+    };
+    const uint32_t before = first > 0 ? a.keys[first - 1] : none;
+    fetch(first);
+    bool head = before == key[0];  // the piece's first run began before it
+    bool open = false;             // the run at hand goes on
+    float sum[N] = {};
+    for (uint32_t i = first; i < last && key[0] != none; i += kAhead) {  // the ids that name no row come last
+        uint32_t row[kAhead + 1];
+#pragma unroll
+        for (int u = 0; u <= kAhead; ++u) row[u] = key[u];
         vec_t<TG, N> v[kAhead];
         vec_t<TW, N> old[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (i + u >= last || key[u] == none) continue;
-            v[u] = load_raw<TG, N, true>(static_cast<const TG*>(a.grad_out) + static_cast<int64_t>(a.tokens[i + u]) * a.width + c, left);
-            if (a.accumulate && key[u + 1] != key[u])
-                old[u] = load_raw<TW, N>(static_cast<const TW*>(a.grad) + static_cast<int64_t>(key[u]) * a.width + c, left);
+            if (i + u >= last || row[u] == none) continue;
+            v[u] = load_raw<TG, N, true>(static_cast<const TG*>(a.grad_out) + static_cast<int64_t>(token[u]) * a.width + c, left);
+            if (a.accumulate && row[u + 1] != row[u])
+                old[u] = load_raw<TW, N>(static_cast<const TW*>(a.grad) + static_cast<int64_t>(row[u]) * a.width + c, left);
         }
+        if (i + kAhead < last) fetch(i + kAhead);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (i + u >= last || key[u] == none) continue;
+            if (i + u >= last || row[u] == none) continue;
 #pragma unroll
             for (int j = 0; j < N; ++j) sum[j] += static_cast<float>(v[u][j]);
-            open = key[u + 1] == key[u];
+            open = row[u + 1] == row[u];
             if (open) continue;
             if (head) {
                 store_some<N>(a.partials + static_cast<int64_t>(piece) * 2 * a.width + c, sum, left);
             } else {
 #pragma unroll
                 for (int j = 0; j < N; ++j) sum[j] = a.accumulate ? fmaf(sum[j], a.scale, static_cast<float>(old[u][j])) : sum[j] * a.scale;
-                store_some<N>(static_cast<TW*>(a.grad) + static_cast<int64_t>(key[u]) * a.width + c, sum, left);
+                store_some<N>(static_cast<TW*>(a.grad) + static_cast<int64_t>(row[u]) * a.width + c, sum, left);
             }
             head = false;
 #pragma unroll
@@ -509,7 +530,7 @@ struct Work {
 Work work_of(int64_t n, int64_t width) {
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     Work w{};
-    const int64_t tiles = (n + kTile - 1) / kTile, list = up(4 * n);
+    const int64_t tiles = (n + kTile - 1) / kTile, list = up(4 * (n + 16));  // sum_pieces_kernel reads a little past n
     w.keys[0] = up(4 * tiles * kDigits);
     w.tokens[0] = w.keys[0] + list, w.keys[1] = w.tokens[0] + list, w.tokens[1] = w.keys[1] + list;
     w.partials = w.tokens[1] + list;
@@ -607,12 +628,12 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
             const auto list = [&](int64_t offset) { return reinterpret_cast<uint32_t*>(at + offset); };
             const uint32_t tiles = static_cast<uint32_t>((n + kTile - 1) / kTile);
             SortArgs o{ids_dev, nullptr, nullptr, nullptr, nullptr, list(work.counts), rows, padding_idx, static_cast<uint32_t>(n),
-                       tiles, id_bytes, 0, 0, nullptr, 0};
+                       tiles, id_bytes, 0, nullptr, 0};
             int32_t bits = 1;
             while (rows >> bits) ++bits;  // of the largest key, `rows`
             const int passes = (bits + kDigitBits - 1) / kDigitBits;
-            o.digit_bits = (bits + passes - 1) / passes;
-            const bool whole = n <= kSortWhole;
+            const bool eight = bits <= 8 * passes;  // bits a pass: 8 where that takes no more of them, else 9
+            const bool whole = n <= kSortWhole && bits <= kWholeKeyBits;
             const int launches = whole ? 1 : 2 * passes;
             // a gradient that is written whole is cleared beside the sort, which leaves most of the chip idle: a share
             // with each launch, by the work-groups past the tiles
@@ -629,17 +650,26 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
             if (whole) {
                 o.keys_out = list(work.keys[0]), o.tokens_out = list(work.tokens[0]);
                 const dim3 grid(1 + clearing(true));
-                if (n <= 2048) hipLaunchKernelGGL((sort_whole_kernel<8, 4>), grid, dim3(512), 0, s, o, bits);
-                else hipLaunchKernelGGL((sort_whole_kernel<16, 8>), grid, dim3(1024), 0, s, o, bits);
+                const auto sort = [&](auto digit) {
+                    constexpr int BITS = decltype(digit)::value;
+                    if (n <= 2048) hipLaunchKernelGGL((sort_whole_kernel<BITS, 8, 4>), grid, dim3(512), 0, s, o, bits);
+                    else if (n <= 4096) hipLaunchKernelGGL((sort_whole_kernel<BITS, 16, 4>), grid, dim3(1024), 0, s, o, bits);
+                    else hipLaunchKernelGGL((sort_whole_kernel<BITS, 16, 8>), grid, dim3(1024), 0, s, o, bits);
+                };
+                if (eight) sort(std::integral_constant<int, 8>{});
+                else sort(std::integral_constant<int, 9>{});
                 if (int rc = launched("sort_whole_kernel")) return rc;
                 side = 1;
             } else {
-                for (o.shift = 0; o.shift < bits; o.shift += o.digit_bits, side ^= 1) {
+                for (o.shift = 0; o.shift < bits; o.shift += eight ? 8 : 9, side ^= 1) {
                     o.keys_out = list(work.keys[side]), o.tokens_out = list(work.tokens[side]);
-                    hipLaunchKernelGGL(count_kernel, dim3(tiles + clearing(false)), dim3(kSortBlock), 0, s, o);
+                    const dim3 counters(tiles + clearing(false));
+                    if (eight) hipLaunchKernelGGL(count_kernel<8>, counters, dim3(kSortBlock), 0, s, o);
+                    else hipLaunchKernelGGL(count_kernel<9>, counters, dim3(kSortBlock), 0, s, o);
                     if (int rc = launched("count_kernel")) return rc;
-                    const dim3 grid(tiles + clearing(o.shift + o.digit_bits >= bits));
-                    hipLaunchKernelGGL(place_kernel, grid, dim3(kSortBlock), 0, s, o);
+                    const dim3 grid(tiles + clearing(o.shift + (eight ? 8 : 9) >= bits));
+                    if (eight) hipLaunchKernelGGL(place_kernel<8>, grid, dim3(kSortBlock), 0, s, o);
+                    else hipLaunchKernelGGL(place_kernel<9>, grid, dim3(kSortBlock), 0, s, o);
                     if (int rc = launched("place_kernel")) return rc;
                     o.keys = o.keys_out, o.tokens = o.tokens_out;
                 }
