@@ -499,11 +499,24 @@ __global__ __launch_bounds__(kBlock) void join_pieces_kernel(SumArgs a) {
     store_some<N>(out, sum, left);
 }
 
-// Which form: the sort's launches cost what reading all ids for each of a few
-// thousand rows does.
-constexpr int64_t kByRowWork = int64_t{1} << 20;  // rows * tokens
-bool by_row(int64_t n, int64_t rows) {
-    return n >= (int64_t{1} << 30) || rows >= (int64_t{1} << 31) || n == 0 || rows <= kByRowWork / n;
+// Which form: a work-group per row, while all of them read the ids in less than
+// the sort's launches take and one row that has all tokens is not long in summing
+// them.  A whole call in us, by row / sorted, ids whose frequency falls as one over
+// their rank and all the same:
+//   tokens  rows   width   by rank        the same
+//   256     96     128      5.1 / 14.1     6.5 / 13.5
+//   1,024   96     128      5.4 / 15.1    17.5 / 17.1
+//   1,024   1,000  256      5.4 / 17.1    30.9 / 18.9
+//   256     1,000  4,096    7.7 / 17.4    60.2 / 17.6
+//   1,024   96     768     17.2 / 14.1   117.8 / 16.4
+//   64      16,000 4,096   29.8 / 25.6    41.1 / 26.4
+//   16      50,304 768     43.5 / 18.4    43.5 / 19.1
+// Lists and weights beyond 30 and 31 bits are not sorted at all.
+constexpr int64_t kByRowWork = int64_t{1} << 19;   // rows * tokens
+constexpr int64_t kByRowTerms = int64_t{1} << 17;  // tokens * width
+bool by_row(int64_t n, int64_t rows, int64_t width) {
+    if (n == 0 || n >= (int64_t{1} << 30) || rows >= (int64_t{1} << 31)) return true;
+    return rows <= kByRowWork / n && width <= kByRowTerms / n;
 }
 
 // Up to here one work-group sorts the whole list: at 8,183 tokens that takes
@@ -590,7 +603,7 @@ MGOPT_API int mgopt_embedding(const void* ids_dev, int32_t id_bytes, int64_t n, 
 
 MGOPT_API int64_t mgopt_embedding_grad_workspace(int64_t n, int64_t rows, int64_t width) {
     if (n < 0 || rows < 1 || width < 1) return -1;
-    return by_row(n, rows) ? 16 : work_of(n, width).bytes;
+    return by_row(n, rows, width) ? 16 : work_of(n, width).bytes;
 }
 
 MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_t n, const void* grad_out_dev,
@@ -612,7 +625,7 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
             const int64_t vecs = (width + N - 1) / N, chunks = (vecs + kBlock - 1) / kBlock;
             if (chunks > max_blocks(kBlock)) return set_error(MGOPT_E_LIMIT, "embedding_grad: rows too long");
             const uint32_t shift = shift_for(vecs);
-            if (by_row(n, rows)) {
+            if (by_row(n, rows, width)) {
                 a.shift = shift;
                 a.chunks = static_cast<uint32_t>(chunks);
                 const int64_t most = max_blocks(kBlock) / chunks;
