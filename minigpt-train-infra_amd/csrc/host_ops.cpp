@@ -459,7 +459,7 @@ py::tuple policy_loss(const Tensor& logits, const Tensor& targets, const Tensor&
     mgopt_policy_args& a = l.p.a;
     const c10::DeviceGuard guard(logits.device());
     const auto f32 = logits.options().dtype(at::kFloat);
-    Tensor log_probs = at::empty(all_but_last(logits), f32), loss = at::empty({}, f32), parts = at::empty({3}, f32);
+    Tensor log_probs = at::empty(all_but_last(logits), f32), results = at::empty({4}, f32);  // loss, policy, kl, clip_fraction
     Tensor work = at::empty({lib.policy_workspace(a.rows)}, logits.options().dtype(at::kByte));
     a.log_probs_dev = log_probs.data_ptr<float>();
     a.workspace_dev = work.data_ptr();
@@ -481,8 +481,10 @@ py::tuple policy_loss(const Tensor& logits, const Tensor& targets, const Tensor&
         }
         a.d_logits_dev = grad->data_ptr();
     }
-    check(lib.policy_loss(&a, loss.data_ptr<float>(), parts.data_ptr<float>(), as_stream(stream)), "policy_loss");
-    return py::make_tuple(loss, log_probs, parts.select(0, 0), parts.select(0, 1), parts.select(0, 2), grad, work);
+    float* const r = results.data_ptr<float>();
+    check(lib.policy_loss(&a, r, r + 1, as_stream(stream)), "policy_loss");
+    const std::vector<Tensor> each = results.unbind(0);
+    return py::make_tuple(each[0], log_probs, each[1], each[2], each[3], grad, work);
 }
 
 Tensor policy_loss_backward(const Tensor& logits, const Tensor& targets, const Tensor& old_logp, const Tensor& advantages,
