@@ -471,7 +471,12 @@ py::tuple policy_loss(const Tensor& logits, const Tensor& targets, const Tensor&
             if (out->sizes() != logits.sizes()) refuse("out has shape " + shape_of(*out) + ", logits " + shape_of(logits));
             const Rows r = rows_of(*out);
             if (!r.t.is_same(*out)) refuse("out needs rows that are contiguous and evenly spaced");
-            if (out->data_ptr() == logits.data_ptr() && (l.p.logits.stride != r.stride || !l.p.logits.t.is_same(logits)))
+            if (r.rows > 1 && r.stride < r.width) refuse("out's rows overlap");
+            // over the logits exactly, or beside them
+            const char *x = static_cast<const char*>(a.logits_dev), *d = static_cast<const char*>(out->data_ptr());
+            const auto bytes = [&](int64_t stride) { return ((a.rows - 1) * stride + a.vocab) * logits.element_size(); };
+            if (a.rows > 0 && x < d + bytes(r.stride) && d < x + bytes(a.logits_stride) &&
+                !(x == d && r.stride == a.logits_stride))
                 refuse("out overlaps the logits and is not them");
             grad = *out;
             a.d_logits_stride = r.stride;

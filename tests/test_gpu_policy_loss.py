@@ -318,6 +318,13 @@ def test_refusals():
         run(x, y, o, a, grad_scale=torch.ones(2, device=DEV))
     with pytest.raises(ValueError, match="out has shape"):
         run(x, y, o, a, out=x[:5])
+    wide = torch.empty(9 * 50 + 7, device=DEV)
+    with pytest.raises(ValueError, match="overlaps the logits"):
+        run(wide[: 8 * 50].view(8, 50), y, o, a, out=wide[7: 8 * 50 + 7].view(8, 50))
+    with pytest.raises(ValueError, match="overlaps the logits"):
+        run(wide[: 8 * 50].view(8, 50), y, o, a, out=wide.as_strided((8, 50), (51, 1)))
+    with pytest.raises(ValueError, match="rows overlap"):
+        run(x, y, o, a, out=torch.empty(50, device=DEV).expand(8, 50))
     with pytest.raises(ValueError, match="evenly spaced"):
         run(x, y, o, a, out=torch.empty((50, 8), device=DEV).t())
     with pytest.raises(RuntimeError, match="no CPU path"):
