@@ -25,9 +25,8 @@
 // takes c's place, which keeps the products finite: what equals m counts 1,
 // all else 0.
 //
-// A row that fits is held in registers between the passes (cached_kernel), as
-// it came, so that it is read once; longer rows are read again, from the
-// Infinity Cache in part.
+// A row is held in registers between the passes (cached_kernel), as it came, so
+// that it is read once; what does not fit is read again.
 //
 // Bound by memory: a row's logits once, its gradient once.
 #include "ops_common.h"
@@ -204,11 +203,12 @@ __device__ __forceinline__ void widen(float (&v)[N], const Raw& raw) {
     for (int j = 0; j < N; ++j) v[j] = static_cast<float>(q[j]);
 }
 
-// Rows of at most NT * NV vectors (and a tail of less than one): each thread
-// holds NV of them.  All loads are issued before
-// the first is used; vectors past the row's end repeat its last one and are
+// The forward forms.  Each thread holds NV vectors of its row, so that rows of at
+// most NT * NV of them (and a tail of less than one) are read once; LONG: what
+// lies beyond is read again for the gradient.  All of a row's first loads are
+// issued before one is used; vectors past its end repeat its last one and are
 // not counted.
-template <typename T, int NT, int NV, Mode MODE>
+template <typename T, int NT, int NV, Mode MODE, bool LONG>
 __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
     constexpr int N = 16 / sizeof(T);
     const int64_t n = a.first_row + blockIdx.x;
@@ -216,11 +216,14 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
     const T* x = static_cast<const T*>(a.logits) + n * a.row_stride;
     T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
     if (w == 0.0f) return skip_row<T, NT, MODE>(a, n, dx);
-    const int V = static_cast<int>(a.vocab), full = V / N, tail = V - full * N, t = threadIdx.x;
+    // vectors of the row; LONG ones have more than 32 bits count
+    using Index = std::conditional_t<LONG, int64_t, int>;
+    const Index V = static_cast<Index>(a.vocab), full = V / N, tail = V - full * N;
+    const int t = threadIdx.x;
     Raw raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int v = i * NT + t;
+        const Index v = i * NT + t;
         raw[i] = full > 0 ? __builtin_bit_cast(Raw, __builtin_nontemporal_load(reinterpret_cast<const vec_t<T, N>*>(x) +
                                                                               (v < full ? v : full - 1)))
                           : Raw{};
@@ -238,6 +241,14 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
         if (i * NT + t < full) take<N>(r, v, a.c);
         asm("" : "+v"(raw[i]));             // widened again below, not kept
     }
+    if constexpr (LONG) {
+#pragma unroll 4
+        for (int64_t i = int64_t{NV} * NT + t; i < full; i += NT) {
+            float v[N];
+            load<N>(v, x + i * N);
+            take<N>(r, v, a.c);
+        }
+    }
     r = join_block<NT>(r);
     __shared__ RowResult shared;
     if (t == 0) shared = row_scalars<MODE>(a, n, in, w, r.m, r.s);
@@ -248,13 +259,22 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
     const int64_t y = id_at(a.targets, n, a.target_bytes);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int at = i * NT + t;
+        const Index at = i * NT + t;
         if (at >= full) continue;
         __builtin_amdgcn_sched_barrier(0);
         float v[N];
         widen<T, N>(v, raw[i]);
         to_gradient<N>(v, q, f, y, static_cast<int64_t>(at) * N);
         store_nt<N>(dx + static_cast<int64_t>(at) * N, v);
+    }
+    if constexpr (LONG) {
+#pragma unroll 4
+        for (int64_t i = int64_t{NV} * NT + t; i < full; i += NT) {
+            float v[N];
+            load<N>(v, x + i * N);
+            to_gradient<N>(v, q, f, y, i * N);
+            store_nt<N>(dx + i * N, v);
+        }
     }
     if (t < tail) {
         to_gradient<1>(last, q, f, y, full * N + t);
@@ -265,52 +285,27 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-template <typename T, int NT, Mode MODE>
-__global__ __launch_bounds__(NT) void policy_kernel(PolicyArgs a) {
+// The gradient from a forward pass's m, s and log-probabilities.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void grad_kernel(PolicyArgs a) {
     constexpr int N = 16 / sizeof(T);
     const int64_t n = a.first_row + blockIdx.x, V = a.vocab;
     const float w = weight_at(a.mask, a.mask_kind, n);
     const T* x = static_cast<const T*>(a.logits) + n * a.row_stride;
     T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
-    const int64_t start = static_cast<int64_t>(threadIdx.x) * N;
-    constexpr int64_t kStep = int64_t{NT} * N;
-    if (w == 0.0f) return skip_row<T, NT, MODE>(a, n, dx);
-    RowInputs in{};
-    if (threadIdx.x == 0) in = row_inputs<T, MODE>(a, n);
-    Running r;
-    if constexpr (MODE == kGrad) {
-        const float2 q = a.stats[n];
-        r.m = q.x, r.s = q.y;
-    } else {
-        // the elements after the last whole vector first, as cached_kernel does: the same bits
-        const int64_t full = V / N * N;
-        if (threadIdx.x < V - full) {
-            const float v[1] = {static_cast<float>(x[full + threadIdx.x])};
-            take<1>(r, v, a.c);
-        }
-        for (int64_t i = start; i < full; i += kStep) {
-            float v[N];
-            load<N>(v, x + i);
-            take<N>(r, v, a.c);
-        }
-        r = join_block<NT>(r);
-    }
+    if (w == 0.0f) return skip_row<T, NT, kGrad>(a, n, dx);
+    const float2 ms = a.stats[n];
     __shared__ RowResult shared;
-    if (threadIdx.x == 0) {
-        const RowResult q = row_scalars<MODE>(a, n, in, w, r.m, r.s);
-        if constexpr (MODE == kLossGrad || MODE == kGrad) shared = q;
-    }
-    if constexpr (MODE == kLossGrad || MODE == kGrad) {
-        __syncthreads();
-        const RowResult q = shared;
-        const Frame f = frame(r.m, a.c);
-        const int64_t y = id_at(a.targets, n, a.target_bytes);
-        for (int64_t i = start; i < V; i += kStep) {
-            float v[N];
-            load_some<N>(v, x + i, V - i);
-            to_gradient<N>(v, q, f, y, i);
-            store_some<N>(dx + i, v, V - i);
-        }
+    if (threadIdx.x == 0) shared = row_scalars<kGrad>(a, n, row_inputs<T, kGrad>(a, n), w, ms.x, ms.y);
+    __syncthreads();
+    const RowResult q = shared;
+    const Frame f = frame(ms.x, a.c);
+    const int64_t y = id_at(a.targets, n, a.target_bytes);
+    for (int64_t i = static_cast<int64_t>(threadIdx.x) * N; i < V; i += int64_t{NT} * N) {
+        float v[N];
+        load_some<N>(v, x + i, V - i);
+        to_gradient<N>(v, q, f, y, i);
+        store_some<N>(dx + i, v, V - i);
     }
 }
 
@@ -332,6 +327,7 @@ __device__ __forceinline__ X sum_block(X x) {
 
 __global__ __launch_bounds__(kSumBlock) void weight_sum_kernel(const void* mask, int32_t kind, int64_t rows, double* out) {
     double x = 0.0;
+#pragma unroll 8
     for (int64_t n = threadIdx.x; n < rows; n += kSumBlock) x += weight_at(mask, kind, n);
     x = sum_block(x);
     if (threadIdx.x == 0) *out = x;
@@ -342,6 +338,7 @@ __global__ __launch_bounds__(kSumBlock) void weight_sum_kernel(const void* mask,
 __global__ __launch_bounds__(kSumBlock) void policy_sum_kernel(const float4* terms, int64_t rows, const double* weight_sum,
                                                                double kl_coef, float* loss, float* parts) {
     double p = 0.0, k = 0.0, h = 0.0;
+#pragma unroll 8
     for (int64_t n = threadIdx.x; n < rows; n += kSumBlock) {
         const float4 t = terms[n];
         p += t.x, k += t.y, h += t.z;
@@ -368,23 +365,19 @@ int launch_rows(PolicyArgs a, hipStream_t s) {
         const auto cached = [&](auto threads, auto held) {
             constexpr int NT = decltype(threads)::value, NV = decltype(held)::value;
             if (vecs > NT * NV) return false;
-            hipLaunchKernelGGL((cached_kernel<T, NT, NV, MODE>), grid, dim3(NT), 0, s, a);
+            hipLaunchKernelGGL((cached_kernel<T, NT, NV, MODE, false>), grid, dim3(NT), 0, s, a);
             return true;
         };
-        const auto again = [&](auto threads) {
-            constexpr int NT = decltype(threads)::value;
-            hipLaunchKernelGGL((policy_kernel<T, NT, MODE>), grid, dim3(NT), 0, s, a);
-        };
         if constexpr (MODE == kGrad) {
-            if (vecs <= 256) again(Int<64>{});
-            else if (vecs <= 2048) again(Int<256>{});
-            else again(Int<1024>{});
+            if (vecs <= 256) hipLaunchKernelGGL((grad_kernel<T, 64>), grid, dim3(64), 0, s, a);
+            else if (vecs <= 2048) hipLaunchKernelGGL((grad_kernel<T, 256>), grid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((grad_kernel<T, 1024>), grid, dim3(1024), 0, s, a);
         } else if (!(cached(Int<64>{}, Int<4>{}) || cached(Int<256>{}, Int<8>{}) || cached(Int<1024>{}, Int<4>{}) ||
                      cached(Int<1024>{}, Int<8>{}) || cached(Int<1024>{}, Int<12>{}) || cached(Int<1024>{}, Int<16>{}) ||
                      cached(Int<1024>{}, Int<20>{}))) {
-            again(Int<1024>{});
+            hipLaunchKernelGGL((cached_kernel<T, 1024, 12, MODE, true>), grid, dim3(1024), 0, s, a);
         }
-        if (int rc = launched("policy_kernel")) return rc;
+        if (int rc = launched("policy_loss")) return rc;
     }
     return 0;
 }

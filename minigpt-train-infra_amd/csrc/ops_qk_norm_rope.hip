@@ -13,9 +13,9 @@
 //     dx = (h - xhat * mean(h * xhat)) / sqrt(mean(x^2) + eps)      dw = sum g * xhat
 //
 // A group of lanes holds a head, each lane VEC pairs of it, so that both halves
-// of a pair are in one lane and the mean is a sum over the group.  A wave's
-// groups take different heads of one token: its cosines, sines and the weights
-// stay in registers from head to head.
+// of a pair are in one lane and the mean is a sum over the group.  `parts` groups
+// share a token's heads: its cosines, sines and the weights stay in registers
+// from head to head.
 //
 // Bound by memory: forward reads and writes the heads once; backward reads x
 // and the gradient and writes dx.  The weights' gradients are summed per lane
@@ -34,7 +34,7 @@ struct Args {
     mgopt_qk_args a;
     uint32_t tokens;
     uint32_t lanes;   // of a head: a power of two
-    uint32_t parts;   // waves that share a token's heads
+    uint32_t parts;   // groups that share a token's heads
     // backward
     uint32_t q_parts, k_parts, q_blocks;
     float* partials;  // [work-groups][dim]
@@ -142,11 +142,11 @@ __device__ __forceinline__ int64_t offset(const int64_t (&stride)[3], const Toke
 
 template <typename T, int VEC, int SLOTS, bool INTER>
 __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_kernel(Args k) {
-    const uint32_t wave = blockIdx.x * kWaves + threadIdx.x / 64, lane = threadIdx.x % 64;
-    const uint32_t n = wave / k.parts, part = wave - n * k.parts;
-    if (n >= k.tokens) return;
+    const uint64_t group = (static_cast<uint64_t>(blockIdx.x) * kRopeBlock + threadIdx.x) / k.lanes;
+    const uint32_t n = static_cast<uint32_t>(group / k.parts), part = static_cast<uint32_t>(group - static_cast<uint64_t>(n) * k.parts);
+    if (n >= k.tokens) return;  // whole groups of lanes
     const Token t = token_of(k, n);
-    const uint32_t l = lane & (k.lanes - 1), groups = 64 / k.lanes, step = groups * k.parts;
+    const uint32_t l = threadIdx.x & (k.lanes - 1);
     const float inv_dim = 1.0f / static_cast<float>(k.a.dim);
     Slot q[SLOTS];
     float c[SLOTS][VEC], d[SLOTS][VEC];
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_kernel(Args k) {
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i)
             if (q[i].on) w[i].read_weights(side.weight_dev, k.a.weight_dtype, q[i]);
-        for (; h < static_cast<uint32_t>(side.heads); h += step) {
+        for (; h < static_cast<uint32_t>(side.heads); h += k.parts) {
             const T* x = static_cast<const T*>(side.x_dev) + offset(side.x_stride, t, h);
             T* out = static_cast<T*>(side.out_dev) + offset(side.out_stride, t, h);
             Pairs<VEC, INTER> v[SLOTS];
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_kernel(Args k) {
         return h - static_cast<uint32_t>(side.heads);
     };
     // the groups count through the queries' heads and on through the keys'
-    const uint32_t first_k = heads(k.a.q, part * groups + lane / k.lanes);
+    const uint32_t first_k = heads(k.a.q, part);
     heads(k.a.k, first_k);
 }
 
@@ -203,8 +203,8 @@ __global__ __launch_bounds__(kRopeBlock, 4) void qk_norm_rope_backward_kernel(Ar
     const mgopt_heads& side = on_q ? k.a.q : k.a.k;
     const uint32_t block = on_q ? blockIdx.x : blockIdx.x - k.q_blocks, blocks = on_q ? k.q_blocks : gridDim.x - k.q_blocks;
     const uint32_t heads = static_cast<uint32_t>(side.heads);
-    const uint32_t lane = threadIdx.x % 64, l = lane & (k.lanes - 1), groups = 64 / k.lanes;
-    const uint32_t parts = on_q ? k.q_parts : k.k_parts, step = groups * parts;
+    const uint32_t lane = threadIdx.x % 64, l = lane & (k.lanes - 1), groups = kRopeBlock / k.lanes;
+    const uint32_t parts = on_q ? k.q_parts : k.k_parts;
     const float inv_dim = 1.0f / static_cast<float>(k.a.dim);
     Slot q[SLOTS];
     Pairs<VEC, INTER> w[SLOTS], sum_w[SLOTS];
@@ -216,14 +216,14 @@ __global__ __launch_bounds__(kRopeBlock, 4) void qk_norm_rope_backward_kernel(Ar
         for (int j = 0; j < VEC; ++j) sum_w[i].a[j] = sum_w[i].b[j] = 0.0f;
     }
     const uint64_t tasks = static_cast<uint64_t>(k.tokens) * parts;
-    for (uint64_t task = static_cast<uint64_t>(block) * kWaves + threadIdx.x / 64; task < tasks;
-         task += static_cast<uint64_t>(blocks) * kWaves) {
+    for (uint64_t task = static_cast<uint64_t>(block) * groups + threadIdx.x / k.lanes; task < tasks;
+         task += static_cast<uint64_t>(blocks) * groups) {
         const uint32_t n = static_cast<uint32_t>(task / parts), part = static_cast<uint32_t>(task - static_cast<uint64_t>(n) * parts);
         const Token t = token_of(k, n);
         float c[SLOTS][VEC], d[SLOTS][VEC];
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) angles<VEC>(k, q[i], l + i * k.lanes, t.pos, c[i], d[i]);
-        for (uint32_t h = part * groups + lane / k.lanes; h < heads; h += step) {
+        for (uint32_t h = part; h < heads; h += parts) {
             const T* x = static_cast<const T*>(side.x_dev) + offset(side.x_stride, t, h);
             const T* grad = static_cast<const T*>(side.grad_dev) + offset(side.grad_stride, t, h);
             T* dx = static_cast<T*>(side.d_x_dev) + offset(side.d_x_stride, t, h);
@@ -344,12 +344,13 @@ int with_form(const mgopt_qk_args& a, Args& k, F&& f) {
         const int pieces = (a.dim + 2 * vec - 1) / (2 * vec);
         k.lanes = 1;
         while (static_cast<int>(k.lanes) * slots < pieces) k.lanes <<= 1;
-        // waves that share a token's heads, while that leaves the chip's 1,024 SIMDs idle and a wave's groups have heads
+        // groups that share a token's heads: four heads each, for the use of one token's cosines, or fewer while
+        // that leaves the chip short of waves
         const int64_t groups = 64 / k.lanes;
         const auto share = [&](int64_t heads) {
-            uint32_t parts = 1;
-            while (parts * groups < heads && static_cast<int64_t>(k.tokens) * parts < 4096) ++parts;
-            return parts;
+            int64_t parts = (heads + 3) / 4;
+            while (parts < heads && k.tokens * parts < 4096 * groups) ++parts;
+            return static_cast<uint32_t>(parts);
         };
         k.parts = share(a.q.heads + a.k.heads);
         k.q_parts = share(a.q.heads), k.k_parts = share(a.k.heads);
@@ -390,9 +391,10 @@ MGOPT_API int mgopt_qk_norm_rope(const mgopt_qk_args* a, void* stream) {
     k.tokens = static_cast<uint32_t>(a->batch * a->length);
     return with_form<false>(*a, k, [&](auto t, auto vec, auto slots, auto inter) {
         using T = decltype(t);
-        const uint32_t blocks = static_cast<uint32_t>((static_cast<uint64_t>(k.tokens) * k.parts + kWaves - 1) / kWaves);
+        const uint64_t groups = kRopeBlock / k.lanes, blocks = (static_cast<uint64_t>(k.tokens) * k.parts + groups - 1) / groups;
+        if (blocks > max_blocks(kRopeBlock)) return set_error(MGOPT_E_LIMIT, "qk_norm_rope: too many heads");
         hipLaunchKernelGGL((qk_norm_rope_kernel<T, decltype(vec)::value, decltype(slots)::value, decltype(inter)::value>),
-                           dim3(blocks), dim3(kRopeBlock), 0, static_cast<hipStream_t>(stream), k);
+                           dim3(static_cast<uint32_t>(blocks)), dim3(kRopeBlock), 0, static_cast<hipStream_t>(stream), k);
         return launched("qk_norm_rope_kernel");
     });
 }
@@ -419,10 +421,10 @@ MGOPT_API int mgopt_qk_norm_rope_backward(const mgopt_qk_args* a, void* stream) 
     if (k.tokens > 0) {
         const int rc = with_form<true>(*a, k, [&](auto t, auto vec, auto slots, auto inter) {
             using T = decltype(t);
-            // work-groups by the sides' shares of the heads, each no more than it has waves' work for
+            // work-groups by the sides' shares of the heads, each no more than it has work for
             const auto blocks_for = [&](uint32_t parts, uint32_t share) {
-                const uint64_t waves = static_cast<uint64_t>(k.tokens) * parts;
-                return static_cast<uint32_t>(std::min<uint64_t>((waves + kWaves - 1) / kWaves, share));
+                const uint64_t groups = kRopeBlock / k.lanes, tasks = static_cast<uint64_t>(k.tokens) * parts;
+                return static_cast<uint32_t>(std::min<uint64_t>((tasks + groups - 1) / groups, share));
             };
             const uint32_t k_share = std::max<uint32_t>(
                 1, static_cast<uint32_t>(static_cast<uint64_t>(kBackwardBlocks) * a->k.heads / (a->q.heads + a->k.heads)));
