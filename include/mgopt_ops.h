@@ -184,7 +184,9 @@ typedef struct mgopt_policy_args {
 
 MGOPT_API int64_t mgopt_policy_workspace(int64_t rows);
 
-/* Writes log_probs_dev.  Reads logits, targets and mask; needs no workspace. */
+/* Writes log_probs_dev.  Reads logits, targets and mask.  The workspace may be
+ * NULL: fewer than 128 long rows are then not cut in slices, and their sums, of
+ * another order, may differ in the last bits. */
 MGOPT_API int mgopt_token_log_probs(const mgopt_policy_args* args, void* stream);
 
 /* With logp = log_softmax(logits / temperature)[target], ratio =

@@ -416,6 +416,11 @@ Tensor token_log_probs(const Tensor& logits, const Tensor& targets, const option
     const c10::DeviceGuard guard(logits.device());
     Tensor out = at::empty(all_but_last(logits), logits.options().dtype(at::kFloat));
     p.a.log_probs_dev = out.data_ptr<float>();
+    Tensor work;
+    if (p.a.rows < 128) {  // few rows, which may be cut in slices
+        work = at::empty({lib.policy_workspace(p.a.rows)}, logits.options().dtype(at::kByte));
+        p.a.workspace_dev = work.data_ptr();
+    }
     check(lib.token_log_probs(&p.a, as_stream(stream)), "token_log_probs");
     return out;
 }

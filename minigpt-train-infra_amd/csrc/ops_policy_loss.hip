@@ -26,7 +26,9 @@
 // all else 0.
 //
 // A row is held in registers between the passes (cached_kernel), as it came, so
-// that it is read once; what does not fit is read again.
+// that it is read once; what does not fit is read again.  Few long rows are cut
+// in slices, a work-group each (slice_kernel), and joined by those that finish
+// them (finish_kernel).
 //
 // Bound by memory: a row's logits once, its gradient once.
 #include "ops_common.h"
@@ -54,6 +56,10 @@ struct PolicyArgs {
     float4* terms;               // w * policy, w * kl, w * clipped
     void* d_logits;
     int64_t d_stride;
+    uint32_t slices = 1;         // of a row
+    int64_t slice;               // elements of one
+    float4* parts;               // m, s and offset of each slice
+    float* picked;               // the targets' logits: a gradient in place may overwrite them before another slice is done
 };
 
 __device__ __forceinline__ float weight_at(const void* mask, int32_t kind, int64_t n) {
@@ -116,10 +122,10 @@ struct RowInputs {
     double total;
 };
 template <typename T, Mode MODE>
-__device__ __forceinline__ RowInputs row_inputs(const PolicyArgs& a, int64_t n) {
+__device__ __forceinline__ RowInputs row_inputs(const PolicyArgs& a, int64_t n, bool pick = MODE != kGrad) {
     RowInputs r{};
     r.target = id_at(a.targets, n, a.target_bytes);
-    if (MODE != kGrad)
+    if (pick)
         r.x = r.target >= 0 && r.target < a.vocab
                   ? static_cast<float>(static_cast<const T*>(a.logits)[n * a.row_stride + r.target])
                   : __builtin_nanf("");
@@ -137,7 +143,8 @@ struct RowResult {
 
 // What one row adds to the loss, and its slope, from m and s.
 template <Mode MODE>
-__device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs& in, float w, float m, float s) {
+__device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs& in, float w, float m, float s,
+                                 bool write = true) {
     double logp;
     if constexpr (MODE == kGrad) {
         logp = a.log_probs[n];
@@ -147,7 +154,7 @@ __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs
         logp = (static_cast<double>(in.x) - static_cast<double>(m)) * a.inv_temp +
                fma(static_cast<double>(m), static_cast<double>(f.c), static_cast<double>(f.offset)) * kLn2 -
                log(static_cast<double>(s));
-        a.log_probs[n] = static_cast<float>(logp);
+        if (write) a.log_probs[n] = static_cast<float>(logp);
     }
     if constexpr (MODE == kLogp) return {};
     const double A = in.advantage, ratio = exp(logp - static_cast<double>(in.old_logp));
@@ -159,7 +166,7 @@ __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs
         kl = e - r;
         slope -= a.kl_coef * e;
     }
-    if constexpr (MODE != kGrad)
+    if (MODE != kGrad && write)
         a.terms[n] = make_float4(static_cast<float>(w * -(held ? s2 : s1)), static_cast<float>(w * kl), held ? w : 0.0f, 0.0f);
     if constexpr (MODE == kLoss) a.stats[n] = make_float2(m, s);
     if constexpr (MODE == kLoss) return {};
@@ -167,19 +174,22 @@ __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs
     return {static_cast<float>(slope), static_cast<float>(-slope / static_cast<double>(s))};
 }
 
+template <typename T, int NT>
+__device__ __forceinline__ void clear(T* dx, int64_t begin, int64_t end) {
+    constexpr int N = 16 / sizeof(T);
+    const float zero[N] = {};
+    for (int64_t i = begin + static_cast<int64_t>(threadIdx.x) * N; i < end; i += int64_t{NT} * N)
+        store_some<N>(dx + i, zero, end - i);
+}
+
 // A row of weight 0: its outputs are zeros.
 template <typename T, int NT, Mode MODE>
 __device__ __forceinline__ void skip_row(const PolicyArgs& a, int64_t n, T* dx) {
-    constexpr int N = 16 / sizeof(T);
-    if (MODE != kGrad && threadIdx.x == 0) {
+    if (threadIdx.x == 0) {
         a.log_probs[n] = 0.0f;
         if (MODE != kLogp) a.terms[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    if constexpr (MODE == kLossGrad || MODE == kGrad) {
-        const float zero[N] = {};
-        for (int64_t i = static_cast<int64_t>(threadIdx.x) * N; i < a.vocab; i += int64_t{NT} * N)
-            store_some<N>(dx + i, zero, a.vocab - i);
-    }
+    if constexpr (MODE == kLossGrad) clear<T, NT>(dx, 0, a.vocab);
 }
 
 // One vector of the gradient, from column i on.
@@ -191,6 +201,19 @@ __device__ __forceinline__ void to_gradient(float (&v)[N], const RowResult& q, c
 #pragma unroll
         for (int j = 0; j < N; ++j)
             if (y == i + j) v[j] += q.slope;
+    }
+}
+
+// The gradient of columns begin to end, from their logits.
+template <typename T, int NT>
+__device__ __forceinline__ void write_gradient(const T* x, T* dx, int64_t begin, int64_t end, const RowResult& q,
+                                               const Frame& f, int64_t y) {
+    constexpr int N = 16 / sizeof(T);
+    for (int64_t i = begin + static_cast<int64_t>(threadIdx.x) * N; i < end; i += int64_t{NT} * N) {
+        float v[N];
+        load_some<N>(v, x + i, end - i);
+        to_gradient<N>(v, q, f, y, i);
+        store_some<N>(dx + i, v, end - i);
     }
 }
 
@@ -285,27 +308,87 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-// The gradient from a forward pass's m, s and log-probabilities.
+// The gradient from a forward pass's m, s and log-probabilities, a slice of a row a work-group.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void grad_kernel(PolicyArgs a) {
-    constexpr int N = 16 / sizeof(T);
-    const int64_t n = a.first_row + blockIdx.x, V = a.vocab;
+    const uint32_t row = blockIdx.x / a.slices, part = blockIdx.x - row * a.slices;
+    const int64_t n = a.first_row + row, begin = part * a.slice, end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
     const float w = weight_at(a.mask, a.mask_kind, n);
     const T* x = static_cast<const T*>(a.logits) + n * a.row_stride;
     T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
-    if (w == 0.0f) return skip_row<T, NT, kGrad>(a, n, dx);
+    if (w == 0.0f) return clear<T, NT>(dx, begin, end);
     const float2 ms = a.stats[n];
     __shared__ RowResult shared;
     if (threadIdx.x == 0) shared = row_scalars<kGrad>(a, n, row_inputs<T, kGrad>(a, n), w, ms.x, ms.y);
     __syncthreads();
-    const RowResult q = shared;
-    const Frame f = frame(ms.x, a.c);
-    const int64_t y = id_at(a.targets, n, a.target_bytes);
-    for (int64_t i = static_cast<int64_t>(threadIdx.x) * N; i < V; i += int64_t{NT} * N) {
+    write_gradient<T, NT>(x, dx, begin, end, shared, frame(ms.x, a.c), id_at(a.targets, n, a.target_bytes));
+}
+
+// m and s of one slice of a row.
+constexpr int kSliceBlock = 256;
+template <typename T>
+__global__ __launch_bounds__(kSliceBlock) void slice_kernel(PolicyArgs a) {
+    constexpr int N = 16 / sizeof(T);
+    const uint32_t n = blockIdx.x / a.slices, part = blockIdx.x - n * a.slices, t = threadIdx.x;
+    if (weight_at(a.mask, a.mask_kind, n) == 0.0f) return;
+    const T* x = static_cast<const T*>(a.logits) + n * a.row_stride;
+    const int64_t begin = part * a.slice, end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
+    const int64_t full = end > begin ? begin + (end - begin) / N * N : begin;
+    if (part == 0 && t == 0) a.picked[n] = row_inputs<T, kLogp>(a, n).x;
+    Running r;
+    if (full + t < end) {
+        const float v[1] = {static_cast<float>(x[full + t])};
+        take<1>(r, v, a.c);
+    }
+#pragma unroll 4
+    for (int64_t i = begin + static_cast<int64_t>(t) * N; i < full; i += kSliceBlock * N) {
         float v[N];
-        load_some<N>(v, x + i, V - i);
-        to_gradient<N>(v, q, f, y, i);
-        store_some<N>(dx + i, v, V - i);
+        load<N>(v, x + i);
+        take<N>(r, v, a.c);
+    }
+    r = join_block<kSliceBlock>(r);
+    if (t == 0) a.parts[blockIdx.x] = make_float4(r.m, r.s, r.offset, 0.0f);
+}
+
+// Joins a row's slices in their order of lanes, and does what the mode asks: a
+// work-group a row, or, for the gradient, a slice.
+template <typename T, Mode MODE>
+__global__ __launch_bounds__(kSliceBlock) void finish_kernel(PolicyArgs a) {
+    constexpr bool kWithGrad = MODE == kLossGrad;
+    const uint32_t n = kWithGrad ? blockIdx.x / a.slices : blockIdx.x, part = kWithGrad ? blockIdx.x - n * a.slices : 0;
+    const float w = weight_at(a.mask, a.mask_kind, n);
+    const int64_t begin = part * a.slice, end = begin + a.slice < a.vocab ? begin + a.slice : a.vocab;
+    T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
+    if (w == 0.0f) {
+        if (part == 0 && threadIdx.x == 0) {
+            a.log_probs[n] = 0.0f;
+            if (MODE != kLogp) a.terms[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        if constexpr (kWithGrad) clear<T, kSliceBlock>(dx, begin, end);
+        return;
+    }
+    __shared__ RowResult shared;
+    __shared__ float top;
+    if (threadIdx.x < 64) {
+        Running r;
+        for (uint32_t i = threadIdx.x; i < a.slices; i += 64) {
+            const float4 p = a.parts[n * a.slices + i];
+            Running q;
+            q.m = p.x, q.s = p.y, q.offset = p.z;
+            r = join(r, q);
+        }
+        r = join_block<64>(r);
+        if (threadIdx.x == 0) {
+            RowInputs in = row_inputs<T, MODE>(a, n, false);  // the target's logit may be overwritten
+            in.x = a.picked[n];
+            shared = row_scalars<MODE>(a, n, in, w, r.m, r.s, part == 0);
+            top = r.m;
+        }
+    }
+    if constexpr (kWithGrad) {
+        __syncthreads();
+        write_gradient<T, kSliceBlock>(static_cast<const T*>(a.logits) + n * a.row_stride, dx, begin, end, shared,
+                                       frame(top, a.c), id_at(a.targets, n, a.target_bytes));
     }
 }
 
@@ -354,12 +437,44 @@ __global__ __launch_bounds__(kSumBlock) void policy_sum_kernel(const float4* ter
     }
 }
 
+// Slices of a row: rows too few for the chip's 256 CUs are cut, in 1,024 slices
+// together at most, where a row makes six slices of 8 vectors a thread or more; a
+// shorter one is done by a work-group of its own in the time of the second launch.
+// Kernels of loss and gradient in bf16, traced, in us, cut / whole: 4 rows of
+// 151,936 12.7 / 19.6, 60 rows 19.5 / 22.1; 8 rows of 50,304 11.4 / 10.4.  Log-
+// probabilities of one row of 151,936: 7.3 / 11.7.
+constexpr int64_t kSplitRows = 128, kSplitSlices = 1024;
+template <typename T>
+void cut(PolicyArgs& a) {
+    constexpr int64_t N = 16 / sizeof(T);
+    const int64_t most = (a.vocab / N + 2047) / 2048;
+    a.slices = 1, a.slice = a.vocab;
+    if (a.rows >= kSplitRows || most < 6 || a.parts == nullptr) return;
+    const int64_t slices = std::min(most, kSplitSlices / a.rows);
+    if (slices < 2) return;
+    a.slices = static_cast<uint32_t>(slices);
+    a.slice = ((a.vocab + slices - 1) / slices + N - 1) / N * N;
+}
+
 // The kernel for rows of this length: threads enough to keep a row's loads in
 // flight, few enough that short rows do not idle.
 template <typename T, Mode MODE>
 int launch_rows(PolicyArgs a, hipStream_t s) {
     constexpr int N = 16 / sizeof(T);
     const int64_t most = max_blocks(1024), vecs = a.vocab / N;
+    cut<T>(a);
+    if (a.slices > 1) {
+        const dim3 every(static_cast<uint32_t>(a.rows * a.slices)), block(kSliceBlock);
+        if constexpr (MODE == kGrad) {
+            hipLaunchKernelGGL((grad_kernel<T, kSliceBlock>), every, block, 0, s, a);
+        } else {
+            hipLaunchKernelGGL((slice_kernel<T>), every, block, 0, s, a);
+            if (int rc = launched("slice_kernel")) return rc;
+            if (MODE == kLossGrad) hipLaunchKernelGGL((finish_kernel<T, MODE>), every, block, 0, s, a);
+            else hipLaunchKernelGGL((finish_kernel<T, MODE>), dim3(static_cast<uint32_t>(a.rows)), dim3(64), 0, s, a);
+        }
+        return launched("policy_loss");
+    }
     for (a.first_row = 0; a.first_row < a.rows; a.first_row += most) {
         const dim3 grid(static_cast<uint32_t>(a.rows - a.first_row < most ? a.rows - a.first_row : most));
         const auto cached = [&](auto threads, auto held) {
@@ -391,6 +506,8 @@ int check(const mgopt_policy_args* p, const char* what) {
     if (p->mask_kind < MGOPT_MASK_NONE || p->mask_kind > MGOPT_MASK_F32) return set_error(MGOPT_E_INVALID, w + ": bad mask kind");
     if (!(p->temperature > 0.0) || !std::isfinite(p->temperature))
         return set_error(MGOPT_E_INVALID, w + ": the temperature must be positive and finite");
+    if (p->workspace_dev && reinterpret_cast<uintptr_t>(p->workspace_dev) % 16 != 0)
+        return set_error(MGOPT_E_ALIGN, w + ": the workspace must be 16-byte aligned");
     if (p->rows > 0 && (!p->logits_dev || !p->targets_dev || !p->log_probs_dev))
         return set_error(MGOPT_E_INVALID, w + ": NULL argument");
     if ((p->mask_kind != MGOPT_MASK_NONE) != (p->mask_dev != nullptr) && p->rows > 0)
@@ -403,8 +520,7 @@ int check_loss(const mgopt_policy_args* p, const char* what) {
     if (int rc = check(p, what)) return rc;
     const std::string w(what);
     if (!(p->clip_low >= 0.0) || !(p->clip_high >= 0.0)) return set_error(MGOPT_E_INVALID, w + ": negative clip range");
-    if (!p->workspace_dev || reinterpret_cast<uintptr_t>(p->workspace_dev) % 16 != 0)
-        return set_error(MGOPT_E_ALIGN, w + ": the workspace must be 16-byte aligned");
+    if (!p->workspace_dev) return set_error(MGOPT_E_ALIGN, w + ": no workspace");
     if (p->rows > 0 && (!p->old_logp_dev || !p->advantages_dev)) return set_error(MGOPT_E_INVALID, w + ": NULL argument");
     return 0;
 }
@@ -418,12 +534,14 @@ PolicyArgs args_of(const mgopt_policy_args* p) {
     a.inv_temp = 1.0 / p->temperature, a.c = static_cast<float>(1.4426950408889634 / p->temperature);
     a.grad_scale = p->grad_scale_dev, a.log_probs = p->log_probs_dev;
     a.d_logits = p->d_logits_dev, a.d_stride = p->d_logits_stride;
-    // workspace: the sum of the weights, then the rows' terms, then their m and s
+    // workspace: the sum of the weights, then the rows' terms, then their m and s, then the slices' and the targets' logits
     char* at = static_cast<char*>(p->workspace_dev);
     if (at != nullptr) {
         a.weight_sum = p->mask_kind == MGOPT_MASK_NONE ? nullptr : reinterpret_cast<const double*>(at);
         a.terms = reinterpret_cast<float4*>(at + 16);
         a.stats = reinterpret_cast<float2*>(at + 16 + 16 * p->rows);
+        a.parts = reinterpret_cast<float4*>(at + 16 + (24 * p->rows + 15) / 16 * 16);
+        a.picked = reinterpret_cast<float*>(a.parts + kSplitSlices);
     }
     return a;
 }
@@ -435,7 +553,11 @@ using namespace mgopt;
 
 extern "C" {
 
-MGOPT_API int64_t mgopt_policy_workspace(int64_t rows) { return rows < 0 ? -1 : 16 + 24 * rows; }
+MGOPT_API int64_t mgopt_policy_workspace(int64_t rows) {
+    // as args_of lays it out; few rows may be cut in slices
+    const int64_t cuts = rows < kSplitRows ? 16 * kSplitSlices + 4 * kSplitRows : 0;
+    return rows < 0 ? -1 : 16 + (24 * rows + 15) / 16 * 16 + cuts;
+}
 
 MGOPT_API int mgopt_token_log_probs(const mgopt_policy_args* p, void* stream) {
     if (int rc = check(p, "token_log_probs")) return rc;

@@ -248,6 +248,28 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(r.loss, want.loss) and bool((grad[:-5:1000] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 7, 127, 128])
+def test_few_long_rows(dtype, rows):
+    """Rows cut in slices, and one row more than is cut: in place, where one
+    slice's gradient overwrites logits that others have read, and by autograd."""
+    V = 90_007 if dtype != "f32" else 60_013
+    case("policy_loss", dtype, "rows", rows, "vocab", V)
+    s = make(rows, V, dtype, rows, mask="bool" if rows > 2 else None)
+    given = (s["targets"], s["old_logp"], s["advantages"])
+    more = {"ref_logp": s["ref_logp"], "mask": s["mask"], "clip": CLIP, "kl_coef": KL}
+    r, grad = mg.policy_loss_grad(s["logits"], *given, **more)
+    check(s, r, grad)
+    copy = s["logits"].clone()
+    again, g = mg.policy_loss_grad(copy, *given, out=copy, **more)
+    assert torch.equal(copy, grad) and all(torch.equal(a, b) for a, b in zip(again, r))
+    assert torch.equal(mg.token_log_probs(s["logits"], s["targets"], mask=s["mask"]), r.log_probs)
+    s["logits"].requires_grad_(True)
+    r = mg.policy_loss(s["logits"], *given, **more)
+    r.loss.backward()
+    check(s, r, s["logits"].grad)
+
+
 def test_many_rows():
     s = make(40_000, 11, "f32", 5, mask="float")
     r, grad = mg.policy_loss_grad(s["logits"], s["targets"], s["old_logp"], s["advantages"], ref_logp=s["ref_logp"],
