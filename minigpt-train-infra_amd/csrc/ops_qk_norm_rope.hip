@@ -30,10 +30,13 @@ constexpr int kWaves = kRopeBlock / 64;
 constexpr int kMaxDim = MGOPT_MAX_HEAD_DIM;
 constexpr uint32_t kBackwardBlocks = 2048;  // work-groups of the backward pass at most, a row of partial weight gradients each
 
+constexpr uint64_t kMaxTasks = uint64_t{1} << 31;  // tokens times the groups that share a token
+
 struct Args {
     mgopt_qk_args a;
     uint32_t tokens;
-    uint32_t lanes;   // of a head: a power of two
+    uint32_t lanes;   // of a head: 1 << shift
+    uint32_t shift;
     uint32_t parts;   // groups that share a token's heads
     // backward
     uint32_t q_parts, k_parts, q_blocks;
@@ -142,8 +145,8 @@ __device__ __forceinline__ int64_t offset(const int64_t (&stride)[3], const Toke
 
 template <typename T, int VEC, int SLOTS, bool INTER>
 __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_kernel(Args k) {
-    const uint64_t group = (static_cast<uint64_t>(blockIdx.x) * kRopeBlock + threadIdx.x) / k.lanes;
-    const uint32_t n = static_cast<uint32_t>(group / k.parts), part = static_cast<uint32_t>(group - static_cast<uint64_t>(n) * k.parts);
+    const uint32_t group = blockIdx.x * (kRopeBlock >> k.shift) + (threadIdx.x >> k.shift);
+    const uint32_t n = group / k.parts, part = group - n * k.parts;
     if (n >= k.tokens) return;  // whole groups of lanes
     const Token t = token_of(k, n);
     const uint32_t l = threadIdx.x & (k.lanes - 1);
@@ -203,7 +206,7 @@ __global__ __launch_bounds__(kRopeBlock, 4) void qk_norm_rope_backward_kernel(Ar
     const mgopt_heads& side = on_q ? k.a.q : k.a.k;
     const uint32_t block = on_q ? blockIdx.x : blockIdx.x - k.q_blocks, blocks = on_q ? k.q_blocks : gridDim.x - k.q_blocks;
     const uint32_t heads = static_cast<uint32_t>(side.heads);
-    const uint32_t lane = threadIdx.x % 64, l = lane & (k.lanes - 1), groups = kRopeBlock / k.lanes;
+    const uint32_t lane = threadIdx.x % 64, l = lane & (k.lanes - 1), groups = kRopeBlock >> k.shift;
     const uint32_t parts = on_q ? k.q_parts : k.k_parts;
     const float inv_dim = 1.0f / static_cast<float>(k.a.dim);
     Slot q[SLOTS];
@@ -215,10 +218,9 @@ __global__ __launch_bounds__(kRopeBlock, 4) void qk_norm_rope_backward_kernel(Ar
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sum_w[i].a[j] = sum_w[i].b[j] = 0.0f;
     }
-    const uint64_t tasks = static_cast<uint64_t>(k.tokens) * parts;
-    for (uint64_t task = static_cast<uint64_t>(block) * groups + threadIdx.x / k.lanes; task < tasks;
-         task += static_cast<uint64_t>(blocks) * groups) {
-        const uint32_t n = static_cast<uint32_t>(task / parts), part = static_cast<uint32_t>(task - static_cast<uint64_t>(n) * parts);
+    const uint32_t tasks = k.tokens * parts;
+    for (uint32_t task = block * groups + (threadIdx.x >> k.shift); task < tasks; task += blocks * groups) {
+        const uint32_t n = task / parts, part = task - n * parts;
         const Token t = token_of(k, n);
         float c[SLOTS][VEC], d[SLOTS][VEC];
 #pragma unroll
@@ -342,8 +344,9 @@ template <bool BACKWARD, typename F>
 int with_form(const mgopt_qk_args& a, Args& k, F&& f) {
     auto shape = [&](int vec, int slots) {
         const int pieces = (a.dim + 2 * vec - 1) / (2 * vec);
-        k.lanes = 1;
-        while (static_cast<int>(k.lanes) * slots < pieces) k.lanes <<= 1;
+        k.shift = 0;
+        while ((1 << k.shift) * slots < pieces) ++k.shift;
+        k.lanes = 1u << k.shift;
         // groups that share a token's heads: four heads each, for the use of one token's cosines, or fewer while
         // that leaves the chip short of waves
         const int64_t groups = 64 / k.lanes;
@@ -391,8 +394,10 @@ MGOPT_API int mgopt_qk_norm_rope(const mgopt_qk_args* a, void* stream) {
     k.tokens = static_cast<uint32_t>(a->batch * a->length);
     return with_form<false>(*a, k, [&](auto t, auto vec, auto slots, auto inter) {
         using T = decltype(t);
-        const uint64_t groups = kRopeBlock / k.lanes, blocks = (static_cast<uint64_t>(k.tokens) * k.parts + groups - 1) / groups;
-        if (blocks > max_blocks(kRopeBlock)) return set_error(MGOPT_E_LIMIT, "qk_norm_rope: too many heads");
+        const uint64_t groups = kRopeBlock / k.lanes, tasks = static_cast<uint64_t>(k.tokens) * k.parts;
+        const uint64_t blocks = (tasks + groups - 1) / groups;
+        if (tasks > kMaxTasks || blocks > max_blocks(kRopeBlock))
+            return set_error(MGOPT_E_LIMIT, "qk_norm_rope: too many heads");
         hipLaunchKernelGGL((qk_norm_rope_kernel<T, decltype(vec)::value, decltype(slots)::value, decltype(inter)::value>),
                            dim3(static_cast<uint32_t>(blocks)), dim3(kRopeBlock), 0, static_cast<hipStream_t>(stream), k);
         return launched("qk_norm_rope_kernel");
@@ -421,6 +426,8 @@ MGOPT_API int mgopt_qk_norm_rope_backward(const mgopt_qk_args* a, void* stream) 
     if (k.tokens > 0) {
         const int rc = with_form<true>(*a, k, [&](auto t, auto vec, auto slots, auto inter) {
             using T = decltype(t);
+            if (static_cast<uint64_t>(k.tokens) * std::max(k.q_parts, k.k_parts) > kMaxTasks)
+                return set_error(MGOPT_E_LIMIT, "qk_norm_rope_backward: too many heads");
             // work-groups by the sides' shares of the heads, each no more than it has work for
             const auto blocks_for = [&](uint32_t parts, uint32_t share) {
                 const uint64_t groups = kRopeBlock / k.lanes, tasks = static_cast<uint64_t>(k.tokens) * parts;
