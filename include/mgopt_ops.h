@@ -42,7 +42,8 @@ MGOPT_API int64_t mgopt_embedding_grad_workspace(int64_t n, int64_t rows, int64_
  * read and written, otherwise every row is written.  grad_out is [n][width],
  * grad [rows][width], both contiguous.  Ids outside [0, rows) and equal to
  * padding_idx (-1: none) add nothing.  workspace_dev:
- * mgopt_embedding_grad_workspace bytes, 16-byte aligned. */
+ * mgopt_embedding_grad_workspace bytes, 16-byte aligned.  Fewer than 2^30 ids
+ * and 2^31 rows (MGOPT_E_LIMIT). */
 MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_t n, const void* grad_out_dev,
                                    int32_t grad_out_dtype, void* grad_dev, int32_t grad_dtype, int64_t rows,
                                    int64_t width, float scale, int64_t padding_idx, int32_t accumulate,

@@ -514,12 +514,10 @@ __global__ __launch_bounds__(kBlock) void join_pieces_kernel(SumArgs a) {
 //   1,024   96     768     17.2 / 14.1   117.8 / 16.4
 //   64      16,000 4,096   29.8 / 25.6    41.1 / 26.4
 //   16      50,304 768     43.5 / 18.4    43.5 / 19.1
-// Lists and weights beyond 30 and 31 bits are not sorted at all.
 constexpr int64_t kByRowWork = int64_t{1} << 19;   // rows * tokens
 constexpr int64_t kByRowTerms = int64_t{1} << 17;  // tokens * width
 bool by_row(int64_t n, int64_t rows, int64_t width) {
-    if (n == 0 || n >= (int64_t{1} << 30) || rows >= (int64_t{1} << 31)) return true;
-    return rows <= kByRowWork / n && width <= kByRowTerms / n;
+    return n == 0 || (rows <= kByRowWork / n && width <= kByRowTerms / n);
 }
 
 // Up to here one work-group sorts the whole list: at 8,183 tokens that takes
@@ -639,6 +637,12 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
                 }
                 return 0;
             }
+            if (n >= (int64_t{1} << 30) || rows >= (int64_t{1} << 31))
+                return set_error(MGOPT_E_LIMIT, "embedding_grad: more than 2^30 tokens or 2^31 rows");
+            const int64_t pieces = (n + piece_for(n, width) - 1) / piece_for(n, width), per_block = kBlock >> shift;
+            const int64_t blocks = (pieces + per_block - 1) / per_block * chunks, join_chunks = (vecs + 63) / 64;
+            if (blocks > max_blocks(kBlock) || join_chunks > max_blocks(kBlock) / pieces)
+                return set_error(MGOPT_E_LIMIT, "embedding_grad: too many tokens of long rows");
             const Work work = work_of(n, width);
             char* const at = static_cast<char*>(workspace_dev);
             const auto list = [&](int64_t offset) { return reinterpret_cast<uint32_t*>(at + offset); };
@@ -693,17 +697,13 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
             SumArgs m{list(work.keys[side ^ 1]), list(work.tokens[side ^ 1]), grad_out_dev, grad_dev,
                       reinterpret_cast<float*>(at + work.partials), rows, width, static_cast<uint32_t>(n), piece_for(n, width), 0, shift,
                       static_cast<uint32_t>(chunks), accumulate, scale};
-            m.pieces = static_cast<uint32_t>((n + m.piece - 1) / m.piece);
-            const int64_t per_block = kBlock >> shift, blocks = (m.pieces + per_block - 1) / per_block * chunks;
-            if (blocks > max_blocks(kBlock)) return set_error(MGOPT_E_LIMIT, "embedding_grad: too many tokens of long rows");
+            m.pieces = static_cast<uint32_t>(pieces);
             if (shift >= 6)
                 hipLaunchKernelGGL((sum_pieces_kernel<TG, TW, true>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, m);
             else
                 hipLaunchKernelGGL((sum_pieces_kernel<TG, TW, false>), dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, m);
             if (int rc = launched("sum_pieces_kernel")) return rc;
-            m.chunks = static_cast<uint32_t>((vecs + 63) / 64);
-            if (static_cast<int64_t>(m.chunks) * m.pieces > max_blocks(kBlock))
-                return set_error(MGOPT_E_LIMIT, "embedding_grad: too many tokens of long rows");
+            m.chunks = static_cast<uint32_t>(join_chunks);
             hipLaunchKernelGGL((join_pieces_kernel<N, TW>), dim3(m.pieces * m.chunks), dim3(kBlock), 0, s, m);
             if (int rc = launched("join_pieces_kernel")) return rc;
             return 0;

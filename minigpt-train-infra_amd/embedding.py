@@ -21,7 +21,8 @@ def embedding_grad_(grad: torch.Tensor, ids: torch.Tensor, grad_out: torch.Tenso
     the output projection, or a later micro-batch, costs no pass over the whole
     gradient.  accumulate=False writes every row instead, zeros where no id
     names it.  grad_out: ids.shape + (width,), of grad's dtype or another of the
-    three.  Ids outside the rows and equal to padding_idx add nothing."""
+    three.  Ids outside the rows and equal to padding_idx add nothing.  Fewer than
+    2^30 ids and 2^31 rows."""
     N.ops().embedding_grad(grad, ids, grad_out, scale, padding_idx, accumulate, N.ops_stream(grad))
     return grad
 

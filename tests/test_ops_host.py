@@ -71,6 +71,8 @@ def test_embedding_rejects_bad_arguments(native):
         _refused(lib, grad(**bad), E_INVALID, b"embedding_grad")
     for bad in (dict(work=None), dict(work=P + 8)):
         _refused(lib, grad(**bad), E_ALIGN, b"workspace")
+    for bad in (dict(n=2**30), dict(rows=2**31, n=1000), dict(n=2**29, width=2**20)):
+        _refused(lib, grad(**bad), E_LIMIT, b"embedding_grad")
     assert lookup(n=0) == 0 and grad(n=0) == 0
 
 
@@ -171,6 +173,10 @@ def test_qk_norm_rope_rejects_bad_arguments(native):
             _refused(lib, call(_qk(side, heads=2**21), vp(None)), E_LIMIT, b"heads")
         _refused(lib, call(None, vp(None)), E_INVALID, b"NULL")
     _refused(lib, forward(_qk("k", out=None), vp(None)), E_INVALID, b"NULL")
+    for call in (forward, backward):
+        many = _qk(batch=2**10, length=2**18)._obj
+        many.q.heads = 2**20
+        _refused(lib, call(ctypes.byref(many), vp(None)), E_LIMIT, b"too many heads")
     for bad in (dict(grad=None), dict(d_x=None), dict(d_weight=None)):
         _refused(lib, backward(_qk("q", **bad), vp(None)), E_INVALID, b"NULL")
     _refused(lib, backward(_qk(workspace=None), vp(None)), E_ALIGN, b"workspace")
