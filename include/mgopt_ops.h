@@ -176,7 +176,7 @@ typedef struct mgopt_policy_args {
     double clip_low;
     double clip_high;
     double kl_coef;
-    double temperature;
+    double temperature; /* from 2^-120 to 2^120 */
     int32_t dtype;
     int32_t target_bytes;
     int32_t mask_kind;

@@ -385,7 +385,7 @@ Policy policy_args(const Tensor& logits, const Tensor& targets, const optional<T
     on_gpu(logits, "logits");
     p.a.dtype = code_of(logits, "logits");
     if (logits.dim() < 1 || logits.size(-1) < 1) refuse("logits need a last dimension of at least 1, got " + shape_of(logits));
-    if (!(temperature > 0.0) || !std::isfinite(temperature)) refuse("the temperature must be positive and finite");
+    if (!(temperature >= 0x1p-120 && temperature <= 0x1p120)) refuse("the temperature must lie between 2^-120 and 2^120");
     p.logits = rows_of(logits);
     const int64_t rows = p.logits.rows;
     if (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt)

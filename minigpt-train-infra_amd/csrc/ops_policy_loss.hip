@@ -17,13 +17,10 @@
 // and a sum s of powers of two; the row's scalars are formed once, in 64 bits; a
 // second pass writes the gradient.  Rows of weight 0 are not read.
 //
-// With c = log2(e) / T and B the integer nearest to m c, s = sum 2^(x c - B):
-// one fused multiply-add forms the exponent with one rounding, of the exponent
-// itself, and sums of other B are joined by exact powers of two.  Where m c
-// passes 2^100 -- a row of the type's lowest value, or a largest one -- all
-// that differs from m is further from it than any exponent reaches, so 1/4
-// takes c's place, which keeps the products finite: what equals m counts 1,
-// all else 0.
+// With c = log2(e) / T, s = sum 2^((x - m) c): the difference is formed first.
+// One fused multiply-add of x c and a rounded m c is an instruction less (153 us
+// for 156 below), but off by m c's rounding, which passes every exponent where
+// m c passes 2^32: a row of -1e10, or a small temperature.
 //
 // A row is held in registers between the passes (cached_kernel), as it came, so
 // that it is read once; what does not fit is read again.  Few long rows are cut
@@ -31,15 +28,13 @@
 // them (finish_kernel).
 //
 // Bound by memory: a row's logits once, its gradient once.  8,192 rows of 50,304
-// bf16: log-probabilities 154 us (5.4 TB/s).  4,096 rows of 151,936 bf16, a quarter
+// bf16: log-probabilities 156 us (5.3 TB/s).  4,096 rows of 151,936 bf16, a quarter
 // of weight 0: loss and gradient 431 us (5.1 TB/s); one such row fills a CU's
 // registers, so that its read, its join and its write follow each other.
 #include "ops_common.h"
 
 namespace mgopt {
 namespace {
-
-constexpr double kLn2 = 0.6931471805599453;
 
 enum Mode { kLogp, kLoss, kLossGrad, kGrad };
 
@@ -51,7 +46,7 @@ struct PolicyArgs {
     const float *old_logp, *ref_logp, *advantages;
     const void* mask;
     double low, high, kl_coef, inv_temp;
-    float c;                     // log2(e) / T
+    float c;                     // log2(e) / T, a normal number
     const float* grad_scale;     // may be NULL
     const double* weight_sum;    // NULL: every row's weight is 1
     float* log_probs;
@@ -61,7 +56,7 @@ struct PolicyArgs {
     int64_t d_stride;
     uint32_t slices = 1;         // of a row
     int64_t slice;               // elements of one
-    float4* parts;               // m, s and offset of each slice
+    float2* parts;               // m and s of each slice
     float* picked;               // the targets' logits: a gradient in place may overwrite them before another slice is done
 };
 
@@ -71,47 +66,38 @@ __device__ __forceinline__ float weight_at(const void* mask, int32_t kind, int64
     return static_cast<const float*>(mask)[n];
 }
 
-// The exponents' factor and offset (-B) at maximum m.  Without a maximum yet
-// (-inf) the offset is finite, so that -inf - -inf does not occur: -inf then
+// The maximum starts at the lowest finite value: -inf - -inf does not occur, -inf
 // counts 0, and a row of nothing else has s = 0, whose log is -inf.
-struct Frame {
-    float c, offset;
-};
-__device__ __forceinline__ Frame frame(float m, float c) {
-    const float k = fabsf(m * c) < 0x1p100f ? c : 0.25f;
-    return {k, m == -INFINITY ? 3e38f : -rintf(m * k)};
-}
 struct Running {
-    float m = -INFINITY, s = 0.0f, offset = 3e38f;  // of frame(m)
+    float m = -3.402823466e38f, s = 0.0f;
 };
-__device__ __forceinline__ Running join(Running a, Running b) {
-    const bool up = b.m > a.m;
-    const float o = up ? b.offset : a.offset;
-    return {up ? b.m : a.m, a.s * exp2_hw(o - a.offset) + b.s * exp2_hw(o - b.offset), o};
+__device__ __forceinline__ Running join(Running a, Running b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    return {m, a.s * exp2_hw((a.m - m) * c) + b.s * exp2_hw((b.m - m) * c)};
 }
 template <int N>
 __device__ __forceinline__ void take(Running& r, const float (&x)[N], float c) {
+    float m = r.m;
 #pragma unroll
-    for (int i = 0; i < N; ++i) r.m = fmaxf(r.m, x[i]);
-    const Frame f = frame(r.m, c);
-    r.s *= exp2_hw(f.offset - r.offset);
-    r.offset = f.offset;
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+    r.s *= exp2_hw((r.m - m) * c);
+    r.m = m;
 #pragma unroll
-    for (int i = 0; i < N; ++i) r.s += exp2_hw(fmaf(x[i], f.c, f.offset));
+    for (int i = 0; i < N; ++i) r.s += exp2_hw((x[i] - m) * c);
 }
 
 template <int NT>
-__device__ __forceinline__ Running join_block(Running r) {
+__device__ __forceinline__ Running join_block(Running r, float c) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) r = join(r, Running{__shfl_xor(r.m, off), __shfl_xor(r.s, off), __shfl_xor(r.offset, off)});
+    for (int off = 1; off < 64; off <<= 1) r = join(r, Running{__shfl_xor(r.m, off), __shfl_xor(r.s, off)}, c);
     if constexpr (NT > 64) {
-        __shared__ float part_m[NT / 64], part_s[NT / 64], part_o[NT / 64];
+        __shared__ float part_m[NT / 64], part_s[NT / 64];
         const int wave = threadIdx.x / 64;
-        if (threadIdx.x % 64 == 0) part_m[wave] = r.m, part_s[wave] = r.s, part_o[wave] = r.offset;
+        if (threadIdx.x % 64 == 0) part_m[wave] = r.m, part_s[wave] = r.s;
         __syncthreads();
-        r = {part_m[0], part_s[0], part_o[0]};
+        r = {part_m[0], part_s[0]};
 #pragma unroll 1
-        for (int i = 1; i < NT / 64; ++i) r = join(r, Running{part_m[i], part_s[i], part_o[i]});
+        for (int i = 1; i < NT / 64; ++i) r = join(r, Running{part_m[i], part_s[i]}, c);
     }
     return r;
 }
@@ -141,7 +127,7 @@ __device__ __forceinline__ RowInputs row_inputs(const PolicyArgs& a, int64_t n, 
 }
 
 struct RowResult {
-    float slope, k;  // of the gradient: slope * [j = y] + k * 2^(x c - B)
+    float slope, k;  // of the gradient: slope * [j = y] + k * 2^((x - m) c)
 };
 
 // What one row adds to the loss, and its slope, from m and s.
@@ -152,11 +138,7 @@ __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs
     if constexpr (MODE == kGrad) {
         logp = a.log_probs[n];
     } else {
-        // to the maximum exactly, and from there as the sum was formed
-        const Frame f = frame(m, a.c);
-        logp = (static_cast<double>(in.x) - static_cast<double>(m)) * a.inv_temp +
-               fma(static_cast<double>(m), static_cast<double>(f.c), static_cast<double>(f.offset)) * kLn2 -
-               log(static_cast<double>(s));
+        logp = (static_cast<double>(in.x) - static_cast<double>(m)) * a.inv_temp - log(static_cast<double>(s));
         if (write) a.log_probs[n] = static_cast<float>(logp);
     }
     if constexpr (MODE == kLogp) return {};
@@ -197,9 +179,9 @@ __device__ __forceinline__ void skip_row(const PolicyArgs& a, int64_t n, T* dx) 
 
 // One vector of the gradient, from column i on.
 template <int N>
-__device__ __forceinline__ void to_gradient(float (&v)[N], const RowResult& q, const Frame& f, int64_t y, int64_t i) {
+__device__ __forceinline__ void to_gradient(float (&v)[N], const RowResult& q, float m, float c, int64_t y, int64_t i) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = q.k * exp2_hw(fmaf(v[j], f.c, f.offset));
+    for (int j = 0; j < N; ++j) v[j] = q.k * exp2_hw((v[j] - m) * c);
     if (y >= i && y < i + N) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -210,12 +192,12 @@ __device__ __forceinline__ void to_gradient(float (&v)[N], const RowResult& q, c
 // The gradient of columns begin to end, from their logits.
 template <typename T, int NT>
 __device__ __forceinline__ void write_gradient(const T* x, T* dx, int64_t begin, int64_t end, const RowResult& q,
-                                               const Frame& f, int64_t y) {
+                                               float m, float c, int64_t y) {
     constexpr int N = 16 / sizeof(T);
     for (int64_t i = begin + static_cast<int64_t>(threadIdx.x) * N; i < end; i += int64_t{NT} * N) {
         float v[N];
         load_some<N>(v, x + i, end - i);
-        to_gradient<N>(v, q, f, y, i);
+        to_gradient<N>(v, q, m, c, y, i);
         store_some<N>(dx + i, v, end - i);
     }
 }
@@ -275,13 +257,12 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
             take<N>(r, v, a.c);
         }
     }
-    r = join_block<NT>(r);
+    r = join_block<NT>(r, a.c);
     __shared__ RowResult shared;
     if (t == 0) shared = row_scalars<MODE>(a, n, in, w, r.m, r.s);
     if constexpr (MODE != kLossGrad) return;
     __syncthreads();
     const RowResult q = shared;
-    const Frame f = frame(r.m, a.c);
     const int64_t y = id_at(a.targets, n, a.target_bytes);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -290,7 +271,7 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         float v[N];
         widen<T, N>(v, raw[i]);
-        to_gradient<N>(v, q, f, y, static_cast<int64_t>(at) * N);
+        to_gradient<N>(v, q, r.m, a.c, y, static_cast<int64_t>(at) * N);
         store_nt<N>(dx + static_cast<int64_t>(at) * N, v);
     }
     if constexpr (LONG) {
@@ -298,12 +279,12 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
         for (int64_t i = int64_t{NV} * NT + t; i < full; i += NT) {
             float v[N];
             load<N>(v, x + i * N);
-            to_gradient<N>(v, q, f, y, i * N);
+            to_gradient<N>(v, q, r.m, a.c, y, i * N);
             store_nt<N>(dx + i * N, v);
         }
     }
     if (t < tail) {
-        to_gradient<1>(last, q, f, y, full * N + t);
+        to_gradient<1>(last, q, r.m, a.c, y, full * N + t);
         dx[full * N + t] = static_cast<T>(last[0]);
     }
 }
@@ -324,7 +305,7 @@ __global__ __launch_bounds__(NT) void grad_kernel(PolicyArgs a) {
     __shared__ RowResult shared;
     if (threadIdx.x == 0) shared = row_scalars<kGrad>(a, n, row_inputs<T, kGrad>(a, n), w, ms.x, ms.y);
     __syncthreads();
-    write_gradient<T, NT>(x, dx, begin, end, shared, frame(ms.x, a.c), id_at(a.targets, n, a.target_bytes));
+    write_gradient<T, NT>(x, dx, begin, end, shared, ms.x, a.c, id_at(a.targets, n, a.target_bytes));
 }
 
 // m and s of one slice of a row.
@@ -349,8 +330,8 @@ __global__ __launch_bounds__(kSliceBlock) void slice_kernel(PolicyArgs a) {
         load<N>(v, x + i);
         take<N>(r, v, a.c);
     }
-    r = join_block<kSliceBlock>(r);
-    if (t == 0) a.parts[blockIdx.x] = make_float4(r.m, r.s, r.offset, 0.0f);
+    r = join_block<kSliceBlock>(r, a.c);
+    if (t == 0) a.parts[blockIdx.x] = make_float2(r.m, r.s);
 }
 
 // Joins a row's slices in their order of lanes, and does what the mode asks: a
@@ -375,12 +356,10 @@ __global__ __launch_bounds__(kSliceBlock) void finish_kernel(PolicyArgs a) {
     if (threadIdx.x < 64) {
         Running r;
         for (uint32_t i = threadIdx.x; i < a.slices; i += 64) {
-            const float4 p = a.parts[n * a.slices + i];
-            Running q;
-            q.m = p.x, q.s = p.y, q.offset = p.z;
-            r = join(r, q);
+            const float2 p = a.parts[n * a.slices + i];
+            r = join(r, Running{p.x, p.y}, a.c);
         }
-        r = join_block<64>(r);
+        r = join_block<64>(r, a.c);
         if (threadIdx.x == 0) {
             RowInputs in = row_inputs<T, MODE>(a, n, false);  // the target's logit may be overwritten
             in.x = a.picked[n];
@@ -390,8 +369,8 @@ __global__ __launch_bounds__(kSliceBlock) void finish_kernel(PolicyArgs a) {
     }
     if constexpr (kWithGrad) {
         __syncthreads();
-        write_gradient<T, kSliceBlock>(static_cast<const T*>(a.logits) + n * a.row_stride, dx, begin, end, shared,
-                                       frame(top, a.c), id_at(a.targets, n, a.target_bytes));
+        write_gradient<T, kSliceBlock>(static_cast<const T*>(a.logits) + n * a.row_stride, dx, begin, end, shared, top,
+                                       a.c, id_at(a.targets, n, a.target_bytes));
     }
 }
 
@@ -507,8 +486,8 @@ int check(const mgopt_policy_args* p, const char* what) {
     if (p->rows < 0 || p->vocab < 1) return set_error(MGOPT_E_INVALID, w + ": need rows >= 0 and vocab >= 1");
     if (p->target_bytes != 4 && p->target_bytes != 8) return set_error(MGOPT_E_INVALID, w + ": targets have 4 or 8 bytes");
     if (p->mask_kind < MGOPT_MASK_NONE || p->mask_kind > MGOPT_MASK_F32) return set_error(MGOPT_E_INVALID, w + ": bad mask kind");
-    if (!(p->temperature > 0.0) || !std::isfinite(p->temperature))
-        return set_error(MGOPT_E_INVALID, w + ": the temperature must be positive and finite");
+    if (!(p->temperature >= 0x1p-120 && p->temperature <= 0x1p120))  // log2(e) / T is a normal 32-bit number
+        return set_error(MGOPT_E_INVALID, w + ": the temperature must lie between 2^-120 and 2^120");
     if (p->workspace_dev && reinterpret_cast<uintptr_t>(p->workspace_dev) % 16 != 0)
         return set_error(MGOPT_E_ALIGN, w + ": the workspace must be 16-byte aligned");
     if (p->rows > 0 && (!p->logits_dev || !p->targets_dev || !p->log_probs_dev))
@@ -543,7 +522,7 @@ PolicyArgs args_of(const mgopt_policy_args* p) {
         a.weight_sum = p->mask_kind == MGOPT_MASK_NONE ? nullptr : reinterpret_cast<const double*>(at);
         a.terms = reinterpret_cast<float4*>(at + 16);
         a.stats = reinterpret_cast<float2*>(at + 16 + 16 * p->rows);
-        a.parts = reinterpret_cast<float4*>(at + 16 + (24 * p->rows + 15) / 16 * 16);
+        a.parts = reinterpret_cast<float2*>(at + 16 + (24 * p->rows + 15) / 16 * 16);
         a.picked = reinterpret_cast<float*>(a.parts + kSplitSlices);
     }
     return a;
@@ -558,7 +537,7 @@ extern "C" {
 
 MGOPT_API int64_t mgopt_policy_workspace(int64_t rows) {
     // as args_of lays it out; few rows may be cut in slices
-    const int64_t cuts = rows < kSplitRows ? 16 * kSplitSlices + 4 * kSplitRows : 0;
+    const int64_t cuts = rows < kSplitRows ? 8 * kSplitSlices + 4 * kSplitRows : 0;
     return rows < 0 ? -1 : 16 + (24 * rows + 15) / 16 * 16 + cuts;
 }
 

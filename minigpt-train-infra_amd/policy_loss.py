@@ -1,7 +1,7 @@
 """The clipped policy loss with a KL term, over the logits of a batch's tokens.
 
 With logp = log_softmax(logits / temperature)[target] of each row, ratio =
-exp(logp - old_logp) and r = ref_logp - logp:
+exp(logp - old_logp), r = ref_logp - logp and a temperature from 2^-120 to 2^120:
 
     policy = -min(ratio * A, clip(ratio, 1 - low, 1 + high) * A)
     kl     = exp(r) - r - 1

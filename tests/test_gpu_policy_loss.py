@@ -19,7 +19,7 @@ import math
 import pytest
 import torch
 
-from tests._ops import DEV, DTYPES, case, generator, mg, near, randn
+from tests._ops import DEV, DTYPES, ROUND, case, generator, mg, near, randn
 
 pytestmark = pytest.mark.gpu
 U = 2.0**-24
@@ -203,6 +203,34 @@ def test_infinities_and_lowest_values(dtype, V):
     part["old_logp"] = (torch.log_softmax(part["logits"].double(), -1)[:, 3] - 0.1).float()
     r, grad = mg.policy_loss_grad(part["logits"], part["targets"], part["old_logp"], part["advantages"], clip=CLIP)
     check(part, r, grad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, V", [(70, 300), (70, 30_000), (3, 151_937)])
+def test_logits_of_large_magnitude_and_small_temperatures(dtype, rows, V):
+    """Every result depends on the logits' differences alone, however large the
+    logits are: the oracle takes them less the row's largest, which 64 bits hold."""
+    t = DTYPES[dtype]
+    levels = [(60_000.0, 1e-6), (-60_000.0, 1e-6)] if dtype == "f16" else [(-1e10, 1.0), (-1e30, 1.0), (1e12, 0.7), (3e38, 1.0)]
+    for level, temperature in [*levels, (None, 1e-9), (None, 1e-30 if dtype != "f16" else 1e-6), (None, 1e9)]:
+        case("policy_loss", dtype, "rows", rows, "vocab", V, "level", level, "temperature", temperature)
+        s = make(rows, V, dtype, 17, ref=False)
+        if level is not None:  # the level, and in two of three columns a step or two below it
+            low = level - abs(level) * 4 * ROUND[t] * (torch.arange(V, device=DEV) % 3).double()
+            s["logits"] = low.to(t).expand(rows, V).contiguous()
+        s["targets"] = s["logits"].argmax(-1)
+        shifted = s["logits"].double() - s["logits"].double().amax(-1, keepdim=True)
+        s["old_logp"] = (torch.log_softmax(shifted / temperature, -1).gather(1, s["targets"][:, None])[:, 0] - 0.1).float()
+        scale = torch.tensor(temperature, device=DEV)
+        given, more = (s["logits"], s["targets"], s["old_logp"], s["advantages"]), {"clip": CLIP, "temperature": temperature}
+        oracle = {**s, "logits": shifted}
+        r, grad = mg.policy_loss_grad(*given, grad_scale=scale, **more)
+        check(oracle, r, grad, temperature, float(scale), kl_coef=0.0)
+        assert torch.equal(mg.token_log_probs(s["logits"], s["targets"], temperature=temperature), r.log_probs)
+        s["logits"].requires_grad_(True)
+        r = mg.policy_loss(*given, **more)
+        (r.loss * scale).backward()
+        check(oracle, r, s["logits"].grad, temperature, float(scale), kl_coef=0.0)
 
 
 def test_layouts_types_and_in_place():

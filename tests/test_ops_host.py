@@ -131,6 +131,16 @@ def test_policy_loss_rejects_bad_arguments(native):
     assert calls["log_probs"](_policy(rows=0)) == 0 and calls["backward"](_policy(rows=0)) == 0
 
 
+def test_policy_loss_rejects_temperatures_beyond_32_bits(native):
+    """log2(e) / T has to be a normal 32-bit number."""
+    lib, vp = native.load_library(), ctypes.c_void_p
+    for bad in (2.0**-121, 2.0**121, float("inf"), -1.0):
+        for rc in (lib.mgopt_token_log_probs(_policy(temperature=bad), vp(None)),
+                   lib.mgopt_policy_loss(_policy(temperature=bad), vp(P), vp(P), vp(None)),
+                   lib.mgopt_policy_loss_backward(_policy(temperature=bad), vp(None))):
+            _refused(lib, rc, E_INVALID, b"temperature")
+
+
 class Heads(ctypes.Structure):                 # mgopt_heads
     _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "out", "grad", "d_x", "d_weight")]
     _fields_ += [(n, ctypes.c_int64 * 3) for n in ("x_stride", "out_stride", "grad_stride", "d_x_stride")]
