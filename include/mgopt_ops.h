@@ -195,7 +195,7 @@ MGOPT_API int mgopt_token_log_probs(const mgopt_policy_args* args, void* stream)
  *   policy = -min(ratio * A, clip(ratio) * A)    kl = exp(r) - r - 1
  * loss_dev[0] = mean(policy) + kl_coef * mean(kl), parts_dev[0..2] =
  * mean(policy), mean(kl) and the share of rows whose gradient the clip holds at
- * 0, all weighted by the mask (0 where every weight is 0).  With d_logits_dev,
+ * 0, all weighted by the mask (0 where the weights' sum is 0).  With d_logits_dev,
  * also the gradient of grad_scale * loss, reading the logits once; without it,
  * the workspace keeps what mgopt_policy_loss_backward needs. */
 MGOPT_API int mgopt_policy_loss(const mgopt_policy_args* args, float* loss_dev, float* parts_dev, void* stream);

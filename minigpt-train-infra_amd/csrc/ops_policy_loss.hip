@@ -155,7 +155,8 @@ __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs
         a.terms[n] = make_float4(static_cast<float>(w * -(held ? s2 : s1)), static_cast<float>(w * kl), held ? w : 0.0f, 0.0f);
     if constexpr (MODE == kLoss) a.stats[n] = make_float2(m, s);
     if constexpr (MODE == kLoss) return {};
-    slope *= w / in.total * a.inv_temp * static_cast<double>(in.scale);
+    // where the weights' sum is 0 the loss is 0, and so is its gradient
+    slope = in.total == 0.0 ? 0.0 : slope * (w / in.total * a.inv_temp * static_cast<double>(in.scale));
     return {static_cast<float>(slope), static_cast<float>(-slope / static_cast<double>(s))};
 }
 
@@ -398,8 +399,8 @@ __global__ __launch_bounds__(kSumBlock) void weight_sum_kernel(const void* mask,
     if (threadIdx.x == 0) *out = x;
 }
 
-// loss, policy, kl, clipped share from the rows' terms.  Rows that all have
-// weight 0 make all four 0.
+// loss, policy, kl, clipped share from the rows' terms.  Weights whose sum is 0
+// make all four 0.
 __global__ __launch_bounds__(kSumBlock) void policy_sum_kernel(const float4* terms, int64_t rows, const double* weight_sum,
                                                                double kl_coef, float* loss, float* parts) {
     double p = 0.0, k = 0.0, h = 0.0;

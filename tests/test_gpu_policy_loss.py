@@ -233,6 +233,21 @@ def test_logits_of_large_magnitude_and_small_temperatures(dtype, rows, V):
         check(oracle, r, s["logits"].grad, temperature, float(scale), kl_coef=0.0)
 
 
+def test_weights_that_cancel():
+    """The weights' sum is 0 without a weight of 0: the means are 0, and their gradient."""
+    for rows, V in ((4, 300), (4, 151_937)):
+        s = make(rows, V, "bf16", 23)
+        mask = torch.tensor([1.0, -1.0, 0.5, -0.5], device=DEV)
+        given = (s["logits"], s["targets"], s["old_logp"], s["advantages"])
+        more = {"ref_logp": s["ref_logp"], "mask": mask, "clip": CLIP, "kl_coef": KL}
+        r, grad = mg.policy_loss_grad(*given, **more)
+        s["logits"].requires_grad_(True)
+        loss = mg.policy_loss(*given, **more).loss
+        loss.backward()
+        assert all(float(v) == 0 for v in (r.loss, r.policy, r.kl, r.clip_fraction, loss))
+        assert bool((grad == 0).all()) and bool((s["logits"].grad == 0).all())
+
+
 def test_layouts_types_and_in_place():
     s = make(30, 700, "bf16", 4, mask="bool")
     more = {"ref_logp": s["ref_logp"], "mask": s["mask"], "clip": CLIP, "kl_coef": KL}
