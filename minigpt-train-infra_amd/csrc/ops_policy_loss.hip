@@ -19,8 +19,9 @@
 //
 // With c = log2(e) / T, s = sum 2^((x - m) c): the difference is formed first.
 // One fused multiply-add of x c and a rounded m c is an instruction less (153 us
-// for 156 below), but off by m c's rounding, which passes every exponent where
-// m c passes 2^32: a row of -1e10, or a small temperature.
+// for 157, vectors taken singly, in the first case below), but off by m c's
+// rounding, which passes every exponent where m c passes 2^32: a row of -1e10, or
+// a small temperature.
 //
 // A row is held in registers between the passes (cached_kernel), as it came, so
 // that it is read once; what does not fit is read again.  Few long rows are cut
@@ -28,8 +29,8 @@
 // them (finish_kernel).
 //
 // Bound by memory: a row's logits once, its gradient once.  8,192 rows of 50,304
-// bf16: log-probabilities 156 us (5.3 TB/s).  4,096 rows of 151,936 bf16, a quarter
-// of weight 0: loss and gradient 431 us (5.1 TB/s); one such row fills a CU's
+// bf16: log-probabilities 154 us (5.3 TB/s).  4,096 rows of 151,936 bf16, a quarter
+// of weight 0: loss and gradient 436 us (5.0 TB/s); one such row fills a CU's
 // registers, so that its read, its join and its write follow each other.
 #include "ops_common.h"
 
@@ -216,7 +217,8 @@ __device__ __forceinline__ void widen(float (&v)[N], const Raw& raw) {
 // most NT * NV of them (and a tail of less than one) are read once; LONG: what
 // lies beyond is read again for the gradient.  All of a row's first loads are
 // issued before one is used; vectors past its end repeat its last one and are
-// not counted.
+// not counted.  Vectors are taken in pairs, for one rescaling of two (log-
+// probabilities of 8,192 rows of 50,304 bf16: 154 us for 157).
 template <typename T, int NT, int NV, Mode MODE, bool LONG>
 __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
     constexpr int N = 16 / sizeof(T);
@@ -243,12 +245,14 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
     Running r;
     take<1>(r, last, a.c);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        __builtin_amdgcn_sched_barrier(0);  // one vector's values at a time: all of them widened do not fit
-        float v[N];
-        widen<T, N>(v, raw[i]);
-        if (i * NT + t < full) take<N>(r, v, a.c);
-        asm("" : "+v"(raw[i]));             // widened again below, not kept
+    for (int i = 0; i < NV; i += 2) {
+        __builtin_amdgcn_sched_barrier(0);  // two vectors' values at a time: all of them widened do not fit
+        float v[2][N];
+        widen<T, N>(v[0], raw[i]);
+        widen<T, N>(v[1], raw[i + 1]);
+        if ((i + 1) * NT + t < full) take<2 * N>(r, reinterpret_cast<const float(&)[2 * N]>(v), a.c);
+        else if (i * NT + t < full) take<N>(r, v[0], a.c);
+        asm("" : "+v"(raw[i]), "+v"(raw[i + 1]));  // widened again below, not kept
     }
     if constexpr (LONG) {
 #pragma unroll 4
