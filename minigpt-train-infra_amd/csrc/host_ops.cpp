@@ -455,6 +455,16 @@ Loss loss_args(const Tensor& logits, const Tensor& targets, const Tensor& old_lo
     return l;
 }
 
+// Element i of a tensor as a scalar tensor that shares its memory alone: no view
+// of it to autograd, with a version of its own.  Callers change a loss in place,
+// which autograd forbids on one of several views that an autograd function returns.
+Tensor scalar_of(const Tensor& t, int64_t i) {
+    Tensor s = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+    s.unsafeGetTensorImpl()->set_storage_offset(t.storage_offset() + i);
+    s.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef{}, at::IntArrayRef{});
+    return s;
+}
+
 // (loss, log_probs, policy, kl, clip_fraction, gradient or None, workspace)
 py::tuple policy_loss(const Tensor& logits, const Tensor& targets, const Tensor& old_logp, const Tensor& advantages,
                       const optional<Tensor>& ref, const optional<Tensor>& mask, double clip_low, double clip_high,
@@ -493,8 +503,8 @@ py::tuple policy_loss(const Tensor& logits, const Tensor& targets, const Tensor&
     }
     float* const r = results.data_ptr<float>();
     check(lib.policy_loss(&a, r, r + 1, as_stream(stream)), "policy_loss");
-    const std::vector<Tensor> each = results.unbind(0);
-    return py::make_tuple(each[0], log_probs, each[1], each[2], each[3], grad, work);
+    return py::make_tuple(scalar_of(results, 0), log_probs, scalar_of(results, 1), scalar_of(results, 2),
+                          scalar_of(results, 3), grad, work);
 }
 
 Tensor policy_loss_backward(const Tensor& logits, const Tensor& targets, const Tensor& old_logp, const Tensor& advantages,

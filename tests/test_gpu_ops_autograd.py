@@ -1,0 +1,45 @@
+"""What autograd, forward-mode derivatives and traces see of the operators: their
+outputs changed in place, tensors that they write in place, dual tensors."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from tests._ops import DEV, generator, mg, randn, same_bits
+from tests.test_gpu_policy_loss import CLIP, KL, make
+
+pytestmark = pytest.mark.gpu
+
+
+def _loss_args(rows=24, V=300, dtype="f32"):
+    s = make(rows, V, dtype, 31)
+    return s["logits"], (s["targets"], s["old_logp"], s["advantages"]), {"ref_logp": s["ref_logp"], "clip": CLIP, "kl_coef": KL}
+
+
+def test_losses_take_in_place_operations():
+    """loss /= n and loss += term before backward, and the other three used as
+    accumulators: each is a tensor of its own."""
+    x, given, more = _loss_args()
+    x.requires_grad_(True)
+    r = mg.policy_loss(x, *given, **more)
+    before = [v.clone() for v in r]
+    want, = torch.autograd.grad(r.loss / 4, x)
+    r = mg.policy_loss(x, *given, **more)
+    r.kl.div_(2)
+    r.policy.add_(1)
+    r.clip_fraction.zero_()
+    loss, aux = r.loss, torch.tensor(3.0, device=DEV, requires_grad=True)
+    loss /= 4
+    loss += aux
+    loss.backward()
+    assert torch.equal(x.grad, want) and float(aux.grad) == 1.0
+    assert torch.equal(loss, before[0] / 4 + 3) and torch.equal(r.kl, before[3] / 2)
+    assert torch.equal(r.policy, before[2] + 1) and float(r.clip_fraction) == 0
+    r, _ = mg.policy_loss_grad(x.detach(), *given, **more)
+    total = r.loss
+    total += aux
+    total.backward()
+    assert float(aux.grad) == 2.0 and torch.equal(total, before[0] + 3)
+    assert all(torch.equal(a, b) for a, b in zip(r[1:], before[1:]))
