@@ -99,6 +99,13 @@ void same_dtype(const Tensor& t, const Tensor& first, const char* name) {
                              c10::toString(first.scalar_type()));
 }
 
+// A caller's tensor that a kernel has overwritten: its version moves on, as after
+// any operation in place, so that a backward pass that saved it raises instead of
+// reading the new values.  Tensors of inference mode have no version.
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void* as_stream(uint64_t s) { return reinterpret_cast<void*>(static_cast<uintptr_t>(s)); }
 
 // A tensor of dimension >= 1 as rows of its last dimension, one stride apart;
@@ -179,6 +186,7 @@ void embedding_grad(const Tensor& grad, const Tensor& ids, const Tensor& grad_ou
                              grad.data_ptr(), code, rows, width, static_cast<float>(scale), padding, accumulate,
                              work.data_ptr(), as_stream(stream)),
           "embedding_grad_");
+    written(grad);
 }
 
 // ------------------------------------------------------------- gated_act
@@ -503,6 +511,7 @@ py::tuple policy_loss(const Tensor& logits, const Tensor& targets, const Tensor&
     }
     float* const r = results.data_ptr<float>();
     check(lib.policy_loss(&a, r, r + 1, as_stream(stream)), "policy_loss");
+    if (want_grad && out.has_value()) written(*out);
     return py::make_tuple(scalar_of(results, 0), log_probs, scalar_of(results, 1), scalar_of(results, 2),
                           scalar_of(results, 3), grad, work);
 }

@@ -46,7 +46,8 @@ def policy_loss_grad(logits: torch.Tensor, targets: torch.Tensor, old_logp: torc
     """The loss and its gradient by the logits in one pass over them, for
     `logits.backward(gradient)`.  grad_scale: a float32 GPU scalar the gradient
     is multiplied by (a GradScaler's scale).  out: where the gradient goes; the
-    logits themselves may be given.  Nothing is recorded for autograd."""
+    logits themselves may be given, where no other backward pass needs them (one
+    that saved them raises).  Nothing is recorded for autograd."""
     *r, grad, _ = N.ops().policy_loss(logits, targets, old_logp, advantages, ref_logp, mask, clip[0], clip[1], kl_coef,
                                       temperature, grad_scale, True, out, N.ops_stream(logits))
     return PolicyLoss(*r), grad

@@ -43,3 +43,39 @@ def test_losses_take_in_place_operations():
     total.backward()
     assert float(aux.grad) == 2.0 and torch.equal(total, before[0] + 3)
     assert all(torch.equal(a, b) for a, b in zip(r[1:], before[1:]))
+
+
+def test_a_gradient_over_the_logits_is_seen_by_autograd():
+    """What was saved of the logits for another backward pass is gone."""
+    x, given, more = _loss_args()
+    x.requires_grad_(True)
+    logits = x * 2
+    z = logits.logsumexp(-1).square().sum()
+    mg.policy_loss_grad(logits.detach(), *given, **more)              # reads them
+    want, = torch.autograd.grad(z, x, retain_graph=True)
+    near = 2 * (2 * logits.logsumexp(-1)[:, None] * logits.softmax(-1))
+    assert float((want - near).abs().max()) < 1e-4
+    mg.policy_loss_grad(logits.detach(), *given, out=torch.empty_like(logits), **more)
+    assert same_bits(torch.autograd.grad(z, x, retain_graph=True), [want])
+    mg.policy_loss_grad(logits.detach(), *given, out=logits.detach(), **more)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(z, x)
+
+
+def test_an_accumulated_gradient_is_seen_by_autograd():
+    gen = generator(1)
+    buf, ids = randn(gen, (50, 16), torch.float32).requires_grad_(True), torch.arange(20, device=DEV)
+    g = randn(gen, (20, 16), torch.float32)
+    for accumulate in (True, False):
+        y = (buf * buf).sum()
+        mg.embedding_grad_(buf.detach(), ids, g, accumulate=accumulate)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():       # tensors without a version
+        grad, logits = torch.zeros((50, 16), device=DEV), _loss_args()[0] * 1.0
+    mg.embedding_grad_(grad, ids, g)
+    assert torch.equal(grad[:20], g)
+    _, given, more = _loss_args()
+    _, want = mg.policy_loss_grad(logits, *given, **more)
+    _, got = mg.policy_loss_grad(logits, *given, out=logits, **more)
+    assert got.data_ptr() == logits.data_ptr() and torch.equal(got, want)
