@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
+from ._autograd import recorded
 
 
 def embedding_grad_(grad: torch.Tensor, ids: torch.Tensor, grad_out: torch.Tensor, *, scale: float = 1.0,
@@ -52,6 +53,6 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, pa
     row that gets no gradient."""
     if padding_idx is not None and not -weight.shape[0] <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx {padding_idx} is outside {weight.shape[0]} rows")
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if recorded(weight):
         return _Embedding.apply(ids, weight, scale, padding_idx, dtype)
     return N.ops().embedding(ids, weight, scale, dtype, N.ops_stream(weight))

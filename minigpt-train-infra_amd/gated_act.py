@@ -16,6 +16,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as N
+from ._autograd import recorded
 
 
 class ActCheckpoint(NamedTuple):
@@ -60,6 +61,6 @@ class _GatedAct(torch.autograd.Function):
 def gated_act(gate: torch.Tensor, up: torch.Tensor | None = None, *, act: str = "silu") -> torch.Tensor:
     """act(gate) * up, or act(gate); where a gradient will be asked for, autograd
     keeps the 8-bit checkpoint and neither gate nor up."""
-    if torch.is_grad_enabled() and (gate.requires_grad or (up is not None and up.requires_grad)):
+    if recorded(gate, up):
         return _GatedAct.apply(gate, up, act)
     return N.ops().gated_act(gate, up, act, False, N.ops_stream(gate))[0]

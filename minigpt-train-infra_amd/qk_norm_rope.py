@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
+from ._autograd import recorded
 
 
 def rope_tables(length: int, rotary: int, *, base: float = 10000.0,
@@ -62,7 +63,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     of shape (length,) or (batch, length); None for 0, 1, ...; one outside the
     tables makes its token's rotated elements NaN.  heads_first: the outputs are
     (batch, heads, length, dim), as attention reads them."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+    if recorded(q, k, q_weight, k_weight):
         return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, heads_first)
     return N.ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, heads_first,
                                 N.ops_stream(q))

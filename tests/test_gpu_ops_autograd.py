@@ -79,3 +79,44 @@ def test_an_accumulated_gradient_is_seen_by_autograd():
     _, want = mg.policy_loss_grad(logits, *given, **more)
     _, got = mg.policy_loss_grad(logits, *given, out=logits, **more)
     assert got.data_ptr() == logits.data_ptr() and torch.equal(got, want)
+
+
+def _differentiable():
+    """(name, function of its differentiable inputs, those inputs)"""
+    gen = generator(2)
+    ids = torch.randint(0, 60, (40,), generator=gen, device=DEV)
+    q, k = randn(gen, (2, 5, 4, 64), torch.float32), randn(gen, (2, 5, 2, 64), torch.float32)
+    wq, wk = randn(gen, (64,), torch.float32), randn(gen, (64,), torch.float32)
+    cos, sin = mg.rope_tables(9, 64, device=DEV)
+    return [("embedding", lambda w: mg.embedding(ids, w, scale=1.5), (randn(gen, (60, 24), torch.float32),)),
+            ("qk_norm_rope", lambda *a: mg.qk_norm_rope(*a, cos, sin), (q, k, wq, wk)),
+            ("gated_act", lambda g: mg.gated_act(g, act="gelu_tanh"), (randn(gen, (9, 200), torch.float32),)),
+            ("gated_act with a gate", lambda g, u: mg.gated_act(g, u),
+             (randn(gen, (9, 200), torch.float32), randn(gen, (9, 200), torch.float32)))]
+
+
+def _outputs(y):
+    return [y] if torch.is_tensor(y) else list(y)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_forward_mode_derivatives_are_refused(i):
+    """A dual tensor asks for no gradient; its tangent is not dropped silently."""
+    name, f, inputs = _differentiable()[i]
+    want = _outputs(f(*inputs))
+    with forward_ad.dual_level():
+        assert same_bits(_outputs(f(*inputs)), want)       # no tangent, no change
+        for j in range(len(inputs)):
+            given = list(inputs)
+            given[j] = forward_ad.make_dual(given[j], torch.ones_like(given[j]))
+            with pytest.raises(NotImplementedError, match="jvp"):
+                f(*given)
+    assert same_bits(_outputs(f(*inputs)), want)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_a_trace_holds_the_operators(i):
+    name, f, inputs = _differentiable()[i]
+    traced = torch.jit.trace(f, inputs)
+    others = tuple(1.5 * x for x in inputs)
+    assert same_bits(_outputs(traced(*others)), _outputs(f(*others)))
