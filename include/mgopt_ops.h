@@ -201,7 +201,8 @@ MGOPT_API int mgopt_token_log_probs(const mgopt_policy_args* args, void* stream)
 MGOPT_API int mgopt_policy_loss(const mgopt_policy_args* args, float* loss_dev, float* parts_dev, void* stream);
 
 /* The gradient of grad_scale * loss, after mgopt_policy_loss without
- * d_logits_dev on the same arguments, log_probs_dev and workspace_dev. */
+ * d_logits_dev on the same arguments, log_probs_dev and workspace_dev: the same
+ * bits as mgopt_policy_loss gives with d_logits_dev. */
 MGOPT_API int mgopt_policy_loss_backward(const mgopt_policy_args* args, void* stream);
 
 #ifdef __cplusplus

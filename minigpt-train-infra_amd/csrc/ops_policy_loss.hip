@@ -39,6 +39,12 @@ namespace {
 
 enum Mode { kLogp, kLoss, kLossGrad, kGrad };
 
+// What a forward pass keeps of a row for a backward pass of its own.
+struct RowStats {
+    float m, s;
+    double slope;  // by the row's log-probability, with neither weight nor scale
+};
+
 struct PolicyArgs {
     const void* logits;
     int64_t row_stride, rows, vocab, first_row;
@@ -51,7 +57,7 @@ struct PolicyArgs {
     const float* grad_scale;     // may be NULL
     const double* weight_sum;    // NULL: every row's weight is 1
     float* log_probs;
-    float2* stats;               // m and s of each row: written by kLoss, read by kGrad
+    RowStats* stats;             // of each row: written by kLoss, read by kGrad
     float4* terms;               // w * policy, w * kl, w * clipped
     void* d_logits;
     int64_t d_stride;
@@ -111,8 +117,12 @@ struct RowInputs {
     float scale;                        // of the gradient, with the weights' sum
     double total;
 };
+__device__ __forceinline__ void gradient_inputs(const PolicyArgs& a, RowInputs& r) {
+    r.scale = a.grad_scale != nullptr ? *a.grad_scale : 1.0f;
+    r.total = a.weight_sum != nullptr ? *a.weight_sum : static_cast<double>(a.rows);
+}
 template <typename T, Mode MODE>
-__device__ __forceinline__ RowInputs row_inputs(const PolicyArgs& a, int64_t n, bool pick = MODE != kGrad) {
+__device__ __forceinline__ RowInputs row_inputs(const PolicyArgs& a, int64_t n, bool pick = true) {
     RowInputs r{};
     r.target = id_at(a.targets, n, a.target_bytes);
     if (pick)
@@ -122,8 +132,7 @@ __device__ __forceinline__ RowInputs row_inputs(const PolicyArgs& a, int64_t n, 
     if (MODE == kLogp) return r;
     r.old_logp = a.old_logp[n], r.advantage = a.advantages[n];
     if (a.ref_logp != nullptr) r.ref = a.ref_logp[n];
-    r.scale = a.grad_scale != nullptr ? *a.grad_scale : 1.0f;
-    r.total = a.weight_sum != nullptr ? *a.weight_sum : static_cast<double>(a.rows);
+    gradient_inputs(a, r);
     return r;
 }
 
@@ -131,17 +140,20 @@ struct RowResult {
     float slope, k;  // of the gradient: slope * [j = y] + k * 2^((x - m) c)
 };
 
-// What one row adds to the loss, and its slope, from m and s.
+__device__ __forceinline__ RowResult row_gradient(const PolicyArgs& a, double slope, const RowInputs& in, float w, float s) {
+    // where the weights' sum is 0 the loss is 0, and so is its gradient
+    slope = in.total == 0.0 ? 0.0 : slope * (w / in.total * a.inv_temp * static_cast<double>(in.scale));
+    return {static_cast<float>(slope), static_cast<float>(-slope / static_cast<double>(s))};
+}
+
+// What one row adds to the loss, and its slope, from m and s.  A backward pass of
+// its own takes the slope from here: formed again from the rounded log-probability,
+// it could hold a row at the clip's edge that the loss did not.
 template <Mode MODE>
 __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs& in, float w, float m, float s,
                                  bool write = true) {
-    double logp;
-    if constexpr (MODE == kGrad) {
-        logp = a.log_probs[n];
-    } else {
-        logp = (static_cast<double>(in.x) - static_cast<double>(m)) * a.inv_temp - log(static_cast<double>(s));
-        if (write) a.log_probs[n] = static_cast<float>(logp);
-    }
+    const double logp = (static_cast<double>(in.x) - static_cast<double>(m)) * a.inv_temp - log(static_cast<double>(s));
+    if (write) a.log_probs[n] = static_cast<float>(logp);
     if constexpr (MODE == kLogp) return {};
     const double A = in.advantage, ratio = exp(logp - static_cast<double>(in.old_logp));
     const double s1 = ratio * A, s2 = fmin(fmax(ratio, a.low), a.high) * A;
@@ -152,13 +164,13 @@ __device__ RowResult row_scalars(const PolicyArgs& a, int64_t n, const RowInputs
         kl = e - r;
         slope -= a.kl_coef * e;
     }
-    if (MODE != kGrad && write)
+    if (write)
         a.terms[n] = make_float4(static_cast<float>(w * -(held ? s2 : s1)), static_cast<float>(w * kl), held ? w : 0.0f, 0.0f);
-    if constexpr (MODE == kLoss) a.stats[n] = make_float2(m, s);
-    if constexpr (MODE == kLoss) return {};
-    // where the weights' sum is 0 the loss is 0, and so is its gradient
-    slope = in.total == 0.0 ? 0.0 : slope * (w / in.total * a.inv_temp * static_cast<double>(in.scale));
-    return {static_cast<float>(slope), static_cast<float>(-slope / static_cast<double>(s))};
+    if constexpr (MODE == kLoss) {
+        a.stats[n] = {m, s, slope};
+        return {};
+    }
+    return row_gradient(a, slope, in, w, s);
 }
 
 template <typename T, int NT>
@@ -297,7 +309,7 @@ __global__ __launch_bounds__(NT) void cached_kernel(PolicyArgs a) {
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-// The gradient from a forward pass's m, s and log-probabilities, a slice of a row a work-group.
+// The gradient from what a forward pass kept, a slice of a row a work-group.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void grad_kernel(PolicyArgs a) {
     const uint32_t row = blockIdx.x / a.slices, part = blockIdx.x - row * a.slices;
@@ -306,11 +318,15 @@ __global__ __launch_bounds__(NT) void grad_kernel(PolicyArgs a) {
     const T* x = static_cast<const T*>(a.logits) + n * a.row_stride;
     T* dx = static_cast<T*>(a.d_logits) + n * a.d_stride;
     if (w == 0.0f) return clear<T, NT>(dx, begin, end);
-    const float2 ms = a.stats[n];
+    const RowStats kept = a.stats[n];
     __shared__ RowResult shared;
-    if (threadIdx.x == 0) shared = row_scalars<kGrad>(a, n, row_inputs<T, kGrad>(a, n), w, ms.x, ms.y);
+    if (threadIdx.x == 0) {
+        RowInputs in{};
+        gradient_inputs(a, in);
+        shared = row_gradient(a, kept.slope, in, w, kept.s);
+    }
     __syncthreads();
-    write_gradient<T, NT>(x, dx, begin, end, shared, ms.x, a.c, id_at(a.targets, n, a.target_bytes));
+    write_gradient<T, NT>(x, dx, begin, end, shared, kept.m, a.c, id_at(a.targets, n, a.target_bytes));
 }
 
 // m and s of one slice of a row.
@@ -521,13 +537,14 @@ PolicyArgs args_of(const mgopt_policy_args* p) {
     a.inv_temp = 1.0 / p->temperature, a.c = static_cast<float>(1.4426950408889634 / p->temperature);
     a.grad_scale = p->grad_scale_dev, a.log_probs = p->log_probs_dev;
     a.d_logits = p->d_logits_dev, a.d_stride = p->d_logits_stride;
-    // workspace: the sum of the weights, then the rows' terms, then their m and s, then the slices' and the targets' logits
+    // workspace: the sum of the weights, then the rows' terms, then what a backward pass needs of them, then the slices'
+    // m and s and the targets' logits
     char* at = static_cast<char*>(p->workspace_dev);
     if (at != nullptr) {
         a.weight_sum = p->mask_kind == MGOPT_MASK_NONE ? nullptr : reinterpret_cast<const double*>(at);
         a.terms = reinterpret_cast<float4*>(at + 16);
-        a.stats = reinterpret_cast<float2*>(at + 16 + 16 * p->rows);
-        a.parts = reinterpret_cast<float2*>(at + 16 + (24 * p->rows + 15) / 16 * 16);
+        a.stats = reinterpret_cast<RowStats*>(at + 16 + 16 * p->rows);
+        a.parts = reinterpret_cast<float2*>(at + 16 + 32 * p->rows);
         a.picked = reinterpret_cast<float*>(a.parts + kSplitSlices);
     }
     return a;
@@ -543,7 +560,7 @@ extern "C" {
 MGOPT_API int64_t mgopt_policy_workspace(int64_t rows) {
     // as args_of lays it out; few rows may be cut in slices
     const int64_t cuts = rows < kSplitRows ? 8 * kSplitSlices + 4 * kSplitRows : 0;
-    return rows < 0 ? -1 : 16 + (24 * rows + 15) / 16 * 16 + cuts;
+    return rows < 0 ? -1 : 16 + 32 * rows + cuts;
 }
 
 MGOPT_API int mgopt_token_log_probs(const mgopt_policy_args* p, void* stream) {

@@ -120,3 +120,23 @@ def test_a_trace_holds_the_operators(i):
     traced = torch.jit.trace(f, inputs)
     others = tuple(1.5 * x for x in inputs)
     assert same_bits(_outputs(traced(*others)), _outputs(f(*others)))
+
+
+@pytest.mark.parametrize("dtype, rows, V", [("f32", 4000, 200), ("bf16", 4000, 200), ("bf16", 100, 120_007)])
+def test_forward_and_backward_clip_the_same_rows(dtype, rows, V):
+    """Ratios that the rounding of old_logp leaves on either side of the clip's
+    edge: the backward pass holds the rows that the loss counted, and gives the
+    gradient of the one-pass form."""
+    s = make(rows, V, dtype, 41, ref=False)
+    logp = torch.log_softmax(s["logits"].double(), -1).gather(1, s["targets"][:, None])[:, 0]
+    s["old_logp"] = (logp - torch.log1p(torch.tensor(CLIP[1], dtype=torch.float64, device=DEV))).float()
+    s["advantages"] = s["advantages"].abs() + 0.1
+    given, more = (s["targets"], s["old_logp"], s["advantages"]), {"clip": CLIP}
+    one, want = mg.policy_loss_grad(s["logits"], *given, **more)
+    x = s["logits"].requires_grad_(True)
+    r = mg.policy_loss(x, *given, **more)
+    r.loss.backward()
+    assert torch.equal(r.clip_fraction, one.clip_fraction) and 0.05 < float(r.clip_fraction) < 0.95
+    held = int((x.grad == 0).all(-1).sum())
+    assert held == round(float(r.clip_fraction) * rows), (held, float(r.clip_fraction) * rows)
+    assert same_bits([x.grad], [want])
