@@ -165,9 +165,9 @@ __global__ __launch_bounds__(kBlock) void grad_by_row_kernel(GradArgs a) {
 // length, whatever rows they touch, and the pieces' sums are joined.
 //
 // The sort is a radix sort, at most kDigitBits a pass, from the low digit up.  A pass
-// counts every tile's digits, and then places each token behind the tokens of
-// smaller digits, those of its digit in earlier tiles, and those before it in
-// its tile.  Ids that name no row, and the padding's, become the key `rows`
+// counts every tile's digits (and, of many tiles, scans the counts), and then
+// places each token behind the tokens of smaller digits, those of its digit in
+// earlier tiles, and those before it in its tile.  Ids that name no row, and the padding's, become the key `rows`
 // and end up last.
 
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;  // at most
@@ -178,10 +178,11 @@ struct SortArgs {
     const void* ids;           // first pass
     const uint32_t *keys, *tokens;
     uint32_t *keys_out, *tokens_out;
-    uint32_t* counts;          // [tiles][kDigits]
+    uint32_t* counts;          // [tiles + 1][kDigits]
     int64_t rows, padding;
     uint32_t n, tiles;
     int32_t id_bytes, shift;   // the digit's lowest bit
+    int32_t scanned;           // counts hold what scan_kernel makes of them
     char* zeros;               // what the work-groups past the tiles clear: a multiple of 16 bytes but in the last launch
     int64_t zero_bytes;
 };
@@ -214,6 +215,40 @@ __global__ __launch_bounds__(kSortBlock) void count_kernel(SortArgs a) {
     }
     __syncthreads();
     a.counts[static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = count[threadIdx.x];
+}
+
+// Each tile's counts become the numbers in the tiles before it, digit by digit,
+// and the row past the tiles the totals.  A work-group takes kScanDigits digits,
+// its threads equal ranges of the tiles.
+constexpr int kScanDigits = 16, kScanBlock = 1024, kScanParts = kScanBlock / kScanDigits;
+__global__ __launch_bounds__(kScanBlock) void scan_kernel(uint32_t* counts, uint32_t tiles) {
+    __shared__ uint32_t sums[kScanParts][kScanDigits];
+    const uint32_t d = threadIdx.x % kScanDigits, part = threadIdx.x / kScanDigits;
+    const uint32_t per = (tiles + kScanParts - 1) / kScanParts;
+    const uint32_t begin = min(part * per, tiles), end = min(begin + per, tiles);
+    uint32_t* const at = counts + blockIdx.x * kScanDigits + d;
+    uint32_t sum = 0;
+#pragma unroll 8
+    for (uint32_t b = begin; b < end; ++b) sum += at[static_cast<int64_t>(b) * kDigits];
+    sums[part][d] = sum;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (uint32_t p = 0; p < kScanParts; ++p) {
+        if (p < part) before += sums[p][d];
+        all += sums[p][d];
+    }
+    constexpr uint32_t kAhead = 8;
+    for (uint32_t b = begin; b < end; b += kAhead) {
+        uint32_t x[kAhead];
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) x[u] = b + u < end ? at[static_cast<int64_t>(b + u) * kDigits] : 0;
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) {
+            if (b + u < end) at[static_cast<int64_t>(b + u) * kDigits] = before;
+            before += x[u];
+        }
+    }
+    if (part == 0) at[static_cast<int64_t>(tiles) * kDigits] = all;
 }
 
 // The exclusive sum of x over the work-group's WAVES waves.
@@ -284,11 +319,16 @@ __global__ __launch_bounds__(kSortBlock) void place_kernel(SortArgs a) {
     __shared__ uint32_t base[kDigits], wave_sums[kSortWaves];
     const uint32_t d = threadIdx.x, lane = d % 64, wave = d / 64, begin = blockIdx.x * kTile;
     uint32_t earlier = 0, all = 0;  // elements of digit d
+    if (a.scanned) {
+        earlier = a.counts[static_cast<int64_t>(blockIdx.x) * kDigits + d];
+        all = a.counts[static_cast<int64_t>(a.tiles) * kDigits + d];
+    } else {
 #pragma unroll 8
-    for (uint32_t b = 0; b < a.tiles; ++b) {
-        const uint32_t x = a.counts[static_cast<int64_t>(b) * kDigits + d];
-        all += x;
-        earlier += b < blockIdx.x ? x : 0;
+        for (uint32_t b = 0; b < a.tiles; ++b) {
+            const uint32_t x = a.counts[static_cast<int64_t>(b) * kDigits + d];
+            all += x;
+            earlier += b < blockIdx.x ? x : 0;
+        }
     }
     uint32_t key[kSortItems], token[kSortItems], digit[kSortItems];
     bool on[kSortItems];
@@ -525,6 +565,13 @@ bool by_row(int64_t n, int64_t rows, int64_t width) {
 // 29; at 16,384, with 16 elements a thread, 44 us against 29.
 constexpr int64_t kSortWhole = 8192;
 
+// Up to here each tile of the sort adds up all tiles' counts itself, which costs
+// tiles^2 reads of 2 KB a pass; beyond, a kernel of its own does it once.  A whole
+// call in us, two passes, direct / scanned, by tiles of 2,048 tokens:
+//   8: 32 / 38    64: 60 / 61    96: 88 / 87    128: 96 / 93    512: 215 / 182
+//   2,048: 953 / 387    8,192: 10,149 / 1,318
+constexpr uint32_t kDirectTiles = 96;
+
 // Sorted positions per piece, a power of two from 8 to 64: about 8,192 waves'
 // pieces, all that fit the chip at once.  Short pieces give the sums more waves,
 // long ones the joining less to do; sums and joining, traced, in us, by the
@@ -545,7 +592,7 @@ Work work_of(int64_t n, int64_t width) {
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     Work w{};
     const int64_t tiles = (n + kTile - 1) / kTile, list = up(4 * (n + 16));  // sum_pieces_kernel reads a little past n
-    w.keys[0] = up(4 * tiles * kDigits);
+    w.keys[0] = up(4 * (tiles + 1) * kDigits);
     w.tokens[0] = w.keys[0] + list, w.keys[1] = w.tokens[0] + list, w.tokens[1] = w.keys[1] + list;
     w.partials = w.tokens[1] + list;
     const int64_t piece = piece_for(n, width);
@@ -648,7 +695,7 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
             const auto list = [&](int64_t offset) { return reinterpret_cast<uint32_t*>(at + offset); };
             const uint32_t tiles = static_cast<uint32_t>((n + kTile - 1) / kTile);
             SortArgs o{ids_dev, nullptr, nullptr, nullptr, nullptr, list(work.counts), rows, padding_idx, static_cast<uint32_t>(n),
-                       tiles, id_bytes, 0, nullptr, 0};
+                       tiles, id_bytes, 0, tiles > kDirectTiles, nullptr, 0};
             int32_t bits = 1;
             while (rows >> bits) ++bits;  // of the largest key, `rows`
             const int passes = (bits + kDigitBits - 1) / kDigitBits;
@@ -687,6 +734,10 @@ MGOPT_API int mgopt_embedding_grad(const void* ids_dev, int32_t id_bytes, int64_
                     if (eight) hipLaunchKernelGGL(count_kernel<8>, counters, dim3(kSortBlock), 0, s, o);
                     else hipLaunchKernelGGL(count_kernel<9>, counters, dim3(kSortBlock), 0, s, o);
                     if (int rc = launched("count_kernel")) return rc;
+                    if (o.scanned) {
+                        hipLaunchKernelGGL(scan_kernel, dim3(kDigits / kScanDigits), dim3(kScanBlock), 0, s, o.counts, tiles);
+                        if (int rc = launched("scan_kernel")) return rc;
+                    }
                     const dim3 grid(tiles + clearing(o.shift + (eight ? 8 : 9) >= bits));
                     if (eight) hipLaunchKernelGGL(place_kernel<8>, grid, dim3(kSortBlock), 0, s, o);
                     else hipLaunchKernelGGL(place_kernel<9>, grid, dim3(kSortBlock), 0, s, o);
