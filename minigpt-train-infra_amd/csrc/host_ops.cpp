@@ -79,10 +79,25 @@ int32_t code_of(const Tensor& t, const char* name) {
 
 [[noreturn]] void refuse(const std::string& text) { throw py::value_error(text); }
 
-std::string shape_of(const Tensor& t) {
+std::string shape_of(at::IntArrayRef sizes) {
     std::string s = "(";
-    for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+    for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
     return s + ")";
+}
+std::string shape_of(const Tensor& t) { return shape_of(t.sizes()); }
+
+// Whether two shapes of one count name the same elements in the same order:
+// equal but for dimensions of one, or one of them a flat list.
+bool same_order(at::IntArrayRef a, at::IntArrayRef b) {
+    const auto real = [](at::IntArrayRef s) {
+        std::vector<int64_t> r;
+        for (const int64_t n : s)
+            if (n != 1) r.push_back(n);
+        return r;
+    };
+    if (a == b) return true;
+    const std::vector<int64_t> x = real(a), y = real(b);
+    return x.size() <= 1 || y.size() <= 1 || x == y;
 }
 
 // On a GPU, and on the first operand's.
@@ -374,6 +389,8 @@ Tensor per_row(const Tensor& t, const Tensor& logits, int64_t rows, const char* 
     beside(t, logits, name);
     if (t.numel() != rows)
         refuse(std::string(name) + " has " + std::to_string(t.numel()) + " values for " + std::to_string(rows) + " rows");
+    if (!same_order(t.sizes(), logits.sizes().slice(0, logits.dim() - 1)))
+        refuse(std::string(name) + " has shape " + shape_of(t) + " for logits " + shape_of(logits));
     return t.contiguous();
 }
 Tensor float_per_row(const Tensor& t, const Tensor& logits, int64_t rows, const char* name) {

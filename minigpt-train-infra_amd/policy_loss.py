@@ -32,9 +32,10 @@ class PolicyLoss(NamedTuple):
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, mask: torch.Tensor | None = None,
                     temperature: float = 1.0) -> torch.Tensor:
     """The log-probability of each row's target, float32 of logits.shape[:-1]
-    (what policy_loss takes as old_logp and ref_logp).  targets: int64 or int32;
-    one outside the vocabulary gives NaN.  mask: bool, or float32 weights; rows
-    of weight 0 give 0.  Nothing is recorded for autograd."""
+    (what policy_loss takes as old_logp and ref_logp).  targets: int64 or int32; a
+    target outside the vocabulary gives NaN.  mask: bool, or float32 weights; rows
+    of weight 0 give 0.  Values per row have the shape logits.shape[:-1] or are a
+    flat list of the rows.  Nothing is recorded for autograd."""
     return N.ops().token_log_probs(logits, targets, mask, temperature, N.ops_stream(logits))
 
 
