@@ -62,7 +62,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     (positions, rotary/2), as rope_tables makes them.  positions: int64 or int32
     of shape (length,) or (batch, length); None for 0, 1, ...; one outside the
     tables makes its token's rotated elements NaN.  heads_first: the outputs are
-    (batch, heads, length, dim), as attention reads them."""
+    (batch, heads, length, dim), as attention reads them.  cos and sin get no
+    gradient; one that asks for it is refused."""
+    if torch.is_grad_enabled():
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.requires_grad:
+                raise ValueError(f"qk_norm_rope has no gradient by {name}: detach it")
     if recorded(q, k, q_weight, k_weight):
         return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, heads_first)
     return N.ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, heads_first,

@@ -35,3 +35,18 @@ def test_values_per_row_in_another_order():
                   (x, y, s["mask"])):
         assert same_bits([mg.token_log_probs(given[0], given[1], mask=given[2]).flatten()], [want])
     assert mg.token_log_probs(x[:0], y[:0]).shape == (0, 4) and mg.token_log_probs(x[:, :0], y[:, :0]).shape == (3, 0)
+
+
+def test_tables_that_ask_for_a_gradient():
+    gen = generator(5)
+    q, k = randn(gen, (1, 3, 2, 32), torch.float32), randn(gen, (1, 3, 1, 32), torch.float32)
+    w = torch.ones(32, device=DEV)
+    cos, sin = mg.rope_tables(3, 32, device=DEV)
+    want = mg.qk_norm_rope(q, k, w, w, cos, sin)
+    for asks in (False, True):
+        q.requires_grad_(asks)
+        for name, c, s in (("cos", cos.clone().requires_grad_(True), sin), ("sin", cos, sin.clone().requires_grad_(True))):
+            with pytest.raises(ValueError, match=f"no gradient by {name}"):
+                mg.qk_norm_rope(q, k, w, w, c, s)
+            with torch.no_grad():
+                assert same_bits(mg.qk_norm_rope(q, k, w, w, c, s), want)
