@@ -241,9 +241,10 @@ std::tuple<Tensor, optional<Tensor>, optional<Tensor>> gated_act(const Tensor& g
     return {y, codes, scales};
 }
 
-// (d_gate, d_up or None, y or None)
+// (d_gate, d_up or None, y or None); shape: the activation's, None where it is not known
 std::tuple<Tensor, optional<Tensor>, optional<Tensor>> gated_act_backward(const Tensor& grad_out, const Tensor& codes,
                                                                           const Tensor& scales, const std::string& act,
+                                                                          const optional<std::vector<int64_t>>& shape,
                                                                           bool want_y, uint64_t stream) {
     const int32_t kind = activation(act);
     on_gpu(grad_out, "grad_out");
@@ -260,6 +261,12 @@ std::tuple<Tensor, optional<Tensor>, optional<Tensor>> gated_act_backward(const 
         scales.size(1) != g.rows || scales.size(2) != groups)
         refuse("the checkpoint is not one of rows like grad_out's " + shape_of(grad_out) + ": codes " + shape_of(codes) +
                ", scales " + shape_of(scales));
+    if (shape.has_value()) {
+        const at::IntArrayRef kept(*shape), lead = grad_out.sizes().slice(0, grad_out.dim() - 1);
+        if (kept.empty() || kept.back() != g.width || !same_order(kept.slice(0, kept.size() - 1), lead))
+            refuse("the checkpoint is not one of rows like grad_out's " + shape_of(grad_out) + ": the activation had shape " +
+                   shape_of(kept));
+    }
     const bool gated = codes.size(0) == 2;
     Tensor d_gate = at::empty(grad_out.sizes(), grad_out.options());
     optional<Tensor> d_up, y;

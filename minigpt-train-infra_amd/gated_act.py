@@ -25,6 +25,7 @@ class ActCheckpoint(NamedTuple):
     codes: torch.Tensor      # int8 [inputs, rows, groups * 128]
     scales: torch.Tensor     # float32 [inputs, rows, groups]
     act: str
+    shape: tuple[int, ...] | None = None     # the activation's; without it, gated_act_backward checks the count of rows only
 
 
 def gated_act_pack(gate: torch.Tensor, up: torch.Tensor | None = None, *,
@@ -33,14 +34,15 @@ def gated_act_pack(gate: torch.Tensor, up: torch.Tensor | None = None, *,
     (the last dimension) are contiguous and evenly spaced; others are copied
     first.  act: "silu" or "gelu_tanh".  Nothing is recorded for autograd."""
     y, codes, scales = N.ops().gated_act(gate, up, act, True, N.ops_stream(gate))
-    return y, ActCheckpoint(codes, scales, act)
+    return y, ActCheckpoint(codes, scales, act, tuple(y.shape))
 
 
 def gated_act_backward(grad_out: torch.Tensor, saved: ActCheckpoint, *,
                        want_y: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
     """(d_gate, d_up, y) from the gradient of y: d_up is None without a gate, y
-    without want_y.  The outputs have grad_out's shape and dtype."""
-    return N.ops().gated_act_backward(grad_out, saved.codes, saved.scales, saved.act, want_y, N.ops_stream(grad_out))
+    without want_y.  The outputs have grad_out's shape and dtype; its rows are
+    those of y, in their order."""
+    return N.ops().gated_act_backward(grad_out, saved.codes, saved.scales, saved.act, saved.shape, want_y, N.ops_stream(grad_out))
 
 
 class _GatedAct(torch.autograd.Function):

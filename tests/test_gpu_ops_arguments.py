@@ -37,6 +37,24 @@ def test_values_per_row_in_another_order():
     assert mg.token_log_probs(x[:0], y[:0]).shape == (0, 4) and mg.token_log_probs(x[:, :0], y[:, :0]).shape == (3, 0)
 
 
+def test_gradient_in_another_order_than_the_checkpoint():
+    """A gradient has to be laid out as the activation was."""
+    gen = generator(4)
+    x, up = randn(gen, (3, 4, 200), torch.bfloat16), randn(gen, (3, 4, 200), torch.bfloat16)
+    dy = randn(gen, (3, 4, 200), torch.bfloat16)
+    _, saved = mg.gated_act_pack(x, up)
+    want = mg.gated_act_backward(dy, saved)
+    for bad in (dy.transpose(0, 1), dy.view(2, 6, 200), dy[..., :130], dy.view(12, 200)[..., :199]):
+        with pytest.raises(ValueError, match="the checkpoint is not one"):
+            mg.gated_act_backward(bad, saved)
+    for good in (dy.view(12, 200), dy[:, None], dy.view(1, 12, 200)):
+        got = mg.gated_act_backward(good, saved)
+        assert same_bits([g.flatten() for g in got], [w.flatten() for w in want])
+    # a checkpoint put together again from its tensors knows its rows only
+    got = mg.gated_act_backward(dy, mg.ActCheckpoint(saved.codes, saved.scales, "silu"))
+    assert same_bits(got, want)
+
+
 def test_tables_that_ask_for_a_gradient():
     gen = generator(5)
     q, k = randn(gen, (1, 3, 2, 32), torch.float32), randn(gen, (1, 3, 1, 32), torch.float32)
