@@ -130,13 +130,9 @@ __device__ __forceinline__ X reduce_lanes(X x, Op op) {
     if constexpr (LANES > 32) x = op(x, __shfl_xor(x, 32));
     return x;
 }
-template <int LANES>
-__device__ __forceinline__ float sum_lanes(float x) {
-    return reduce_lanes<LANES>(x, [](float a, float b) { return a + b; });
-}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32: 1 ulp, tiny results to 0
-__device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }    // v_rcp_f32: 1 ulp
+__device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }    // v_rcp_f32: 1 ulp, tiny results to 0
 
 // An id of a list of 4- or 8-byte signed integers.
 __device__ __forceinline__ int64_t id_at(const void* p, int64_t i, int bytes) {

@@ -542,18 +542,25 @@ __global__ __launch_bounds__(kBlock) void join_pieces_kernel(SumArgs a) {
     store_some<N>(out, sum, left);
 }
 
-// Which form: a work-group per row, while all of them read the ids in less than
-// the sort's launches take and one row that has all tokens is not long in summing
-// them.  A whole call in us, by row / sorted, ids whose frequency falls as one over
-// their rank and all the same:
-//   tokens  rows   width   by rank        the same
-//   256     96     128      5.1 / 14.1     6.5 / 13.5
-//   1,024   96     128      5.4 / 15.1    17.5 / 17.1
-//   1,024   1,000  256      5.4 / 17.1    30.9 / 18.9
-//   256     1,000  4,096    7.7 / 17.4    60.2 / 17.6
-//   1,024   96     768     17.2 / 14.1   117.8 / 16.4
-//   64      16,000 4,096   29.8 / 25.6    41.1 / 26.4
-//   16      50,304 768     43.5 / 18.4    43.5 / 19.1
+// Which form: a work-group per row, or the sort.  A whole call in us, by row /
+// sorted, bf16, ids whose frequency falls as one over their rank and all the same:
+//                          accumulated                   written whole
+//   tokens  rows    width  by rank       the same        by rank        the same
+//   256     96      128    5.0 / 15.3    6.5 / 13.7      4.6 / 14.1     6.5 / 13.5
+//   1,024   96      128    5.6 / 16.2    17.7 / 16.7     5.6 / 15.1     17.4 / 16.5
+//   1,024   1,000   256    6.0 / 18.9    30.9 / 20.7     5.9 / 18.2     30.8 / 20.6
+//   64      8,192   768    7.3 / 15.8    11.5 / 14.1     9.9 / 16.5     13.2 / 15.1
+//   10      50,304  768    32.7 / 12.9   32.4 / 13.2     43.3 / 18.3    43.4 / 19.0
+//   3       151,936 4,096  187 / 11.7    186 / 11.4      245 / 285      245 / 286
+// and beyond the bounds:
+//   256     1,000   4,096  7.3 / 17.0    59.0 / 17.2     8.0 / 17.6     60.2 / 17.9
+//   1,024   96      768    19.4 / 15.0   117 / 17.0      19.2 / 14.7    117 / 16.8
+//   64      16,000  4,096  22.7 / 16.2   25.2 / 14.8     31.3 / 27.6    39.3 / 26.7
+//   16      50,304  768    32.5 / 13.1   32.4 / 13.2     43.2 / 18.6    43.4 / 19.0
+// rows * tokens is what all rows read, tokens * width what a row that has all
+// tokens sums alone.  The rows by themselves are not bounded, and a work-group each
+// costs 0.6 to 1.6 ns: the few tokens (10 of 50,304 rows, 3 of 151,936) that still
+// take the by-row form there would mostly be faster sorted.
 constexpr int64_t kByRowWork = int64_t{1} << 19;   // rows * tokens
 constexpr int64_t kByRowTerms = int64_t{1} << 17;  // tokens * width
 bool by_row(int64_t n, int64_t rows, int64_t width) {

@@ -17,7 +17,7 @@
 //
 // Bound by memory: forward moves (2 + 1) * b + 2 * (1 + 4/128) bytes per
 // element of b bytes, backward (1 + 3) * b + 2 * (1 + 4/128).  8,192 rows of
-// 12,288 in bf16: 158 us forward (5.1 TB/s), 172 to 181 us backward (5.6 to 5.9).
+// 12,288 in bf16: 133 us forward (6.1 TB/s), 179 us backward (5.7).
 // A lane takes 16 bytes of each input, 16 or 32 lanes a group of 128, so that a
 // group's largest magnitude is a few exchanges within a wave.
 #include "ops_common.h"
@@ -26,14 +26,16 @@ namespace mgopt {
 namespace {
 
 // One wave a work-group, which starts as soon as any SIMD has room: against 256
-// threads, at 8,192 rows of 12,288 in bf16, 172 against 180 us for the backward
-// pass; at 2,049 of 2,731 in fp16, 11.9 against 13.9 and 11.8 against 13.7.
+// threads, at 8,192 rows of 12,288 in bf16, 180 against 189 us for the backward
+// pass; at 2,049 of 2,731 in fp16, 12.1 against 14.1 for each.
 constexpr int kActBlock = 64;
 // A forward pass that moves more than the Infinity Cache holds reads its inputs
-// and writes y past the caches: 152 against 168 us at 8,192 rows of 12,288 in
-// bf16.  On 100 MB in fp16, whose inputs are still cached, such loads cost 15.6
-// against 11.9 us, and in the backward pass, with its three outputs, they and such
-// stores never paid (178 to 181 against 172 us).
+// and writes y past the caches: 133 against 145 us at 8,192 rows of 12,288 in
+// bf16.  A backward pass right behind it finds less of what it reads in the cache,
+// 179 against 167 us, so that the two alone take the same; in a training step
+// other passes lie between.  On 100 MB in fp16, whose inputs are still cached, such
+// loads cost 15.2 against 12.2 us, and in the backward pass, with its three
+// outputs, they and such stores never paid.
 constexpr int64_t kStreamBytes = int64_t{256} << 20;
 constexpr int kGroup = MGOPT_ACT_GROUP;  // elements per scale
 constexpr float kTiny = 0x1p-119f;
@@ -44,9 +46,11 @@ constexpr double kLog2e = 1.4426950408889634;
 // The activation and its derivative.  Both are x * s for a logistic s:
 // SiLU's is of x, and GELU's tanh form of v = 2 sqrt(2/pi) (x + 0.044715 x^3),
 // as (1 + tanh(v / 2)) / 2 is the logistic function of v; written so, neither
-// tail cancels.  exp(-v) overflows to inf for large negative v and s is then 0.
-// GELU's v * log2(e) is formed in 64 bits, which run at the 32-bit rate here: an
-// error of v is one of exp(-v) times |v|, and v goes through four roundings.
+// tail cancels.  exp(-v) overflows to inf for large negative v and s is then 0, as
+// it is wherever it would lie below 2^-126: under v = -87.
+// An error of v * log2(e) is one of exp(-v) times |v|.  SiLU's has one rounding,
+// within |v| 2^-24 of s, and stays in 32 bits.  GELU's v goes through four, and is
+// formed in 64 bits, which run at the 32-bit rate here.
 template <int ACT>
 __device__ __forceinline__ void act(float x, float& a, float& d) {
     float w = x * static_cast<float>(kLog2e), dv = 1.0f;
