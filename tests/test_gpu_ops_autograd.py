@@ -3,6 +3,9 @@ outputs changed in place, tensors that they write in place, dual tensors."""
 
 from __future__ import annotations
 
+import copy
+import io
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -140,3 +143,23 @@ def test_forward_and_backward_clip_the_same_rows(dtype, rows, V):
     held = int((x.grad == 0).all(-1).sum())
     assert held == round(float(r.clip_fraction) * rows), (held, float(r.clip_fraction) * rows)
     assert same_bits([x.grad], [want])
+
+
+def test_losses_as_ordinary_tensors():
+    """In inference mode, copied, saved, reshaped: no trace of the shared memory."""
+    x, given, more = _loss_args()
+    want, grad = mg.policy_loss_grad(x, *given, **more)
+    with torch.inference_mode():
+        r, g = mg.policy_loss_grad(x, *given, **more)
+        r.loss.mul_(2)
+        assert same_bits([g], [grad]) and torch.equal(r.loss, want.loss * 2) and torch.equal(r.policy, want.policy)
+    for v in (want.loss, want.policy, want.kl, want.clip_fraction):
+        assert v.shape == () and v.dtype == torch.float32 and v.is_contiguous() and not v._is_view()
+        file = io.BytesIO()
+        torch.save(v, file)
+        file.seek(0)
+        for other in (copy.deepcopy(v), v.clone(), torch.load(file, weights_only=True), v.view(1)[0], v.cpu().to(DEV)):
+            assert same_bits([other], [v])
+        assert float(v) == v.item() == v.cpu().numpy()
+    total = torch.stack([want.loss, want.policy, want.kl, want.clip_fraction])
+    assert same_bits([total[0], total[3]], [want.loss, want.clip_fraction])
