@@ -1,9 +1,10 @@
 /*
  * mgopt_ops.h -- C ABI of the operators of a training step around its matrix
  * products and attention (libmgopt.so): token embedding, query/key norms with
- * the rotary rotation, the MLP's activation with an 8-bit checkpoint, and the
- * clipped policy loss.  Their gradients are the ones the optimizer step
- * (mgopt.h) reads.
+ * the rotary rotation, attention, the residual's norm, the MLP's activation with
+ * an 8-bit checkpoint, and the clipped policy loss; and, for forward passes that
+ * need no gradient, products of 8-bit integers.  The gradients are the ones the
+ * optimizer step (mgopt.h) reads.
  *
  * Conventions are those of mgopt.h: *_dev arguments are device pointers to
  * memory of the caller's, calls are asynchronous on `stream` and wait for
@@ -75,6 +76,39 @@ MGOPT_API int mgopt_gated_act_backward(const void* grad_out_dev, int64_t grad_ou
                                        const float* scales_dev, int32_t gated, int32_t dtype, int64_t rows,
                                        int64_t width, int32_t act, void* d_gate_dev, int64_t d_gate_stride,
                                        void* d_up_dev, int64_t d_up_stride, void* y_dev, void* stream);
+
+/* ---- the residual's norm, and rows in 8 bits --------------------------------- */
+
+#define MGOPT_MAX_NORM_WIDTH 32768
+
+/* h = round(x + residual) to `dtype`, contiguous (residual_dev and h_dev NULL: h
+ * is x), and of h's rows y = (h * r) * weight with r = 1 / sqrt(mean(h^2) + eps),
+ * the mean in 64 bits.  Exactly one of y_dev (contiguous, of `dtype`) and
+ * codes_dev with scales_dev: the rows of y, unrounded, as 8-bit codes (below).
+ * Strides are those between rows. */
+MGOPT_API int mgopt_rms_norm(const void* x_dev, int64_t x_stride, const void* residual_dev, int64_t residual_stride,
+                             const void* weight_dev, int32_t weight_dtype, int32_t dtype, int64_t rows, int64_t width,
+                             double eps, void* h_dev, void* y_dev, int8_t* codes_dev, int64_t codes_stride,
+                             float* scales_dev, void* stream);
+
+MGOPT_API int64_t mgopt_rms_norm_workspace(int64_t rows, int64_t width);
+
+/* From the gradient of y, that of h (or NULL) and h itself: d_x, contiguous, the
+ * gradient of x and of the residual, and d_weight, of weight_dtype (NULL: not
+ * wanted).  workspace_dev (with d_weight_dev): mgopt_rms_norm_workspace bytes,
+ * 16-byte aligned. */
+MGOPT_API int mgopt_rms_norm_backward(const void* grad_y_dev, int64_t grad_y_stride, const void* grad_h_dev,
+                                      int64_t grad_h_stride, const void* h_dev, int64_t h_stride, const void* weight_dev,
+                                      int32_t weight_dtype, int32_t dtype, int64_t rows, int64_t width, double eps,
+                                      void* d_x_dev, void* d_weight_dev, void* workspace_dev, void* stream);
+
+/* Rows in 8 bits: a row whose largest magnitude is m holds scale = m * (1/127) and
+ * the integers nearest to x * (127 / m), ties to even, in fp32; m below 2^-119
+ * counts as 0, and a row with an inf or a NaN has the scale NaN.  codes_stride is
+ * the width rounded up to 16, codes_dev 16-byte aligned; the codes behind the
+ * width are 0. */
+MGOPT_API int mgopt_int8_rows(const void* x_dev, int64_t x_stride, int32_t dtype, int64_t rows, int64_t width,
+                              int8_t* codes_dev, int64_t codes_stride, float* scales_dev, void* stream);
 
 /* ---- query/key norms and the rotation -------------------------------------- */
 

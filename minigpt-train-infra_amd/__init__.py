@@ -30,8 +30,10 @@ from .clip_grad import clip_grad_norm_
 from .embedding import embedding, embedding_grad_
 from .gated_act import ActCheckpoint, gated_act, gated_act_backward, gated_act_pack
 from .grad_scaler import GradScaler
+from .int8_linear import Int8Rows, int8_rows
 from .policy_loss import PolicyLoss, policy_loss, policy_loss_grad, token_log_probs
 from .qk_norm_rope import qk_norm_rope, qk_norm_rope_backward, rope_tables
+from .rms_norm import add_rms_norm, rms_norm, rms_norm_backward, rms_norm_int8
 from .schedule import build_adamw_param_groups, cosine_lr, optimizer_completed_steps, set_optimizer_lr
 from .state_load import load_grad_scaler_state, load_optimizer_state
 from . import paramsets
@@ -60,4 +62,10 @@ __all__ = [
     "qk_norm_rope_backward",
     "rope_tables",
     "token_log_probs",
+    "add_rms_norm",
+    "rms_norm",
+    "rms_norm_backward",
+    "rms_norm_int8",
+    "Int8Rows",
+    "int8_rows",
 ]

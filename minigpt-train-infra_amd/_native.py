@@ -52,6 +52,10 @@ OPS_EXPORTS = (
     "mgopt_token_log_probs",
     "mgopt_policy_loss",
     "mgopt_policy_loss_backward",
+    "mgopt_rms_norm",
+    "mgopt_rms_norm_workspace",
+    "mgopt_rms_norm_backward",
+    "mgopt_int8_rows",
 )
 
 

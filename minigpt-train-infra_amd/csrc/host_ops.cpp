@@ -33,6 +33,10 @@ struct Entries {
     decltype(&mgopt_token_log_probs) token_log_probs = nullptr;
     decltype(&mgopt_policy_loss) policy_loss = nullptr;
     decltype(&mgopt_policy_loss_backward) policy_loss_backward = nullptr;
+    decltype(&mgopt_rms_norm) rms_norm = nullptr;
+    decltype(&mgopt_rms_norm_workspace) rms_norm_workspace = nullptr;
+    decltype(&mgopt_rms_norm_backward) rms_norm_backward = nullptr;
+    decltype(&mgopt_int8_rows) int8_rows = nullptr;
     decltype(&mgopt_last_error) last_error = nullptr;
     PyObject* error = nullptr;  // the package's MgoptError
 } lib;
@@ -54,6 +58,10 @@ void bind_ops(const py::dict& addresses, const py::object& error) {
     take(lib.token_log_probs, "mgopt_token_log_probs");
     take(lib.policy_loss, "mgopt_policy_loss");
     take(lib.policy_loss_backward, "mgopt_policy_loss_backward");
+    take(lib.rms_norm, "mgopt_rms_norm");
+    take(lib.rms_norm_workspace, "mgopt_rms_norm_workspace");
+    take(lib.rms_norm_backward, "mgopt_rms_norm_backward");
+    take(lib.int8_rows, "mgopt_int8_rows");
     take(lib.last_error, "mgopt_last_error");
     Py_XDECREF(lib.error);
     lib.error = error.inc_ref().ptr();
@@ -556,6 +564,110 @@ Tensor policy_loss_backward(const Tensor& logits, const Tensor& targets, const T
     return grad;
 }
 
+// -------------------------------------------------------------- rms_norm
+
+// Codes and scales of rows, as the kernels write them: rows of codes start 16 bytes apart or a multiple of it.
+struct Codes {
+    Tensor codes, scales;
+    int64_t stride;
+};
+Codes codes_for(const Tensor& x, int64_t rows, int64_t width) {
+    const int64_t stride = (width + 15) / 16 * 16;
+    std::vector<int64_t> shape = x.sizes().vec(), lead(shape.begin(), shape.end() - 1);
+    Tensor codes = at::empty({rows, stride}, x.options().dtype(at::kChar)), scales = at::empty(lead, x.options().dtype(at::kFloat));
+    std::vector<int64_t> strides(shape.size(), 1);
+    int64_t next = stride;
+    for (int64_t i = static_cast<int64_t>(shape.size()) - 2; i >= 0; --i) strides[i] = next, next *= std::max<int64_t>(shape[i], 1);
+    return {codes.as_strided(shape, strides), scales, stride};
+}
+
+void norm_width(const Tensor& x, const char* name) {
+    if (x.dim() < 1 || x.size(-1) < 1) refuse(std::string(name) + " needs a last dimension of at least 1, got " + shape_of(x));
+    if (x.size(-1) > MGOPT_MAX_NORM_WIDTH) refuse("rows of more than " + std::to_string(MGOPT_MAX_NORM_WIDTH) + " elements");
+}
+Tensor norm_weight(const Tensor& weight, const Tensor& x, int32_t& code) {
+    beside(weight, x, "weight");
+    code = code_of(weight, "weight");
+    if (weight.dim() != 1 || weight.size(0) != x.size(-1))
+        refuse("weight needs shape (" + std::to_string(x.size(-1)) + ",), got " + shape_of(weight));
+    return weight.contiguous();
+}
+
+// (y, h), or (codes, scales, h): h is x itself where there is no residual
+py::tuple rms_norm(const Tensor& x, const optional<Tensor>& residual, const Tensor& weight, double eps, bool int8,
+                   uint64_t stream) {
+    on_gpu(x, "x");
+    const int32_t dtype = code_of(x, "x");
+    norm_width(x, "x");
+    if (residual.has_value()) {
+        beside(*residual, x, "residual");
+        same_dtype(*residual, x, "residual");
+        if (residual->sizes() != x.sizes()) refuse("x and residual differ in shape: " + shape_of(x) + ", " + shape_of(*residual));
+    }
+    if (!(eps >= 0.0)) refuse("eps must not be negative");
+    const c10::DeviceGuard guard(x.device());
+    int32_t weight_dtype;
+    const Tensor w = norm_weight(weight, x, weight_dtype);
+    const Rows a = rows_of(x), b = residual.has_value() ? rows_of(*residual) : Rows{};
+    Tensor h = residual.has_value() ? at::empty(x.sizes(), x.options()) : x, y;
+    Codes c;
+    if (int8) c = codes_for(x, a.rows, a.width);
+    else y = at::empty(x.sizes(), x.options());
+    check(lib.rms_norm(a.t.data_ptr(), a.stride, residual.has_value() ? b.t.data_ptr() : nullptr,
+                       residual.has_value() ? b.stride : 0, w.data_ptr(), weight_dtype, dtype, a.rows, a.width, eps,
+                       residual.has_value() ? h.data_ptr() : nullptr, int8 ? nullptr : y.data_ptr(),
+                       int8 ? c.codes.data_ptr<int8_t>() : nullptr, c.stride, int8 ? c.scales.data_ptr<float>() : nullptr,
+                       as_stream(stream)),
+          "rms_norm");
+    return int8 ? py::make_tuple(c.codes, c.scales, h) : py::make_tuple(y, h);
+}
+
+// (d_x, d_weight or None)
+py::tuple rms_norm_backward(const Tensor& grad_y, const optional<Tensor>& grad_h, const Tensor& h, const Tensor& weight,
+                            double eps, bool want_weight, uint64_t stream) {
+    on_gpu(h, "h");
+    const int32_t dtype = code_of(h, "h");
+    norm_width(h, "h");
+    const auto like_h = [&](const Tensor& g, const char* name) {
+        beside(g, h, name);
+        same_dtype(g, h, name);
+        if (g.sizes() != h.sizes()) refuse(std::string(name) + " needs h's shape " + shape_of(h) + ", got " + shape_of(g));
+    };
+    like_h(grad_y, "grad_y");
+    if (grad_h.has_value()) like_h(*grad_h, "grad_h");
+    if (!(eps >= 0.0)) refuse("eps must not be negative");
+    const c10::DeviceGuard guard(h.device());
+    int32_t weight_dtype;
+    const Tensor w = norm_weight(weight, h, weight_dtype);
+    const Rows gy = rows_of(grad_y), gh = grad_h.has_value() ? rows_of(*grad_h) : Rows{}, s = rows_of(h);
+    Tensor dx = at::empty(h.sizes(), h.options()), work;
+    optional<Tensor> dw;
+    if (want_weight) {
+        dw = at::empty(weight.sizes(), weight.options());
+        work = at::empty({lib.rms_norm_workspace(s.rows, s.width)}, h.options().dtype(at::kByte));
+    }
+    check(lib.rms_norm_backward(gy.t.data_ptr(), gy.stride, grad_h.has_value() ? gh.t.data_ptr() : nullptr,
+                                grad_h.has_value() ? gh.stride : 0, s.t.data_ptr(), s.stride, w.data_ptr(), weight_dtype,
+                                dtype, s.rows, s.width, eps, dx.data_ptr(), want_weight ? dw->data_ptr() : nullptr,
+                                want_weight ? work.data_ptr() : nullptr, as_stream(stream)),
+          "rms_norm_backward");
+    return py::make_tuple(dx, dw);
+}
+
+// (codes, scales)
+py::tuple int8_rows(const Tensor& x, uint64_t stream) {
+    on_gpu(x, "x");
+    const int32_t dtype = code_of(x, "x");
+    if (x.dim() < 1 || x.size(-1) < 1) refuse("x needs a last dimension of at least 1, got " + shape_of(x));
+    const c10::DeviceGuard guard(x.device());
+    const Rows r = rows_of(x);
+    Codes c = codes_for(x, r.rows, r.width);
+    check(lib.int8_rows(r.t.data_ptr(), r.stride, dtype, r.rows, r.width, c.codes.data_ptr<int8_t>(), c.stride,
+                        c.scales.data_ptr<float>(), as_stream(stream)),
+          "int8_rows");
+    return py::make_tuple(c.codes, c.scales);
+}
+
 }  // namespace
 
 void define_ops(py::module_& m) {
@@ -569,4 +681,7 @@ void define_ops(py::module_& m) {
     m.def("token_log_probs", &token_log_probs);
     m.def("policy_loss", &policy_loss);
     m.def("policy_loss_backward", &policy_loss_backward);
+    m.def("rms_norm", &rms_norm);
+    m.def("rms_norm_backward", &rms_norm_backward);
+    m.def("int8_rows", &int8_rows);
 }

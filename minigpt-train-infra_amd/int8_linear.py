@@ -1,0 +1,29 @@
+"""Products of 8-bit integers with a scale for each token and each output
+channel, for forward passes that need no gradient (a rollout's).
+
+    y[t, n] = x.scales[t] * weight.scales[n] * sum of x.codes[t] * weight.codes[n]  (+ bias[n])
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _native as N
+
+
+class Int8Rows(NamedTuple):
+    """Rows in 8 bits: row t stands for codes[t] * scales[t]."""
+
+    codes: torch.Tensor      # int8 (..., width); rows may lie further apart than their width
+    scales: torch.Tensor     # float32 (...)
+
+
+def int8_rows(x: torch.Tensor) -> Int8Rows:
+    """x (..., width) in 8 bits, a scale for each row: tokens of an activation, or
+    the output channels of a weight (channels, width).  With m a row's largest
+    magnitude, scale = m / 127 and the codes are the integers nearest to
+    x * (127 / m); m below 2^-119 counts as 0, a row with an inf or a NaN has the
+    scale NaN.  Nothing is recorded for autograd."""
+    return Int8Rows(*N.ops().int8_rows(x, N.ops_stream(x)))
