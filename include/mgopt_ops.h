@@ -169,6 +169,72 @@ MGOPT_API int64_t mgopt_qk_norm_rope_workspace(int32_t dim);
 /* d_x and d_weight from x and the gradient of out. */
 MGOPT_API int mgopt_qk_norm_rope_backward(const mgopt_qk_args* args, void* stream);
 
+/* ---- attention --------------------------------------------------------------- */
+
+#define MGOPT_MAX_ATTENTION_DIM 128
+
+/* Query i of a sequence of n queries and m keys sees key j of it where j <= i + m
+ * - n (causal: the last query sees the last key), or always.  With x = scale q . k
+ * over the keys seen, lse = log(sum(exp(x))) and out = sum(exp(x - lse) v); a query
+ * that sees none has out 0, lse -inf and no gradient.  Query head h reads key head
+ * h / (q_heads / k_heads).
+ *   *_stride       {batch, token, head}, in elements; a head's `dim` elements are
+ *                  contiguous.
+ *   lse_dev        [batch][q_heads][queries]; mgopt_attention takes NULL.
+ *   q_lengths_dev,
+ *   k_lengths_dev  [batch]: the queries (keys) of each row of the batch that are
+ *                  real, or NULL: all.  Clamped to 0 .. queries (keys).
+ *   q_offsets_dev,
+ *   k_offsets_dev  [sequences + 1], not decreasing: packed sequences.  Sequence s has
+ *                  the tokens from offset s to offset s + 1 of a batch of 1.
+ * Both of offset_bytes (4 or 8) bytes.  Queries (keys) of no sequence are not read;
+ * out, d_q (d_k, d_v) are 0 there.  Offsets beyond the tokens are clamped; where
+ * they decrease, what their sequences and the tokens between hold is not specified. */
+typedef struct mgopt_attention_args {
+    const void* q_dev;
+    const void* k_dev;
+    const void* v_dev;
+    void* out_dev;            /* backward: read */
+    float* lse_dev;           /* backward: read */
+    const void* grad_out_dev; /* backward only, as those that follow */
+    void* d_q_dev;
+    void* d_k_dev;
+    void* d_v_dev;
+    const void* q_offsets_dev;
+    const void* k_offsets_dev;
+    const void* q_lengths_dev;
+    const void* k_lengths_dev;
+    void* workspace_dev; /* mgopt_attention_workspace bytes, 16-byte aligned */
+    int64_t q_stride[3];
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t out_stride[3];
+    int64_t grad_out_stride[3];
+    int64_t d_q_stride[3];
+    int64_t d_k_stride[3];
+    int64_t d_v_stride[3];
+    int64_t batch;
+    int64_t queries; /* tokens of q in a row of the batch */
+    int64_t keys;
+    int64_t sequences;
+    double scale; /* positive, below 2^100 */
+    int32_t q_heads;
+    int32_t k_heads; /* divides q_heads */
+    int32_t dim;
+    int32_t dtype;
+    int32_t offset_bytes;
+    int32_t causal;
+} mgopt_attention_args;
+
+/* Bytes of workspace that a call with these arguments needs (0: none; -1: they are
+ * refused). */
+MGOPT_API int64_t mgopt_attention_workspace(const mgopt_attention_args* args, int32_t backward);
+
+MGOPT_API int mgopt_attention(const mgopt_attention_args* args, void* stream);
+
+/* d_q, d_k and d_v from the gradient of out, out, lse and the inputs. */
+MGOPT_API int mgopt_attention_backward(const mgopt_attention_args* args, void* stream);
+
 /* ---- the clipped policy loss ---------------------------------------------- */
 
 #define MGOPT_MASK_NONE 0   /* every row counts once */

@@ -26,6 +26,7 @@ importlib.import_module("minigpt-train-infra_amd").
 """
 
 from .adamw import AdamW
+from .attention import attention, attention_backward, attention_lse
 from .clip_grad import clip_grad_norm_
 from .embedding import embedding, embedding_grad_
 from .gated_act import ActCheckpoint, gated_act, gated_act_backward, gated_act_pack
@@ -62,6 +63,9 @@ __all__ = [
     "qk_norm_rope_backward",
     "rope_tables",
     "token_log_probs",
+    "attention",
+    "attention_backward",
+    "attention_lse",
     "add_rms_norm",
     "rms_norm",
     "rms_norm_backward",

@@ -37,6 +37,9 @@ struct Entries {
     decltype(&mgopt_rms_norm_workspace) rms_norm_workspace = nullptr;
     decltype(&mgopt_rms_norm_backward) rms_norm_backward = nullptr;
     decltype(&mgopt_int8_rows) int8_rows = nullptr;
+    decltype(&mgopt_attention_workspace) attention_workspace = nullptr;
+    decltype(&mgopt_attention) attention = nullptr;
+    decltype(&mgopt_attention_backward) attention_backward = nullptr;
     decltype(&mgopt_last_error) last_error = nullptr;
     PyObject* error = nullptr;  // the package's MgoptError
 } lib;
@@ -62,6 +65,9 @@ void bind_ops(const py::dict& addresses, const py::object& error) {
     take(lib.rms_norm_workspace, "mgopt_rms_norm_workspace");
     take(lib.rms_norm_backward, "mgopt_rms_norm_backward");
     take(lib.int8_rows, "mgopt_int8_rows");
+    take(lib.attention_workspace, "mgopt_attention_workspace");
+    take(lib.attention, "mgopt_attention");
+    take(lib.attention_backward, "mgopt_attention_backward");
     take(lib.last_error, "mgopt_last_error");
     Py_XDECREF(lib.error);
     lib.error = error.inc_ref().ptr();
@@ -668,6 +674,137 @@ py::tuple int8_rows(const Tensor& x, uint64_t stream) {
     return py::make_tuple(c.codes, c.scales);
 }
 
+// ------------------------------------------------------------- attention
+
+// The arguments both passes share, with the tensors that keep them alive.
+struct Attention {
+    mgopt_attention_args a{};
+    Tensor q, k, v, q_offsets, k_offsets, q_lengths, k_lengths;
+    bool first;  // heads before tokens
+};
+
+Tensor integers(const Tensor& t, const Tensor& q, const char* name, int64_t count, int32_t& bytes) {
+    beside(t, q, name);
+    if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
+        throw py::type_error(std::string(name) + " must be int64 or int32");
+    if (t.dim() != 1 || (count >= 0 ? t.size(0) != count : t.size(0) < 1))
+        refuse(std::string(name) + " needs " + (count >= 0 ? std::to_string(count) + " values" : "one value at least") + ", got shape " +
+               shape_of(t));
+    const int32_t size = static_cast<int32_t>(t.element_size());
+    if (bytes != 0 && bytes != size) throw py::type_error(std::string(name) + " has another integer type than those before it");
+    bytes = size;
+    return t.contiguous();
+}
+
+Attention attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& offsets,
+                         const optional<Tensor>& key_offsets, const optional<Tensor>& lengths, const optional<Tensor>& key_lengths,
+                         bool causal, const optional<double>& scale, bool heads_first) {
+    Attention r;
+    mgopt_attention_args& a = r.a;
+    r.first = heads_first;
+    on_gpu(q, "q");
+    a.dtype = code_of(q, "q");
+    beside(k, q, "k");
+    beside(v, q, "v");
+    same_dtype(k, q, "k");
+    same_dtype(v, q, "v");
+    const int64_t head = heads_first ? 1 : 2, token = heads_first ? 2 : 1;
+    const char* order = heads_first ? "(batch, heads, length, dim)" : "(batch, length, heads, dim)";
+    if (q.dim() != 4 || k.dim() != 4 || k.sizes() != v.sizes() || q.size(0) != k.size(0) || q.size(3) != k.size(3))
+        refuse("q, k and v need shapes " + std::string(order) + " with k's and v's alike and q's batch and dim, got " + shape_of(q) +
+               ", " + shape_of(k) + " and " + shape_of(v));
+    if (q.size(head) < 1 || k.size(head) < 1 || q.size(head) % k.size(head) != 0)
+        refuse("q's heads must be a multiple of k's, got " + std::to_string(q.size(head)) + " and " + std::to_string(k.size(head)));
+    if (q.size(3) < 1) refuse("heads need at least one element, got " + shape_of(q));
+    if (q.size(3) > MGOPT_MAX_ATTENTION_DIM)
+        refuse("heads of more than " + std::to_string(MGOPT_MAX_ATTENTION_DIM) + " elements");
+    a.scale = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3)));
+    if (!(a.scale > 0.0) || !(a.scale < 0x1p100)) refuse("the scale must be positive and below 2^100");
+    a.batch = q.size(0), a.queries = q.size(token), a.keys = k.size(token);
+    a.q_heads = static_cast<int32_t>(q.size(head)), a.k_heads = static_cast<int32_t>(k.size(head));
+    a.dim = static_cast<int32_t>(q.size(3)), a.causal = causal;
+    if (key_offsets.has_value() && !offsets.has_value()) refuse("key_offsets without offsets");
+    if (offsets.has_value()) {
+        if (a.batch != 1) refuse("packed sequences need a batch of 1, got " + shape_of(q));
+        if (lengths.has_value() || key_lengths.has_value()) refuse("packed sequences have offsets, not lengths");
+        if (!key_offsets.has_value() && a.keys != a.queries)
+            refuse("q and k differ in tokens: give key_offsets too, got " + shape_of(q) + " and " + shape_of(k));
+        r.q_offsets = integers(*offsets, q, "offsets", -1, a.offset_bytes);
+        r.k_offsets = key_offsets.has_value() ? integers(*key_offsets, q, "key_offsets", r.q_offsets.size(0), a.offset_bytes) : r.q_offsets;
+        a.sequences = r.q_offsets.size(0) - 1;
+        a.q_offsets_dev = r.q_offsets.data_ptr(), a.k_offsets_dev = r.k_offsets.data_ptr();
+    }
+    if (lengths.has_value()) {
+        r.q_lengths = integers(*lengths, q, "lengths", a.batch, a.offset_bytes);
+        a.q_lengths_dev = r.q_lengths.data_ptr();
+    }
+    if (key_lengths.has_value()) {
+        r.k_lengths = integers(*key_lengths, q, "key_lengths", a.batch, a.offset_bytes);
+        a.k_lengths_dev = r.k_lengths.data_ptr();
+    }
+    r.q = heads_in(q, a.q_stride, heads_first), r.k = heads_in(k, a.k_stride, heads_first), r.v = heads_in(v, a.v_stride, heads_first);
+    a.q_dev = r.q.data_ptr(), a.k_dev = r.k.data_ptr(), a.v_dev = r.v.data_ptr();
+    return r;
+}
+
+int64_t attention_workspace(const mgopt_attention_args& a, bool backward) {
+    const int64_t bytes = lib.attention_workspace(&a, backward);
+    check(bytes < 0 ? MGOPT_E_LIMIT : 0, "attention");
+    return bytes;
+}
+
+// (out, lse or None): out is (batch, length, heads, dim) whichever order the inputs have
+py::tuple attention(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& offsets,
+                    const optional<Tensor>& key_offsets, const optional<Tensor>& lengths, const optional<Tensor>& key_lengths,
+                    bool causal, const optional<double>& scale, bool heads_first, bool want_lse, uint64_t stream) {
+    on_gpu(q, "q");
+    const c10::DeviceGuard guard(q.device());
+    Attention r = attention_args(q, k, v, offsets, key_offsets, lengths, key_lengths, causal, scale, heads_first);
+    mgopt_attention_args& a = r.a;
+    Tensor out = at::empty({a.batch, a.queries, a.q_heads, a.dim}, q.options()), work;
+    heads_in(out, a.out_stride, false);
+    a.out_dev = out.data_ptr();
+    optional<Tensor> lse;
+    if (want_lse) {
+        lse = at::empty({a.batch, a.q_heads, a.queries}, q.options().dtype(at::kFloat));
+        a.lse_dev = lse->data_ptr<float>();
+    }
+    if (const int64_t bytes = attention_workspace(a, false)) {
+        work = at::empty({bytes}, q.options().dtype(at::kByte));
+        a.workspace_dev = work.data_ptr();
+    }
+    check(lib.attention(&a, as_stream(stream)), "attention");
+    return py::make_tuple(out, lse);
+}
+
+py::tuple attention_backward(const Tensor& grad_out, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                             const Tensor& lse, const optional<Tensor>& offsets, const optional<Tensor>& key_offsets,
+                             const optional<Tensor>& lengths, const optional<Tensor>& key_lengths, bool causal,
+                             const optional<double>& scale, bool heads_first, uint64_t stream) {
+    on_gpu(q, "q");
+    const c10::DeviceGuard guard(q.device());
+    Attention r = attention_args(q, k, v, offsets, key_offsets, lengths, key_lengths, causal, scale, heads_first);
+    mgopt_attention_args& a = r.a;
+    beside(grad_out, q, "grad_out");
+    beside(out, q, "out");
+    beside(lse, q, "lse");
+    same_dtype(grad_out, q, "grad_out");
+    same_dtype(out, q, "out");
+    const std::vector<int64_t> shape{a.batch, a.queries, a.q_heads, a.dim}, stats{a.batch, a.q_heads, a.queries};
+    if (grad_out.sizes() != at::IntArrayRef(shape) || out.sizes() != at::IntArrayRef(shape))
+        refuse("grad_out and out need shape " + shape_of(shape) + ", got " + shape_of(grad_out) + " and " + shape_of(out));
+    if (lse.scalar_type() != at::kFloat || lse.sizes() != at::IntArrayRef(stats)) refuse("lse needs float32 of shape " + shape_of(stats));
+    const Tensor g = heads_in(grad_out, a.grad_out_stride, false), o = heads_in(out, a.out_stride, false), l = lse.contiguous();
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+    heads_in(dq, a.d_q_stride, heads_first), heads_in(dk, a.d_k_stride, heads_first), heads_in(dv, a.d_v_stride, heads_first);
+    a.grad_out_dev = g.data_ptr(), a.out_dev = o.data_ptr(), a.lse_dev = l.data_ptr<float>();
+    a.d_q_dev = dq.data_ptr(), a.d_k_dev = dk.data_ptr(), a.d_v_dev = dv.data_ptr();
+    Tensor work = at::empty({attention_workspace(a, true)}, q.options().dtype(at::kByte));
+    a.workspace_dev = work.data_ptr();
+    check(lib.attention_backward(&a, as_stream(stream)), "attention_backward");
+    return py::make_tuple(dq, dk, dv);
+}
+
 }  // namespace
 
 void define_ops(py::module_& m) {
@@ -684,4 +821,6 @@ void define_ops(py::module_& m) {
     m.def("rms_norm", &rms_norm);
     m.def("rms_norm_backward", &rms_norm_backward);
     m.def("int8_rows", &int8_rows);
+    m.def("attention", &attention);
+    m.def("attention_backward", &attention_backward);
 }

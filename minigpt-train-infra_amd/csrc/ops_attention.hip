@@ -1,0 +1,864 @@
+// ops_attention.hip -- attention of grouped heads over batches, packed sequences
+// and caches, and its backward pass.
+//
+// For a sequence of n queries and m keys, query i and key j of a head, x_ij =
+// scale * q_i . k_j where j is seen (j <= i + m - n if causal, so that the last
+// query sees the last key):
+//
+//     lse_i = log sum_j exp(x_ij)      p_ij = exp(x_ij - lse_i)      out_i = sum_j p_ij v_j
+//
+// and with g the gradient of out, delta_i = g_i . out_i:
+//
+//     ds_ij = p_ij (g_i . v_j - delta_i)    dq_i = scale sum_j ds_ij k_j
+//     dv_j = sum_i p_ij g_i                 dk_j = scale sum_i ds_ij q_i
+//
+// A query that sees no key has out 0, lse -inf and no gradient.
+//
+// The query heads that share a key head are rows of one matrix: row r of a
+// sequence is query r / group, head r % group of the group, so that keys and
+// values are read once for all of them and few queries of many heads fill a tile.
+//
+// All products run on the matrix cores in blocks of 32 x 32.  The block's C layout
+// leaves in a lane one column and, in its 16 registers, rows 8 (e/4) + 4 (lane/32) +
+// e%4.  Scores are formed transposed (forward, dq: a column a query; dk and dv: a
+// column a key), so that softmax statistics are one lane's and its partner's, and the
+// probabilities are already the B operand of the product that follows, for that order
+// of the contraction; the A operand is read from LDS transposed, in the same order.
+//
+// dq and dk, dv are kernels of their own, without atomics: scores and g v^T are
+// formed twice, 7 products instead of 5, and the sums' order is fixed.
+#include "ops_common.h"
+
+namespace mgopt {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTile = 128;  // rows (queries x group), or keys, of a work-group: 32 a wave
+constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Eight elements of a lane along the contraction: k = 16 c + 8 (lane/32) + 0..7 of chunk c.
+template <typename T>
+using Frag = T __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x16 mma(Frag<__bf16> a, Frag<__bf16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(Frag<_Float16> a, Frag<_Float16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(Frag<float> a, Frag<float> b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+// Probabilities in fp16 are kept times 2^15 (at most 2^15): those of long rows would be subnormal.
+template <typename T>
+constexpr float kShift = std::is_same_v<T, _Float16> ? 15.0f : 0.0f;
+
+// A tile of rows of DP elements in LDS.  Chunk c (16 bytes) of row r lies at chunk c ^ turn(r) of the
+// row: reads of one chunk of 16 rows, and transposed reads of 4 chunks of 4 rows, fall on different banks.
+template <typename T, int DP>
+struct Tile {
+    static constexpr int kPer = 16 / sizeof(T);          // elements of a chunk
+    static constexpr int kChunks = DP / kPer;            // of a row
+    static __device__ __forceinline__ int turn(int r) {
+        if constexpr (sizeof(T) == 4) {
+            if constexpr (kChunks % 16 == 0) return (r >> 2 & 1) << 3 | (r >> 3 & 1) << 2 | (r & 3);
+            else return r >> 1 & 7;
+        } else if constexpr (kChunks % 16 == 0) {
+            return (r & 3) << 2 | (r >> 2 & 3);
+        } else if constexpr (kChunks == 8) {
+            return (r >> 1 & 1) << 2 | (r >> 2 & 3);
+        } else {
+            return r >> 2 & 3;
+        }
+    }
+    static __device__ __forceinline__ int at(int r, int chunk) { return r * DP + ((chunk ^ turn(r)) * kPer); }
+
+    // chunk c of row r of the A operand
+    static __device__ __forceinline__ Frag<T> rows(const T* lds, int r, int c, int h) {
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const Frag<T>*>(lds + at(r, 2 * c + h));
+        } else {
+            typedef T four __attribute__((ext_vector_type(4)));
+            const four x = *reinterpret_cast<const four*>(lds + at(r, 4 * c + 2 * h));
+            const four y = *reinterpret_cast<const four*>(lds + at(r, 4 * c + 2 * h + 1));
+            return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // Transposed: row 32 db + lane%32 of the A operand, its contraction over the tile's rows 16 c .. 16 c + 15 in
+    // the order of the C layout: element e is row 16 c + 8 (e/4) + 4 h + e%4.
+    static __device__ __forceinline__ Frag<T> columns(const T* lds, int db, int c, int lane) {
+        const int h = lane / 32;
+        Frag<T> f;
+        if constexpr (sizeof(T) == 2) {
+            // of 16 lanes, lane i names 4 elements of row i/4 and takes column i of the 4 rows
+            const int d = 32 * db + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+            s16x4 part[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = 16 * c + 8 * j + 4 * h + lane % 16 / 4;
+                part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4*)(lds + at(r, d / kPer) + d % kPer));
+            }
+            f = __builtin_bit_cast(Frag<T>, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int d = 32 * db + lane % 32;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = lds[at(16 * c + 8 * (e / 4) + 4 * h + e % 4, d / kPer) + d % kPer];
+        }
+        return f;
+    }
+};
+
+// N elements from p, those from n on 0.
+template <typename T, int N>
+__device__ __forceinline__ vec_t<T, N> load_part(const T* p, int n) {
+    if (n >= N) return *reinterpret_cast<const vec_t<T, N>*>(p);
+    vec_t<T, N> v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < n ? p[i] : static_cast<T>(0.0f);
+    return v;
+}
+
+// A tile's way from memory to LDS, through registers.
+template <typename T, int DP, int ROWS>
+struct Stage {
+    using L = Tile<T, DP>;
+    static constexpr int kVecs = ROWS * L::kChunks, kEach = (kVecs + kThreads - 1) / kThreads;
+    vec_t<T, L::kPer> reg[kEach];
+    // row(r): where row r of the tile lies, or NULL for zeros
+    template <typename F>
+    __device__ __forceinline__ void load(int dim, F&& row) {
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const int v = x * kThreads + threadIdx.x, r = v / L::kChunks, c = v % L::kChunks;
+            reg[x] = vec_t<T, L::kPer>{};
+            if (kVecs % kThreads == 0 || v < kVecs)
+                if (const T* p = row(r)) reg[x] = load_part<T, L::kPer>(p + c * L::kPer, dim - c * L::kPer);
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const int v = x * kThreads + threadIdx.x, r = v / L::kChunks, c = v % L::kChunks;
+            typedef T chunk __attribute__((ext_vector_type(L::kPer)));
+            if (kVecs % kThreads == 0 || v < kVecs) *reinterpret_cast<chunk*>(lds + L::at(r, c)) = reg[x];
+        }
+    }
+};
+
+struct AttArgs {
+    mgopt_attention_args a;
+    uint32_t group;      // query heads of a key head
+    uint32_t tiles;      // of a batch's row (padded batches)
+    uint32_t splits;
+    float scale2;        // scale * log2(e)
+    float* delta;        // [batch][q_heads][queries]
+    float* part_out;     // [splits][rows][dim]
+    float* part_ml;      // [splits][rows][2]
+};
+
+__device__ __forceinline__ int64_t clamp64(int64_t x, int64_t low, int64_t high) { return x < low ? low : x > high ? high : x; }
+
+// The sequence of a work-group, and its tile's first row in it.
+struct Part {
+    int64_t batch;       // its row of the batch
+    int64_t q0, k0;      // its first query and key there
+    int32_t n, m;        // its queries and keys
+    int32_t total;       // queries (keys) of its place in memory: those from n (m) on are padding
+    int64_t first;       // of the tile, in rows
+};
+
+// Tile `slot` of the queries (`per` rows each), or of the keys with KEYS.  Packed sequences, with what lies before the
+// first and behind the last as two more that hold nothing, have places of their own for floor(rows / kTile) + 1
+// tiles each; `first` is beyond `total` where a place stays empty.  Offsets are clamped to the tokens.
+template <bool KEYS>
+__device__ Part find(const AttArgs& p, uint32_t slot, uint32_t per) {
+    const mgopt_attention_args& a = p.a;
+    Part s{};
+    const int64_t tokens = KEYS ? a.keys : a.queries;
+    if (a.q_offsets_dev == nullptr) {
+        s.batch = slot / p.tiles;
+        s.first = static_cast<int64_t>(slot % p.tiles) * kTile;
+        s.total = static_cast<int32_t>(tokens);
+        s.n = static_cast<int32_t>(a.q_lengths_dev ? clamp64(id_at(a.q_lengths_dev, s.batch, a.offset_bytes), 0, a.queries) : a.queries);
+        s.m = static_cast<int32_t>(a.k_lengths_dev ? clamp64(id_at(a.k_lengths_dev, s.batch, a.offset_bytes), 0, a.keys) : a.keys);
+        return s;
+    }
+    const void* offsets = KEYS ? a.k_offsets_dev : a.q_offsets_dev;
+    const int32_t count = static_cast<int32_t>(a.sequences) + 2;
+    const auto edge = [&](int32_t j) {
+        return j <= 0 ? 0 : j >= count ? tokens : clamp64(id_at(offsets, j - 1, a.offset_bytes), 0, tokens);
+    };
+    const auto base = [&](int32_t j) { return edge(j) * per / kTile + j; };
+    // the last part whose places begin at `slot` or before, 64 of them looked at at once
+    int32_t low = 0, left = count;
+    while (left > 1) {
+        const int32_t step = (left + 63) / 64, at = low + static_cast<int32_t>(threadIdx.x % 64) * step;
+        const uint64_t hit = __ballot(at < low + left && base(at) <= static_cast<int64_t>(slot));
+        const int32_t k = max(1, __popcll(hit)) - 1;
+        left = min(step, left - k * step);
+        low += k * step;
+    }
+    const int64_t from = edge(low), to = edge(low + 1);
+    s.first = (static_cast<int64_t>(slot) - base(low)) * kTile;
+    s.total = static_cast<int32_t>(to > from ? to - from : 0);
+    if (s.first < 0) s.first = 0, s.total = 0;
+    s.q0 = s.k0 = from;
+    if (low >= 1 && low + 1 < count) {
+        const void* others = KEYS ? a.q_offsets_dev : a.k_offsets_dev;
+        const int64_t all = KEYS ? a.queries : a.keys;
+        const int64_t x = clamp64(id_at(others, low - 1, a.offset_bytes), 0, all), y = clamp64(id_at(others, low, a.offset_bytes), 0, all);
+        const int32_t len = static_cast<int32_t>(y > x ? y - x : 0);
+        (KEYS ? s.q0 : s.k0) = x;
+        s.n = KEYS ? len : s.total, s.m = KEYS ? s.total : len;
+    }
+    return s;
+}
+
+// How many keys, from the first, query i of the sequence sees.
+__device__ __forceinline__ int32_t seen(const AttArgs& p, const Part& s, int32_t i) {
+    if (i >= s.n) return 0;
+    return p.a.causal ? max(0, min(s.m, i + 1 + s.m - s.n)) : s.m;
+}
+
+// f of a lane and of the lane 32 away.
+template <typename Op>
+__device__ __forceinline__ float with_partner(float x, Op op) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+
+// One row's elements as the B operand: chunk c's 8 elements of this half of the wave.
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(Frag<T> (&f)[DP / 16], const T* row, int dim, int h) {
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        f[c] = Frag<T>{};
+        if (row != nullptr) {
+            const int d = 16 * c + 8 * h;
+            const vec_t<T, 8> v = load_part<T, 8>(row + d, dim - d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[c][e] = v[e];
+        }
+    }
+}
+
+// Chunk c (of two) of a block of scores as the B operand.
+template <typename T>
+__device__ __forceinline__ Frag<T> as_operand(const f32x16& s, int c) {
+    Frag<T> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = static_cast<T>(s[8 * c + e]);
+    return f;
+}
+
+// A column of the accumulators (rows are the elements of a head) times `by`.
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DP / 32], float by, int dim, int h) {
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int d = 32 * b + 8 * q + 4 * h;
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = acc[b][4 * q + e] * by;
+            store_some<4>(row + d, f, dim - d);
+        }
+}
+
+// Row r's place: query r / group, head r % group of the group.
+struct Place {
+    int32_t query, head;
+};
+__device__ __forceinline__ Place place_of(const AttArgs& p, int64_t r) {
+    const uint32_t x = static_cast<uint32_t>(r), i = x / p.group;
+    return {static_cast<int32_t>(i), static_cast<int32_t>(x - i * p.group)};
+}
+
+template <typename T>
+__device__ __forceinline__ T* row_of(const void* base, const int64_t (&stride)[3], int64_t batch, int64_t token, int64_t head) {
+    return const_cast<T*>(static_cast<const T*>(base)) + batch * stride[0] + token * stride[1] + head * stride[2];
+}
+
+// Which (slot, key head) a work-group has: key heads next to each other, so that with 8 of them each XCD keeps
+// the keys and values of one; the last tiles of causal batches, which see most keys, first.
+struct Unit {
+    uint32_t slot, head;
+};
+__device__ __forceinline__ Unit unit_of(const AttArgs& p, bool last_first) {
+    const uint32_t heads = static_cast<uint32_t>(p.a.k_heads);
+    uint32_t slot = blockIdx.x / heads;
+    const uint32_t head = blockIdx.x - slot * heads;
+    if (p.a.q_offsets_dev == nullptr) {
+        // tiles outermost, the batch's rows within
+        const uint32_t rows = static_cast<uint32_t>(p.a.batch);
+        uint32_t t = slot / rows;
+        const uint32_t b = slot - t * rows;
+        if (last_first) t = p.tiles - 1 - t;
+        slot = b * p.tiles + t;
+    }
+    return {slot, head};
+}
+
+// What any of `rows` rows from r on sees at most; later queries see no fewer keys than earlier ones.
+__device__ __forceinline__ int32_t most_seen(const AttArgs& p, const Part& s, int64_t r, int rows) {
+    return place_of(p, r).query < s.n ? seen(p, s, min(place_of(p, r + rows - 1).query, s.n - 1)) : 0;
+}
+
+// ------------------------------------------------------------------- forward
+
+template <typename T, int DP>
+constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;  // keys of a tile in LDS
+template <typename T, int DP>
+constexpr int kMinWaves = sizeof(T) == 4 ? 1 : 2;  // a SIMD
+
+template <typename T, int DP, bool SPLIT>
+__global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel(AttArgs p) {
+    constexpr int BN = kKeys<T, DP>;
+    using L = Tile<T, DP>;
+    __shared__ alignas(16) T keys[2][BN * DP], values[2][BN * DP];
+    const mgopt_attention_args& a = p.a;
+    const Unit u = unit_of(p, a.causal);
+    const Part s = find<false>(p, u.slot, p.group);
+    if (s.first >= static_cast<int64_t>(s.total) * p.group) return;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 32, h = lane / 32;
+    const Place at = place_of(p, s.first + wave * 32 + col);
+    const int64_t head = static_cast<int64_t>(u.head) * p.group + at.head;
+    const bool inside = at.query < s.total;
+    const int32_t mine = seen(p, s, at.query);
+    Frag<T> q[DP / 16];
+    load_row<T, DP>(q, mine > 0 ? row_of<T>(a.q_dev, a.q_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
+    // what the work-group's rows, and the wave's, see at most, and the wave's at least
+    const int32_t most = most_seen(p, s, s.first, kTile);
+    const int32_t wave_most = most_seen(p, s, s.first + wave * 32, 32);
+    const int32_t wave_least = seen(p, s, place_of(p, s.first + wave * 32).query);
+    int32_t from = 0, to = most;
+    if constexpr (SPLIT) {
+        const int32_t share = (most + BN * static_cast<int32_t>(p.splits) - 1) / (BN * static_cast<int32_t>(p.splits)) * BN;
+        from = static_cast<int32_t>(min(static_cast<int64_t>(blockIdx.y) * share, static_cast<int64_t>(most)));
+        to = min(from + share, most);
+    }
+    Stage<T, DP, BN> stage_k, stage_v;
+    const T* const kp = row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0, u.head);
+    const T* const vp = row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0, u.head);
+    const auto fetch = [&](int32_t k0) {
+        stage_k.load(a.dim, [&](int r) { return k0 + r < to ? kp + (k0 + r) * a.k_stride[1] : nullptr; });
+        stage_v.load(a.dim, [&](int r) { return k0 + r < to ? vp + (k0 + r) * a.v_stride[1] : nullptr; });
+    };
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) o[b] = f32x16{};
+    float top = -INFINITY, sum = 0.0f;
+    if (from < to) {
+        fetch(from);
+        stage_k.store(keys[0]), stage_v.store(values[0]);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int32_t k0 = from; k0 < to; k0 += BN, buf ^= 1) {
+        const bool more = k0 + BN < to;
+        if (more) fetch(k0 + BN);
+        if (k0 < wave_most) {
+            f32x16 x[BN / 32];
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b) {
+                x[b] = f32x16{};
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) x[b] = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x[b]);
+            }
+            if (k0 + BN > wave_least || k0 + BN > to) {
+#pragma unroll
+                for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (k0 + 32 * b + 8 * (e / 4) + 4 * h + e % 4 >= min(mine, to)) x[b][e] = -INFINITY;
+            }
+            float big = x[0][0];
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) big = fmaxf(big, x[b][e]);
+            big = with_partner(big, [](float y, float z) { return fmaxf(y, z); });
+            const float next = fmaxf(top, big);
+            const float ref = next == -INFINITY ? 0.0f : next;
+            if (__any(next > top)) {
+                const float alpha = exp2_hw((top - ref) * p.scale2);
+                sum *= alpha;
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
+                top = next;
+            }
+            const float off = fmaf(ref, p.scale2, -kShift<T>);
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    x[b][e] = exp2_hw(fmaf(x[b][e], p.scale2, -off));
+                    sum += x[b][e];
+                }
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Frag<T> w = as_operand<T>(x[b], c);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) o[d] = mma(L::columns(values[buf], d, 2 * b + c, lane), w, o[d]);
+                }
+        }
+        if (more) stage_k.store(keys[buf ^ 1]), stage_v.store(values[buf ^ 1]);
+        __syncthreads();
+    }
+    sum = with_partner(sum, add);
+    if (!inside) return;
+    if (mine == 0) {  // padding, or no key to see: what its column holds is of a query of zeros without a mask
+        top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) o[b] = f32x16{};
+    }
+    if constexpr (SPLIT) {
+        // rows in the order (batch, query, head)
+        const int64_t rows = a.batch * a.queries * a.q_heads;
+        const int64_t row = blockIdx.y * rows + (s.batch * a.queries + s.q0 + at.query) * a.q_heads + head;
+        store_row<float, DP>(p.part_out + row * a.dim, o, 1.0f, a.dim, h);
+        if (h == 0) p.part_ml[2 * row] = top, p.part_ml[2 * row + 1] = sum;
+    } else {
+        T* const out = row_of<T>(a.out_dev, a.out_stride, s.batch, s.q0 + at.query, head);
+        store_row<T, DP>(out, o, sum == 0.0f ? 0.0f : 1.0f / sum, a.dim, h);
+        if (h == 0 && a.lse_dev != nullptr)
+            a.lse_dev[(s.batch * a.q_heads + head) * a.queries + s.q0 + at.query] =
+                sum == 0.0f ? -INFINITY : static_cast<float>(kLn2) * (top * p.scale2 - kShift<T> + log2f(sum));
+    }
+}
+
+// Joins the parts of a row: a wave a row.
+template <typename T>
+__global__ __launch_bounds__(64) void join_kernel(AttArgs p) {
+    const mgopt_attention_args& a = p.a;
+    const int64_t rows = a.batch * a.queries * a.q_heads, row = blockIdx.x;
+    const int64_t head = row % a.q_heads, t = row / a.q_heads, query = t % a.queries, batch = t / a.queries;
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t i = 0; i < p.splits; ++i) top = fmaxf(top, p.part_ml[2 * (i * rows + row)]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float acc[2] = {};  // elements lane and lane + 64
+    for (uint32_t i = 0; i < p.splits; ++i) {
+        const float* ml = p.part_ml + 2 * (i * rows + row);
+        const float w = exp2_hw((ml[0] - ref) * p.scale2);
+        sum = fmaf(w, ml[1], sum);
+        const float* o = p.part_out + (i * rows + row) * a.dim;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int d = threadIdx.x + 64 * j;
+            if (d < a.dim) acc[j] = fmaf(w, o[d], acc[j]);
+        }
+    }
+    T* out = row_of<T>(a.out_dev, a.out_stride, batch, query, head);
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int d = threadIdx.x + 64 * j;
+        if (d < a.dim) out[d] = static_cast<T>(acc[j] * by);
+    }
+    if (threadIdx.x == 0 && a.lse_dev != nullptr)
+        a.lse_dev[(batch * a.q_heads + head) * a.queries + query] =
+            sum == 0.0f ? -INFINITY : static_cast<float>(kLn2) * (top * p.scale2 - kShift<T> + log2f(sum));
+}
+
+// ------------------------------------------------------------------ backward
+
+// The score gradients of fp16 heads are rounded to fp16 times a power of two of each column's own, lowered
+// with the accumulators when a value would pass 2^15: without it those of long rows, a probability times a
+// small gradient, are subnormal or 0.
+template <typename T>
+struct Range {
+    template <int B>
+    __device__ __forceinline__ void fit(f32x16&, f32x16 (&)[B]) {}
+    __device__ __forceinline__ float back() const { return 1.0f; }
+};
+template <>
+struct Range<_Float16> {
+    float by = 0x1p100f;
+    template <int B>
+    __device__ __forceinline__ void fit(f32x16& ds, f32x16 (&acc)[B]) {
+        float big = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) big = fmaxf(big, fabsf(ds[e]));
+        big = with_partner(big, [](float y, float z) { return fmaxf(y, z); });
+        if (__any(big * by > 32768.0f)) {
+            // the power of two that takes big to [2^13, 2^14); an inf or a NaN is not fitted
+            const bool lower = big * by > 32768.0f && big < INFINITY;
+            const float next = lower ? __uint_as_float((267u - (__float_as_uint(big) >> 23)) << 23) : by;
+            const float change = next / by;
+            by = next;
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[b][e] *= change;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[e] *= by;
+    }
+    __device__ __forceinline__ float back() const { return 1.0f / by; }
+};
+
+// dq, and delta for the kernel that follows.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_kernel(AttArgs p) {
+    constexpr int BN = kKeys<T, DP>;
+    using L = Tile<T, DP>;
+    __shared__ alignas(16) T keys[2][BN * DP], values[2][BN * DP];
+    const mgopt_attention_args& a = p.a;
+    const Unit u = unit_of(p, a.causal);
+    const Part s = find<false>(p, u.slot, p.group);
+    if (s.first >= static_cast<int64_t>(s.total) * p.group) return;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 32, h = lane / 32;
+    const Place at = place_of(p, s.first + wave * 32 + col);
+    const int64_t head = static_cast<int64_t>(u.head) * p.group + at.head;
+    const bool inside = at.query < s.total;
+    const int32_t mine = seen(p, s, at.query);
+    Frag<T> q[DP / 16], g[DP / 16];
+    load_row<T, DP>(q, mine > 0 ? row_of<T>(a.q_dev, a.q_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
+    load_row<T, DP>(g, mine > 0 ? row_of<T>(a.grad_out_dev, a.grad_out_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
+    const int64_t stat = (s.batch * a.q_heads + head) * a.queries + s.q0 + at.query;
+    float delta = 0.0f, lse = INFINITY;
+    {
+        Frag<T> o[DP / 16];
+        load_row<T, DP>(o, mine > 0 ? row_of<T>(a.out_dev, a.out_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = fmaf(static_cast<float>(g[c][e]), static_cast<float>(o[c][e]), delta);
+        delta = with_partner(delta, add);
+        if (inside && h == 0) p.delta[stat] = delta;
+        if (mine > 0) lse = a.lse_dev[stat] * static_cast<float>(kLog2e);
+    }
+    const int32_t to = most_seen(p, s, s.first, kTile);
+    const int32_t wave_most = most_seen(p, s, s.first + wave * 32, 32);
+    const int32_t wave_least = seen(p, s, place_of(p, s.first + wave * 32).query);
+    Stage<T, DP, BN> stage_k, stage_v;
+    const T* const kp = row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0, u.head);
+    const T* const vp = row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0, u.head);
+    const auto fetch = [&](int32_t k0) {
+        stage_k.load(a.dim, [&](int r) { return k0 + r < to ? kp + (k0 + r) * a.k_stride[1] : nullptr; });
+        stage_v.load(a.dim, [&](int r) { return k0 + r < to ? vp + (k0 + r) * a.v_stride[1] : nullptr; });
+    };
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) acc[b] = f32x16{};
+    Range<T> range;
+    if (to > 0) {
+        fetch(0);
+        stage_k.store(keys[0]), stage_v.store(values[0]);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int32_t k0 = 0; k0 < to; k0 += BN, buf ^= 1) {
+        const bool more = k0 + BN < to;
+        if (more) fetch(k0 + BN);
+        if (k0 < wave_most) {
+            const bool edge = k0 + BN > wave_least;
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b) {
+                f32x16 x{}, ds{};
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) x = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x);
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) ds = mma(L::rows(values[buf], 32 * b + col, c, h), g[c], ds);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ds[e] = exp2_hw(fmaf(x[e], p.scale2, -lse)) * (ds[e] - delta);
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (k0 + 32 * b + 8 * (e / 4) + 4 * h + e % 4 >= mine) ds[e] = 0.0f;
+                }
+                range.fit(ds, acc);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Frag<T> w = as_operand<T>(ds, c);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) acc[d] = mma(L::columns(keys[buf], d, 2 * b + c, lane), w, acc[d]);
+                }
+            }
+        }
+        if (more) stage_k.store(keys[buf ^ 1]), stage_v.store(values[buf ^ 1]);
+        __syncthreads();
+    }
+    if (!inside) return;
+    if (mine == 0) {
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) acc[b] = f32x16{};
+    }
+    store_row<T, DP>(row_of<T>(a.d_q_dev, a.d_q_stride, s.batch, s.q0 + at.query, head), acc,
+                     static_cast<float>(a.scale) * range.back(), a.dim, h);
+}
+
+template <typename T, int DP>
+constexpr int kRows = sizeof(T) == 4 ? 32 : 64;  // rows of a tile in LDS, for dk and dv
+
+// dk and dv of 128 keys over all rows that see them.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
+    constexpr int BM = kRows<T, DP>;
+    using L = Tile<T, DP>;
+    __shared__ alignas(16) T queries[2][BM * DP], grads[2][BM * DP];
+    __shared__ alignas(16) float lses[2][BM], deltas[2][BM];
+    __shared__ alignas(16) int32_t limits[2][BM];
+    const mgopt_attention_args& a = p.a;
+    const Unit u = unit_of(p, false);
+    const Part s = find<true>(p, u.slot, 1);
+    if (s.first >= s.total) return;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 32, h = lane / 32;
+    const int32_t tile0 = static_cast<int32_t>(s.first), key = tile0 + wave * 32 + col;
+    const bool live = key < s.m;
+    Frag<T> k[DP / 16], v[DP / 16];
+    load_row<T, DP>(k, live ? row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0 + key, u.head) : nullptr, a.dim, h);
+    load_row<T, DP>(v, live ? row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0 + key, u.head) : nullptr, a.dim, h);
+    // the first row that sees the tile's first key
+    const int32_t rows = s.n * static_cast<int32_t>(p.group);
+    int32_t from = 0;
+    if (a.causal) from = min(max(0, tile0 - (s.m - s.n)), s.n) * static_cast<int32_t>(p.group) / BM * BM;
+    if (tile0 >= s.m) from = rows;
+    const int32_t blind = a.causal ? s.n - s.m : 0;  // queries before this one see no key, and have no gradient
+    Stage<T, DP, BM> stage_q, stage_g;
+    float stat = 0.0f;
+    int32_t limit = 0;
+    const auto fetch = [&](int32_t r0) {
+        const auto row = [&](int r, const void* base, const int64_t (&stride)[3]) -> const T* {
+            if (r0 + r >= rows) return nullptr;
+            const Place at = place_of(p, r0 + r);
+            if (at.query < blind) return nullptr;
+            return row_of<T>(base, stride, s.batch, s.q0 + at.query, static_cast<int64_t>(u.head) * p.group + at.head);
+        };
+        stage_q.load(a.dim, [&](int r) { return row(r, a.q_dev, a.q_stride); });
+        stage_g.load(a.dim, [&](int r) { return row(r, a.grad_out_dev, a.grad_out_stride); });
+        // a row's statistics: thread r of the first BM its lse, r of the second its delta
+        if (threadIdx.x < 2 * BM) {
+            const int r = threadIdx.x % BM;
+            const bool first = threadIdx.x < BM;
+            stat = first ? INFINITY : 0.0f, limit = -1;
+            if (r0 + r < rows) {
+                const Place at = place_of(p, r0 + r);
+                const int64_t i = (s.batch * a.q_heads + static_cast<int64_t>(u.head) * p.group + at.head) * a.queries + s.q0 + at.query;
+                limit = seen(p, s, at.query) - 1;
+                if (!first) stat = p.delta[i];
+                else if (limit >= 0) stat = a.lse_dev[i] * static_cast<float>(kLog2e) - kShift<T>;
+            }
+        }
+    };
+    const auto put = [&](int to) {
+        stage_q.store(queries[to]), stage_g.store(grads[to]);
+        if (threadIdx.x < BM) lses[to][threadIdx.x] = stat, limits[to][threadIdx.x] = limit;
+        else if (threadIdx.x < 2 * BM) deltas[to][threadIdx.x - BM] = stat;
+    };
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) dk[b] = f32x16{}, dv[b] = f32x16{};
+    Range<T> range;
+    if (from < rows) fetch(from), put(0);
+    __syncthreads();
+    int buf = 0;
+    for (int32_t r0 = from; r0 < rows; r0 += BM, buf ^= 1) {
+        const bool more = r0 + BM < rows;
+        if (more) fetch(r0 + BM);
+        // the tile's rows see no fewer keys than its first and no more than its last
+        if (seen(p, s, place_of(p, min(r0 + BM, rows) - 1).query) > tile0 + wave * 32) {
+            const bool edge = seen(p, s, place_of(p, r0).query) < min(tile0 + wave * 32 + 32, s.m);
+#pragma unroll
+            for (int b = 0; b < BM / 32; ++b) {
+                f32x16 x{};
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) x = mma(L::rows(queries[buf], 32 * b + col, c, h), k[c], x);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int r = 32 * b + 8 * (e / 4) + 4 * h + e % 4;
+                    x[e] = exp2_hw(fmaf(x[e], p.scale2, -lses[buf][r]));
+                    if (edge) x[e] = key > limits[buf][r] ? 0.0f : x[e];
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Frag<T> w = as_operand<T>(x, c);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) dv[d] = mma(L::columns(grads[buf], d, 2 * b + c, lane), w, dv[d]);
+                }
+                f32x16 ds{};
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) ds = mma(L::rows(grads[buf], 32 * b + col, c, h), v[c], ds);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int r = 32 * b + 8 * (e / 4) + 4 * h + e % 4;
+                    ds[e] = x[e] * (ds[e] - deltas[buf][r]);
+                    if (edge) ds[e] = key > limits[buf][r] ? 0.0f : ds[e];
+                }
+                range.fit(ds, dk);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Frag<T> w = as_operand<T>(ds, c);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) dk[d] = mma(L::columns(queries[buf], d, 2 * b + c, lane), w, dk[d]);
+                }
+            }
+        }
+        if (more) put(buf ^ 1);
+        __syncthreads();
+    }
+    if (key >= s.total) return;
+    const float down = exp2_hw(-kShift<T>);
+    store_row<T, DP>(row_of<T>(a.d_k_dev, a.d_k_stride, s.batch, s.k0 + key, u.head), dk,
+                     live ? static_cast<float>(a.scale) * range.back() * down : 0.0f, a.dim, h);
+    store_row<T, DP>(row_of<T>(a.d_v_dev, a.d_v_stride, s.batch, s.k0 + key, u.head), dv, live ? down : 0.0f, a.dim, h);
+}
+
+// ---------------------------------------------------------------------- host
+
+int check(const mgopt_attention_args* a, const char* what) {
+    const std::string w(what);
+    if (!a) return set_error(MGOPT_E_INVALID, w + ": NULL arguments");
+    if (!known_dtype(a->dtype)) return set_error(MGOPT_E_INVALID, w + ": bad dtype");
+    if (a->batch < 0 || a->queries < 0 || a->keys < 0 || a->sequences < 0)
+        return set_error(MGOPT_E_INVALID, w + ": negative sizes");
+    if (a->q_heads < 1 || a->k_heads < 1 || a->q_heads % a->k_heads != 0)
+        return set_error(MGOPT_E_INVALID, w + ": the query heads must be a multiple of the key heads");
+    if (a->dim < 1) return set_error(MGOPT_E_INVALID, w + ": heads need at least one element");
+    if (a->dim > MGOPT_MAX_ATTENTION_DIM)
+        return set_error(MGOPT_E_LIMIT, w + ": heads of more than " + std::to_string(MGOPT_MAX_ATTENTION_DIM) + " elements");
+    if (!(a->scale > 0.0) || !(a->scale < 0x1p100)) return set_error(MGOPT_E_INVALID, w + ": the scale must be positive and below 2^100");
+    if ((a->q_offsets_dev == nullptr) != (a->k_offsets_dev == nullptr))
+        return set_error(MGOPT_E_INVALID, w + ": offsets of both sides, or of none");
+    if (a->q_offsets_dev && (a->batch != 1 || a->q_lengths_dev || a->k_lengths_dev))
+        return set_error(MGOPT_E_INVALID, w + ": packed sequences are a batch of 1 and have no lengths");
+    if ((a->q_offsets_dev || a->q_lengths_dev || a->k_lengths_dev) && a->offset_bytes != 4 && a->offset_bytes != 8)
+        return set_error(MGOPT_E_INVALID, w + ": offsets and lengths have 4 or 8 bytes");
+    const int64_t most = int64_t{1} << 30;
+    if (a->keys > most || a->queries > most / a->q_heads || a->sequences > most || a->q_heads > (1 << 20))
+        return set_error(MGOPT_E_LIMIT, w + ": more than 2^30 keys, sequences or queries times heads");
+    return 0;
+}
+
+// Work-groups of `per` rows a token on one side.
+int places(const mgopt_attention_args& a, int64_t tokens, int64_t per, const char* what, uint32_t& tiles, uint32_t& blocks) {
+    const int64_t each = (tokens * per + kTile - 1) / kTile;
+    const int64_t slots = a.q_offsets_dev ? tokens * per / kTile + a.sequences + 2 : each;
+    tiles = static_cast<uint32_t>(each);
+    const int64_t most = max_blocks(kThreads);
+    if (a.q_offsets_dev ? slots > most / a.k_heads : a.batch > 0 && each > most / a.k_heads / a.batch)
+        return set_error(MGOPT_E_LIMIT, std::string(what) + ": too many work-groups");
+    blocks = static_cast<uint32_t>(slots * (a.q_offsets_dev ? 1 : a.batch) * a.k_heads);
+    return 0;
+}
+
+// Parts that the keys of each row are cut in, where the rows alone leave the chip short of work.
+constexpr int64_t kMinShare = 256;   // keys of a part at least
+uint32_t splits_for(const mgopt_attention_args& a) {
+    const int64_t per = a.q_heads / a.k_heads;
+    const int64_t tiles = a.q_offsets_dev ? a.queries * per / kTile + a.sequences : (a.queries * per + kTile - 1) / kTile * a.batch;
+    const int64_t groups = std::max<int64_t>(1, tiles * a.k_heads);
+    const int64_t keys = a.q_offsets_dev ? a.keys / std::max<int64_t>(1, a.sequences) : a.keys;
+    const int64_t s = std::min((512 + groups - 1) / groups, keys / kMinShare);
+    return static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(s, 256)));
+}
+
+template <typename F>
+int with_dim(int32_t dim, F&& f) {
+    if (dim <= 32) return f(std::integral_constant<int, 32>{});
+    if (dim <= 64) return f(std::integral_constant<int, 64>{});
+    if (dim <= 96) return f(std::integral_constant<int, 96>{});
+    return f(std::integral_constant<int, 128>{});
+}
+
+int64_t rows_of_all(const mgopt_attention_args& a) { return a.batch * a.queries * a.q_heads; }
+
+AttArgs args_of(const mgopt_attention_args& a) {
+    AttArgs p{};
+    p.a = a;
+    p.group = static_cast<uint32_t>(a.q_heads / a.k_heads);
+    p.scale2 = static_cast<float>(a.scale * kLog2e);
+    return p;
+}
+
+}  // namespace
+}  // namespace mgopt
+
+using namespace mgopt;
+
+extern "C" {
+
+MGOPT_API int64_t mgopt_attention_workspace(const mgopt_attention_args* a, int32_t backward) {
+    if (check(a, "attention_workspace")) return -1;
+    if (backward) return rows_of_all(*a) * 4;
+    const int64_t splits = splits_for(*a);
+    return splits > 1 ? splits * rows_of_all(*a) * (a->dim + 2) * 4 : 0;
+}
+
+MGOPT_API int mgopt_attention(const mgopt_attention_args* a, void* stream) {
+    if (int rc = check(a, "attention")) return rc;
+    if (rows_of_all(*a) == 0) return 0;
+    if (!a->q_dev || !a->out_dev || (a->keys > 0 && (!a->k_dev || !a->v_dev)))
+        return set_error(MGOPT_E_INVALID, "attention: NULL argument");
+    AttArgs p = args_of(*a);
+    p.splits = splits_for(*a);
+    if (p.splits > 1) {
+        if (!a->workspace_dev || reinterpret_cast<uintptr_t>(a->workspace_dev) % 16 != 0)
+            return set_error(MGOPT_E_ALIGN, "attention: the workspace must be 16-byte aligned and not NULL");
+        p.part_out = static_cast<float*>(a->workspace_dev);
+        p.part_ml = p.part_out + p.splits * rows_of_all(*a) * a->dim;
+    }
+    uint32_t blocks;
+    if (int rc = places(*a, a->queries, p.group, "attention", p.tiles, blocks)) return rc;
+    if (p.splits > 1 && rows_of_all(*a) > max_blocks(64)) return set_error(MGOPT_E_LIMIT, "attention: too many rows");
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return with_dtype(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        return with_dim(a->dim, [&](auto d) {
+            constexpr int DP = decltype(d)::value;
+            if (p.splits == 1) {
+                hipLaunchKernelGGL((attention_kernel<T, DP, false>), dim3(blocks), dim3(kThreads), 0, s, p);
+                return launched("attention");
+            }
+            hipLaunchKernelGGL((attention_kernel<T, DP, true>), dim3(blocks, p.splits), dim3(kThreads), 0, s, p);
+            if (int rc = launched("attention")) return rc;
+            hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<uint32_t>(rows_of_all(*a))), dim3(64), 0, s, p);
+            return launched("attention");
+        });
+    });
+}
+
+MGOPT_API int mgopt_attention_backward(const mgopt_attention_args* a, void* stream) {
+    if (int rc = check(a, "attention_backward")) return rc;
+    const bool rows = rows_of_all(*a) > 0, keys = a->batch * a->keys > 0;
+    if (rows && (!a->q_dev || !a->out_dev || !a->grad_out_dev || !a->lse_dev || !a->d_q_dev))
+        return set_error(MGOPT_E_INVALID, "attention_backward: NULL argument");
+    if (keys && (!a->k_dev || !a->v_dev || !a->d_k_dev || !a->d_v_dev))
+        return set_error(MGOPT_E_INVALID, "attention_backward: NULL argument");
+    if (rows && (!a->workspace_dev || reinterpret_cast<uintptr_t>(a->workspace_dev) % 16 != 0))
+        return set_error(MGOPT_E_ALIGN, "attention_backward: the workspace must be 16-byte aligned and not NULL");
+    AttArgs p = args_of(*a);
+    p.delta = static_cast<float*>(a->workspace_dev);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return with_dtype(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        return with_dim(a->dim, [&](auto d) -> int {
+            constexpr int DP = decltype(d)::value;
+            uint32_t blocks;
+            if (rows) {
+                if (int rc = places(*a, a->queries, p.group, "attention_backward", p.tiles, blocks)) return rc;
+                hipLaunchKernelGGL((attention_dq_kernel<T, DP>), dim3(blocks), dim3(kThreads), 0, s, p);
+                if (int rc = launched("attention_backward")) return rc;
+            }
+            if (!keys) return 0;
+            if (int rc = places(*a, a->keys, 1, "attention_backward", p.tiles, blocks)) return rc;
+            hipLaunchKernelGGL((attention_dkv_kernel<T, DP>), dim3(blocks), dim3(kThreads), 0, s, p);
+            return launched("attention_backward");
+        });
+    });
+}
+
+}  // extern "C"
