@@ -110,6 +110,17 @@ MGOPT_API int mgopt_rms_norm_backward(const void* grad_y_dev, int64_t grad_y_str
 MGOPT_API int mgopt_int8_rows(const void* x_dev, int64_t x_stride, int32_t dtype, int64_t rows, int64_t width,
                               int8_t* codes_dev, int64_t codes_stride, float* scales_dev, void* stream);
 
+/* ---- products of 8-bit integers ---------------------------------------------- */
+
+#define MGOPT_MAX_INT8_WIDTH 131071
+
+/* y[t][n] = (x_scales[t] * w_scales[n]) * sum_k x[t][k] * w[n][k] + bias[n], the sum
+ * exact in 32 bits, y contiguous; x has `rows` rows, w `channels`, of `width` codes.
+ * Strides are those between rows; bias_dev may be NULL. */
+MGOPT_API int mgopt_int8_linear(const int8_t* x_dev, int64_t x_stride, const float* x_scales_dev, const int8_t* w_dev,
+                                int64_t w_stride, const float* w_scales_dev, const void* bias_dev, int32_t bias_dtype,
+                                int64_t rows, int64_t width, int64_t channels, void* y_dev, int32_t dtype, void* stream);
+
 /* ---- query/key norms and the rotation -------------------------------------- */
 
 #define MGOPT_MAX_HEAD_DIM 512

@@ -31,7 +31,7 @@ from .clip_grad import clip_grad_norm_
 from .embedding import embedding, embedding_grad_
 from .gated_act import ActCheckpoint, gated_act, gated_act_backward, gated_act_pack
 from .grad_scaler import GradScaler
-from .int8_linear import Int8Rows, int8_rows
+from .int8_linear import Int8Rows, int8_linear, int8_rows
 from .policy_loss import PolicyLoss, policy_loss, policy_loss_grad, token_log_probs
 from .qk_norm_rope import qk_norm_rope, qk_norm_rope_backward, rope_tables
 from .rms_norm import add_rms_norm, rms_norm, rms_norm_backward, rms_norm_int8
@@ -71,5 +71,6 @@ __all__ = [
     "rms_norm_backward",
     "rms_norm_int8",
     "Int8Rows",
+    "int8_linear",
     "int8_rows",
 ]

@@ -56,6 +56,7 @@ OPS_EXPORTS = (
     "mgopt_rms_norm_workspace",
     "mgopt_rms_norm_backward",
     "mgopt_int8_rows",
+    "mgopt_int8_linear",
     "mgopt_attention_workspace",
     "mgopt_attention",
     "mgopt_attention_backward",

@@ -15,7 +15,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 #: the optimizer step and the training-step operators
 SRCS = [HERE / "csrc" / name for name in ("mgopt.hip", "ops_attention.hip", "ops_embedding.hip", "ops_gated_act.hip",
-                                          "ops_policy_loss.hip", "ops_qk_norm_rope.hip", "ops_rms_norm.hip")]
+                                          "ops_int8_linear.hip", "ops_policy_loss.hip", "ops_qk_norm_rope.hip", "ops_rms_norm.hip")]
 INCLUDE = HERE.parent / "include"
 OUT_DIR = HERE / "_build"
 LIB = OUT_DIR / "libmgopt.so"

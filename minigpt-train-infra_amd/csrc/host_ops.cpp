@@ -37,6 +37,7 @@ struct Entries {
     decltype(&mgopt_rms_norm_workspace) rms_norm_workspace = nullptr;
     decltype(&mgopt_rms_norm_backward) rms_norm_backward = nullptr;
     decltype(&mgopt_int8_rows) int8_rows = nullptr;
+    decltype(&mgopt_int8_linear) int8_linear = nullptr;
     decltype(&mgopt_attention_workspace) attention_workspace = nullptr;
     decltype(&mgopt_attention) attention = nullptr;
     decltype(&mgopt_attention_backward) attention_backward = nullptr;
@@ -65,6 +66,7 @@ void bind_ops(const py::dict& addresses, const py::object& error) {
     take(lib.rms_norm_workspace, "mgopt_rms_norm_workspace");
     take(lib.rms_norm_backward, "mgopt_rms_norm_backward");
     take(lib.int8_rows, "mgopt_int8_rows");
+    take(lib.int8_linear, "mgopt_int8_linear");
     take(lib.attention_workspace, "mgopt_attention_workspace");
     take(lib.attention, "mgopt_attention");
     take(lib.attention_backward, "mgopt_attention_backward");
@@ -674,6 +676,49 @@ py::tuple int8_rows(const Tensor& x, uint64_t stream) {
     return py::make_tuple(c.codes, c.scales);
 }
 
+// ----------------------------------------------------------- int8_linear
+
+// Codes (..., width) as rows, and a scale for each of them.
+Rows int8_operand(const Tensor& codes, const Tensor& scales, const std::string& name) {
+    if (codes.scalar_type() != at::kChar || scales.scalar_type() != at::kFloat)
+        throw py::type_error(name + " needs int8 codes and float32 scales");
+    if (codes.dim() < 1 || codes.size(-1) < 1) refuse(name + "'s codes need a last dimension of at least 1, got " + shape_of(codes));
+    if (scales.sizes() != codes.sizes().slice(0, codes.dim() - 1))
+        refuse(name + " needs a scale for each row, got codes " + shape_of(codes) + " and scales " + shape_of(scales));
+    return rows_of(codes);
+}
+
+Tensor int8_linear(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Tensor& w_scales, const optional<Tensor>& bias,
+                   const py::object& dtype, uint64_t stream) {
+    on_gpu(x, "x");
+    beside(x_scales, x, "x's scales");
+    beside(w, x, "weight");
+    beside(w_scales, x, "weight's scales");
+    if (w.dim() != 2) refuse("weight needs codes (channels, width), got " + shape_of(w));
+    const c10::DeviceGuard guard(x.device());
+    const Rows a = int8_operand(x, x_scales, "x"), b = int8_operand(w, w_scales, "weight");
+    if (a.width != b.width) refuse("x and weight differ in width: " + shape_of(x) + ", " + shape_of(w));
+    if (a.width > MGOPT_MAX_INT8_WIDTH) refuse("rows of more than " + std::to_string(MGOPT_MAX_INT8_WIDTH) + " codes, whose sums pass 32 bits");
+    Tensor c;
+    int32_t bias_dtype = MGOPT_F32;
+    if (bias.has_value()) {
+        beside(*bias, x, "bias");
+        bias_dtype = code_of(*bias, "bias");
+        if (bias->dim() != 1 || bias->size(0) != b.rows) refuse("bias needs shape (" + std::to_string(b.rows) + ",), got " + shape_of(*bias));
+        c = bias->contiguous();
+    }
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = b.rows;
+    Tensor y = at::empty(shape, x.options().dtype(torch::python::detail::py_object_to_dtype(dtype)));
+    const int32_t code = code_of(y, "the output");
+    const Tensor sx = x_scales.contiguous(), sw = w_scales.contiguous();
+    check(lib.int8_linear(a.t.data_ptr<int8_t>(), a.stride, sx.data_ptr<float>(), b.t.data_ptr<int8_t>(), b.stride,
+                          sw.data_ptr<float>(), bias.has_value() ? c.data_ptr() : nullptr, bias_dtype, a.rows, a.width, b.rows,
+                          y.data_ptr(), code, as_stream(stream)),
+          "int8_linear");
+    return y;
+}
+
 // ------------------------------------------------------------- attention
 
 // The arguments both passes share, with the tensors that keep them alive.
@@ -821,6 +866,7 @@ void define_ops(py::module_& m) {
     m.def("rms_norm", &rms_norm);
     m.def("rms_norm_backward", &rms_norm_backward);
     m.def("int8_rows", &int8_rows);
+    m.def("int8_linear", &int8_linear);
     m.def("attention", &attention);
     m.def("attention_backward", &attention_backward);
 }

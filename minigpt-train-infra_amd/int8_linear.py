@@ -27,3 +27,18 @@ def int8_rows(x: torch.Tensor) -> Int8Rows:
     x * (127 / m); m below 2^-119 counts as 0, a row with an inf or a NaN has the
     scale NaN.  Nothing is recorded for autograd."""
     return Int8Rows(*N.ops().int8_rows(x, N.ops_stream(x)))
+
+
+def int8_linear(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, *,
+                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y (..., channels) of `dtype` (float32, float16 or bfloat16) from x (...,
+    width) and weight (channels, width), of at most 131,071 codes a row: their sums
+    are exact in 32 bits.  bias: (channels,), of any of the three types.  Rows of
+    codes may lie any distance apart, as int8_rows and rms_norm_int8 leave them.
+    Nothing is recorded for autograd: scales and a bias that ask for a gradient are
+    refused."""
+    if torch.is_grad_enabled():
+        for name, t in (("x's scales", x.scales), ("weight's scales", weight.scales), ("bias", bias)):
+            if t is not None and t.requires_grad:
+                raise ValueError(f"int8_linear has no gradient by {name}: detach it")
+    return N.ops().int8_linear(x.codes, x.scales, weight.codes, weight.scales, bias, dtype, N.ops_stream(x.codes))
