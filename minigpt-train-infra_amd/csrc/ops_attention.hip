@@ -59,25 +59,15 @@ __device__ __forceinline__ f32x16 mma(Frag<float> a, Frag<float> b, f32x16 c) {
 template <typename T>
 constexpr float kShift = std::is_same_v<T, _Float16> ? 15.0f : 0.0f;
 
-// A tile of rows of DP elements in LDS.  Chunk c (16 bytes) of row r lies at chunk c ^ turn(r) of the
-// row: reads of one chunk of 16 rows, and transposed reads of 4 chunks of 4 rows, fall on different banks.
+// A tile of rows of DP elements in LDS, kPitch elements apart: a lane's place plus a constant is every address, and
+// neither 8 rows' reads of a chunk (16 bytes) nor 4 rows' transposed reads of two fall on a bank twice: the
+// pitch is 3, 7, 9 or 13 chunks more than a multiple of 16 (4-byte types: an odd number).
 template <typename T, int DP>
 struct Tile {
     static constexpr int kPer = 16 / sizeof(T);          // elements of a chunk
     static constexpr int kChunks = DP / kPer;            // of a row
-    static __device__ __forceinline__ int turn(int r) {
-        if constexpr (sizeof(T) == 4) {
-            if constexpr (kChunks % 16 == 0) return (r >> 2 & 1) << 3 | (r >> 3 & 1) << 2 | (r & 3);
-            else return r >> 1 & 7;
-        } else if constexpr (kChunks % 16 == 0) {
-            return (r & 3) << 2 | (r >> 2 & 3);
-        } else if constexpr (kChunks == 8) {
-            return (r >> 1 & 1) << 2 | (r >> 2 & 3);
-        } else {
-            return r >> 2 & 3;
-        }
-    }
-    static __device__ __forceinline__ int at(int r, int chunk) { return r * DP + ((chunk ^ turn(r)) * kPer); }
+    static constexpr int kPitch = (sizeof(T) == 4 ? kChunks + 1 : kChunks == 4 ? 7 : kChunks == 16 ? 19 : kChunks + 1) * kPer;
+    static __device__ __forceinline__ int at(int r, int chunk) { return r * kPitch + chunk * kPer; }
 
     // chunk c of row r of the A operand
     static __device__ __forceinline__ Frag<T> rows(const T* lds, int r, int c, int h) {
@@ -130,27 +120,65 @@ template <typename T, int DP, int ROWS>
 struct Stage {
     using L = Tile<T, DP>;
     static constexpr int kVecs = ROWS * L::kChunks, kEach = (kVecs + kThreads - 1) / kThreads;
+    static constexpr bool kWhole = kVecs % kThreads == 0;
+    static constexpr int kStep = kThreads % L::kChunks == 0 ? kThreads / L::kChunks : 0;  // rows from vector to vector
     vec_t<T, L::kPer> reg[kEach];
-    // row(r): where row r of the tile lies, or NULL for zeros
-    template <typename F>
-    __device__ __forceinline__ void load(int dim, F&& row) {
+
+    static __device__ __forceinline__ bool has(int tid, int x) { return kWhole || x * kThreads + tid < kVecs; }
+    static __device__ __forceinline__ int row(int tid, int x) { return (x * kThreads + tid) / L::kChunks; }
+    static __device__ __forceinline__ int chunk(int tid, int x) { return (x * kThreads + tid) % L::kChunks; }
+    static __device__ __forceinline__ vec_t<T, L::kPer> get(const T* base, uint32_t bytes) {
+        return *reinterpret_cast<const vec_t<T, L::kPer>*>(reinterpret_cast<const char*>(base) + bytes);
+    }
+
+    // A whole tile of whole rows, row r at r / group * stride + r % group * inner: offsets of 32 bits from a base that
+    // is alike in all lanes.
+    __device__ __forceinline__ void load_whole(const T* base, uint32_t group, int64_t stride, int64_t inner) {
+        const int tid = threadIdx.x;
+        const auto offset = [&](uint32_t r) {
+            const uint32_t i = group == 1 ? r : r / group;
+            return (i * static_cast<uint32_t>(stride) + (r - i * group) * static_cast<uint32_t>(inner)) * static_cast<uint32_t>(sizeof(T));
+        };
+        if constexpr (kStep > 0 && kWhole) {  // the group divides kStep
+            const uint32_t bytes = offset(row(tid, 0)) + chunk(tid, 0) * 16;
+            const int64_t step = group == 1 ? kStep * stride : kStep / group * stride;
 #pragma unroll
-        for (int x = 0; x < kEach; ++x) {
-            const int v = x * kThreads + threadIdx.x, r = v / L::kChunks, c = v % L::kChunks;
-            reg[x] = vec_t<T, L::kPer>{};
-            if (kVecs % kThreads == 0 || v < kVecs)
-                if (const T* p = row(r)) reg[x] = load_part<T, L::kPer>(p + c * L::kPer, dim - c * L::kPer);
+            for (int x = 0; x < kEach; ++x) reg[x] = get(base + x * step, bytes);
+        } else {
+#pragma unroll
+            for (int x = 0; x < kEach; ++x)
+                if (has(tid, x)) reg[x] = get(base, offset(row(tid, x)) + chunk(tid, x) * 16);
         }
+    }
+    // at(r): where row r lies.
+    template <typename F>
+    __device__ __forceinline__ void load_rows(int dim, F&& at) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));  // this way is rare: nothing of it is worth a register between the tiles
+#pragma unroll
+        for (int x = 0; x < kEach; ++x)
+            if (has(tid, x)) reg[x] = load_part<T, L::kPer>(at(row(tid, x)) + chunk(tid, x) * L::kPer, dim - chunk(tid, x) * L::kPer);
+    }
+    // Rows of one stride from `base` on, of which `rows` (one at least) are there; the last one stands for those behind it.
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int dim) {
+        if (rows >= ROWS && dim == DP) load_whole(base, 1, stride, 0);
+        else load_rows(dim, [&](int r) { return base + min(r, rows - 1) * stride; });
     }
     __device__ __forceinline__ void store(T* lds) const {
+        typedef T chunk_t __attribute__((ext_vector_type(L::kPer)));
+        const int tid = threadIdx.x;
 #pragma unroll
-        for (int x = 0; x < kEach; ++x) {
-            const int v = x * kThreads + threadIdx.x, r = v / L::kChunks, c = v % L::kChunks;
-            typedef T chunk __attribute__((ext_vector_type(L::kPer)));
-            if (kVecs % kThreads == 0 || v < kVecs) *reinterpret_cast<chunk*>(lds + L::at(r, c)) = reg[x];
-        }
+        for (int x = 0; x < kEach; ++x)
+            if (has(tid, x)) *reinterpret_cast<chunk_t*>(lds + L::at(row(tid, x), chunk(tid, x))) = reg[x];
     }
 };
+
+// A value that all lanes hold alike, in a scalar register.
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const uint32_t low = static_cast<uint32_t>(uniform(static_cast<int32_t>(x)));
+    return static_cast<int64_t>(uniform(static_cast<int32_t>(x >> 32))) << 32 | low;
+}
 
 struct AttArgs {
     mgopt_attention_args a;
@@ -158,6 +186,7 @@ struct AttArgs {
     uint32_t tiles;      // of a batch's row (padded batches)
     uint32_t splits;
     float scale2;        // scale * log2(e)
+    bool even_rows;      // backward: see attention_dkv_kernel
     float* delta;        // [batch][q_heads][queries]
     float* part_out;     // [splits][rows][dim]
     float* part_ml;      // [splits][rows][2]
@@ -178,7 +207,7 @@ struct Part {
 // first and behind the last as two more that hold nothing, have places of their own for floor(rows / kTile) + 1
 // tiles each; `first` is beyond `total` where a place stays empty.  Offsets are clamped to the tokens.
 template <bool KEYS>
-__device__ Part find(const AttArgs& p, uint32_t slot, uint32_t per) {
+__device__ Part find_part(const AttArgs& p, uint32_t slot, uint32_t per) {
     const mgopt_attention_args& a = p.a;
     Part s{};
     const int64_t tokens = KEYS ? a.keys : a.queries;
@@ -219,6 +248,12 @@ __device__ Part find(const AttArgs& p, uint32_t slot, uint32_t per) {
         s.n = KEYS ? len : s.total, s.m = KEYS ? s.total : len;
     }
     return s;
+}
+
+template <bool KEYS>
+__device__ __forceinline__ Part find(const AttArgs& p, uint32_t slot, uint32_t per) {
+    const Part s = find_part<KEYS>(p, slot, per);
+    return {uniform(s.batch), uniform(s.q0), uniform(s.k0), uniform(s.n), uniform(s.m), uniform(s.total), uniform(s.first)};
 }
 
 // How many keys, from the first, query i of the sequence sees.
@@ -324,12 +359,12 @@ template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel(AttArgs p) {
     constexpr int BN = kKeys<T, DP>;
     using L = Tile<T, DP>;
-    __shared__ alignas(16) T keys[2][BN * DP], values[2][BN * DP];
+    __shared__ alignas(16) T keys[2][BN * L::kPitch], values[2][BN * L::kPitch];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, a.causal);
     const Part s = find<false>(p, u.slot, p.group);
     if (s.first >= static_cast<int64_t>(s.total) * p.group) return;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 32, h = lane / 32;
+    const int lane = threadIdx.x % 64, wave = uniform(static_cast<int32_t>(threadIdx.x / 64)), col = lane % 32, h = lane / 32;
     const Place at = place_of(p, s.first + wave * 32 + col);
     const int64_t head = static_cast<int64_t>(u.head) * p.group + at.head;
     const bool inside = at.query < s.total;
@@ -350,8 +385,8 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
     const T* const kp = row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0, u.head);
     const T* const vp = row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0, u.head);
     const auto fetch = [&](int32_t k0) {
-        stage_k.load(a.dim, [&](int r) { return k0 + r < to ? kp + (k0 + r) * a.k_stride[1] : nullptr; });
-        stage_v.load(a.dim, [&](int r) { return k0 + r < to ? vp + (k0 + r) * a.v_stride[1] : nullptr; });
+        stage_k.load(kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
+        stage_v.load(vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
     };
     f32x16 o[DP / 32];
 #pragma unroll
@@ -440,33 +475,45 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
     }
 }
 
-// Joins the parts of a row: a wave a row.
+// Joins the parts of a row, which a work-group's waves share.
+constexpr uint32_t kMostSplits = kThreads;
 template <typename T>
-__global__ __launch_bounds__(64) void join_kernel(AttArgs p) {
+__global__ __launch_bounds__(kThreads) void join_kernel(AttArgs p) {
+    __shared__ float weight[kMostSplits], tops[kThreads / 64], sums[kThreads / 64], part[kThreads / 64][128];
     const mgopt_attention_args& a = p.a;
     const int64_t rows = a.batch * a.queries * a.q_heads, row = blockIdx.x;
     const int64_t head = row % a.q_heads, t = row / a.q_heads, query = t % a.queries, batch = t / a.queries;
-    float top = -INFINITY, sum = 0.0f;
-    for (uint32_t i = 0; i < p.splits; ++i) top = fmaxf(top, p.part_ml[2 * (i * rows + row)]);
-    const float ref = top == -INFINITY ? 0.0f : top;
+    const uint32_t i = threadIdx.x, wave = i / 64, lane = i % 64;
+    const bool mine = i < p.splits;
+    float top = mine ? p.part_ml[2 * (i * rows + row)] : -INFINITY;
+    const float kept = top, len = mine ? p.part_ml[2 * (i * rows + row) + 1] : 0.0f;
+    top = reduce_lanes<64>(top, [](float x, float y) { return fmaxf(x, y); });
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float w = exp2_hw((kept - (top == -INFINITY ? 0.0f : top)) * p.scale2);
+    if (mine) weight[i] = w;
+    float sum = reduce_lanes<64>(w * len, add);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     float acc[2] = {};  // elements lane and lane + 64
-    for (uint32_t i = 0; i < p.splits; ++i) {
-        const float* ml = p.part_ml + 2 * (i * rows + row);
-        const float w = exp2_hw((ml[0] - ref) * p.scale2);
-        sum = fmaf(w, ml[1], sum);
-        const float* o = p.part_out + (i * rows + row) * a.dim;
+#pragma unroll 8
+    for (uint32_t k = wave; k < p.splits; k += kThreads / 64) {
+        const float* o = p.part_out + (k * rows + row) * a.dim;
+        const float by = weight[k];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int d = threadIdx.x + 64 * j;
-            if (d < a.dim) acc[j] = fmaf(w, o[d], acc[j]);
+            const int d = lane + 64 * j;
+            if (d < a.dim) acc[j] = fmaf(by, o[d], acc[j]);
         }
     }
-    T* out = row_of<T>(a.out_dev, a.out_stride, batch, query, head);
-    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int d = threadIdx.x + 64 * j;
-        if (d < a.dim) out[d] = static_cast<T>(acc[j] * by);
+    part[wave][lane] = acc[0], part[wave][lane + 64] = acc[1];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < a.dim) {
+        const float x = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+        row_of<T>(a.out_dev, a.out_stride, batch, query, head)[d] = static_cast<T>(x * (sum == 0.0f ? 0.0f : 1.0f / sum));
     }
     if (threadIdx.x == 0 && a.lse_dev != nullptr)
         a.lse_dev[(batch * a.q_heads + head) * a.queries + query] =
@@ -515,12 +562,12 @@ template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_kernel(AttArgs p) {
     constexpr int BN = kKeys<T, DP>;
     using L = Tile<T, DP>;
-    __shared__ alignas(16) T keys[2][BN * DP], values[2][BN * DP];
+    __shared__ alignas(16) T keys[2][BN * L::kPitch], values[2][BN * L::kPitch];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, a.causal);
     const Part s = find<false>(p, u.slot, p.group);
     if (s.first >= static_cast<int64_t>(s.total) * p.group) return;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 32, h = lane / 32;
+    const int lane = threadIdx.x % 64, wave = uniform(static_cast<int32_t>(threadIdx.x / 64)), col = lane % 32, h = lane / 32;
     const Place at = place_of(p, s.first + wave * 32 + col);
     const int64_t head = static_cast<int64_t>(u.head) * p.group + at.head;
     const bool inside = at.query < s.total;
@@ -528,9 +575,15 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_ker
     Frag<T> q[DP / 16], g[DP / 16];
     load_row<T, DP>(q, mine > 0 ? row_of<T>(a.q_dev, a.q_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
     load_row<T, DP>(g, mine > 0 ? row_of<T>(a.grad_out_dev, a.grad_out_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
+    const int32_t to = most_seen(p, s, s.first, kTile);
+    const int32_t wave_most = most_seen(p, s, s.first + wave * 32, 32);
+    const int32_t wave_least = seen(p, s, place_of(p, s.first + wave * 32).query);
     const int64_t stat = (s.batch * a.q_heads + head) * a.queries + s.q0 + at.query;
-    float delta = 0.0f, lse = INFINITY;
-    {
+    // Rows whose keys are one tile take delta from it, as sum_j p_ij g_i . v_j: of few keys, what is left of
+    // g_i . v_j - delta_i can be less than the rounding of out.
+    const bool one_tile = wave_most <= BN;
+    float delta = 0.0f, lse = mine > 0 ? a.lse_dev[stat] * static_cast<float>(kLog2e) : INFINITY;
+    if (!one_tile) {
         Frag<T> o[DP / 16];
         load_row<T, DP>(o, mine > 0 ? row_of<T>(a.out_dev, a.out_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
 #pragma unroll
@@ -538,18 +591,13 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_ker
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = fmaf(static_cast<float>(g[c][e]), static_cast<float>(o[c][e]), delta);
         delta = with_partner(delta, add);
-        if (inside && h == 0) p.delta[stat] = delta;
-        if (mine > 0) lse = a.lse_dev[stat] * static_cast<float>(kLog2e);
     }
-    const int32_t to = most_seen(p, s, s.first, kTile);
-    const int32_t wave_most = most_seen(p, s, s.first + wave * 32, 32);
-    const int32_t wave_least = seen(p, s, place_of(p, s.first + wave * 32).query);
     Stage<T, DP, BN> stage_k, stage_v;
     const T* const kp = row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0, u.head);
     const T* const vp = row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0, u.head);
     const auto fetch = [&](int32_t k0) {
-        stage_k.load(a.dim, [&](int r) { return k0 + r < to ? kp + (k0 + r) * a.k_stride[1] : nullptr; });
-        stage_v.load(a.dim, [&](int r) { return k0 + r < to ? vp + (k0 + r) * a.v_stride[1] : nullptr; });
+        stage_k.load(kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
+        stage_v.load(vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
     };
     f32x16 acc[DP / 32];
 #pragma unroll
@@ -565,34 +613,59 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_ker
         const bool more = k0 + BN < to;
         if (more) fetch(k0 + BN);
         if (k0 < wave_most) {
-            const bool edge = k0 + BN > wave_least;
-#pragma unroll
-            for (int b = 0; b < BN / 32; ++b) {
-                f32x16 x{}, ds{};
+            // p_ij and g_i . v_j of keys 32 b .. 32 b + 31 of the tile
+            const auto scores = [&](int b, f32x16& x, f32x16& dp) {
+                x = f32x16{}, dp = f32x16{};
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c) x = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x);
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) ds = mma(L::rows(values[buf], 32 * b + col, c, h), g[c], ds);
+                for (int c = 0; c < DP / 16; ++c) dp = mma(L::rows(values[buf], 32 * b + col, c, h), g[c], dp);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) ds[e] = exp2_hw(fmaf(x[e], p.scale2, -lse)) * (ds[e] - delta);
-                if (edge) {
+                for (int e = 0; e < 16; ++e) x[e] = exp2_hw(fmaf(x[e], p.scale2, -lse));
+            };
+            const auto hide = [&](int b, f32x16& x, f32x16& dp) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (k0 + 32 * b + 8 * (e / 4) + 4 * h + e % 4 >= mine) ds[e] = 0.0f;
+                for (int e = 0; e < 16; ++e) {
+                    const bool out = k0 + 32 * b + 8 * (e / 4) + 4 * h + e % 4 >= mine;
+                    x[e] = out ? 0.0f : x[e], dp[e] = out ? 0.0f : dp[e];
                 }
-                range.fit(ds, acc);
+            };
+            const auto sum_up = [&](int b, const f32x16& x, f32x16& dp) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dp[e] = x[e] * (dp[e] - delta);
+                range.fit(dp, acc);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const Frag<T> w = as_operand<T>(ds, c);
+                    const Frag<T> w = as_operand<T>(dp, c);
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) acc[d] = mma(L::columns(keys[buf], d, 2 * b + c, lane), w, acc[d]);
                 }
+            };
+            const bool edge = k0 + BN > wave_least;
+            if (one_tile) {
+#pragma unroll
+                for (int b = 0; b < BN / 32; ++b) {
+                    f32x16 x, dp;
+                    scores(b, x, dp);
+                    hide(b, x, dp);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) delta = fmaf(x[e], dp[e], delta);
+                }
+                delta = with_partner(delta, add);
+            }
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b) {
+                f32x16 x, dp;
+                scores(b, x, dp);
+                if (edge) hide(b, x, dp);
+                sum_up(b, x, dp);
             }
         }
         if (more) stage_k.store(keys[buf ^ 1]), stage_v.store(values[buf ^ 1]);
         __syncthreads();
     }
     if (!inside) return;
+    if (h == 0) p.delta[stat] = mine > 0 ? delta : 0.0f;
     if (mine == 0) {
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b) acc[b] = f32x16{};
@@ -609,14 +682,14 @@ template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
     constexpr int BM = kRows<T, DP>;
     using L = Tile<T, DP>;
-    __shared__ alignas(16) T queries[2][BM * DP], grads[2][BM * DP];
+    __shared__ alignas(16) T queries[2][BM * L::kPitch], grads[2][BM * L::kPitch];
     __shared__ alignas(16) float lses[2][BM], deltas[2][BM];
     __shared__ alignas(16) int32_t limits[2][BM];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, false);
     const Part s = find<true>(p, u.slot, 1);
     if (s.first >= s.total) return;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 32, h = lane / 32;
+    const int lane = threadIdx.x % 64, wave = uniform(static_cast<int32_t>(threadIdx.x / 64)), col = lane % 32, h = lane / 32;
     const int32_t tile0 = static_cast<int32_t>(s.first), key = tile0 + wave * 32 + col;
     const bool live = key < s.m;
     Frag<T> k[DP / 16], v[DP / 16];
@@ -631,15 +704,21 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
     Stage<T, DP, BM> stage_q, stage_g;
     float stat = 0.0f;
     int32_t limit = 0;
+    // whole tiles whose rows are (query, head) alike from tile to tile, with offsets of 32 bits
+    const bool even = p.even_rows;
+    const T* const qp = row_of<T>(a.q_dev, a.q_stride, s.batch, s.q0, static_cast<int64_t>(u.head) * p.group);
+    const T* const gp = row_of<T>(a.grad_out_dev, a.grad_out_stride, s.batch, s.q0, static_cast<int64_t>(u.head) * p.group);
     const auto fetch = [&](int32_t r0) {
-        const auto row = [&](int r, const void* base, const int64_t (&stride)[3]) -> const T* {
-            if (r0 + r >= rows) return nullptr;
-            const Place at = place_of(p, r0 + r);
-            if (at.query < blind) return nullptr;
-            return row_of<T>(base, stride, s.batch, s.q0 + at.query, static_cast<int64_t>(u.head) * p.group + at.head);
-        };
-        stage_q.load(a.dim, [&](int r) { return row(r, a.q_dev, a.q_stride); });
-        stage_g.load(a.dim, [&](int r) { return row(r, a.grad_out_dev, a.grad_out_stride); });
+        if (even && r0 + BM <= rows && r0 >= blind * static_cast<int32_t>(p.group)) {
+            const int64_t i0 = r0 / static_cast<int32_t>(p.group);
+            stage_q.load_whole(qp + i0 * a.q_stride[1], p.group, a.q_stride[1], a.q_stride[2]);
+            stage_g.load_whole(gp + i0 * a.grad_out_stride[1], p.group, a.grad_out_stride[1], a.grad_out_stride[2]);
+        } else {
+            // rows that are not there, or see no key, are others here: their probabilities are 0
+            const auto at = [&](int r) { return place_of(p, min(max(r0 + r, blind * static_cast<int32_t>(p.group)), rows - 1)); };
+            stage_q.load_rows(a.dim, [&](int r) { const Place x = at(r); return qp + x.query * a.q_stride[1] + x.head * a.q_stride[2]; });
+            stage_g.load_rows(a.dim, [&](int r) { const Place x = at(r); return gp + x.query * a.grad_out_stride[1] + x.head * a.grad_out_stride[2]; });
+        }
         // a row's statistics: thread r of the first BM its lse, r of the second its delta
         if (threadIdx.x < 2 * BM) {
             const int r = threadIdx.x % BM;
@@ -674,29 +753,29 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
             const bool edge = seen(p, s, place_of(p, r0).query) < min(tile0 + wave * 32 + 32, s.m);
 #pragma unroll
             for (int b = 0; b < BM / 32; ++b) {
-                f32x16 x{};
+                f32x16 x{}, ds{};
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c) x = mma(L::rows(queries[buf], 32 * b + col, c, h), k[c], x);
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) ds = mma(L::rows(grads[buf], 32 * b + col, c, h), v[c], ds);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int r = 32 * b + 8 * (e / 4) + 4 * h + e % 4;
                     x[e] = exp2_hw(fmaf(x[e], p.scale2, -lses[buf][r]));
-                    if (edge) x[e] = key > limits[buf][r] ? 0.0f : x[e];
+                    ds[e] = x[e] * (ds[e] - deltas[buf][r]);
+                }
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const bool out = key > limits[buf][32 * b + 8 * (e / 4) + 4 * h + e % 4];
+                        x[e] = out ? 0.0f : x[e], ds[e] = out ? 0.0f : ds[e];
+                    }
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Frag<T> w = as_operand<T>(x, c);
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) dv[d] = mma(L::columns(grads[buf], d, 2 * b + c, lane), w, dv[d]);
-                }
-                f32x16 ds{};
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c) ds = mma(L::rows(grads[buf], 32 * b + col, c, h), v[c], ds);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int r = 32 * b + 8 * (e / 4) + 4 * h + e % 4;
-                    ds[e] = x[e] * (ds[e] - deltas[buf][r]);
-                    if (edge) ds[e] = key > limits[buf][r] ? 0.0f : ds[e];
                 }
                 range.fit(ds, dk);
 #pragma unroll
@@ -719,6 +798,8 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
 
 // ---------------------------------------------------------------------- host
 
+constexpr int64_t kNear = int64_t{1} << 30;  // elements: what a lane's offset of 32 bits reaches, in bytes
+
 int check(const mgopt_attention_args* a, const char* what) {
     const std::string w(what);
     if (!a) return set_error(MGOPT_E_INVALID, w + ": NULL arguments");
@@ -737,6 +818,11 @@ int check(const mgopt_attention_args* a, const char* what) {
         return set_error(MGOPT_E_INVALID, w + ": packed sequences are a batch of 1 and have no lengths");
     if ((a->q_offsets_dev || a->q_lengths_dev || a->k_lengths_dev) && a->offset_bytes != 4 && a->offset_bytes != 8)
         return set_error(MGOPT_E_INVALID, w + ": offsets and lengths have 4 or 8 bytes");
+    for (const int64_t* stride : {a->q_stride, a->k_stride, a->v_stride, a->out_stride, a->grad_out_stride, a->d_q_stride,
+                                  a->d_k_stride, a->d_v_stride})
+        if (stride[0] < 0 || stride[1] < 0 || stride[2] < 0) return set_error(MGOPT_E_INVALID, w + ": negative strides");
+    if (a->k_stride[1] >= kNear / 64 || a->v_stride[1] >= kNear / 64)
+        return set_error(MGOPT_E_LIMIT, w + ": keys or values 2^24 elements apart or more");
     const int64_t most = int64_t{1} << 30;
     if (a->keys > most || a->queries > most / a->q_heads || a->sequences > most || a->q_heads > (1 << 20))
         return set_error(MGOPT_E_LIMIT, w + ": more than 2^30 keys, sequences or queries times heads");
@@ -763,7 +849,7 @@ uint32_t splits_for(const mgopt_attention_args& a) {
     const int64_t groups = std::max<int64_t>(1, tiles * a.k_heads);
     const int64_t keys = a.q_offsets_dev ? a.keys / std::max<int64_t>(1, a.sequences) : a.keys;
     const int64_t s = std::min((512 + groups - 1) / groups, keys / kMinShare);
-    return static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(s, 256)));
+    return static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(s, kMostSplits)));
 }
 
 template <typename F>
@@ -813,7 +899,7 @@ MGOPT_API int mgopt_attention(const mgopt_attention_args* a, void* stream) {
     }
     uint32_t blocks;
     if (int rc = places(*a, a->queries, p.group, "attention", p.tiles, blocks)) return rc;
-    if (p.splits > 1 && rows_of_all(*a) > max_blocks(64)) return set_error(MGOPT_E_LIMIT, "attention: too many rows");
+    if (p.splits > 1 && rows_of_all(*a) > max_blocks(kThreads)) return set_error(MGOPT_E_LIMIT, "attention: too many rows");
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
@@ -825,7 +911,7 @@ MGOPT_API int mgopt_attention(const mgopt_attention_args* a, void* stream) {
             }
             hipLaunchKernelGGL((attention_kernel<T, DP, true>), dim3(blocks, p.splits), dim3(kThreads), 0, s, p);
             if (int rc = launched("attention")) return rc;
-            hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<uint32_t>(rows_of_all(*a))), dim3(64), 0, s, p);
+            hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<uint32_t>(rows_of_all(*a))), dim3(kThreads), 0, s, p);
             return launched("attention");
         });
     });
@@ -847,6 +933,11 @@ MGOPT_API int mgopt_attention_backward(const mgopt_attention_args* a, void* stre
         using T = decltype(t);
         return with_dim(a->dim, [&](auto d) -> int {
             constexpr int DP = decltype(d)::value;
+            const auto near = [&](const int64_t (&stride)[3]) {
+                return stride[1] < kNear / 128 && stride[2] < kNear / 2 / p.group;
+            };
+            constexpr int step = Stage<T, DP, kRows<T, DP>>::kStep;
+            p.even_rows = a->dim == DP && kRows<T, DP> % p.group == 0 && step % p.group == 0 && near(a->q_stride) && near(a->grad_out_stride);
             uint32_t blocks;
             if (rows) {
                 if (int rc = places(*a, a->queries, p.group, "attention_backward", p.tiles, blocks)) return rc;
