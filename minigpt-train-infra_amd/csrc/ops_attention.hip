@@ -115,64 +115,6 @@ __device__ __forceinline__ vec_t<T, N> load_part(const T* p, int n) {
     return v;
 }
 
-// A tile's way from memory to LDS, through registers.
-template <typename T, int DP, int ROWS>
-struct Stage {
-    using L = Tile<T, DP>;
-    static constexpr int kVecs = ROWS * L::kChunks, kEach = (kVecs + kThreads - 1) / kThreads;
-    static constexpr bool kWhole = kVecs % kThreads == 0;
-    static constexpr int kStep = kThreads % L::kChunks == 0 ? kThreads / L::kChunks : 0;  // rows from vector to vector
-    vec_t<T, L::kPer> reg[kEach];
-
-    static __device__ __forceinline__ bool has(int tid, int x) { return kWhole || x * kThreads + tid < kVecs; }
-    static __device__ __forceinline__ int row(int tid, int x) { return (x * kThreads + tid) / L::kChunks; }
-    static __device__ __forceinline__ int chunk(int tid, int x) { return (x * kThreads + tid) % L::kChunks; }
-    static __device__ __forceinline__ vec_t<T, L::kPer> get(const T* base, uint32_t bytes) {
-        return *reinterpret_cast<const vec_t<T, L::kPer>*>(reinterpret_cast<const char*>(base) + bytes);
-    }
-
-    // A whole tile of whole rows, row r at r / group * stride + r % group * inner: offsets of 32 bits from a base that
-    // is alike in all lanes.
-    __device__ __forceinline__ void load_whole(const T* base, uint32_t group, int64_t stride, int64_t inner) {
-        const int tid = threadIdx.x;
-        const auto offset = [&](uint32_t r) {
-            const uint32_t i = group == 1 ? r : r / group;
-            return (i * static_cast<uint32_t>(stride) + (r - i * group) * static_cast<uint32_t>(inner)) * static_cast<uint32_t>(sizeof(T));
-        };
-        if constexpr (kStep > 0 && kWhole) {  // the group divides kStep
-            const uint32_t bytes = offset(row(tid, 0)) + chunk(tid, 0) * 16;
-            const int64_t step = group == 1 ? kStep * stride : kStep / group * stride;
-#pragma unroll
-            for (int x = 0; x < kEach; ++x) reg[x] = get(base + x * step, bytes);
-        } else {
-#pragma unroll
-            for (int x = 0; x < kEach; ++x)
-                if (has(tid, x)) reg[x] = get(base, offset(row(tid, x)) + chunk(tid, x) * 16);
-        }
-    }
-    // at(r): where row r lies.
-    template <typename F>
-    __device__ __forceinline__ void load_rows(int dim, F&& at) {
-        int tid = threadIdx.x;
-        asm volatile("" : "+v"(tid));  // this way is rare: nothing of it is worth a register between the tiles
-#pragma unroll
-        for (int x = 0; x < kEach; ++x)
-            if (has(tid, x)) reg[x] = load_part<T, L::kPer>(at(row(tid, x)) + chunk(tid, x) * L::kPer, dim - chunk(tid, x) * L::kPer);
-    }
-    // Rows of one stride from `base` on, of which `rows` (one at least) are there; the last one stands for those behind it.
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int dim) {
-        if (rows >= ROWS && dim == DP) load_whole(base, 1, stride, 0);
-        else load_rows(dim, [&](int r) { return base + min(r, rows - 1) * stride; });
-    }
-    __device__ __forceinline__ void store(T* lds) const {
-        typedef T chunk_t __attribute__((ext_vector_type(L::kPer)));
-        const int tid = threadIdx.x;
-#pragma unroll
-        for (int x = 0; x < kEach; ++x)
-            if (has(tid, x)) *reinterpret_cast<chunk_t*>(lds + L::at(row(tid, x), chunk(tid, x))) = reg[x];
-    }
-};
-
 // A value that all lanes hold alike, in a scalar register.
 __device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t uniform(int64_t x) {
@@ -180,14 +122,85 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
     return static_cast<int64_t>(uniform(static_cast<int32_t>(x >> 32))) << 32 | low;
 }
 
+// A tile's way from memory to LDS.  Rows whose chunks are aligned to 16 bytes go there without passing through
+// registers: a wave's load puts its 64 chunks behind each other in LDS, those between a row's end and the
+// pitch as well.  Chunks behind `dim` are copies of the row's first: the operand that meets them is 0 there.
+template <typename T, int DP, int ROWS>
+struct Stage {
+    using L = Tile<T, DP>;
+    static constexpr int kRowChunks = L::kPitch / L::kPer;
+    static constexpr int kLoads = (ROWS * kRowChunks + 63) / 64, kEach = (kLoads + kThreads / 64 - 1) / (kThreads / 64);
+    static constexpr int kSize = kLoads * 64 * L::kPer;  // elements of LDS
+    uint32_t off[kEach];
+
+    static __device__ __forceinline__ void load(T* lds, int i, const T* base, uint32_t bytes) {
+        const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) T*)lds)) + i * 1024;
+        // not counted by the compiler: landed() waits for it
+        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(bytes), "s"(base) : "memory", "m0");
+    }
+    static __device__ __forceinline__ uint32_t chunk_bytes(int v, int dim) {
+        const int c = v % kRowChunks;
+        return c * L::kPer < dim ? c * 16 : 0;
+    }
+    // For whole(): row r of a tile lies at r / group * stride + r % group * inner from its base.
+    __device__ __forceinline__ void plan(int wave, uint32_t group, int64_t stride, int64_t inner, int dim) {
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const int v = (x * (kThreads / 64) + wave) * 64 + static_cast<int>(threadIdx.x % 64);
+            const uint32_t r = min(v / kRowChunks, ROWS - 1), i = r / group;
+            off[x] = (i * static_cast<uint32_t>(stride) + (r - i * group) * static_cast<uint32_t>(inner)) * static_cast<uint32_t>(sizeof(T)) +
+                     chunk_bytes(v, dim);
+        }
+    }
+    __device__ __forceinline__ void whole(T* lds, int wave, const T* base) const {
+#pragma unroll
+        for (int x = 0; x < kEach; ++x)
+            if (const int i = x * (kThreads / 64) + wave; i < kLoads) load(lds, i, base, off[x]);
+    }
+    // `rows` rows (one at least) of one stride; the last one stands for those behind it.
+    __device__ __forceinline__ void some(T* lds, int wave, const T* base, int64_t stride, int rows, int dim) const {
+#pragma unroll
+        for (int x = 0; x < kEach; ++x)
+            if (const int i = x * (kThreads / 64) + wave; i < kLoads) {
+                const int v = i * 64 + static_cast<int>(threadIdx.x % 64);
+                const uint32_t row = min(v / kRowChunks, min(rows, ROWS) - 1);
+                load(lds, i, base, row * static_cast<uint32_t>(stride) * static_cast<uint32_t>(sizeof(T)) + chunk_bytes(v, dim));
+            }
+    }
+    // Rows anywhere, through registers; at(r): where row r lies.
+    template <typename F>
+    static __device__ __forceinline__ void copy(T* lds, int dim, F&& at) {
+        typedef T chunk_t __attribute__((ext_vector_type(L::kPer)));
+        int v = threadIdx.x;
+        asm volatile("" : "+v"(v));  // nothing of this rare way is worth a register between the tiles
+        for (; v < ROWS * L::kChunks; v += kThreads) {
+            const int r = v / L::kChunks, c = v % L::kChunks;
+            *reinterpret_cast<chunk_t*>(lds + L::at(r, c)) = load_part<T, L::kPer>(at(r) + c * L::kPer, dim - c * L::kPer);
+        }
+    }
+    __device__ __forceinline__ void fetch(T* lds, int wave, bool aligned, const T* base, int64_t stride, int rows, int dim) const {
+        if (!aligned) copy(lds, dim, [&](int r) { return base + min(r, rows - 1) * stride; });
+        else if (rows >= ROWS) whole(lds, wave, base);
+        else some(lds, wave, base, stride, rows, dim);
+    }
+};
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// 4 bytes from each lane's address to LDS, 256 bytes a wave.
+__device__ __forceinline__ void load_word(void* lds, const void* at) {
+    const uint32_t to = uniform(static_cast<int32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds)));
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(at) : "memory", "m0");
+}
+
 struct AttArgs {
     mgopt_attention_args a;
     uint32_t group;      // query heads of a key head
+    uint32_t magic, shift;  // x / group = (x * magic >> 32) >> shift for x < 2^31, but for a group of 1
     uint32_t tiles;      // of a batch's row (padded batches)
     uint32_t splits;
     float scale2;        // scale * log2(e)
-    bool even_rows;      // backward: see attention_dkv_kernel
-    float* delta;        // [batch][q_heads][queries]
+    bool aligned_keys;   // keys' and values' chunks are aligned to 16 bytes
+    bool aligned_rows;   // queries' and gradients' too, tiles of them have (query, head) alike, and 32 bits reach over them
+    float* stats;        // backward: [2][batch][q_heads][queries], lse * log2(e) - kShift (inf: sees no key), and delta
     float* part_out;     // [splits][rows][dim]
     float* part_ml;      // [splits][rows][2]
 };
@@ -314,7 +327,7 @@ struct Place {
     int32_t query, head;
 };
 __device__ __forceinline__ Place place_of(const AttArgs& p, int64_t r) {
-    const uint32_t x = static_cast<uint32_t>(r), i = x / p.group;
+    const uint32_t x = static_cast<uint32_t>(r), i = p.group == 1 ? x : __umulhi(x, p.magic) >> p.shift;
     return {static_cast<int32_t>(i), static_cast<int32_t>(x - i * p.group)};
 }
 
@@ -324,7 +337,7 @@ __device__ __forceinline__ T* row_of(const void* base, const int64_t (&stride)[3
 }
 
 // Which (slot, key head) a work-group has: key heads next to each other, so that with 8 of them each XCD keeps
-// the keys and values of one; the last tiles of causal batches, which see most keys, first.
+// the keys and values of one; with last_first, for causal batches' queries, the last tiles, which see most keys, first.
 struct Unit {
     uint32_t slot, head;
 };
@@ -359,7 +372,7 @@ template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel(AttArgs p) {
     constexpr int BN = kKeys<T, DP>;
     using L = Tile<T, DP>;
-    __shared__ alignas(16) T keys[2][BN * L::kPitch], values[2][BN * L::kPitch];
+    __shared__ alignas(16) T keys[2][Stage<T, DP, BN>::kSize], values[2][Stage<T, DP, BN>::kSize];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, a.causal);
     const Part s = find<false>(p, u.slot, p.group);
@@ -384,31 +397,29 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
     Stage<T, DP, BN> stage_k, stage_v;
     const T* const kp = row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0, u.head);
     const T* const vp = row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0, u.head);
-    const auto fetch = [&](int32_t k0) {
-        stage_k.load(kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
-        stage_v.load(vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
+    stage_k.plan(wave, 1, a.k_stride[1], 0, a.dim), stage_v.plan(wave, 1, a.v_stride[1], 0, a.dim);
+    const auto fetch = [&](int32_t k0, int buf) {
+        stage_k.fetch(keys[buf], wave, p.aligned_keys, kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
+        stage_v.fetch(values[buf], wave, p.aligned_keys, vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
     };
     f32x16 o[DP / 32];
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) o[b] = f32x16{};
     float top = -INFINITY, sum = 0.0f;
-    if (from < to) {
-        fetch(from);
-        stage_k.store(keys[0]), stage_v.store(values[0]);
-    }
+    if (from < to) fetch(from, 0);
+    landed();
     __syncthreads();
     int buf = 0;
     for (int32_t k0 = from; k0 < to; k0 += BN, buf ^= 1) {
-        const bool more = k0 + BN < to;
-        if (more) fetch(k0 + BN);
+        if (k0 + BN < to) fetch(k0 + BN, buf ^ 1);
         if (k0 < wave_most) {
             f32x16 x[BN / 32];
 #pragma unroll
-            for (int b = 0; b < BN / 32; ++b) {
-                x[b] = f32x16{};
+            for (int b = 0; b < BN / 32; ++b) x[b] = f32x16{};
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) x[b] = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x[b]);
-            }
+            for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+                for (int b = 0; b < BN / 32; ++b) x[b] = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x[b]);
             if (k0 + BN > wave_least || k0 + BN > to) {
 #pragma unroll
                 for (int b = 0; b < BN / 32; ++b)
@@ -450,7 +461,7 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
                     for (int d = 0; d < DP / 32; ++d) o[d] = mma(L::columns(values[buf], d, 2 * b + c, lane), w, o[d]);
                 }
         }
-        if (more) stage_k.store(keys[buf ^ 1]), stage_v.store(values[buf ^ 1]);
+        landed();
         __syncthreads();
     }
     sum = with_partner(sum, add);
@@ -562,7 +573,7 @@ template <typename T, int DP>
 __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_kernel(AttArgs p) {
     constexpr int BN = kKeys<T, DP>;
     using L = Tile<T, DP>;
-    __shared__ alignas(16) T keys[2][BN * L::kPitch], values[2][BN * L::kPitch];
+    __shared__ alignas(16) T keys[2][Stage<T, DP, BN>::kSize], values[2][Stage<T, DP, BN>::kSize];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, a.causal);
     const Part s = find<false>(p, u.slot, p.group);
@@ -595,31 +606,30 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_ker
     Stage<T, DP, BN> stage_k, stage_v;
     const T* const kp = row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0, u.head);
     const T* const vp = row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0, u.head);
-    const auto fetch = [&](int32_t k0) {
-        stage_k.load(kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
-        stage_v.load(vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
+    stage_k.plan(wave, 1, a.k_stride[1], 0, a.dim), stage_v.plan(wave, 1, a.v_stride[1], 0, a.dim);
+    const auto fetch = [&](int32_t k0, int buf) {
+        stage_k.fetch(keys[buf], wave, p.aligned_keys, kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
+        stage_v.fetch(values[buf], wave, p.aligned_keys, vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
     };
     f32x16 acc[DP / 32];
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) acc[b] = f32x16{};
     Range<T> range;
-    if (to > 0) {
-        fetch(0);
-        stage_k.store(keys[0]), stage_v.store(values[0]);
-    }
+    if (to > 0) fetch(0, 0);
+    landed();
     __syncthreads();
     int buf = 0;
     for (int32_t k0 = 0; k0 < to; k0 += BN, buf ^= 1) {
-        const bool more = k0 + BN < to;
-        if (more) fetch(k0 + BN);
+        if (k0 + BN < to) fetch(k0 + BN, buf ^ 1);
         if (k0 < wave_most) {
             // p_ij and g_i . v_j of keys 32 b .. 32 b + 31 of the tile
             const auto scores = [&](int b, f32x16& x, f32x16& dp) {
                 x = f32x16{}, dp = f32x16{};
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) x = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x);
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c) dp = mma(L::rows(values[buf], 32 * b + col, c, h), g[c], dp);
+                for (int c = 0; c < DP / 16; ++c) {
+                    x = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x);
+                    dp = mma(L::rows(values[buf], 32 * b + col, c, h), g[c], dp);
+                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[e] = exp2_hw(fmaf(x[e], p.scale2, -lse));
             };
@@ -661,11 +671,11 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_ker
                 sum_up(b, x, dp);
             }
         }
-        if (more) stage_k.store(keys[buf ^ 1]), stage_v.store(values[buf ^ 1]);
+        landed();
         __syncthreads();
     }
     if (!inside) return;
-    if (h == 0) p.delta[stat] = mine > 0 ? delta : 0.0f;
+    if (h == 0) p.stats[stat] = lse - kShift<T>, p.stats[a.batch * a.q_heads * a.queries + stat] = mine > 0 ? delta : 0.0f;
     if (mine == 0) {
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b) acc[b] = f32x16{};
@@ -675,16 +685,22 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_ker
 }
 
 template <typename T, int DP>
-constexpr int kRows = sizeof(T) == 4 ? 32 : 64;  // rows of a tile in LDS, for dk and dv
+constexpr int kRows = sizeof(T) == 4 || DP > 64 ? 32 : 64;  // rows of a tile in LDS, for dk and dv
+
+// Whether the values stay in LDS: with the keys and both sums they pass the registers of two waves a SIMD.
+template <typename T, int DP>
+constexpr bool kValuesInLds = sizeof(T) == 2 && DP > 64;
 
 // dk and dv of 128 keys over all rows that see them.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
+__global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dkv_kernel(AttArgs p) {
     constexpr int BM = kRows<T, DP>;
+    constexpr bool LDS_V = kValuesInLds<T, DP>;
     using L = Tile<T, DP>;
-    __shared__ alignas(16) T queries[2][BM * L::kPitch], grads[2][BM * L::kPitch];
-    __shared__ alignas(16) float lses[2][BM], deltas[2][BM];
-    __shared__ alignas(16) int32_t limits[2][BM];
+    using Rows = Stage<T, DP, BM>;
+    __shared__ alignas(16) T queries[2][Rows::kSize], grads[2][Rows::kSize];
+    __shared__ alignas(16) T values[LDS_V ? Stage<T, DP, kTile>::kSize : 8];
+    __shared__ alignas(16) float lses[2][64], deltas[2][64];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, false);
     const Part s = find<true>(p, u.slot, 1);
@@ -692,72 +708,68 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
     const int lane = threadIdx.x % 64, wave = uniform(static_cast<int32_t>(threadIdx.x / 64)), col = lane % 32, h = lane / 32;
     const int32_t tile0 = static_cast<int32_t>(s.first), key = tile0 + wave * 32 + col;
     const bool live = key < s.m;
-    Frag<T> k[DP / 16], v[DP / 16];
+    Frag<T> k[DP / 16], v[LDS_V ? 1 : DP / 16];
     load_row<T, DP>(k, live ? row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0 + key, u.head) : nullptr, a.dim, h);
-    load_row<T, DP>(v, live ? row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0 + key, u.head) : nullptr, a.dim, h);
+    if constexpr (!LDS_V) load_row<T, DP>(v, live ? row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0 + key, u.head) : nullptr, a.dim, h);
+    else if (tile0 < s.m)
+        Stage<T, DP, kTile>::copy(values, a.dim, [&](int r) { return row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0 + min(tile0 + r, s.m - 1), u.head); });
     // the first row that sees the tile's first key
-    const int32_t rows = s.n * static_cast<int32_t>(p.group);
+    const int32_t group = static_cast<int32_t>(p.group), rows = s.n * group;
     int32_t from = 0;
-    if (a.causal) from = min(max(0, tile0 - (s.m - s.n)), s.n) * static_cast<int32_t>(p.group) / BM * BM;
+    if (a.causal) from = min(max(0, tile0 - (s.m - s.n)), s.n) * group / BM * BM;
     if (tile0 >= s.m) from = rows;
-    const int32_t blind = a.causal ? s.n - s.m : 0;  // queries before this one see no key, and have no gradient
-    Stage<T, DP, BM> stage_q, stage_g;
-    float stat = 0.0f;
-    int32_t limit = 0;
-    // whole tiles whose rows are (query, head) alike from tile to tile, with offsets of 32 bits
-    const bool even = p.even_rows;
-    const T* const qp = row_of<T>(a.q_dev, a.q_stride, s.batch, s.q0, static_cast<int64_t>(u.head) * p.group);
-    const T* const gp = row_of<T>(a.grad_out_dev, a.grad_out_stride, s.batch, s.q0, static_cast<int64_t>(u.head) * p.group);
-    const auto fetch = [&](int32_t r0) {
-        if (even && r0 + BM <= rows && r0 >= blind * static_cast<int32_t>(p.group)) {
-            const int64_t i0 = r0 / static_cast<int32_t>(p.group);
-            stage_q.load_whole(qp + i0 * a.q_stride[1], p.group, a.q_stride[1], a.q_stride[2]);
-            stage_g.load_whole(gp + i0 * a.grad_out_stride[1], p.group, a.grad_out_stride[1], a.grad_out_stride[2]);
+    const int32_t blind = a.causal ? max(0, s.n - s.m) * group : 0;  // rows before this one see no key, and have no gradient
+    Rows stage_q, stage_g;
+    const int64_t head0 = static_cast<int64_t>(u.head) * group;
+    const T* const qp = row_of<T>(a.q_dev, a.q_stride, s.batch, s.q0, head0);
+    const T* const gp = row_of<T>(a.grad_out_dev, a.grad_out_stride, s.batch, s.q0, head0);
+    stage_q.plan(wave, p.group, a.q_stride[1], a.q_stride[2], a.dim);
+    stage_g.plan(wave, p.group, a.grad_out_stride[1], a.grad_out_stride[2], a.dim);
+    const float* const stats = p.stats + (s.batch * a.q_heads + head0) * a.queries + s.q0;
+    const int64_t all = a.batch * a.q_heads * a.queries;
+    const auto q_row = [&](const Place& x) { return qp + x.query * a.q_stride[1] + x.head * a.q_stride[2]; };
+    const auto g_row = [&](const Place& x) { return gp + x.query * a.grad_out_stride[1] + x.head * a.grad_out_stride[2]; };
+    // rows that are not there, or see no key, are others here: their probabilities are 0
+    const auto at = [&](int32_t r) { return place_of(p, min(max(r, blind), rows - 1)); };
+    const auto fetch = [&](int32_t r0, int buf) {
+        if (p.aligned_rows && r0 + BM <= rows && r0 >= blind) {
+            const int64_t first = place_of(p, r0).query;
+            stage_q.whole(queries[buf], wave, qp + first * a.q_stride[1]);
+            stage_g.whole(grads[buf], wave, gp + first * a.grad_out_stride[1]);
         } else {
-            // rows that are not there, or see no key, are others here: their probabilities are 0
-            const auto at = [&](int r) { return place_of(p, min(max(r0 + r, blind * static_cast<int32_t>(p.group)), rows - 1)); };
-            stage_q.load_rows(a.dim, [&](int r) { const Place x = at(r); return qp + x.query * a.q_stride[1] + x.head * a.q_stride[2]; });
-            stage_g.load_rows(a.dim, [&](int r) { const Place x = at(r); return gp + x.query * a.grad_out_stride[1] + x.head * a.grad_out_stride[2]; });
+            Rows::copy(queries[buf], a.dim, [&](int r) { return q_row(at(r0 + r)); });
+            Rows::copy(grads[buf], a.dim, [&](int r) { return g_row(at(r0 + r)); });
         }
-        // a row's statistics: thread r of the first BM its lse, r of the second its delta
-        if (threadIdx.x < 2 * BM) {
-            const int r = threadIdx.x % BM;
-            const bool first = threadIdx.x < BM;
-            stat = first ? INFINITY : 0.0f, limit = -1;
-            if (r0 + r < rows) {
-                const Place at = place_of(p, r0 + r);
-                const int64_t i = (s.batch * a.q_heads + static_cast<int64_t>(u.head) * p.group + at.head) * a.queries + s.q0 + at.query;
-                limit = seen(p, s, at.query) - 1;
-                if (!first) stat = p.delta[i];
-                else if (limit >= 0) stat = a.lse_dev[i] * static_cast<float>(kLog2e) - kShift<T>;
-            }
+        if (wave < 2) {
+            const Place x = at(r0 + min(lane, BM - 1));
+            load_word(wave == 0 ? lses[buf] : deltas[buf], stats + (wave == 0 ? 0 : all) + x.head * a.queries + x.query);
         }
-    };
-    const auto put = [&](int to) {
-        stage_q.store(queries[to]), stage_g.store(grads[to]);
-        if (threadIdx.x < BM) lses[to][threadIdx.x] = stat, limits[to][threadIdx.x] = limit;
-        else if (threadIdx.x < 2 * BM) deltas[to][threadIdx.x - BM] = stat;
     };
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) dk[b] = f32x16{}, dv[b] = f32x16{};
     Range<T> range;
-    if (from < rows) fetch(from), put(0);
+    // from the last rows, which all key tiles have, to the first, so that the tiles of a head read the same rows at
+    // about the same time
+    const int32_t last = (rows - 1) / BM * BM;
+    if (from < rows) fetch(last, 0);
+    landed();
     __syncthreads();
     int buf = 0;
-    for (int32_t r0 = from; r0 < rows; r0 += BM, buf ^= 1) {
-        const bool more = r0 + BM < rows;
-        if (more) fetch(r0 + BM);
+    for (int32_t r0 = last; r0 >= from && from < rows; r0 -= BM, buf ^= 1) {
+        if (r0 > from) fetch(r0 - BM, buf ^ 1);
         // the tile's rows see no fewer keys than its first and no more than its last
         if (seen(p, s, place_of(p, min(r0 + BM, rows) - 1).query) > tile0 + wave * 32) {
-            const bool edge = seen(p, s, place_of(p, r0).query) < min(tile0 + wave * 32 + 32, s.m);
+            const bool edge = r0 + BM > rows || seen(p, s, place_of(p, r0).query) < min(tile0 + wave * 32 + 32, s.m);
 #pragma unroll
             for (int b = 0; b < BM / 32; ++b) {
                 f32x16 x{}, ds{};
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) x = mma(L::rows(queries[buf], 32 * b + col, c, h), k[c], x);
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c) ds = mma(L::rows(grads[buf], 32 * b + col, c, h), v[c], ds);
+                for (int c = 0; c < DP / 16; ++c) {
+                    x = mma(L::rows(queries[buf], 32 * b + col, c, h), k[c], x);
+                    if constexpr (LDS_V) ds = mma(L::rows(grads[buf], 32 * b + col, c, h), L::rows(values, wave * 32 + col, c, h), ds);
+                    else ds = mma(L::rows(grads[buf], 32 * b + col, c, h), v[c], ds);
+                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int r = 32 * b + 8 * (e / 4) + 4 * h + e % 4;
@@ -767,7 +779,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
                 if (edge) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const bool out = key > limits[buf][32 * b + 8 * (e / 4) + 4 * h + e % 4];
+                        const bool out = key >= seen(p, s, place_of(p, r0 + 32 * b + 8 * (e / 4) + 4 * h + e % 4).query);
                         x[e] = out ? 0.0f : x[e], ds[e] = out ? 0.0f : ds[e];
                     }
                 }
@@ -786,7 +798,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
                 }
             }
         }
-        if (more) put(buf ^ 1);
+        landed();
         __syncthreads();
     }
     if (key >= s.total) return;
@@ -798,7 +810,13 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv_kernel(AttArgs p) {
 
 // ---------------------------------------------------------------------- host
 
-constexpr int64_t kNear = int64_t{1} << 30;  // elements: what a lane's offset of 32 bits reaches, in bytes
+constexpr int64_t kNear = int64_t{1} << 30;  // elements that a lane's offset of 32 bits, in bytes, reaches over
+
+// Whether heads' chunks of 16 bytes are whole and aligned.
+bool aligned(const void* at, const int64_t* stride, int bytes, int32_t dim) {
+    return reinterpret_cast<uintptr_t>(at) % 16 == 0 && dim * bytes % 16 == 0 && stride[0] * bytes % 16 == 0 &&
+           stride[1] * bytes % 16 == 0 && stride[2] * bytes % 16 == 0;
+}
 
 int check(const mgopt_attention_args* a, const char* what) {
     const std::string w(what);
@@ -866,7 +884,11 @@ AttArgs args_of(const mgopt_attention_args& a) {
     AttArgs p{};
     p.a = a;
     p.group = static_cast<uint32_t>(a.q_heads / a.k_heads);
+    uint32_t bits = 0;
+    while ((uint64_t{1} << bits) < p.group) ++bits;
+    if (bits > 0) p.magic = static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + p.group - 1) / p.group), p.shift = bits - 1;
     p.scale2 = static_cast<float>(a.scale * kLog2e);
+    p.aligned_keys = aligned(a.k_dev, a.k_stride, dtype_bytes(a.dtype), a.dim) && aligned(a.v_dev, a.v_stride, dtype_bytes(a.dtype), a.dim);
     return p;
 }
 
@@ -879,7 +901,7 @@ extern "C" {
 
 MGOPT_API int64_t mgopt_attention_workspace(const mgopt_attention_args* a, int32_t backward) {
     if (check(a, "attention_workspace")) return -1;
-    if (backward) return rows_of_all(*a) * 4;
+    if (backward) return rows_of_all(*a) * 8;
     const int64_t splits = splits_for(*a);
     return splits > 1 ? splits * rows_of_all(*a) * (a->dim + 2) * 4 : 0;
 }
@@ -927,17 +949,15 @@ MGOPT_API int mgopt_attention_backward(const mgopt_attention_args* a, void* stre
     if (rows && (!a->workspace_dev || reinterpret_cast<uintptr_t>(a->workspace_dev) % 16 != 0))
         return set_error(MGOPT_E_ALIGN, "attention_backward: the workspace must be 16-byte aligned and not NULL");
     AttArgs p = args_of(*a);
-    p.delta = static_cast<float*>(a->workspace_dev);
+    p.stats = static_cast<float*>(a->workspace_dev);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         return with_dim(a->dim, [&](auto d) -> int {
             constexpr int DP = decltype(d)::value;
-            const auto near = [&](const int64_t (&stride)[3]) {
-                return stride[1] < kNear / 128 && stride[2] < kNear / 2 / p.group;
-            };
-            constexpr int step = Stage<T, DP, kRows<T, DP>>::kStep;
-            p.even_rows = a->dim == DP && kRows<T, DP> % p.group == 0 && step % p.group == 0 && near(a->q_stride) && near(a->grad_out_stride);
+            p.aligned_rows = kRows<T, DP> % p.group == 0;
+            for (const auto& [at, stride] : {std::pair<const void*, const int64_t*>{a->q_dev, a->q_stride}, {a->grad_out_dev, a->grad_out_stride}})
+                p.aligned_rows = p.aligned_rows && aligned(at, stride, sizeof(T), a->dim) && stride[1] < kNear / 256 && stride[2] < kNear / 8 / p.group;
             uint32_t blocks;
             if (rows) {
                 if (int rc = places(*a, a->queries, p.group, "attention_backward", p.tiles, blocks)) return rc;
