@@ -28,15 +28,30 @@ struct LinearArgs {
     int32_t bias_dtype;
 };
 
-// 16 codes from p, those from n on 0.
-__device__ __forceinline__ i32x4 load_codes(const int8_t* p, int64_t n) {
+// 16 codes at an address of any alignment.
+__device__ __forceinline__ i32x4 load_codes(const int8_t* p) {
     typedef int unaligned __attribute__((ext_vector_type(4), aligned(1)));
-    if (n >= 16) return *reinterpret_cast<const unaligned*>(p);
+    return *reinterpret_cast<const unaligned*>(p);
+}
+// 16 codes from code `at` of a row of `width`, those behind the row 0: the last 16 of the row, moved down.
+__device__ __forceinline__ i32x4 load_codes(const int8_t* p, int64_t at, int64_t width) {
+    const int64_t n = width - at;
+    if (n >= 16) return load_codes(p);
     i32x4 v{};
+    if (n <= 0) return v;
+    if (width < 16) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (i < n) v[i / 4] |= static_cast<int>((static_cast<uint32_t>(p[i]) & 0xFFu) << (8 * (i % 4)));
-    return v;
+        for (int i = 0; i < 16; ++i)
+            if (i < n) v[i / 4] |= static_cast<int>((static_cast<uint32_t>(p[i]) & 0xFFu) << (8 * (i % 4)));
+        return v;
+    }
+    typedef uint64_t two __attribute__((ext_vector_type(2)));
+    const two x = __builtin_bit_cast(two, load_codes(p + n - 16));
+    const uint32_t bits = static_cast<uint32_t>(16 - n) * 8;  // 8 .. 120
+    two y;
+    y[0] = bits < 64 ? x[0] >> bits | x[1] << (64 - bits) : x[1] >> (bits - 64);
+    y[1] = bits < 64 ? x[1] >> bits : 0;
+    return __builtin_bit_cast(i32x4, y);
 }
 
 __device__ __forceinline__ i32x16 mma(i32x4 a, i32x4 b, i32x16 c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
@@ -47,30 +62,40 @@ __device__ __forceinline__ float bias_at(const LinearArgs& a, int64_t n) {
     return static_cast<float>(static_cast<const __bf16*>(a.bias)[n]);
 }
 
-// Four channels from n on of token t.
-template <typename T>
-__device__ __forceinline__ void finish(const LinearArgs& a, int64_t t, int64_t n, const int (&sum)[4], float x_scale) {
-    const int64_t left = a.channels - n;
-    if (left <= 0) return;
-    float y[4];
+// Four channels from n on of a token of scale x_scale; those behind the last are the last's.
+__device__ __forceinline__ void scaled(float (&y)[4], const LinearArgs& a, int64_t n, const int (&sum)[4], float x_scale) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t at = i < left ? n + i : n;
+        const int64_t at = min(n + i, a.channels - 1);
         y[i] = static_cast<float>(sum[i]) * (x_scale * a.w_scales[at]);
         if (a.bias != nullptr) y[i] += bias_at(a, at);
     }
-    store_some<4>(static_cast<T*>(a.y) + t * a.channels + n, y, left);
 }
 
-// Tiles of WC * TC * 32 channels and WT * TT * 32 tokens, WC * WT waves with TC x TT blocks of 32 x 32 each.
-// 128 codes of each row at a time lie in LDS, twice: the next ones are on their way while these are multiplied.
-// Chunk c (16 codes) of row r lies at chunk c ^ (r / 2 % 8), so that a chunk of 16 rows falls on all banks.
-template <typename T, int WC, int WT, int TC, int TT>
+// Where chunk c (16 codes) of row r of a tile lies in LDS: chunk c ^ turn(r) of the row, so that a chunk of 16
+// rows falls on all banks.
+template <int CHUNKS>
+__device__ __forceinline__ int turn(int r) { return r / (16 / CHUNKS) % CHUNKS; }
+
+// A wave's load of 64 chunks, each lane's from an address of its own, to LDS behind each other.  The compiler does not
+// count it: waiting is the caller's.
+__device__ __forceinline__ void load_direct(i32x4* lds, const int8_t* from) {
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) i32x4*)lds));
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory", "m0");
+}
+template <int LEFT>
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%0)" ::"i"(LEFT) : "memory"); }
+
+// Tiles of WC * TC * 32 channels and WT * TT * 32 tokens, WC * WT waves with TC x TT blocks of 32 x 32 each, BK codes of
+// the contraction at a time.  ALIGNED (rows start on 16 bytes): codes go to LDS directly, AHEAD stages before they are
+// multiplied.  Otherwise they are AHEAD stages ahead in registers and one in LDS.
+template <typename T, int WC, int WT, int TC, int TT, int BK, int AHEAD, bool ALIGNED>
 __global__ __launch_bounds__(WC* WT * 64, 2) void int8_linear_kernel(LinearArgs a) {
-    constexpr int THREADS = WC * WT * 64, BC = WC * TC * 32, BT = WT * TT * 32, BK = 128, CHUNKS = BK / 16;
-    constexpr int EACH = (BC + BT) * CHUNKS / THREADS;
-    static_assert((BC + BT) * CHUNKS % THREADS == 0 && BC * CHUNKS % THREADS == 0);
-    __shared__ i32x4 lds[2][(BC + BT) * CHUNKS];
+    constexpr int THREADS = WC * WT * 64, BC = WC * TC * 32, BT = WT * TT * 32, CHUNKS = BK / 16, SIZE = (BC + BT) * CHUNKS;
+    constexpr int EACH = SIZE / THREADS, STEP = THREADS / CHUNKS;  // STEP: rows from a thread's chunk to its next
+    constexpr int BUFFERS = ALIGNED ? AHEAD + 1 : 2;
+    static_assert(SIZE % THREADS == 0 && BC * CHUNKS % THREADS == 0 && STEP % 16 == 0);
+    __shared__ i32x4 lds[BUFFERS][SIZE];
     const uint32_t total = a.row_tiles * a.channel_tiles, share = (total + 7) / 8;
     // an XCD's work-groups (every eighth) take neighbouring tiles, eight tiles of tokens at a time
     const uint32_t place = blockIdx.x % 8 * share + blockIdx.x / 8;
@@ -78,138 +103,207 @@ __global__ __launch_bounds__(WC* WT * 64, 2) void int8_linear_kernel(LinearArgs 
     const uint32_t band = place / (8 * a.channel_tiles), in = place - band * 8 * a.channel_tiles;
     const uint32_t high = min(8u, a.row_tiles - band * 8);
     const int64_t t0 = static_cast<int64_t>(band * 8 + in % high) * BT, n0 = static_cast<int64_t>(in / high) * BC;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 32, h = lane / 32;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, h = lane / 32;
     const int wc = wave % WC * TC * 32, wt = wave / WC * TT * 32;
 
-    // rows beyond the last are the last once more: their results are not stored
+    // A thread's chunks: places e * THREADS + threadIdx.x of LDS, one chunk of every STEP-th row.
+    // Rows beyond the last are the last once more: their results are not stored.
+    const int row = threadIdx.x / CHUNKS, mine = ((threadIdx.x % CHUNKS) ^ turn<CHUNKS>(row)) * 16;
     const int8_t* from[EACH];
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        const int v = e * THREADS + threadIdx.x, r = v / CHUNKS, c = v % CHUNKS;
-        from[e] = (r < BC ? a.w + min(n0 + r, a.channels - 1) * a.w_stride : a.x + min(t0 + r - BC, a.rows - 1) * a.x_stride) + c * 16;
-    }
-    const int mine = threadIdx.x % CHUNKS * 16;  // all of a thread's chunks have one column
-    i32x4 next[EACH];
-    const auto fetch = [&](int64_t k) {
-        if (k + BK <= a.width) {
-#pragma unroll
-            for (int e = 0; e < EACH; ++e) next[e] = load_codes(from[e] + k, 16);
-        } else {
-#pragma unroll
-            for (int e = 0; e < EACH; ++e) next[e] = load_codes(from[e] + k, a.width - k - mine);
-        }
-    };
-    const auto put = [&](int to) {
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-            const int v = e * THREADS + threadIdx.x, r = v / CHUNKS, c = v % CHUNKS;
-            lds[to][r * CHUNKS + (c ^ (r / 2 % 8))] = next[e];
-        }
-    };
+    for (int e = 0; e < EACH; ++e)
+        from[e] = (e * STEP < BC ? a.w + min(n0 + e * STEP + row, a.channels - 1) * a.w_stride
+                                 : a.x + min(t0 + e * STEP + row - BC, a.rows - 1) * a.x_stride) + mine;
+    const int32_t stages = static_cast<int32_t>((a.width + BK - 1) / BK), whole = static_cast<int32_t>(a.width / BK);
     i32x16 acc[TC][TT];
 #pragma unroll
     for (int i = 0; i < TC; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) acc[i][j] = i32x16{};
-    fetch(0);
-    put(0);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t k = 0; k < a.width; k += BK, buf ^= 1) {
-        const bool more = k + BK < a.width;
-        if (more) fetch(k + BK);
+    const auto multiply = [&](const i32x4* codes) {
 #pragma unroll
         for (int s = 0; s < BK / 32; ++s) {
             i32x4 w[TC], x[TT];
 #pragma unroll
             for (int i = 0; i < TC; ++i) {
                 const int r = wc + 32 * i + col;
-                w[i] = lds[buf][r * CHUNKS + ((2 * s + h) ^ (r / 2 % 8))];
+                w[i] = codes[r * CHUNKS + ((2 * s + h) ^ turn<CHUNKS>(r))];
             }
 #pragma unroll
             for (int j = 0; j < TT; ++j) {
                 const int r = BC + wt + 32 * j + col;
-                x[j] = lds[buf][r * CHUNKS + ((2 * s + h) ^ (r / 2 % 8))];
+                x[j] = codes[r * CHUNKS + ((2 * s + h) ^ turn<CHUNKS>(r))];
             }
 #pragma unroll
             for (int i = 0; i < TC; ++i)
 #pragma unroll
                 for (int j = 0; j < TT; ++j) acc[i][j] = mma(w[i], x[j], acc[i][j]);
         }
-        if (more) put(buf ^ 1);
+    };
+    if constexpr (ALIGNED) {
+        const auto fetch = [&](int32_t stage, int to) {
+            const int64_t k = static_cast<int64_t>(stage) * BK;
+            if (stage < whole) {
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) load_direct(&lds[to][e * THREADS + wave * 64], from[e] + k);
+            } else if (stage < stages) {
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) lds[to][e * THREADS + threadIdx.x] = load_codes(from[e] + k, k + mine, a.width);
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) fetch(u, u);
+        int buf = 0;
+        for (int32_t stage = 0; stage < stages; ++stage) {
+            // this stage's loads are done when only those of the AHEAD - 1 behind it are not
+            if (stage + AHEAD - 1 < whole) landed<EACH*(AHEAD - 1)>();
+            else landed<0>();
+            __syncthreads();
+            fetch(stage + AHEAD, buf == 0 ? AHEAD : buf - 1);  // where the stage before this one was: all waves have left it
+            multiply(lds[buf]);
+            buf = buf == AHEAD ? 0 : buf + 1;
+        }
+    } else {
+        i32x4 next[AHEAD][EACH];
+        const auto fetch = [&](int32_t stage, int set) {
+            const int64_t k = static_cast<int64_t>(stage) * BK;
+            if (stage < whole) {
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) next[set][e] = load_codes(from[e] + k);
+            } else if (stage < stages) {
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) next[set][e] = load_codes(from[e] + k, k + mine, a.width);
+            }
+        };
+        const auto put = [&](int to, int set) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) lds[to][e * THREADS + threadIdx.x] = next[set][e];
+        };
+        fetch(0, 0);
+        put(0, 0);
+#pragma unroll
+        for (int u = 1; u <= AHEAD; ++u) fetch(u, u % AHEAD);
         __syncthreads();
+        int buf = 0;
+        for (int32_t first = 0; first < stages; first += AHEAD)
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int32_t stage = first + u;
+                if (stage >= stages) break;
+                multiply(lds[buf]);
+                if (stage + 1 < stages) {
+                    put(buf ^ 1, (u + 1) % AHEAD);
+                    fetch(stage + 1 + AHEAD, (u + 1) % AHEAD);
+                }
+                __syncthreads();
+                buf ^= 1;
+            }
     }
+    // A token's channels lie four by four in lanes that are rows of y apart: they pass through LDS, to be written in
+    // rows.  8,192 x 4,096 x 12,288 in bf16: 60 us less than writing 8 bytes a lane.
+    constexpr int PITCH = BC + 16 / static_cast<int>(sizeof(T)), PER = 16 / static_cast<int>(sizeof(T));
+    static_assert(sizeof(lds) >= WT * 32 * PITCH * sizeof(T));
+    T* const out = reinterpret_cast<T*>(&lds[0][0]);
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
-        const int64_t t = t0 + wt + 32 * j + col;
-        if (t >= a.rows) continue;
-        const float x_scale = a.x_scales[t];
+        const float x_scale = a.x_scales[min(t0 + wt + 32 * j + col, a.rows - 1)];
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < TC; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int sum[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                finish<T>(a, t, n0 + wc + 32 * i + 8 * q + 4 * h, sum, x_scale);
+                const int c = wc + 32 * i + 8 * q + 4 * h;
+                float y[4];
+                scaled(y, a, n0 + c, sum, x_scale);
+                store<4>(out + (wave / WC * 32 + col) * PITCH + c, y);
             }
+        __syncthreads();
+        for (int v = threadIdx.x; v < WT * 32 * (BC / PER); v += THREADS) {
+            const int r = v / (BC / PER), c = v % (BC / PER) * PER;
+            const int64_t t = t0 + r / 32 * (TT * 32) + 32 * j + r % 32, n = n0 + c;
+            if (t >= a.rows) continue;
+            const T* const at = out + r * PITCH + c;
+            T* const to = static_cast<T*>(a.y) + t * a.channels + n;
+            if (n + PER <= a.channels) {
+                *reinterpret_cast<vec_t<T, PER>*>(to) = *reinterpret_cast<const vec_t<T, PER>*>(at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; ++e)
+                    if (n + e < a.channels) to[e] = at[e];
+            }
+        }
     }
 }
 
-// Few tokens (TT blocks of 32): a work-group takes 32 channels, its eight waves an eighth of the contraction
-// each, straight from memory to the matrix cores; their sums meet in LDS, as integers in any order.
-constexpr int kFewWaves = 8;
-template <typename T, int TT>
+// Few tokens (TT blocks of 32): a work-group takes 32 channels, its eight waves an eighth of each 256 codes of the
+// contraction; their sums meet in LDS, as integers in any order.  Three stages of codes are in LDS or on
+// their way: two work-groups a CU have up to 96 KB in flight, which is what the weights' stream needs.
+constexpr int kFewWaves = 8, kFewCodes = 32 * kFewWaves, kStages = 3;
+template <typename T, int TT, bool ALIGNED>
 __global__ __launch_bounds__(kFewWaves * 64) void int8_few_kernel(LinearArgs a) {
+    constexpr int CHUNKS = kFewCodes / 16, ROWS = 32 + 32 * TT, THREADS = kFewWaves * 64, EACH = ROWS * CHUNKS / THREADS;
+    static_assert(ROWS * CHUNKS % THREADS == 0 && THREADS / CHUNKS == 32);
+    __shared__ i32x4 lds[kStages][ROWS * CHUNKS];
     __shared__ int sums[TT * 32][33];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 32, h = lane / 32;
-    for (int i = threadIdx.x; i < TT * 32 * 33; i += kFewWaves * 64) sums[i / 33][i % 33] = 0;
-    __syncthreads();
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, h = lane / 32;
+    for (int i = threadIdx.x; i < TT * 32 * 33; i += THREADS) sums[i / 33][i % 33] = 0;
     const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 32;
-    const int8_t* w = a.w + min(n0 + col, a.channels - 1) * a.w_stride;
-    const int8_t* x[TT];
+    // a thread's chunks: row threadIdx.x / CHUNKS of the weights and of each block of tokens; chunk c of row r lies at chunk
+    // c ^ r % 16
+    const int row = threadIdx.x / CHUNKS, mine = ((threadIdx.x % CHUNKS) ^ (row % 16)) * 16;
+    const int8_t* from[EACH];
+    from[0] = a.w + min(n0 + row, a.channels - 1) * a.w_stride + mine;
 #pragma unroll
-    for (int j = 0; j < TT; ++j) x[j] = a.x + min(static_cast<int64_t>(32 * j + col), a.rows - 1) * a.x_stride;
+    for (int e = 1; e < EACH; ++e) from[e] = a.x + min(static_cast<int64_t>(32 * (e - 1) + row), a.rows - 1) * a.x_stride + mine;
+    const int64_t stages = (a.width + kFewCodes - 1) / kFewCodes, direct = ALIGNED ? a.width / kFewCodes : 0;
+    const auto fetch = [&](int64_t stage, int to) {
+        const int64_t k = stage * kFewCodes;
+        if (stage < direct) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) load_direct(&lds[to][e * THREADS + wave * 64], from[e] + k);
+        } else if (stage < stages) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) lds[to][e * THREADS + threadIdx.x] = load_codes(from[e] + k, k + mine, a.width);
+        }
+    };
     i32x16 acc[TT];
 #pragma unroll
     for (int j = 0; j < TT; ++j) acc[j] = i32x16{};
-    // 128 codes a turn: this half of the wave takes 64 consecutive ones of a row
-    const int64_t turns = (a.width + 127) / 128;
-    for (int64_t turn = wave; turn < turns; turn += kFewWaves) {
-        const int64_t k = turn * 128 + 64 * h;
-        if (turn * 128 + 128 <= a.width) {
-            i32x4 f[4];
+    fetch(0, 0), fetch(1, 1);
+    int buf = 0;
+    for (int64_t stage = 0; stage < stages; ++stage) {
+        // this stage's loads are done when only the next one's EACH are not
+        if (stage + 1 < direct) landed<EACH>();
+        else landed<0>();
+        __syncthreads();
+        fetch(stage + 2, buf == 0 ? 2 : buf - 1);  // where the stage before this one was: all waves have left it
+        const int c = (2 * wave + h) ^ (col % 16);
+        const i32x4 w = lds[buf][col * CHUNKS + c];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) f[s] = load_codes(w + k + 16 * s, 16);
-#pragma unroll
-            for (int j = 0; j < TT; ++j) {
-                i32x4 g[4];
-#pragma unroll
-                for (int s = 0; s < 4; ++s) g[s] = load_codes(x[j] + k + 16 * s, 16);
-#pragma unroll
-                for (int s = 0; s < 4; ++s) acc[j] = mma(f[s], g[s], acc[j]);
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int64_t left = a.width - k - 16 * s;
-                const i32x4 f = load_codes(w + k + 16 * s, left);
-#pragma unroll
-                for (int j = 0; j < TT; ++j) acc[j] = mma(f, load_codes(x[j] + k + 16 * s, left), acc[j]);
-            }
-        }
+        for (int j = 0; j < TT; ++j) acc[j] = mma(w, lds[buf][(32 + 32 * j + col) * CHUNKS + c], acc[j]);
+        buf = buf == 2 ? 0 : buf + 1;
     }
 #pragma unroll
     for (int j = 0; j < TT; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) atomicAdd(&sums[32 * j + col][8 * (e / 4) + 4 * h + e % 4], acc[j][e]);
     __syncthreads();
-    for (int i = threadIdx.x; i < TT * 32 * 8; i += kFewWaves * 64) {
+    for (int i = threadIdx.x; i < TT * 32 * 8; i += THREADS) {
         const int64_t t = i / 8;
         const int c = i % 8 * 4;
         if (t >= a.rows) continue;
         const int sum[4] = {sums[t][c], sums[t][c + 1], sums[t][c + 2], sums[t][c + 3]};
-        finish<T>(a, t, n0 + c, sum, a.x_scales[t]);
+        float y[4];
+        if (n0 + c >= a.channels) continue;
+        scaled(y, a, n0 + c, sum, a.x_scales[t]);
+        store_some<4>(static_cast<T*>(a.y) + t * a.channels + n0 + c, y, a.channels - n0 - c);
     }
 }
+
+template <int V>
+using Int = std::integral_constant<int, V>;
+constexpr int kBigCodes = 128, kBigAhead = 1, kMidAhead = 1, kSmallAhead = 2;
 
 }  // namespace
 }  // namespace mgopt
@@ -231,14 +325,17 @@ MGOPT_API int mgopt_int8_linear(const int8_t* x_dev, int64_t x_stride, const flo
     a.x = x_dev, a.w = w_dev, a.x_stride = x_stride, a.w_stride = w_stride, a.x_scales = x_scales_dev, a.w_scales = w_scales_dev;
     a.bias = bias_dev, a.bias_dtype = bias_dtype, a.y = y_dev, a.rows = rows, a.width = width, a.channels = channels;
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool aligned = (reinterpret_cast<uintptr_t>(x_dev) | reinterpret_cast<uintptr_t>(w_dev) | static_cast<uint64_t>(x_stride | w_stride)) % 16 == 0;
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
         if (rows <= 64) {
             const int64_t blocks = (channels + 31) / 32;
             if (blocks > max_blocks(kFewWaves * 64)) return set_error(MGOPT_E_LIMIT, "int8_linear: too many channels");
             const dim3 grid(static_cast<uint32_t>(blocks)), block(kFewWaves * 64);
-            if (rows <= 32) hipLaunchKernelGGL((int8_few_kernel<T, 1>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((int8_few_kernel<T, 2>), grid, block, 0, s, a);
+            if (rows <= 32 && aligned) hipLaunchKernelGGL((int8_few_kernel<T, 1, true>), grid, block, 0, s, a);
+            else if (rows <= 32) hipLaunchKernelGGL((int8_few_kernel<T, 1, false>), grid, block, 0, s, a);
+            else if (aligned) hipLaunchKernelGGL((int8_few_kernel<T, 2, true>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((int8_few_kernel<T, 2, false>), grid, block, 0, s, a);
             return launched("int8_linear");
         }
         const auto tiles = [&](int64_t bt, int64_t bc, int threads) -> int64_t {
@@ -247,16 +344,20 @@ MGOPT_API int mgopt_int8_linear(const int8_t* x_dev, int64_t x_stride, const flo
             a.row_tiles = static_cast<uint32_t>(r), a.channel_tiles = static_cast<uint32_t>(c);
             return (r * c + 7) / 8 * 8;
         };
-        if ((rows + 255) / 256 * ((channels + 255) / 256) >= 256) {
-            const int64_t grid = tiles(256, 256, 512);
+        const auto launch = [&](auto wc, auto wt, auto tc, auto tt, auto bk, auto ahead) -> int {
+            constexpr int WC = decltype(wc)::value, WT = decltype(wt)::value, TC = decltype(tc)::value, TT = decltype(tt)::value;
+            constexpr int BK = decltype(bk)::value, AHEAD = decltype(ahead)::value, THREADS = WC * WT * 64;
+            const int64_t grid = tiles(WT * TT * 32, WC * TC * 32, THREADS);
             if (grid < 0) return set_error(MGOPT_E_LIMIT, "int8_linear: too many tiles");
-            hipLaunchKernelGGL((int8_linear_kernel<T, 4, 2, 2, 4>), dim3(static_cast<uint32_t>(grid)), dim3(512), 0, s, a);
-        } else {
-            const int64_t grid = tiles(64, 64, 256);
-            if (grid < 0) return set_error(MGOPT_E_LIMIT, "int8_linear: too many tiles");
-            hipLaunchKernelGGL((int8_linear_kernel<T, 2, 2, 1, 1>), dim3(static_cast<uint32_t>(grid)), dim3(256), 0, s, a);
-        }
-        return launched("int8_linear");
+            const dim3 blocks(static_cast<uint32_t>(grid)), threads(THREADS);
+            if (aligned) hipLaunchKernelGGL((int8_linear_kernel<T, WC, WT, TC, TT, BK, AHEAD, true>), blocks, threads, 0, s, a);
+            else hipLaunchKernelGGL((int8_linear_kernel<T, WC, WT, TC, TT, BK, (TC * TT > 4 ? 1 : 2), false>), blocks, threads, 0, s, a);
+            return launched("int8_linear");
+        };
+        const auto count = [&](int64_t side) { return (rows + side - 1) / side * ((channels + side - 1) / side); };
+        if (count(256) >= 256) return launch(Int<4>{}, Int<2>{}, Int<2>{}, Int<4>{}, Int<kBigCodes>{}, Int<kBigAhead>{});
+        if (count(128) >= 256) return launch(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<128>{}, Int<kMidAhead>{});
+        return launch(Int<2>{}, Int<2>{}, Int<1>{}, Int<1>{}, Int<128>{}, Int<kSmallAhead>{});
     });
 }
 
