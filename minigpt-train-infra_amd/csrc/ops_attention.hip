@@ -34,6 +34,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTile = 128;  // rows (queries x group), or keys, of a work-group: 32 a wave
+constexpr int kShared = 32; // rows of one whose waves share them, and the keys out among them
 constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -217,16 +218,16 @@ struct Part {
 };
 
 // Tile `slot` of the queries (`per` rows each), or of the keys with KEYS.  Packed sequences, with what lies before the
-// first and behind the last as two more that hold nothing, have places of their own for floor(rows / kTile) + 1
+// first and behind the last as two more that hold nothing, have places of their own for floor(rows / TILE) + 1
 // tiles each; `first` is beyond `total` where a place stays empty.  Offsets are clamped to the tokens.
-template <bool KEYS>
+template <bool KEYS, int TILE>
 __device__ Part find_part(const AttArgs& p, uint32_t slot, uint32_t per) {
     const mgopt_attention_args& a = p.a;
     Part s{};
     const int64_t tokens = KEYS ? a.keys : a.queries;
     if (a.q_offsets_dev == nullptr) {
         s.batch = slot / p.tiles;
-        s.first = static_cast<int64_t>(slot % p.tiles) * kTile;
+        s.first = static_cast<int64_t>(slot % p.tiles) * TILE;
         s.total = static_cast<int32_t>(tokens);
         s.n = static_cast<int32_t>(a.q_lengths_dev ? clamp64(id_at(a.q_lengths_dev, s.batch, a.offset_bytes), 0, a.queries) : a.queries);
         s.m = static_cast<int32_t>(a.k_lengths_dev ? clamp64(id_at(a.k_lengths_dev, s.batch, a.offset_bytes), 0, a.keys) : a.keys);
@@ -237,7 +238,7 @@ __device__ Part find_part(const AttArgs& p, uint32_t slot, uint32_t per) {
     const auto edge = [&](int32_t j) {
         return j <= 0 ? 0 : j >= count ? tokens : clamp64(id_at(offsets, j - 1, a.offset_bytes), 0, tokens);
     };
-    const auto base = [&](int32_t j) { return edge(j) * per / kTile + j; };
+    const auto base = [&](int32_t j) { return edge(j) * per / TILE + j; };
     // the last part whose places begin at `slot` or before, 64 of them looked at at once
     int32_t low = 0, left = count;
     while (left > 1) {
@@ -248,7 +249,7 @@ __device__ Part find_part(const AttArgs& p, uint32_t slot, uint32_t per) {
         low += k * step;
     }
     const int64_t from = edge(low), to = edge(low + 1);
-    s.first = (static_cast<int64_t>(slot) - base(low)) * kTile;
+    s.first = (static_cast<int64_t>(slot) - base(low)) * TILE;
     s.total = static_cast<int32_t>(to > from ? to - from : 0);
     if (s.first < 0) s.first = 0, s.total = 0;
     s.q0 = s.k0 = from;
@@ -263,9 +264,9 @@ __device__ Part find_part(const AttArgs& p, uint32_t slot, uint32_t per) {
     return s;
 }
 
-template <bool KEYS>
+template <bool KEYS, int TILE = kTile>
 __device__ __forceinline__ Part find(const AttArgs& p, uint32_t slot, uint32_t per) {
-    const Part s = find_part<KEYS>(p, slot, per);
+    const Part s = find_part<KEYS, TILE>(p, slot, per);
     return {uniform(s.batch), uniform(s.q0), uniform(s.k0), uniform(s.n), uniform(s.m), uniform(s.total), uniform(s.first)};
 }
 
@@ -343,8 +344,11 @@ struct Unit {
 };
 __device__ __forceinline__ Unit unit_of(const AttArgs& p, bool last_first) {
     const uint32_t heads = static_cast<uint32_t>(p.a.k_heads);
-    uint32_t slot = blockIdx.x / heads;
-    const uint32_t head = blockIdx.x - slot * heads;
+    uint32_t place = blockIdx.x;
+    if (p.tiles == 1 && gridDim.x % 8 == 0) place = place % 8 * (gridDim.x / 8) + place / 8;
+    uint32_t slot = place / heads;
+    const uint32_t head = place - slot * heads;
+    if (p.a.q_offsets_dev != nullptr && last_first) slot = gridDim.x / heads - 1 - slot;
     if (p.a.q_offsets_dev == nullptr) {
         // tiles outermost, the batch's rows within
         const uint32_t rows = static_cast<uint32_t>(p.a.batch);
@@ -368,39 +372,47 @@ constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;  // keys of a tile in LDS
 template <typename T, int DP>
 constexpr int kMinWaves = sizeof(T) == 4 ? 1 : 2;  // a SIMD
 
-template <typename T, int DP, bool SPLIT>
+// SPLIT: a work-group takes one of `splits` parts of the keys and leaves its sums for join_kernel.  SHARED: its waves
+// take the same 32 rows and a quarter of each 128 keys, and join their sums in LDS, for rows so few that 128 of them
+// fill no work-group, or the work-groups do not fill the chip.
+template <typename T, int DP, bool SPLIT, bool SHARED>
 __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel(AttArgs p) {
-    constexpr int BN = kKeys<T, DP>;
+    constexpr int TILE = SHARED ? kShared : kTile, BN = SHARED ? 128 : kKeys<T, DP>, BLOCKS = SHARED ? 1 : BN / 32;
     using L = Tile<T, DP>;
-    __shared__ alignas(16) T keys[2][Stage<T, DP, BN>::kSize], values[2][Stage<T, DP, BN>::kSize];
+    using Keys = Stage<T, DP, BN>;
+    // two work-groups a CU where their tiles leave room for it
+    constexpr int BUFFERS = SHARED && Keys::kSize * sizeof(T) > 20 * 1024 ? 1 : 2;
+    __shared__ alignas(16) T tiles[2][BUFFERS][Keys::kSize];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, a.causal);
-    const Part s = find<false>(p, u.slot, p.group);
+    const Part s = find<false, TILE>(p, u.slot, p.group);
     if (s.first >= static_cast<int64_t>(s.total) * p.group) return;
     const int lane = threadIdx.x % 64, wave = uniform(static_cast<int32_t>(threadIdx.x / 64)), col = lane % 32, h = lane / 32;
-    const Place at = place_of(p, s.first + wave * 32 + col);
+    const int64_t first = SHARED ? s.first : s.first + wave * 32;  // of the wave's rows
+    const int block0 = SHARED ? wave : 0;                          // of its keys in a tile
+    const Place at = place_of(p, first + col);
     const int64_t head = static_cast<int64_t>(u.head) * p.group + at.head;
     const bool inside = at.query < s.total;
     const int32_t mine = seen(p, s, at.query);
     Frag<T> q[DP / 16];
     load_row<T, DP>(q, mine > 0 ? row_of<T>(a.q_dev, a.q_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
     // what the work-group's rows, and the wave's, see at most, and the wave's at least
-    const int32_t most = most_seen(p, s, s.first, kTile);
-    const int32_t wave_most = most_seen(p, s, s.first + wave * 32, 32);
-    const int32_t wave_least = seen(p, s, place_of(p, s.first + wave * 32).query);
+    const int32_t most = most_seen(p, s, s.first, TILE);
+    const int32_t wave_most = most_seen(p, s, first, 32);
+    const int32_t wave_least = seen(p, s, place_of(p, first).query);
     int32_t from = 0, to = most;
     if constexpr (SPLIT) {
         const int32_t share = (most + BN * static_cast<int32_t>(p.splits) - 1) / (BN * static_cast<int32_t>(p.splits)) * BN;
         from = static_cast<int32_t>(min(static_cast<int64_t>(blockIdx.y) * share, static_cast<int64_t>(most)));
         to = min(from + share, most);
     }
-    Stage<T, DP, BN> stage_k, stage_v;
+    Keys stage_k, stage_v;
     const T* const kp = row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0, u.head);
     const T* const vp = row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0, u.head);
     stage_k.plan(wave, 1, a.k_stride[1], 0, a.dim), stage_v.plan(wave, 1, a.v_stride[1], 0, a.dim);
     const auto fetch = [&](int32_t k0, int buf) {
-        stage_k.fetch(keys[buf], wave, p.aligned_keys, kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
-        stage_v.fetch(values[buf], wave, p.aligned_keys, vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
+        stage_k.fetch(tiles[0][buf], wave, p.aligned_keys, kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
+        stage_v.fetch(tiles[1][buf], wave, p.aligned_keys, vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
     };
     f32x16 o[DP / 32];
 #pragma unroll
@@ -410,26 +422,27 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
     landed();
     __syncthreads();
     int buf = 0;
-    for (int32_t k0 = from; k0 < to; k0 += BN, buf ^= 1) {
-        if (k0 + BN < to) fetch(k0 + BN, buf ^ 1);
-        if (k0 < wave_most) {
-            f32x16 x[BN / 32];
+    for (int32_t k0 = from; k0 < to; k0 += BN) {
+        if (BUFFERS == 2 && k0 + BN < to) fetch(k0 + BN, buf ^ 1);
+        const T *const keys = tiles[0][buf], *const values = tiles[1][buf];
+        if (k0 + 32 * block0 < wave_most) {
+            f32x16 x[BLOCKS];
 #pragma unroll
-            for (int b = 0; b < BN / 32; ++b) x[b] = f32x16{};
+            for (int b = 0; b < BLOCKS; ++b) x[b] = f32x16{};
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
-                for (int b = 0; b < BN / 32; ++b) x[b] = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x[b]);
-            if (k0 + BN > wave_least || k0 + BN > to) {
+                for (int b = 0; b < BLOCKS; ++b) x[b] = mma(L::rows(keys, 32 * (block0 + b) + col, c, h), q[c], x[b]);
+            if (k0 + 32 * (block0 + BLOCKS) > min(wave_least, to)) {
 #pragma unroll
-                for (int b = 0; b < BN / 32; ++b)
+                for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (k0 + 32 * b + 8 * (e / 4) + 4 * h + e % 4 >= min(mine, to)) x[b][e] = -INFINITY;
+                        if (k0 + 32 * (block0 + b) + 8 * (e / 4) + 4 * h + e % 4 >= min(mine, to)) x[b][e] = -INFINITY;
             }
             float big = x[0][0];
 #pragma unroll
-            for (int b = 0; b < BN / 32; ++b)
+            for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) big = fmaxf(big, x[b][e]);
             big = with_partner(big, [](float y, float z) { return fmaxf(y, z); });
@@ -446,43 +459,86 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
             }
             const float off = fmaf(ref, p.scale2, -kShift<T>);
 #pragma unroll
-            for (int b = 0; b < BN / 32; ++b)
+            for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     x[b][e] = exp2_hw(fmaf(x[b][e], p.scale2, -off));
                     sum += x[b][e];
                 }
 #pragma unroll
-            for (int b = 0; b < BN / 32; ++b)
+            for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Frag<T> w = as_operand<T>(x[b], c);
 #pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) o[d] = mma(L::columns(values[buf], d, 2 * b + c, lane), w, o[d]);
+                    for (int d = 0; d < DP / 32; ++d) o[d] = mma(L::columns(values, d, 2 * (block0 + b) + c, lane), w, o[d]);
                 }
+        }
+        if constexpr (BUFFERS == 2) {
+            buf ^= 1;
+        } else {
+            __syncthreads();
+            if (k0 + BN < to) fetch(k0 + BN, 0);
         }
         landed();
         __syncthreads();
     }
     sum = with_partner(sum, add);
-    if (!inside) return;
     if (mine == 0) {  // padding, or no key to see: what its column holds is of a query of zeros without a mask
         top = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b) o[b] = f32x16{};
     }
-    if constexpr (SPLIT) {
-        // rows in the order (batch, query, head)
-        const int64_t rows = a.batch * a.queries * a.q_heads;
-        const int64_t row = blockIdx.y * rows + (s.batch * a.queries + s.q0 + at.query) * a.q_heads + head;
-        store_row<float, DP>(p.part_out + row * a.dim, o, 1.0f, a.dim, h);
-        if (h == 0) p.part_ml[2 * row] = top, p.part_ml[2 * row + 1] = sum;
+    const int64_t rows = a.batch * a.queries * a.q_heads;  // of parts: in the order (batch, query, head)
+    const auto part = [&](const Place& x) {
+        return blockIdx.y * rows + (s.batch * a.queries + s.q0 + x.query) * a.q_heads + static_cast<int64_t>(u.head) * p.group + x.head;
+    };
+    const auto write_lse = [&](const Place& x, float m, float l) {
+        if (a.lse_dev != nullptr)
+            a.lse_dev[(s.batch * a.q_heads + static_cast<int64_t>(u.head) * p.group + x.head) * a.queries + s.q0 + x.query] =
+                l == 0.0f ? -INFINITY : static_cast<float>(kLn2) * (m * p.scale2 - kShift<T> + log2f(l));
+    };
+    if constexpr (SHARED) {
+        constexpr int PITCH = DP + 4, EACH = DP / 8;  // a row's eight threads take EACH elements each
+        static_assert(sizeof(tiles) >= sizeof(float) * 4 * 32 * PITCH);
+        __shared__ float stats[2][4][32];
+        float(*const sums)[32][PITCH] = reinterpret_cast<float(*)[32][PITCH]>(&tiles[0][0][0]);
+        store_row<float, DP>(sums[wave][col], o, 1.0f, DP, h);
+        if (h == 0) stats[0][wave][col] = top, stats[1][wave][col] = sum;
+        __syncthreads();
+        const int r = threadIdx.x / 8, d0 = threadIdx.x % 8 * EACH;
+        const Place x = place_of(p, first + r);
+        if (x.query >= s.total) return;
+        const float m = fmaxf(fmaxf(stats[0][0][r], stats[0][1][r]), fmaxf(stats[0][2][r], stats[0][3][r]));
+        float l = 0.0f, y[EACH] = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float by = exp2_hw((stats[0][w][r] - (m == -INFINITY ? 0.0f : m)) * p.scale2);
+            l = fmaf(by, stats[1][w][r], l);
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) y[e] = fmaf(by, sums[w][r][d0 + e], y[e]);
+        }
+        if constexpr (SPLIT) {
+            store_some<EACH>(p.part_out + part(x) * a.dim + d0, y, a.dim - d0);
+            if (d0 == 0) p.part_ml[2 * part(x)] = m, p.part_ml[2 * part(x) + 1] = l;
+        } else {
+            const float by = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) y[e] *= by;
+            store_some<EACH>(row_of<T>(a.out_dev, a.out_stride, s.batch, s.q0 + x.query, static_cast<int64_t>(u.head) * p.group + x.head) + d0, y,
+                             a.dim - d0);
+            if (d0 == 0) write_lse(x, m, l);
+        }
     } else {
-        T* const out = row_of<T>(a.out_dev, a.out_stride, s.batch, s.q0 + at.query, head);
-        store_row<T, DP>(out, o, sum == 0.0f ? 0.0f : 1.0f / sum, a.dim, h);
-        if (h == 0 && a.lse_dev != nullptr)
-            a.lse_dev[(s.batch * a.q_heads + head) * a.queries + s.q0 + at.query] =
-                sum == 0.0f ? -INFINITY : static_cast<float>(kLn2) * (top * p.scale2 - kShift<T> + log2f(sum));
+        if (!inside) return;
+        if constexpr (SPLIT) {
+            store_row<float, DP>(p.part_out + part(at) * a.dim, o, 1.0f, a.dim, h);
+            if (h == 0) p.part_ml[2 * part(at)] = top, p.part_ml[2 * part(at) + 1] = sum;
+        } else {
+            T* const out = row_of<T>(a.out_dev, a.out_stride, s.batch, s.q0 + at.query, head);
+            store_row<T, DP>(out, o, sum == 0.0f ? 0.0f : 1.0f / sum, a.dim, h);
+            if (h == 0) write_lse(at, top, sum);
+        }
     }
 }
 
@@ -847,10 +903,10 @@ int check(const mgopt_attention_args* a, const char* what) {
     return 0;
 }
 
-// Work-groups of `per` rows a token on one side.
-int places(const mgopt_attention_args& a, int64_t tokens, int64_t per, const char* what, uint32_t& tiles, uint32_t& blocks) {
-    const int64_t each = (tokens * per + kTile - 1) / kTile;
-    const int64_t slots = a.q_offsets_dev ? tokens * per / kTile + a.sequences + 2 : each;
+// Work-groups of `tile` rows, `per` a token, on one side.
+int places(const mgopt_attention_args& a, int64_t tokens, int64_t per, int tile, const char* what, uint32_t& tiles, uint32_t& blocks) {
+    const int64_t each = (tokens * per + tile - 1) / tile;
+    const int64_t slots = a.q_offsets_dev ? tokens * per / tile + a.sequences + 2 : each;
     tiles = static_cast<uint32_t>(each);
     const int64_t most = max_blocks(kThreads);
     if (a.q_offsets_dev ? slots > most / a.k_heads : a.batch > 0 && each > most / a.k_heads / a.batch)
@@ -859,15 +915,28 @@ int places(const mgopt_attention_args& a, int64_t tokens, int64_t per, const cha
     return 0;
 }
 
-// Parts that the keys of each row are cut in, where the rows alone leave the chip short of work.
+// How the forward pass takes its rows: whether the waves of a work-group share 32 of them, and in how many parts the
+// keys of each row are cut where the rows alone leave the chip short of work.
+struct Form {
+    bool shared;
+    uint32_t splits;
+};
 constexpr int64_t kMinShare = 256;   // keys of a part at least
-uint32_t splits_for(const mgopt_attention_args& a) {
+constexpr int64_t kFill = 512;       // work-groups that fill the chip: two a CU
+Form form_of(const mgopt_attention_args& a) {
     const int64_t per = a.q_heads / a.k_heads;
-    const int64_t tiles = a.q_offsets_dev ? a.queries * per / kTile + a.sequences : (a.queries * per + kTile - 1) / kTile * a.batch;
-    const int64_t groups = std::max<int64_t>(1, tiles * a.k_heads);
+    const auto groups = [&](int tile) {
+        return a.k_heads * (a.q_offsets_dev ? a.queries * per / tile + a.sequences : (a.queries * per + tile - 1) / tile * a.batch);
+    };
+    Form f;
+    f.shared = groups(kTile) < kFill;
+    const int64_t work = std::max<int64_t>(1, groups(f.shared ? kShared : kTile));
     const int64_t keys = a.q_offsets_dev ? a.keys / std::max<int64_t>(1, a.sequences) : a.keys;
-    const int64_t s = std::min((512 + groups - 1) / groups, keys / kMinShare);
-    return static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(s, kMostSplits)));
+    const int64_t s = std::min((kFill + work - 1) / work, keys / kMinShare);
+    f.splits = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(s, kMostSplits)));
+    // few rows over long caches are bound by memory, and two tiles a work-group on their way matter more than its waves
+    if (a.queries * per <= kShared && a.dim > 64 && a.dtype != MGOPT_F32 && keys / f.splits >= 1024) f.shared = false;
+    return f;
 }
 
 template <typename F>
@@ -902,7 +971,7 @@ extern "C" {
 MGOPT_API int64_t mgopt_attention_workspace(const mgopt_attention_args* a, int32_t backward) {
     if (check(a, "attention_workspace")) return -1;
     if (backward) return rows_of_all(*a) * 8;
-    const int64_t splits = splits_for(*a);
+    const int64_t splits = form_of(*a).splits;
     return splits > 1 ? splits * rows_of_all(*a) * (a->dim + 2) * 4 : 0;
 }
 
@@ -912,7 +981,8 @@ MGOPT_API int mgopt_attention(const mgopt_attention_args* a, void* stream) {
     if (!a->q_dev || !a->out_dev || (a->keys > 0 && (!a->k_dev || !a->v_dev)))
         return set_error(MGOPT_E_INVALID, "attention: NULL argument");
     AttArgs p = args_of(*a);
-    p.splits = splits_for(*a);
+    const Form form = form_of(*a);
+    p.splits = form.splits;
     if (p.splits > 1) {
         if (!a->workspace_dev || reinterpret_cast<uintptr_t>(a->workspace_dev) % 16 != 0)
             return set_error(MGOPT_E_ALIGN, "attention: the workspace must be 16-byte aligned and not NULL");
@@ -920,19 +990,20 @@ MGOPT_API int mgopt_attention(const mgopt_attention_args* a, void* stream) {
         p.part_ml = p.part_out + p.splits * rows_of_all(*a) * a->dim;
     }
     uint32_t blocks;
-    if (int rc = places(*a, a->queries, p.group, "attention", p.tiles, blocks)) return rc;
+    if (int rc = places(*a, a->queries, p.group, form.shared ? kShared : kTile, "attention", p.tiles, blocks)) return rc;
     if (p.splits > 1 && rows_of_all(*a) > max_blocks(kThreads)) return set_error(MGOPT_E_LIMIT, "attention: too many rows");
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         return with_dim(a->dim, [&](auto d) {
             constexpr int DP = decltype(d)::value;
-            if (p.splits == 1) {
-                hipLaunchKernelGGL((attention_kernel<T, DP, false>), dim3(blocks), dim3(kThreads), 0, s, p);
-                return launched("attention");
-            }
-            hipLaunchKernelGGL((attention_kernel<T, DP, true>), dim3(blocks, p.splits), dim3(kThreads), 0, s, p);
+            const dim3 grid(blocks, p.splits), threads(kThreads);
+            if (form.shared && p.splits > 1) hipLaunchKernelGGL((attention_kernel<T, DP, true, true>), grid, threads, 0, s, p);
+            else if (form.shared) hipLaunchKernelGGL((attention_kernel<T, DP, false, true>), grid, threads, 0, s, p);
+            else if (p.splits > 1) hipLaunchKernelGGL((attention_kernel<T, DP, true, false>), grid, threads, 0, s, p);
+            else hipLaunchKernelGGL((attention_kernel<T, DP, false, false>), grid, threads, 0, s, p);
             if (int rc = launched("attention")) return rc;
+            if (p.splits == 1) return 0;
             hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<uint32_t>(rows_of_all(*a))), dim3(kThreads), 0, s, p);
             return launched("attention");
         });
@@ -960,12 +1031,12 @@ MGOPT_API int mgopt_attention_backward(const mgopt_attention_args* a, void* stre
                 p.aligned_rows = p.aligned_rows && aligned(at, stride, sizeof(T), a->dim) && stride[1] < kNear / 256 && stride[2] < kNear / 8 / p.group;
             uint32_t blocks;
             if (rows) {
-                if (int rc = places(*a, a->queries, p.group, "attention_backward", p.tiles, blocks)) return rc;
+                if (int rc = places(*a, a->queries, p.group, kTile, "attention_backward", p.tiles, blocks)) return rc;
                 hipLaunchKernelGGL((attention_dq_kernel<T, DP>), dim3(blocks), dim3(kThreads), 0, s, p);
                 if (int rc = launched("attention_backward")) return rc;
             }
             if (!keys) return 0;
-            if (int rc = places(*a, a->keys, 1, "attention_backward", p.tiles, blocks)) return rc;
+            if (int rc = places(*a, a->keys, 1, kTile, "attention_backward", p.tiles, blocks)) return rc;
             hipLaunchKernelGGL((attention_dkv_kernel<T, DP>), dim3(blocks), dim3(kThreads), 0, s, p);
             return launched("attention_backward");
         });
