@@ -372,6 +372,24 @@ constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;  // keys of a tile in LDS
 template <typename T, int DP>
 constexpr int kMinWaves = sizeof(T) == 4 ? 1 : 2;  // a SIMD
 
+// Where the sums of the waves that share rows or keys meet, a column's elements behind each other, and the thread's
+// part of them in the join: row r, EACH elements from d0 on.
+template <int DP>
+struct Join {
+    static constexpr int kPitch = DP + 4, kEach = DP / 8, kBytes = 4 * 32 * kPitch * 4;
+    float (*sums)[32][kPitch];
+    int r = threadIdx.x / 8, d0 = threadIdx.x % 8 * kEach;
+    __device__ __forceinline__ explicit Join(void* lds) : sums(static_cast<float (*)[32][kPitch]>(lds)) {}
+    __device__ __forceinline__ void put(int wave, int col, const f32x16 (&acc)[DP / 32], float by, int h) {
+        store_row<float, DP>(sums[wave][col], acc, by, DP, h);
+    }
+    // y += by * wave w's elements
+    __device__ __forceinline__ void get(float (&y)[kEach], int w, float by) const {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) y[e] = fmaf(by, sums[w][r][d0 + e], y[e]);
+    }
+};
+
 // SPLIT: a work-group takes one of `splits` parts of the keys and leaves its sums for join_kernel.  SHARED: its waves
 // take the same 32 rows and a quarter of each 128 keys, and join their sums in LDS, for rows so few that 128 of them
 // fill no work-group, or the work-groups do not fill the chip.
@@ -499,14 +517,14 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
                 l == 0.0f ? -INFINITY : static_cast<float>(kLn2) * (m * p.scale2 - kShift<T> + log2f(l));
     };
     if constexpr (SHARED) {
-        constexpr int PITCH = DP + 4, EACH = DP / 8;  // a row's eight threads take EACH elements each
-        static_assert(sizeof(tiles) >= sizeof(float) * 4 * 32 * PITCH);
+        constexpr int EACH = Join<DP>::kEach;
+        static_assert(sizeof(tiles) >= Join<DP>::kBytes);
         __shared__ float stats[2][4][32];
-        float(*const sums)[32][PITCH] = reinterpret_cast<float(*)[32][PITCH]>(&tiles[0][0][0]);
-        store_row<float, DP>(sums[wave][col], o, 1.0f, DP, h);
+        Join<DP> join(&tiles[0][0][0]);
+        join.put(wave, col, o, 1.0f, h);
         if (h == 0) stats[0][wave][col] = top, stats[1][wave][col] = sum;
         __syncthreads();
-        const int r = threadIdx.x / 8, d0 = threadIdx.x % 8 * EACH;
+        const int r = join.r, d0 = join.d0;
         const Place x = place_of(p, first + r);
         if (x.query >= s.total) return;
         const float m = fmaxf(fmaxf(stats[0][0][r], stats[0][1][r]), fmaxf(stats[0][2][r], stats[0][3][r]));
@@ -515,8 +533,7 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
         for (int w = 0; w < 4; ++w) {
             const float by = exp2_hw((stats[0][w][r] - (m == -INFINITY ? 0.0f : m)) * p.scale2);
             l = fmaf(by, stats[1][w][r], l);
-#pragma unroll
-            for (int e = 0; e < EACH; ++e) y[e] = fmaf(by, sums[w][r][d0 + e], y[e]);
+            join.get(y, w, by);
         }
         if constexpr (SPLIT) {
             store_some<EACH>(p.part_out + part(x) * a.dim + d0, y, a.dim - d0);
@@ -624,27 +641,32 @@ struct Range<_Float16> {
     __device__ __forceinline__ float back() const { return 1.0f / by; }
 };
 
-// dq, and delta for the kernel that follows.
-template <typename T, int DP>
+// dq, and delta for the kernel that follows.  SHARED: as in the forward pass.
+template <typename T, int DP, bool SHARED>
 __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_kernel(AttArgs p) {
-    constexpr int BN = kKeys<T, DP>;
+    constexpr int TILE = SHARED ? kShared : kTile, BN = SHARED ? 128 : kKeys<T, DP>, BLOCKS = SHARED ? 1 : BN / 32;
     using L = Tile<T, DP>;
-    __shared__ alignas(16) T keys[2][Stage<T, DP, BN>::kSize], values[2][Stage<T, DP, BN>::kSize];
+    using Keys = Stage<T, DP, BN>;
+    constexpr int BUFFERS = SHARED && Keys::kSize * sizeof(T) > 20 * 1024 ? 1 : 2;
+    __shared__ alignas(16) T tiles[2][BUFFERS][Keys::kSize];
+    __shared__ float deltas[SHARED ? 4 : 1][32];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, a.causal);
-    const Part s = find<false>(p, u.slot, p.group);
+    const Part s = find<false, TILE>(p, u.slot, p.group);
     if (s.first >= static_cast<int64_t>(s.total) * p.group) return;
     const int lane = threadIdx.x % 64, wave = uniform(static_cast<int32_t>(threadIdx.x / 64)), col = lane % 32, h = lane / 32;
-    const Place at = place_of(p, s.first + wave * 32 + col);
+    const int64_t first = SHARED ? s.first : s.first + wave * 32;  // of the wave's rows
+    const int block0 = SHARED ? wave : 0;                          // of its keys in a tile
+    const Place at = place_of(p, first + col);
     const int64_t head = static_cast<int64_t>(u.head) * p.group + at.head;
     const bool inside = at.query < s.total;
     const int32_t mine = seen(p, s, at.query);
     Frag<T> q[DP / 16], g[DP / 16];
     load_row<T, DP>(q, mine > 0 ? row_of<T>(a.q_dev, a.q_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
     load_row<T, DP>(g, mine > 0 ? row_of<T>(a.grad_out_dev, a.grad_out_stride, s.batch, s.q0 + at.query, head) : nullptr, a.dim, h);
-    const int32_t to = most_seen(p, s, s.first, kTile);
-    const int32_t wave_most = most_seen(p, s, s.first + wave * 32, 32);
-    const int32_t wave_least = seen(p, s, place_of(p, s.first + wave * 32).query);
+    const int32_t to = most_seen(p, s, s.first, TILE);
+    const int32_t wave_most = most_seen(p, s, first, 32);
+    const int32_t wave_least = seen(p, s, place_of(p, first).query);
     const int64_t stat = (s.batch * a.q_heads + head) * a.queries + s.q0 + at.query;
     // Rows whose keys are one tile take delta from it, as sum_j p_ij g_i . v_j: of few keys, what is left of
     // g_i . v_j - delta_i can be less than the rounding of out.
@@ -659,13 +681,32 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_ker
             for (int e = 0; e < 8; ++e) delta = fmaf(static_cast<float>(g[c][e]), static_cast<float>(o[c][e]), delta);
         delta = with_partner(delta, add);
     }
-    Stage<T, DP, BN> stage_k, stage_v;
+    Keys stage_k, stage_v;
     const T* const kp = row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0, u.head);
     const T* const vp = row_of<T>(a.v_dev, a.v_stride, s.batch, s.k0, u.head);
     stage_k.plan(wave, 1, a.k_stride[1], 0, a.dim), stage_v.plan(wave, 1, a.v_stride[1], 0, a.dim);
     const auto fetch = [&](int32_t k0, int buf) {
-        stage_k.fetch(keys[buf], wave, p.aligned_keys, kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
-        stage_v.fetch(values[buf], wave, p.aligned_keys, vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
+        stage_k.fetch(tiles[0][buf], wave, p.aligned_keys, kp + k0 * a.k_stride[1], a.k_stride[1], to - k0, a.dim);
+        stage_v.fetch(tiles[1][buf], wave, p.aligned_keys, vp + k0 * a.v_stride[1], a.v_stride[1], to - k0, a.dim);
+    };
+    int buf = 0;
+    // p_ij and g_i . v_j of block b of the keys from k0 on
+    const auto scores = [&](int b, f32x16& x, f32x16& dp) {
+        x = f32x16{}, dp = f32x16{};
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            x = mma(L::rows(tiles[0][buf], 32 * b + col, c, h), q[c], x);
+            dp = mma(L::rows(tiles[1][buf], 32 * b + col, c, h), g[c], dp);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = exp2_hw(fmaf(x[e], p.scale2, -lse));
+    };
+    const auto hide = [&](int32_t k, f32x16& x, f32x16& dp) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const bool out = k + 8 * (e / 4) + 4 * h + e % 4 >= mine;
+            x[e] = out ? 0.0f : x[e], dp[e] = out ? 0.0f : dp[e];
+        }
     };
     f32x16 acc[DP / 32];
 #pragma unroll
@@ -674,70 +715,75 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dq_ker
     if (to > 0) fetch(0, 0);
     landed();
     __syncthreads();
-    int buf = 0;
-    for (int32_t k0 = 0; k0 < to; k0 += BN, buf ^= 1) {
-        if (k0 + BN < to) fetch(k0 + BN, buf ^ 1);
-        if (k0 < wave_most) {
-            // p_ij and g_i . v_j of keys 32 b .. 32 b + 31 of the tile
-            const auto scores = [&](int b, f32x16& x, f32x16& dp) {
-                x = f32x16{}, dp = f32x16{};
+    if (one_tile) {
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) {
-                    x = mma(L::rows(keys[buf], 32 * b + col, c, h), q[c], x);
-                    dp = mma(L::rows(values[buf], 32 * b + col, c, h), g[c], dp);
-                }
+        for (int b = 0; b < BLOCKS; ++b)
+            if (32 * (block0 + b) < wave_most) {
+                f32x16 x, dp;
+                scores(block0 + b, x, dp);
+                hide(32 * (block0 + b), x, dp);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = exp2_hw(fmaf(x[e], p.scale2, -lse));
-            };
-            const auto hide = [&](int b, f32x16& x, f32x16& dp) {
+                for (int e = 0; e < 16; ++e) delta = fmaf(x[e], dp[e], delta);
+            }
+        delta = with_partner(delta, add);
+        if constexpr (SHARED) {  // wave_most is the work-group's: all waves are here
+            if (h == 0) deltas[wave][col] = delta;
+            __syncthreads();
+            delta = (deltas[0][col] + deltas[1][col]) + (deltas[2][col] + deltas[3][col]);
+        }
+    }
+    for (int32_t k0 = 0; k0 < to; k0 += BN) {
+        if (BUFFERS == 2 && k0 + BN < to) fetch(k0 + BN, buf ^ 1);
+        if (k0 + 32 * block0 < wave_most) {
+            const bool edge = k0 + 32 * (block0 + BLOCKS) > wave_least;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const bool out = k0 + 32 * b + 8 * (e / 4) + 4 * h + e % 4 >= mine;
-                    x[e] = out ? 0.0f : x[e], dp[e] = out ? 0.0f : dp[e];
-                }
-            };
-            const auto sum_up = [&](int b, const f32x16& x, f32x16& dp) {
+            for (int b = 0; b < BLOCKS; ++b) {
+                f32x16 x, ds;
+                scores(block0 + b, x, ds);
+                if (edge) hide(k0 + 32 * (block0 + b), x, ds);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) dp[e] = x[e] * (dp[e] - delta);
-                range.fit(dp, acc);
+                for (int e = 0; e < 16; ++e) ds[e] = x[e] * (ds[e] - delta);
+                range.fit(ds, acc);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const Frag<T> w = as_operand<T>(dp, c);
+                    const Frag<T> w = as_operand<T>(ds, c);
 #pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) acc[d] = mma(L::columns(keys[buf], d, 2 * b + c, lane), w, acc[d]);
+                    for (int d = 0; d < DP / 32; ++d) acc[d] = mma(L::columns(tiles[0][buf], d, 2 * (block0 + b) + c, lane), w, acc[d]);
                 }
-            };
-            const bool edge = k0 + BN > wave_least;
-            if (one_tile) {
-#pragma unroll
-                for (int b = 0; b < BN / 32; ++b) {
-                    f32x16 x, dp;
-                    scores(b, x, dp);
-                    hide(b, x, dp);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) delta = fmaf(x[e], dp[e], delta);
-                }
-                delta = with_partner(delta, add);
             }
-#pragma unroll
-            for (int b = 0; b < BN / 32; ++b) {
-                f32x16 x, dp;
-                scores(b, x, dp);
-                if (edge) hide(b, x, dp);
-                sum_up(b, x, dp);
-            }
+        }
+        if constexpr (BUFFERS == 2) {
+            buf ^= 1;
+        } else {
+            __syncthreads();
+            if (k0 + BN < to) fetch(k0 + BN, 0);
         }
         landed();
         __syncthreads();
     }
-    if (!inside) return;
-    if (h == 0) p.stats[stat] = lse - kShift<T>, p.stats[a.batch * a.q_heads * a.queries + stat] = mine > 0 ? delta : 0.0f;
+    if (inside && h == 0 && (!SHARED || wave == 0))
+        p.stats[stat] = lse - kShift<T>, p.stats[a.batch * a.q_heads * a.queries + stat] = mine > 0 ? delta : 0.0f;
     if (mine == 0) {
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b) acc[b] = f32x16{};
     }
-    store_row<T, DP>(row_of<T>(a.d_q_dev, a.d_q_stride, s.batch, s.q0 + at.query, head), acc,
-                     static_cast<float>(a.scale) * range.back(), a.dim, h);
+    const float by = static_cast<float>(a.scale) * range.back();
+    if constexpr (SHARED) {
+        static_assert(sizeof(tiles) >= Join<DP>::kBytes);
+        Join<DP> join(&tiles[0][0][0]);
+        join.put(wave, col, acc, by, h);
+        __syncthreads();
+        const Place x = place_of(p, first + join.r);
+        if (x.query >= s.total) return;
+        float y[Join<DP>::kEach] = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) join.get(y, w, 1.0f);
+        store_some<Join<DP>::kEach>(
+            row_of<T>(a.d_q_dev, a.d_q_stride, s.batch, s.q0 + x.query, static_cast<int64_t>(u.head) * p.group + x.head) + join.d0, y,
+            a.dim - join.d0);
+    } else if (inside) {
+        store_row<T, DP>(row_of<T>(a.d_q_dev, a.d_q_stride, s.batch, s.q0 + at.query, head), acc, by, a.dim, h);
+    }
 }
 
 template <typename T, int DP>
@@ -747,22 +793,25 @@ constexpr int kRows = sizeof(T) == 4 || DP > 64 ? 32 : 64;  // rows of a tile in
 template <typename T, int DP>
 constexpr bool kValuesInLds = sizeof(T) == 2 && DP > 64;
 
-// dk and dv of 128 keys over all rows that see them.
-template <typename T, int DP>
+// dk and dv of 128 keys over all rows that see them.  SHARED: of 32 keys, and the waves take a quarter each of 128 rows at
+// a time, and join their sums in LDS.
+template <typename T, int DP, bool SHARED>
 __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dkv_kernel(AttArgs p) {
-    constexpr int BM = kRows<T, DP>;
-    constexpr bool LDS_V = kValuesInLds<T, DP>;
+    constexpr int BM = SHARED ? 128 : kRows<T, DP>, TILE = SHARED ? kShared : kTile, BLOCKS = SHARED ? 1 : BM / 32;
+    constexpr bool LDS_V = !SHARED && kValuesInLds<T, DP>;
     using L = Tile<T, DP>;
     using Rows = Stage<T, DP, BM>;
-    __shared__ alignas(16) T queries[2][Rows::kSize], grads[2][Rows::kSize];
+    constexpr int BUFFERS = SHARED && Rows::kSize * sizeof(T) > 20 * 1024 ? 1 : 2;
+    __shared__ alignas(16) T tiles[2][BUFFERS][Rows::kSize];
     __shared__ alignas(16) T values[LDS_V ? Stage<T, DP, kTile>::kSize : 8];
-    __shared__ alignas(16) float lses[2][64], deltas[2][64];
+    __shared__ alignas(16) float lses[BUFFERS][SHARED ? 128 : 64], deltas[BUFFERS][SHARED ? 128 : 64];
     const mgopt_attention_args& a = p.a;
     const Unit u = unit_of(p, false);
-    const Part s = find<true>(p, u.slot, 1);
+    const Part s = find<true, TILE>(p, u.slot, 1);
     if (s.first >= s.total) return;
     const int lane = threadIdx.x % 64, wave = uniform(static_cast<int32_t>(threadIdx.x / 64)), col = lane % 32, h = lane / 32;
-    const int32_t tile0 = static_cast<int32_t>(s.first), key = tile0 + wave * 32 + col;
+    const int32_t tile0 = static_cast<int32_t>(s.first), key0 = tile0 + (SHARED ? 0 : wave * 32), key = key0 + col;
+    const int block0 = SHARED ? wave : 0;  // of the wave's rows in a tile
     const bool live = key < s.m;
     Frag<T> k[DP / 16], v[LDS_V ? 1 : DP / 16];
     load_row<T, DP>(k, live ? row_of<T>(a.k_dev, a.k_stride, s.batch, s.k0 + key, u.head) : nullptr, a.dim, h);
@@ -790,15 +839,17 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dkv_ke
     const auto fetch = [&](int32_t r0, int buf) {
         if (p.aligned_rows && r0 + BM <= rows && r0 >= blind) {
             const int64_t first = place_of(p, r0).query;
-            stage_q.whole(queries[buf], wave, qp + first * a.q_stride[1]);
-            stage_g.whole(grads[buf], wave, gp + first * a.grad_out_stride[1]);
+            stage_q.whole(tiles[0][buf], wave, qp + first * a.q_stride[1]);
+            stage_g.whole(tiles[1][buf], wave, gp + first * a.grad_out_stride[1]);
         } else {
-            Rows::copy(queries[buf], a.dim, [&](int r) { return q_row(at(r0 + r)); });
-            Rows::copy(grads[buf], a.dim, [&](int r) { return g_row(at(r0 + r)); });
+            Rows::copy(tiles[0][buf], a.dim, [&](int r) { return q_row(at(r0 + r)); });
+            Rows::copy(tiles[1][buf], a.dim, [&](int r) { return g_row(at(r0 + r)); });
         }
-        if (wave < 2) {
-            const Place x = at(r0 + min(lane, BM - 1));
-            load_word(wave == 0 ? lses[buf] : deltas[buf], stats + (wave == 0 ? 0 : all) + x.head * a.queries + x.query);
+        // waves 0 and 1 (of 128 rows 0 to 3) bring 64 rows' statistics each
+        if (wave < (BM > 64 ? 4 : 2)) {
+            const int half = wave / 2 * 64;
+            const Place x = at(r0 + min(half + lane, BM - 1));
+            load_word((wave % 2 == 0 ? lses[buf] : deltas[buf]) + half, stats + (wave % 2 == 0 ? 0 : all) + x.head * a.queries + x.query);
         }
     };
     f32x16 dk[DP / 32], dv[DP / 32];
@@ -812,19 +863,21 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dkv_ke
     landed();
     __syncthreads();
     int buf = 0;
-    for (int32_t r0 = last; r0 >= from && from < rows; r0 -= BM, buf ^= 1) {
-        if (r0 > from) fetch(r0 - BM, buf ^ 1);
+    for (int32_t r0 = last; r0 >= from && from < rows; r0 -= BM) {
+        if (BUFFERS == 2 && r0 > from) fetch(r0 - BM, buf ^ 1);
+        const T *const queries = tiles[0][buf], *const grads = tiles[1][buf];
         // the tile's rows see no fewer keys than its first and no more than its last
-        if (seen(p, s, place_of(p, min(r0 + BM, rows) - 1).query) > tile0 + wave * 32) {
-            const bool edge = r0 + BM > rows || seen(p, s, place_of(p, r0).query) < min(tile0 + wave * 32 + 32, s.m);
+        const int32_t r1 = r0 + 32 * block0, r2 = r1 + 32 * BLOCKS;
+        if (r1 < rows && seen(p, s, place_of(p, min(r2, rows) - 1).query) > key0) {
+            const bool edge = r2 > rows || seen(p, s, place_of(p, r1).query) < min(key0 + 32, s.m);
 #pragma unroll
-            for (int b = 0; b < BM / 32; ++b) {
+            for (int b = block0; b < block0 + BLOCKS; ++b) {
                 f32x16 x{}, ds{};
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c) {
-                    x = mma(L::rows(queries[buf], 32 * b + col, c, h), k[c], x);
-                    if constexpr (LDS_V) ds = mma(L::rows(grads[buf], 32 * b + col, c, h), L::rows(values, wave * 32 + col, c, h), ds);
-                    else ds = mma(L::rows(grads[buf], 32 * b + col, c, h), v[c], ds);
+                    x = mma(L::rows(queries, 32 * b + col, c, h), k[c], x);
+                    if constexpr (LDS_V) ds = mma(L::rows(grads, 32 * b + col, c, h), L::rows(values, wave * 32 + col, c, h), ds);
+                    else ds = mma(L::rows(grads, 32 * b + col, c, h), v[c], ds);
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -843,25 +896,50 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dkv_ke
                 for (int c = 0; c < 2; ++c) {
                     const Frag<T> w = as_operand<T>(x, c);
 #pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) dv[d] = mma(L::columns(grads[buf], d, 2 * b + c, lane), w, dv[d]);
+                    for (int d = 0; d < DP / 32; ++d) dv[d] = mma(L::columns(grads, d, 2 * b + c, lane), w, dv[d]);
                 }
                 range.fit(ds, dk);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Frag<T> w = as_operand<T>(ds, c);
 #pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) dk[d] = mma(L::columns(queries[buf], d, 2 * b + c, lane), w, dk[d]);
+                    for (int d = 0; d < DP / 32; ++d) dk[d] = mma(L::columns(queries, d, 2 * b + c, lane), w, dk[d]);
                 }
             }
+        }
+        if constexpr (BUFFERS == 2) {
+            buf ^= 1;
+        } else {
+            __syncthreads();
+            if (r0 > from) fetch(r0 - BM, 0);
         }
         landed();
         __syncthreads();
     }
-    if (key >= s.total) return;
     const float down = exp2_hw(-kShift<T>);
-    store_row<T, DP>(row_of<T>(a.d_k_dev, a.d_k_stride, s.batch, s.k0 + key, u.head), dk,
-                     live ? static_cast<float>(a.scale) * range.back() * down : 0.0f, a.dim, h);
-    store_row<T, DP>(row_of<T>(a.d_v_dev, a.d_v_stride, s.batch, s.k0 + key, u.head), dv, live ? down : 0.0f, a.dim, h);
+    const float by_k = live ? static_cast<float>(a.scale) * range.back() * down : 0.0f, by_v = live ? down : 0.0f;
+    if constexpr (SHARED) {
+        static_assert(sizeof(tiles) >= Join<DP>::kBytes);
+        Join<DP> join(&tiles[0][0][0]);
+        const int32_t row = tile0 + join.r;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            join.put(wave, col, side == 0 ? dk : dv, side == 0 ? by_k : by_v, h);
+            __syncthreads();
+            if (row < s.total) {
+                float y[Join<DP>::kEach] = {};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) join.get(y, w, 1.0f);
+                T* const to = side == 0 ? row_of<T>(a.d_k_dev, a.d_k_stride, s.batch, s.k0 + row, u.head)
+                                        : row_of<T>(a.d_v_dev, a.d_v_stride, s.batch, s.k0 + row, u.head);
+                store_some<Join<DP>::kEach>(to + join.d0, y, a.dim - join.d0);
+            }
+            __syncthreads();
+        }
+    } else if (key < s.total) {
+        store_row<T, DP>(row_of<T>(a.d_k_dev, a.d_k_stride, s.batch, s.k0 + key, u.head), dk, by_k, a.dim, h);
+        store_row<T, DP>(row_of<T>(a.d_v_dev, a.d_v_stride, s.batch, s.k0 + key, u.head), dv, by_v, a.dim, h);
+    }
 }
 
 // ---------------------------------------------------------------------- host
@@ -923,14 +1001,15 @@ struct Form {
 };
 constexpr int64_t kMinShare = 256;   // keys of a part at least
 constexpr int64_t kFill = 512;       // work-groups that fill the chip: two a CU
+constexpr int64_t kFew = 128, kFewF32 = 512;  // fewer than this in the backward pass, and waves share rows, or keys
+int64_t groups_of(const mgopt_attention_args& a, int64_t tokens, int64_t per, int tile) {
+    return a.k_heads * (a.q_offsets_dev ? tokens * per / tile + a.sequences : (tokens * per + tile - 1) / tile * a.batch);
+}
 Form form_of(const mgopt_attention_args& a) {
     const int64_t per = a.q_heads / a.k_heads;
-    const auto groups = [&](int tile) {
-        return a.k_heads * (a.q_offsets_dev ? a.queries * per / tile + a.sequences : (a.queries * per + tile - 1) / tile * a.batch);
-    };
     Form f;
-    f.shared = groups(kTile) < kFill;
-    const int64_t work = std::max<int64_t>(1, groups(f.shared ? kShared : kTile));
+    f.shared = groups_of(a, a.queries, per, kTile) < kFill;
+    const int64_t work = std::max<int64_t>(1, groups_of(a, a.queries, per, f.shared ? kShared : kTile));
     const int64_t keys = a.q_offsets_dev ? a.keys / std::max<int64_t>(1, a.sequences) : a.keys;
     const int64_t s = std::min((kFill + work - 1) / work, keys / kMinShare);
     f.splits = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(s, kMostSplits)));
@@ -1021,23 +1100,27 @@ MGOPT_API int mgopt_attention_backward(const mgopt_attention_args* a, void* stre
         return set_error(MGOPT_E_ALIGN, "attention_backward: the workspace must be 16-byte aligned and not NULL");
     AttArgs p = args_of(*a);
     p.stats = static_cast<float*>(a->workspace_dev);
+    const int64_t few = a->dtype == MGOPT_F32 ? kFewF32 : kFew;
+    const bool shared_rows = groups_of(*a, a->queries, p.group, kTile) < few, shared_keys = groups_of(*a, a->keys, 1, kTile) < few;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         return with_dim(a->dim, [&](auto d) -> int {
             constexpr int DP = decltype(d)::value;
-            p.aligned_rows = kRows<T, DP> % p.group == 0;
+            p.aligned_rows = (shared_keys ? 128 : kRows<T, DP>) % p.group == 0;
             for (const auto& [at, stride] : {std::pair<const void*, const int64_t*>{a->q_dev, a->q_stride}, {a->grad_out_dev, a->grad_out_stride}})
-                p.aligned_rows = p.aligned_rows && aligned(at, stride, sizeof(T), a->dim) && stride[1] < kNear / 256 && stride[2] < kNear / 8 / p.group;
+                p.aligned_rows = p.aligned_rows && aligned(at, stride, sizeof(T), a->dim) && stride[1] < kNear / 512 && stride[2] < kNear / 8 / p.group;
             uint32_t blocks;
             if (rows) {
-                if (int rc = places(*a, a->queries, p.group, kTile, "attention_backward", p.tiles, blocks)) return rc;
-                hipLaunchKernelGGL((attention_dq_kernel<T, DP>), dim3(blocks), dim3(kThreads), 0, s, p);
+                if (int rc = places(*a, a->queries, p.group, shared_rows ? kShared : kTile, "attention_backward", p.tiles, blocks)) return rc;
+                if (shared_rows) hipLaunchKernelGGL((attention_dq_kernel<T, DP, true>), dim3(blocks), dim3(kThreads), 0, s, p);
+                else hipLaunchKernelGGL((attention_dq_kernel<T, DP, false>), dim3(blocks), dim3(kThreads), 0, s, p);
                 if (int rc = launched("attention_backward")) return rc;
             }
             if (!keys) return 0;
-            if (int rc = places(*a, a->keys, 1, kTile, "attention_backward", p.tiles, blocks)) return rc;
-            hipLaunchKernelGGL((attention_dkv_kernel<T, DP>), dim3(blocks), dim3(kThreads), 0, s, p);
+            if (int rc = places(*a, a->keys, 1, shared_keys ? kShared : kTile, "attention_backward", p.tiles, blocks)) return rc;
+            if (shared_keys) hipLaunchKernelGGL((attention_dkv_kernel<T, DP, true>), dim3(blocks), dim3(kThreads), 0, s, p);
+            else hipLaunchKernelGGL((attention_dkv_kernel<T, DP, false>), dim3(blocks), dim3(kThreads), 0, s, p);
             return launched("attention_backward");
         });
     });
