@@ -217,7 +217,7 @@ typedef struct mgopt_attention_args {
     const void* k_lengths_dev;
     void* workspace_dev; /* mgopt_attention_workspace bytes, 16-byte aligned */
     int64_t q_stride[3];
-    int64_t k_stride[3];
+    int64_t k_stride[3]; /* of tokens below 2^23, as v's */
     int64_t v_stride[3];
     int64_t out_stride[3];
     int64_t grad_out_stride[3];

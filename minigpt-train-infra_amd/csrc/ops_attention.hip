@@ -168,12 +168,26 @@ struct Stage {
                 load(lds, i, base, row * static_cast<uint32_t>(stride) * static_cast<uint32_t>(sizeof(T)) + chunk_bytes(v, dim));
             }
     }
-    // Rows anywhere, through registers; at(r): where row r lies.
+    // Rows anywhere; at(r): where row r lies.
+    template <typename F>
+    static __device__ __forceinline__ void scattered(T* lds, int wave, int dim, F&& at) {
+        int lane = threadIdx.x % 64;
+        asm volatile("" : "+v"(lane));  // nothing of this way is worth a register between the tiles
+#pragma unroll 1
+        for (int x = 0; x < kEach; ++x)
+            if (const int i = x * (kThreads / 64) + wave; i < kLoads) {
+                const int v = i * 64 + lane;
+                const char* from = reinterpret_cast<const char*>(at(min(v / kRowChunks, ROWS - 1))) + chunk_bytes(v, dim);
+                const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) T*)lds)) + i * 1024;
+                asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
+            }
+    }
+    // The same through registers, for rows of any alignment.
     template <typename F>
     static __device__ __forceinline__ void copy(T* lds, int dim, F&& at) {
         typedef T chunk_t __attribute__((ext_vector_type(L::kPer)));
         int v = threadIdx.x;
-        asm volatile("" : "+v"(v));  // nothing of this rare way is worth a register between the tiles
+        asm volatile("" : "+v"(v));
         for (; v < ROWS * L::kChunks; v += kThreads) {
             const int r = v / L::kChunks, c = v % L::kChunks;
             *reinterpret_cast<chunk_t*>(lds + L::at(r, c)) = load_part<T, L::kPer>(at(r) + c * L::kPer, dim - c * L::kPer);
@@ -200,7 +214,8 @@ struct AttArgs {
     uint32_t splits;
     float scale2;        // scale * log2(e)
     bool aligned_keys;   // keys' and values' chunks are aligned to 16 bytes
-    bool aligned_rows;   // queries' and gradients' too, tiles of them have (query, head) alike, and 32 bits reach over them
+    bool aligned_rows;   // queries' and gradients' too
+    bool even_rows;      // and their tiles have (query, head) alike, and 32 bits reach over them
     float* stats;        // backward: [2][batch][q_heads][queries], lse * log2(e) - kShift (inf: sees no key), and delta
     float* part_out;     // [splits][rows][dim]
     float* part_ml;      // [splits][rows][2]
@@ -837,13 +852,15 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dkv_ke
     // rows that are not there, or see no key, are others here: their probabilities are 0
     const auto at = [&](int32_t r) { return place_of(p, min(max(r, blind), rows - 1)); };
     const auto fetch = [&](int32_t r0, int buf) {
-        if (p.aligned_rows && r0 + BM <= rows && r0 >= blind) {
+        if (p.even_rows && r0 + BM <= rows && r0 >= blind) {
             const int64_t first = place_of(p, r0).query;
             stage_q.whole(tiles[0][buf], wave, qp + first * a.q_stride[1]);
             stage_g.whole(tiles[1][buf], wave, gp + first * a.grad_out_stride[1]);
         } else {
-            Rows::copy(tiles[0][buf], a.dim, [&](int r) { return q_row(at(r0 + r)); });
-            Rows::copy(tiles[1][buf], a.dim, [&](int r) { return g_row(at(r0 + r)); });
+            const auto q_at = [&](int r) { return q_row(at(r0 + r)); };
+            const auto g_at = [&](int r) { return g_row(at(r0 + r)); };
+            if (p.aligned_rows) Rows::scattered(tiles[0][buf], wave, a.dim, q_at), Rows::scattered(tiles[1][buf], wave, a.dim, g_at);
+            else Rows::copy(tiles[0][buf], a.dim, q_at), Rows::copy(tiles[1][buf], a.dim, g_at);
         }
         // waves 0 and 1 (of 128 rows 0 to 3) bring 64 rows' statistics each
         if (wave < (BM > 64 ? 4 : 2)) {
@@ -973,8 +990,8 @@ int check(const mgopt_attention_args* a, const char* what) {
     for (const int64_t* stride : {a->q_stride, a->k_stride, a->v_stride, a->out_stride, a->grad_out_stride, a->d_q_stride,
                                   a->d_k_stride, a->d_v_stride})
         if (stride[0] < 0 || stride[1] < 0 || stride[2] < 0) return set_error(MGOPT_E_INVALID, w + ": negative strides");
-    if (a->k_stride[1] >= kNear / 64 || a->v_stride[1] >= kNear / 64)
-        return set_error(MGOPT_E_LIMIT, w + ": keys or values 2^24 elements apart or more");
+    if (a->k_stride[1] >= kNear / 128 || a->v_stride[1] >= kNear / 128)  // offsets over a tile of 128 of them have 32 bits
+        return set_error(MGOPT_E_LIMIT, w + ": keys or values 2^23 elements apart or more");
     const int64_t most = int64_t{1} << 30;
     if (a->keys > most || a->queries > most / a->q_heads || a->sequences > most || a->q_heads > (1 << 20))
         return set_error(MGOPT_E_LIMIT, w + ": more than 2^30 keys, sequences or queries times heads");
@@ -1002,6 +1019,9 @@ struct Form {
 constexpr int64_t kMinShare = 256;   // keys of a part at least
 constexpr int64_t kFill = 512;       // work-groups that fill the chip: two a CU
 constexpr int64_t kFew = 128, kFewF32 = 512;  // fewer than this in the backward pass, and waves share rows, or keys
+// but for 2-byte heads of more than 64 and keys of more rows: 2 x 2,000 queries of 6 + 2 heads of 128 391 us, shared 438;
+// 2,048 of 4 + 4 160 us, shared 100
+constexpr int64_t kFewRows = 4096;
 int64_t groups_of(const mgopt_attention_args& a, int64_t tokens, int64_t per, int tile) {
     return a.k_heads * (a.q_offsets_dev ? tokens * per / tile + a.sequences : (tokens * per + tile - 1) / tile * a.batch);
 }
@@ -1101,15 +1121,17 @@ MGOPT_API int mgopt_attention_backward(const mgopt_attention_args* a, void* stre
     AttArgs p = args_of(*a);
     p.stats = static_cast<float*>(a->workspace_dev);
     const int64_t few = a->dtype == MGOPT_F32 ? kFewF32 : kFew;
-    const bool shared_rows = groups_of(*a, a->queries, p.group, kTile) < few, shared_keys = groups_of(*a, a->keys, 1, kTile) < few;
+    const bool shared_rows = groups_of(*a, a->queries, p.group, kTile) < few, shared_keys = groups_of(*a, a->keys, 1, kTile) < few &&
+        (a->dim <= 64 || a->dtype == MGOPT_F32 || a->queries * p.group <= kFewRows);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         return with_dim(a->dim, [&](auto d) -> int {
             constexpr int DP = decltype(d)::value;
-            p.aligned_rows = (shared_keys ? 128 : kRows<T, DP>) % p.group == 0;
-            for (const auto& [at, stride] : {std::pair<const void*, const int64_t*>{a->q_dev, a->q_stride}, {a->grad_out_dev, a->grad_out_stride}})
-                p.aligned_rows = p.aligned_rows && aligned(at, stride, sizeof(T), a->dim) && stride[1] < kNear / 512 && stride[2] < kNear / 8 / p.group;
+            p.aligned_rows = aligned(a->q_dev, a->q_stride, sizeof(T), a->dim) && aligned(a->grad_out_dev, a->grad_out_stride, sizeof(T), a->dim);
+            p.even_rows = p.aligned_rows && (shared_keys ? 128 : kRows<T, DP>) % p.group == 0;
+            for (const int64_t* stride : {a->q_stride, a->grad_out_stride})
+                p.even_rows = p.even_rows && stride[1] < kNear / 512 && stride[2] < kNear / 8 / p.group;
             uint32_t blocks;
             if (rows) {
                 if (int rc = places(*a, a->queries, p.group, shared_rows ? kShared : kTile, "attention_backward", p.tiles, blocks)) return rc;
