@@ -178,3 +178,23 @@ def test_refusals():
             mg.int8_linear(*bad)
         with torch.no_grad():
             mg.int8_linear(*bad)
+
+
+@pytest.mark.parametrize("M, K, N", [(1, 1000, 70), (40, 2731, 100), (64, 20, 33), (300, 2731, 300), (70, 250, 66), (2050, 1000, 2060),
+                                     (4133, 1000, 4101), (2050, 100, 2060)])
+def test_rows_that_start_on_16_bytes(M, K, N):
+    """As int8_rows lays them out, and packed: the same bits, in every form."""
+    case("int8_linear, aligned", M, K, N)
+    gen = generator(9)
+    x, w, b = mg.Int8Rows(*codes(gen, M, K, -128)), mg.Int8Rows(*codes(gen, N, K, -128)), randn(gen, (N,), torch.float32)
+    want = mg.int8_linear(x, w, b, dtype=torch.float32)
+    check(want, x, w, b, slice(max(0, M - 70), M))
+
+    def laid_out(r):
+        n, pitch = r.codes.shape[0], (K + 15) // 16 * 16
+        room = torch.full((n, pitch), 77, dtype=torch.int8, device=DEV)          # what lies between the rows counts for nothing
+        return mg.Int8Rows(room[:, :K].copy_(r.codes), r.scales)
+
+    assert same_bits([mg.int8_linear(laid_out(x), laid_out(w), b, dtype=torch.float32)], [want])
+    half = mg.int8_linear(laid_out(x), laid_out(w), b, dtype=torch.bfloat16)
+    assert same_bits([half], [want.to(torch.bfloat16)])
