@@ -10,10 +10,13 @@ Drop-in replacements for the torch calls of the reference's training loop
 plus the loop's host helpers (build_adamw_param_groups, set_optimizer_lr,
 cosine_lr, optimizer_completed_steps) and the checkpoint loaders it calls on
 resume (load_optimizer_state, load_grad_scaler_state).  Beside them, the
-operators of a training step around its matrix products and attention:
+operators of a training step around its matrix products, and of a rollout:
 
     embedding       lookup of scaled rows, and the weight's gradient
+    add_rms_norm    the residual's addition and the RMS norm of the sum
     qk_norm_rope    RMS norms of query and key heads and the rotary rotation
+    attention       grouped heads over batches, packed sequences and caches
+    int8_linear     products of 8-bit integers with scales per token and channel
     gated_act       the MLP's activation with an 8-bit checkpoint
     policy_loss     the clipped policy loss with a KL term over the logits
 

@@ -7,6 +7,11 @@
 // 2^14), so neither tiles nor parts of the contraction change a result; it is turned
 // into a 32-bit float, scaled, added to the bias and rounded once.
 //
+// Many tokens are bound by the matrix cores' chain of loads from LDS and products: 8,192 x
+// 4,096 x 12,288 in bf16 426 to 479 us (1.7 to 1.9 POP/s; the same loop without its
+// loads reaches 2.9).  Few tokens are bound by the weights' way from memory:
+// 12,288 x 4,096 codes 10 us for one token (5.0 TB/s), 17 for 64.
+//
 // The matrix cores take the channels as rows and the tokens as columns, so that a
 // lane holds four consecutive channels of one token in each group of registers.
 #include "ops_common.h"
@@ -200,7 +205,7 @@ __global__ __launch_bounds__(WC* WT * 64, 2) void int8_linear_kernel(LinearArgs 
             }
     }
     // A token's channels lie four by four in lanes that are rows of y apart: they pass through LDS, to be written in
-    // rows.  8,192 x 4,096 x 12,288 in bf16: 60 us less than writing 8 bytes a lane.
+    // rows.  8,192 x 4,096 x 12,288 in bf16: 479 us, 512 with 8 bytes a lane written as they lie.
     constexpr int PITCH = BC + 16 / static_cast<int>(sizeof(T)), PER = 16 / static_cast<int>(sizeof(T));
     static_assert(sizeof(lds) >= WT * 32 * PITCH * sizeof(T));
     T* const out = reinterpret_cast<T*>(&lds[0][0]);
@@ -355,6 +360,9 @@ MGOPT_API int mgopt_int8_linear(const int8_t* x_dev, int64_t x_stride, const flo
             return launched("int8_linear");
         };
         const auto count = [&](int64_t side) { return (rows + side - 1) / side * ((channels + side - 1) / side); };
+        // tiles of 256 where they fill the chip, of 128 where those do, of 64 otherwise: 1,024 x 12,288 x 4,096 84 us with
+        // tiles of 128, 130 of 64; 512 x 4,096 x 4,096 20 us with tiles of 64, 30 of 128; 8,192 x 12,288 x 4,096 479 us
+        // with tiles of 256, 587 of 128
         if (count(256) >= 256) return launch(Int<4>{}, Int<2>{}, Int<2>{}, Int<4>{}, Int<kBigCodes>{}, Int<kBigAhead>{});
         if (count(128) >= 256) return launch(Int<2>{}, Int<2>{}, Int<2>{}, Int<2>{}, Int<128>{}, Int<kMidAhead>{});
         return launch(Int<2>{}, Int<2>{}, Int<1>{}, Int<1>{}, Int<128>{}, Int<kSmallAhead>{});
