@@ -760,6 +760,7 @@ Attention attention_args(const Tensor& q, const Tensor& k, const Tensor& v, cons
                ", " + shape_of(k) + " and " + shape_of(v));
     if (q.size(head) < 1 || k.size(head) < 1 || q.size(head) % k.size(head) != 0)
         refuse("q's heads must be a multiple of k's, got " + std::to_string(q.size(head)) + " and " + std::to_string(k.size(head)));
+    if (q.size(head) > (1 << 20)) refuse("more than 2^20 heads, got " + shape_of(q));
     if (q.size(3) < 1) refuse("heads need at least one element, got " + shape_of(q));
     if (q.size(3) > MGOPT_MAX_ATTENTION_DIM)
         refuse("heads of more than " + std::to_string(MGOPT_MAX_ATTENTION_DIM) + " elements");

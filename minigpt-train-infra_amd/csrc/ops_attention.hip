@@ -1015,11 +1015,13 @@ int check(const mgopt_attention_args* a, const char* what) {
     for (const int64_t* stride : {a->q_stride, a->k_stride, a->v_stride, a->out_stride, a->grad_out_stride, a->d_q_stride,
                                   a->d_k_stride, a->d_v_stride})
         if (stride[0] < 0 || stride[1] < 0 || stride[2] < 0) return set_error(MGOPT_E_INVALID, w + ": negative strides");
-    if (a->k_stride[1] >= kNear / 128 || a->v_stride[1] >= kNear / 128)  // offsets over a tile of 128 of them have 32 bits
+    // offsets over a tile of 128 of them have 32 bits; one alone has no next
+    if (a->keys > 1 && (a->k_stride[1] >= kNear / 128 || a->v_stride[1] >= kNear / 128))
         return set_error(MGOPT_E_LIMIT, w + ": keys or values 2^23 elements apart or more");
     const int64_t most = int64_t{1} << 30;
     if (a->keys > most || a->queries > most / a->q_heads || a->sequences > most || a->q_heads > (1 << 20))
         return set_error(MGOPT_E_LIMIT, w + ": more than 2^30 keys, sequences or queries times heads");
+    if (a->batch > max_blocks(kThreads)) return set_error(MGOPT_E_LIMIT, w + ": more rows of the batch than work-groups");
     return 0;
 }
 

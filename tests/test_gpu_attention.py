@@ -421,3 +421,18 @@ def test_refusals():
                       ((out, q, k, k, out, lse[0]), "lse"), ((out, q, k, k, out, lse.double()), "lse")):
         with pytest.raises(ValueError, match=what):
             mg.attention_backward(*bad)
+
+
+def test_one_key_of_any_stride():
+    """A single key has no next: its token stride says nothing."""
+    q, k, v, g = inputs(2, 3, 1, 4, 2, 32, torch.bfloat16, 24)
+    far = [t.as_strided(t.shape, (64, 2**25, 32, 1)) for t in (k, v)]
+    got, want = run(q, *far, g), run(q, k, v, g)
+    assert all(same_bits([got[n]], [want[n]]) for n in want)
+
+
+def test_too_many_heads():
+    """Heads beyond 32 bits are refused before they are counted in 32."""
+    x = torch.ones(1, 1, 1, 8, device=DEV)
+    with pytest.raises(ValueError, match="2\\^20 heads"):
+        mg.attention(x.expand(1, 1, 2**32 + 1, 8), x, x)

@@ -151,3 +151,11 @@ def test_operators_have_no_cpu_path(mg):
                  lambda: mg.int8_rows(x), lambda: mg.int8_linear(codes, codes), lambda: mg.attention(heads, heads, heads)):
         with pytest.raises(RuntimeError, match="no CPU"):
             call()
+
+
+def test_attention_batches_beyond_a_grid(lib):
+    """Batches that no grid takes, or whose rows pass 64 bits, are refused, not taken for empty ones."""
+    for batch in (2**24 + 1, 2**62):
+        for call in (lib.mgopt_attention, lib.mgopt_attention_backward):
+            _refused(lib, call(_attention(batch=batch, queries=1, keys=1), vp(None)), E_LIMIT, b"attention")
+        assert lib.mgopt_attention_workspace(_attention(batch=batch, queries=1, keys=1), 1) == -1
