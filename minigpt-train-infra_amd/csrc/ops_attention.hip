@@ -300,7 +300,7 @@ __device__ __forceinline__ Part find(const AttArgs& p, uint32_t slot, uint32_t p
 // How many keys, from the first, query i of the sequence sees.
 __device__ __forceinline__ int32_t seen(const AttArgs& p, const Part& s, int32_t i) {
     if (i >= s.n) return 0;
-    return p.a.causal ? max(0, min(s.m, i + 1 + s.m - s.n)) : s.m;
+    return p.a.causal ? max(0, min(s.m, (i + 1 - s.n) + s.m)) : s.m;
 }
 
 // f of a lane and of the lane 32 away.
