@@ -958,8 +958,13 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_dkv_ke
         landed();
         __syncthreads();
     }
-    const float down = exp2_hw(-kShift<T>);
-    const float by_k = live ? static_cast<float>(a.scale) * range.back() * down : 0.0f, by_v = live ? down : 0.0f;
+    // a key that is not there: its column holds exp(0 - lse) of the rows, where they see all keys that are, which may
+    // have passed the type's range
+    if (!live) {
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) dk[b] = dv[b] = f32x16{};
+    }
+    const float by_v = exp2_hw(-kShift<T>), by_k = static_cast<float>(a.scale) * range.back() * by_v;
     if constexpr (SHARED) {
         static_assert(sizeof(tiles) >= Join<DP>::kBytes);
         Join<DP> join(&tiles[0][0][0]);
