@@ -20,6 +20,9 @@
 // underflow there, and r, rounded to 32 bits once, does not hang on the order of
 // the sum but in one of some 2^28 rows, so that the codes are the format's and not
 // this kernel's.
+// The backward pass sums gw * h there too, since h is as it came and not yet normed:
+// with rows near the largest values that sum passes 32 bits, and mean(gw * xhat) does
+// not.  8,192 rows of 4,096 in bf16 take 1 us more for it.
 //
 // Bound by memory.  A row is read once and held in registers, packed in its own
 // type, by one wave, 256 or 1,024 threads, whichever needs no more than a few
@@ -46,10 +49,9 @@ __device__ __forceinline__ void load_weight(float (&f)[N], const void* w, int32_
 // The sums of x and y over a work-group of BLOCK threads in a fixed order, in each of them; `part` is
 // free again when all threads have passed the next barrier.
 template <int BLOCK>
-__device__ __forceinline__ void block_sum(double& x, float& y, double (&part)[BLOCK / 64], float (&other)[BLOCK / 64]) {
+__device__ __forceinline__ void block_sum(double& x, double& y, double (&part)[BLOCK / 64], double (&other)[BLOCK / 64]) {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-    y = reduce_lanes<64>(y, [](float a, float b) { return a + b; });
+    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d), y += __shfl_xor(y, d);
     if constexpr (BLOCK > 64) {
         if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x, other[threadIdx.x / 64] = y;
         __syncthreads();
@@ -191,7 +193,7 @@ template <typename T, int BLOCK, int NV>
 __global__ __launch_bounds__(BLOCK) void rms_norm_backward_kernel(NormArgs a) {
     constexpr int N = 16 / sizeof(T);
     __shared__ double squares[2][BLOCK / 64];
-    __shared__ float dots[2][BLOCK / 64];
+    __shared__ double dots[2][BLOCK / 64];
     float dw[NV][N];
 #pragma unroll
     for (int v = 0; v < NV; ++v)
@@ -200,8 +202,7 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_backward_kernel(NormArgs a) {
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
         float h[NV][N], g[NV][N];
-        double sum = 0.0;
-        float dot = 0.0f;
+        double sum = 0.0, dot = 0.0;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int64_t at = (static_cast<int64_t>(v) * BLOCK + threadIdx.x) * N, n = a.width - at;
@@ -216,13 +217,13 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_backward_kernel(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 sum = fma(static_cast<double>(h[v][i]), static_cast<double>(h[v][i]), sum);
-                dot = fmaf(g[v][i] * w[i], h[v][i], dot);
+                dot = fma(static_cast<double>(g[v][i] * w[i]), static_cast<double>(h[v][i]), dot);
             }
         }
         // two sets of partial sums in turn: a wave that is a row ahead writes the other one
         block_sum<BLOCK>(sum, dot, squares[turn], dots[turn]);
         const float r = rstd_of(sum, a.width, a.eps);
-        const float mean = dot * r / static_cast<float>(a.width);
+        const float mean = static_cast<float>(dot * static_cast<double>(r) / static_cast<double>(a.width));
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int64_t at = (static_cast<int64_t>(v) * BLOCK + threadIdx.x) * N, n = a.width - at;
