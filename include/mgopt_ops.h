@@ -228,7 +228,7 @@ typedef struct mgopt_attention_args {
     int64_t queries; /* tokens of q in a row of the batch */
     int64_t keys;
     int64_t sequences;
-    double scale; /* positive, below 2^100 */
+    double scale; /* 2^-100 or more, below 2^100 */
     int32_t q_heads;
     int32_t k_heads; /* divides q_heads */
     int32_t dim;

@@ -75,7 +75,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
     offsets[s] to offsets[s + 1]; key_offsets where the keys are packed otherwise.
     Tokens of no sequence are not read, and out is 0 there.
 
-    scale: positive, 1/sqrt(dim) by default.  A key or value that is not finite
+    scale: from 2^-100 to below 2^100, 1/sqrt(dim) by default.  A key or value that is not finite
     reaches queries of its own sequence only, but there also some before it."""
     if recorded(q, k, v):
         return _Attention.apply(q, k, v, offsets, key_offsets, lengths, key_lengths, causal, scale, heads_first)

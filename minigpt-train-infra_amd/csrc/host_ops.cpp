@@ -765,7 +765,7 @@ Attention attention_args(const Tensor& q, const Tensor& k, const Tensor& v, cons
     if (q.size(3) > MGOPT_MAX_ATTENTION_DIM)
         refuse("heads of more than " + std::to_string(MGOPT_MAX_ATTENTION_DIM) + " elements");
     a.scale = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3)));
-    if (!(a.scale > 0.0) || !(a.scale < 0x1p100)) refuse("the scale must be positive and below 2^100");
+    if (!(a.scale >= 0x1p-100) || !(a.scale < 0x1p100)) refuse("the scale must be at least 2^-100 and below 2^100");
     a.batch = q.size(0), a.queries = q.size(token), a.keys = k.size(token);
     a.q_heads = static_cast<int32_t>(q.size(head)), a.k_heads = static_cast<int32_t>(k.size(head));
     a.dim = static_cast<int32_t>(q.size(3)), a.causal = causal;

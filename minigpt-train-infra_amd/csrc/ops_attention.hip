@@ -1010,7 +1010,9 @@ int check(const mgopt_attention_args* a, const char* what) {
     if (a->dim < 1) return set_error(MGOPT_E_INVALID, w + ": heads need at least one element");
     if (a->dim > MGOPT_MAX_ATTENTION_DIM)
         return set_error(MGOPT_E_LIMIT, w + ": heads of more than " + std::to_string(MGOPT_MAX_ATTENTION_DIM) + " elements");
-    if (!(a->scale > 0.0) || !(a->scale < 0x1p100)) return set_error(MGOPT_E_INVALID, w + ": the scale must be positive and below 2^100");
+    // far smaller ones are 0 in fp32, and 0 times a masked score's -inf a NaN
+    if (!(a->scale >= 0x1p-100) || !(a->scale < 0x1p100))
+        return set_error(MGOPT_E_INVALID, w + ": the scale must be at least 2^-100 and below 2^100");
     if ((a->q_offsets_dev == nullptr) != (a->k_offsets_dev == nullptr))
         return set_error(MGOPT_E_INVALID, w + ": offsets of both sides, or of none");
     if (a->q_offsets_dev && (a->batch != 1 || a->q_lengths_dev || a->k_lengths_dev))
