@@ -503,7 +503,8 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
                     for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
                 top = next;
             }
-            const float off = fmaf(ref, p.scale2, -kShift<T>);
+            float off = fmaf(ref, p.scale2, -kShift<T>);
+            if (off == INFINITY) off = NAN;  // a score beyond 32 bits: what inf - inf is, and not a row without keys
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
