@@ -79,6 +79,11 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None,
                   eps: float = 1e-6) -> tuple[Int8Rows, torch.Tensor]:
     """(rows, h): y in 8 bits with a scale for each row, rounded from 32 bits,
-    and h (x itself without a residual).  Nothing is recorded for autograd."""
+    and h (x itself without a residual).  Nothing is recorded for autograd: an x
+    and a residual that ask for a gradient, which h would lose, are refused."""
+    if torch.is_grad_enabled():
+        for name, t in (("x", x), ("the residual", residual)):
+            if t is not None and t.requires_grad:
+                raise ValueError(f"rms_norm_int8 has no gradient by {name}: detach it")
     codes, scales, h = N.ops().rms_norm(x, residual, weight, eps, True, N.ops_stream(x))
     return Int8Rows(codes, scales), h
