@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from ._autograd import recorded
+from ._autograd import apart, recorded
 
 
 def attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
@@ -45,6 +45,10 @@ class _Attention(torch.autograd.Function):
         return (*N.ops().attention_backward(grad_out, *given, *ctx.how, N.ops_stream(given[0])),) + (None,) * 7
 
 
+def _with_lse(q, *given) -> tuple[torch.Tensor, ...]:
+    return N.ops().attention(q, *given, True, N.ops_stream(q))
+
+
 def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: torch.Tensor | None = None,
                   key_offsets: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
                   key_lengths: torch.Tensor | None = None, causal: bool = True, scale: float | None = None,
@@ -52,8 +56,7 @@ def attention_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets:
     """(out, lse): attention and, for attention_backward or to join parts of the
     keys, the logarithm of each row's sum of exp(scores), float32 (batch, heads,
     length).  Nothing is recorded for autograd."""
-    return N.ops().attention(q, k, v, offsets, key_offsets, lengths, key_lengths, causal, scale, heads_first, True,
-                             N.ops_stream(q))
+    return apart(_with_lse, q, k, v, offsets, key_offsets, lengths, key_lengths, causal, scale, heads_first)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: torch.Tensor | None = None,

@@ -11,6 +11,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as N
+from ._autograd import apart
 
 
 class Int8Rows(NamedTuple):
@@ -20,13 +21,21 @@ class Int8Rows(NamedTuple):
     scales: torch.Tensor     # float32 (...)
 
 
+def _rows(x) -> tuple[torch.Tensor, ...]:
+    return N.ops().int8_rows(x, N.ops_stream(x))
+
+
 def int8_rows(x: torch.Tensor) -> Int8Rows:
     """x (..., width) in 8 bits, a scale for each row: tokens of an activation, or
     the output channels of a weight (channels, width).  With m a row's largest
     magnitude, scale = m / 127 and the codes are the integers nearest to
     x * (127 / m); m below 2^-119 counts as 0, a row with an inf or a NaN has the
     scale NaN.  Nothing is recorded for autograd."""
-    return Int8Rows(*N.ops().int8_rows(x, N.ops_stream(x)))
+    return Int8Rows(*apart(_rows, x))
+
+
+def _linear(codes, *given) -> tuple[torch.Tensor]:
+    return (N.ops().int8_linear(codes, *given, N.ops_stream(codes)),)
 
 
 def int8_linear(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, *,
@@ -41,4 +50,4 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
         for name, t in (("x's scales", x.scales), ("weight's scales", weight.scales), ("bias", bias)):
             if t is not None and t.requires_grad:
                 raise ValueError(f"int8_linear has no gradient by {name}: detach it")
-    return N.ops().int8_linear(x.codes, x.scales, weight.codes, weight.scales, bias, dtype, N.ops_stream(x.codes))
+    return apart(_linear, x.codes, x.scales, weight.codes, weight.scales, bias, dtype)[0]

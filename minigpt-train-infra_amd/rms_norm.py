@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from ._autograd import recorded
+from ._autograd import apart, recorded
 from .int8_linear import Int8Rows
 
 
@@ -76,6 +76,11 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     return N.ops().rms_norm(x, residual, weight, eps, False, N.ops_stream(x))
 
 
+def _normed_rows(x, residual, weight, eps) -> tuple[torch.Tensor, ...]:
+    codes, scales, h = N.ops().rms_norm(x, residual, weight, eps, True, N.ops_stream(x))
+    return (codes, scales) if residual is None else (codes, scales, h)
+
+
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None,
                   eps: float = 1e-6) -> tuple[Int8Rows, torch.Tensor]:
     """(rows, h): y in 8 bits with a scale for each row, rounded from 32 bits,
@@ -85,5 +90,5 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tens
         for name, t in (("x", x), ("the residual", residual)):
             if t is not None and t.requires_grad:
                 raise ValueError(f"rms_norm_int8 has no gradient by {name}: detach it")
-    codes, scales, h = N.ops().rms_norm(x, residual, weight, eps, True, N.ops_stream(x))
-    return Int8Rows(codes, scales), h
+    rows = apart(_normed_rows, x, residual, weight, eps)
+    return Int8Rows(*rows[:2]), x if residual is None else rows[2]
