@@ -20,9 +20,12 @@
 // underflow there, and r, rounded to 32 bits once, does not hang on the order of
 // the sum but in one of some 2^28 rows, so that the codes are the format's and not
 // this kernel's.
-// The backward pass sums gw * h there too, since h is as it came and not yet normed:
-// with rows near the largest values that sum passes 32 bits, and mean(gw * xhat) does
-// not.  8,192 rows of 4,096 in bf16 take 1 us more for it.
+//
+// The backward pass norms a row before it sums gw * xhat, though a sum of gw * h
+// beside the squares' saves a join of the waves: with h near its type's largest values
+// that sum passes 32 bits.  On the same inputs over and over, with and without it: 8,192
+// rows of 4,096 in bf16 46.5 and 45.7 us, 4,096 of 16,384 119 and 128, 2,048 of 32,768
+// in fp32 340 and 301.  (The sum of gw * h in 64 bits: 47, 157 and 342, for the registers.)
 //
 // Bound by memory.  A row is read once and held in registers, packed in its own
 // type, by one wave, 256 or 1,024 threads, whichever needs no more than a few
@@ -46,24 +49,16 @@ __device__ __forceinline__ void load_weight(float (&f)[N], const void* w, int32_
     else load_some<N>(f, static_cast<const __bf16*>(w) + at, n);
 }
 
-// The sums of x and y over a work-group of BLOCK threads in a fixed order, in each of them; `part` is
-// free again when all threads have passed the next barrier.
-template <int BLOCK>
-__device__ __forceinline__ void block_sum(double& x, double& y, double (&part)[BLOCK / 64], double (&other)[BLOCK / 64]) {
+// The sum of x over a work-group of BLOCK threads in a fixed order, in each of them; `part` is free again
+// when all threads have passed the next barrier.
+template <int BLOCK, typename X>
+__device__ __forceinline__ X block_sum(X x, X (&part)[BLOCK / 64]) {
+    if constexpr (sizeof(X) == 4) {
+        x = reduce_lanes<64>(x, [](X a, X b) { return a + b; });
+    } else {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d), y += __shfl_xor(y, d);
-    if constexpr (BLOCK > 64) {
-        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x, other[threadIdx.x / 64] = y;
-        __syncthreads();
-        x = part[0], y = other[0];
-#pragma unroll
-        for (int i = 1; i < BLOCK / 64; ++i) x += part[i], y += other[i];
+        for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
     }
-}
-template <int BLOCK>
-__device__ __forceinline__ double block_sum(double x, double (&part)[BLOCK / 64]) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
     if constexpr (BLOCK > 64) {
         if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = x;
         __syncthreads();
@@ -193,7 +188,7 @@ template <typename T, int BLOCK, int NV>
 __global__ __launch_bounds__(BLOCK) void rms_norm_backward_kernel(NormArgs a) {
     constexpr int N = 16 / sizeof(T);
     __shared__ double squares[2][BLOCK / 64];
-    __shared__ double dots[2][BLOCK / 64];
+    __shared__ float dots[2][BLOCK / 64];
     float dw[NV][N];
 #pragma unroll
     for (int v = 0; v < NV; ++v)
@@ -202,7 +197,7 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_backward_kernel(NormArgs a) {
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
         float h[NV][N], g[NV][N];
-        double sum = 0.0, dot = 0.0;
+        double sum = 0.0;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int64_t at = (static_cast<int64_t>(v) * BLOCK + threadIdx.x) * N, n = a.width - at;
@@ -210,20 +205,21 @@ __global__ __launch_bounds__(BLOCK) void rms_norm_backward_kernel(NormArgs a) {
             load_some<N>(g[v], static_cast<const T*>(a.x) + row * a.x_stride + at, n);
         }
 #pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum = fma(static_cast<double>(h[v][i]), static_cast<double>(h[v][i]), sum);
+        // two sets of partial sums in turn: a wave that is a row ahead writes the other one
+        const float r = rstd_of(block_sum<BLOCK>(sum, squares[turn]), a.width, a.eps);
+        float dot = 0.0f;
+#pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int64_t at = (static_cast<int64_t>(v) * BLOCK + threadIdx.x) * N, n = a.width - at;
             float w[N];
             load_weight<N>(w, a.weight, a.weight_dtype, at, n);
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                sum = fma(static_cast<double>(h[v][i]), static_cast<double>(h[v][i]), sum);
-                dot = fma(static_cast<double>(g[v][i] * w[i]), static_cast<double>(h[v][i]), dot);
-            }
+            for (int i = 0; i < N; ++i) dot = fmaf(g[v][i] * w[i], h[v][i] * r, dot);
         }
-        // two sets of partial sums in turn: a wave that is a row ahead writes the other one
-        block_sum<BLOCK>(sum, dot, squares[turn], dots[turn]);
-        const float r = rstd_of(sum, a.width, a.eps);
-        const float mean = static_cast<float>(dot * static_cast<double>(r) / static_cast<double>(a.width));
+        const float mean = block_sum<BLOCK>(dot, dots[turn]) / static_cast<float>(a.width);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int64_t at = (static_cast<int64_t>(v) * BLOCK + threadIdx.x) * N, n = a.width - at;
