@@ -298,17 +298,19 @@ __global__ __launch_bounds__(BLOCK) void int8_rows_kernel(NormArgs a) {
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-// Threads of a row, and vectors a thread, by the row's vectors.
-template <typename F>
-int with_shape(int64_t vecs, F&& f) {
+// Threads of a row, and vectors of N elements a thread.
+template <int N, typename F>
+int with_shape(int64_t width, F&& f) {
+    const int64_t vecs = (width + N - 1) / N;
     if (vecs <= 64) return f(Int<64>{}, Int<1>{});
     if (vecs <= 128) return f(Int<64>{}, Int<2>{});
     if (vecs <= 256) return f(Int<256>{}, Int<1>{});
     if (vecs <= 512) return f(Int<256>{}, Int<2>{});
     if (vecs <= 1024) return f(Int<256>{}, Int<4>{});
     if (vecs <= 2048) return f(Int<1024>{}, Int<2>{});
-    if (vecs <= 4096) return f(Int<1024>{}, Int<4>{});
-    return f(Int<1024>{}, Int<8>{});
+    if constexpr (kMaxWidth / N > 4096)
+        if (vecs > 4096) return f(Int<1024>{}, Int<8>{});
+    return f(Int<1024>{}, Int<4>{});
 }
 
 // The launches that cover the rows, one work-group each, in pieces of at most a grid.
@@ -374,7 +376,7 @@ MGOPT_API int mgopt_rms_norm(const void* x_dev, int64_t x_stride, const void* re
         using T = decltype(t);
         constexpr int N = 16 / sizeof(T);
         // codes fill their rows up to the stride
-        return with_shape(((codes_dev ? codes_stride : width) + N - 1) / N, [&](auto block, auto nv) {
+        return with_shape<N>(codes_dev ? codes_stride : width, [&](auto block, auto nv) {
             constexpr int B = decltype(block)::value, NV = decltype(nv)::value;
             return over_rows(a, B, "rms_norm", [&](dim3 grid) {
                 if (codes_dev) hipLaunchKernelGGL((rms_norm_kernel<T, B, NV, true>), grid, dim3(B), 0, s, a);
@@ -412,7 +414,7 @@ MGOPT_API int mgopt_rms_norm_backward(const void* grad_y_dev, int64_t grad_y_str
         const int rc = with_dtype(dtype, [&](auto t) {
             using T = decltype(t);
             constexpr int N = 16 / sizeof(T);
-            return with_shape((width + N - 1) / N, [&](auto block, auto nv) {
+            return with_shape<N>(width, [&](auto block, auto nv) {
                 constexpr int B = decltype(block)::value, NV = decltype(nv)::value;
                 hipLaunchKernelGGL((rms_norm_backward_kernel<T, B, NV>), dim3(blocks), dim3(B), 0, s, a);
                 return launched("rms_norm_backward");
