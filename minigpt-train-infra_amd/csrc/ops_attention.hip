@@ -503,8 +503,7 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
                     for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
                 top = next;
             }
-            float off = fmaf(ref, p.scale2, -kShift<T>);
-            if (off == INFINITY) off = NAN;  // a score beyond 32 bits: what inf - inf is, and not a row without keys
+            const float off = fmaf(ref, p.scale2, -kShift<T>);
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
@@ -531,6 +530,8 @@ __global__ __launch_bounds__(kThreads, (kMinWaves<T, DP>)) void attention_kernel
         __syncthreads();
     }
     sum = with_partner(sum, add);
+    // a score beyond 32 bits took all others' probabilities, and its own, to 0: what inf - inf is, and not a row without keys
+    if (top * p.scale2 == INFINITY) sum = NAN;
     if (mine == 0) {  // padding, or no key to see: what its column holds is of a query of zeros without a mask
         top = -INFINITY, sum = 0.0f;
 #pragma unroll
