@@ -187,8 +187,8 @@ MGOPT_API int mgopt_qk_norm_rope_backward(const mgopt_qk_args* args, void* strea
 /* Query i of a sequence of n queries and m keys sees key j of it where j <= i + m
  * - n (causal: the last query sees the last key), or always.  With x = scale q . k
  * over the keys seen, lse = log(sum(exp(x))) and out = sum(exp(x - lse) v); a query
- * that sees none has out 0, lse -inf and no gradient.  Query head h reads key head
- * h / (q_heads / k_heads).
+ * that sees none has out 0, lse -inf and no gradient, one whose largest x passes 32
+ * bits NaN.  Query head h reads key head h / (q_heads / k_heads).
  *   *_stride       {batch, token, head}, in elements; a head's `dim` elements are
  *                  contiguous.
  *   lse_dev        [batch][q_heads][queries]; mgopt_attention takes NULL.

@@ -5,8 +5,8 @@ over a cache; and its backward pass.
 
 over the keys that query i of a sequence of n queries and m keys sees: j <= i +
 m - n if causal, so that the last query sees the last key, and else all.  A query
-that sees none has out 0, lse -inf and no gradient.  Scores, softmax statistics
-and sums are held in 32 bits; probabilities and the scores' gradients are rounded
+that sees none has out 0, lse -inf and no gradient; one whose largest score passes
+32 bits is NaN.  Scores, softmax statistics and sums are held in 32 bits; probabilities and the scores' gradients are rounded
 to the inputs' type for the products that follow them.
 """
 

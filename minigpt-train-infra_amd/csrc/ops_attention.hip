@@ -12,7 +12,8 @@
 //     ds_ij = p_ij (g_i . v_j - delta_i)    dq_i = scale sum_j ds_ij k_j
 //     dv_j = sum_i p_ij g_i                 dk_j = scale sum_i ds_ij q_i
 //
-// A query that sees no key has out 0, lse -inf and no gradient.
+// A query that sees no key has out 0, lse -inf and no gradient; one whose largest
+// score passes 32 bits is NaN.
 //
 // The query heads that share a key head are rows of one matrix: row r of a
 // sequence is query r / group, head r % group of the group, so that keys and
@@ -30,7 +31,8 @@
 //
 // Probabilities and ds are rounded to the inputs' type for the products that follow
 // them: a result has up to 1.5 times the error of its own rounding.  dq of rows of few
-// keys, which hold much of its norm, also takes what that rounding leaves.
+// keys (one tile of them, 64 or where waves share rows 128), which hold much of its norm,
+// also takes what that rounding leaves.
 //
 // What bounds it.  2 x 4,096 tokens of 32 + 8 heads of 128 in bf16: 304 us forward (904
 // TFLOP/s), 398 for dq (1,036, of its three products), 804 for dk and dv (684, four
@@ -39,6 +41,12 @@
 // waves a SIMD, as many as the registers hold, hide a part.  An operand read from LDS
 // feeds one product, so that LDS would bound the matrix cores next.  Few tokens
 // over a cache are bound by memory: 64 caches of 2,048 to 4,096 tokens 172 us (4.85 TB/s).
+//
+// fp32: 2 x 4,096 tokens as above 2,536 us forward (108 TFLOP/s of a library product's
+// 154) and 8,430 backward (114); heads of 128, dq of 96 and dk and dv of 64 too, have
+// one wave a SIMD.  A token over 64 caches of 4,096 of them takes 1,310 us (1.6 TB/s): its
+// four rows are one wave's, whose 128 products of 32 x 32 x 2 a tile of 32 keys, 64
+// cycles each, are 870 us in two rounds of one work-group a CU.
 #include "ops_common.h"
 
 namespace mgopt {

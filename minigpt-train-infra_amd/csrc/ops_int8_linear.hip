@@ -243,7 +243,9 @@ __global__ __launch_bounds__(WC* WT * 64, 2) void int8_linear_kernel(LinearArgs 
 
 // Few tokens (TT blocks of 32): a work-group takes 32 channels, its eight waves an eighth of each 256 codes of the
 // contraction; their sums meet in LDS, as integers in any order.  Three stages of codes are in LDS or on
-// their way: two work-groups a CU have up to 96 KB in flight, which is what the weights' stream needs.
+// their way.  With one block of tokens a CU holds three work-groups (53,376 bytes of LDS each) and has up to 96 KB in flight,
+// which is what the weights' stream needs: 12,288 x 4,096 codes at 5.0 TB/s.  With two it holds one (82,176 bytes; two
+// work-groups are 512 too many), with 48 KB in flight: 2.8 TB/s for 64 tokens.
 constexpr int kFewWaves = 8, kFewCodes = 32 * kFewWaves, kStages = 3;
 template <typename T, int TT, bool ALIGNED>
 __global__ __launch_bounds__(kFewWaves * 64) void int8_few_kernel(LinearArgs a) {

@@ -27,12 +27,18 @@
 // rows of 4,096 in bf16 46.5 and 45.7 us, 4,096 of 16,384 119 and 128, 2,048 of 32,768
 // in fp32 340 and 301.  (The sum of gw * h in 64 bits: 47, 157 and 342, for the registers.)
 //
-// Bound by memory.  A row is read once and held in registers, packed in its own
-// type, by one wave, 256 or 1,024 threads, whichever needs no more than a few
-// vectors of 16 bytes a thread.  8,192 rows of 4,096 in bf16: 46 us forward (5.9
-// TB/s); 73 us backward (3.7 TB/s with the weight's partial sums) and 8 for the sums of
-// those.  The backward pass with 512 threads a row took 79 us, with each next row's
-// loads ahead of this row's sums 85: both cost more registers than they hide latency.
+// Bound by memory.  A row is read once and held by one wave, 256 or 1,024 threads,
+// whichever needs no more than a few vectors of 16 bytes a thread.  8,192 rows of
+// 4,096 in bf16: 46 us forward (5.9 TB/s); 75 us backward (3.6 TB/s with the weight's
+// partial sums) and 8 for the sums of those.  The backward pass with 512 threads a row
+// took 79 us and with each next row's loads ahead of this row's sums 85, where this one
+// took 72: both cost more registers than they hide latency.
+//
+// Wide rows do not stay in the registers of 1,024 threads, 128 each: forward, fp32 rows
+// over 16,384 in 8 bits spill 12 of them; backward, rows over 16,384 spill 106 (fp32) and
+// 118 (2 bytes), fp32 rows over 8,192 23.  On the same inputs over and over, backward:
+// 4,096 x 8,192 in bf16 70 us (2.9 TB/s), 4,096 x 16,384 119 (3.4), 2,048 x 32,768 301 (1.3);
+// in fp32 100 (4.0), 187 (4.3) and 340 (2.4).
 #include "ops_common.h"
 
 namespace mgopt {
@@ -338,9 +344,10 @@ int check_codes(const char* what, const int8_t* codes, int64_t stride, int64_t w
     return 0;
 }
 
-// Work-groups of the backward pass, each with a row of partial weight gradients: enough for 16 waves a
-// compute unit.  8,192 rows of 4,096 in bf16, with the sums of the partial rows: 80 us with 1,024
-// work-groups, 109 with 512 and 163 with 256, whose waves do not cover the memory's latency.
+// Work-groups of the backward pass, each with a row of partial weight gradients: 8 waves a compute unit where a
+// row is one wave's, 16 or more for the others.  8,192 rows of 4,096 in bf16, with the sums of the partial
+// rows: 80 us with 1,024 work-groups, 109 with 512 and 163 with 256, whose waves do not cover the memory's
+// latency.
 uint32_t backward_blocks(int64_t rows, int64_t width) {
     const int64_t most = width <= 1024 ? 2048 : width <= 8192 ? 1024 : 256;
     return static_cast<uint32_t>(std::max<int64_t>(1, std::min(rows, most)));
