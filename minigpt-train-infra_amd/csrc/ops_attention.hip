@@ -46,7 +46,7 @@
 // 154) and 8,430 backward (114); heads of 128, dq of 96 and dk and dv of 64 too, have
 // one wave a SIMD.  A token over 64 caches of 4,096 of them takes 1,310 us (1.6 TB/s): its
 // four rows are one wave's, whose 128 products of 32 x 32 x 2 a tile of 32 keys, 64
-// cycles each, are 870 us in two rounds of one work-group a CU.
+// cycles each, are 870 us in two turns of one work-group a CU.
 #include "ops_common.h"
 
 namespace mgopt {
